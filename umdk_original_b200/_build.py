@@ -46,8 +46,13 @@ KERNEL_SOURCES = [
     "kernels/dispatch_noalloc.cu",
     "kernels/sync_p2p.cu",
     "kernels/tp_exchange.cu",
+    "kernels/quant_fp4.cu",
+    "kernels/grouped_gemm_fp4.cu",
     "runtime/cam_runtime.cpp",
+    "runtime/expert_ops.cpp",
 ]
+
+BINDING_SOURCES = ["bindings.cpp", "bindings_expert.cpp"]
 
 
 def _nvcc() -> str:
@@ -71,7 +76,7 @@ def _check_gemm_registers(ptxas_log: str, src: Path) -> None:
     CTA is launched with; that count must be the kLaunchRegs constant of the source, or the
     kernel would wait for registers that never come."""
     import re
-    want = int(re.search(r"k(?:Mx|P2|I8|Fm|MT)?LaunchRegs\s*=\s*(\d+)", src.read_text()).group(1))
+    want = int(re.search(r"k(?:Mx|P2|I8|Fm|MT|F4|Em)?LaunchRegs\s*=\s*(\d+)", src.read_text()).group(1))
     # only the GEMM kernels re-partition registers; a file may hold other kernels as well
     got = [int(n) for name, n in re.findall(r"Compiling entry function '([^']+)'.*?Used (\d+) registers", ptxas_log, re.S)
            if "grouped_gemm" in name or "fused_moe" in name]
@@ -126,7 +131,7 @@ def build_kernels(force: bool = False, debug: bool = False) -> Path:
             logs = list(ex.map(lambda j: _run(j[0]), jobs))
         for (_, src, obj), log in zip(jobs, logs):
             if src.name in ("grouped_gemm.cu", "grouped_gemm_mx.cu", "grouped_gemm_mx2.cu", "grouped_gemm_i8.cu",
-                            "grouped_gemm_rows_n_mx.cu", "grouped_gemm_rows_n_i8.cu", "fused_moe_mx.cu"):
+                            "grouped_gemm_rows_n_mx.cu", "grouped_gemm_rows_n_i8.cu", "fused_moe_mx.cu", "grouped_gemm_fp4.cu"):
                 _check_gemm_registers(log, src)
             _mark(src, obj, stamp)
     so = LIB / "libumdk_cam.so"
@@ -142,8 +147,8 @@ def build_bindings(force: bool = False, debug: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     out = PKG / ("_C" + suffix)
-    src = CSRC / "bindings.cpp"
-    obj = OBJ / "bindings.o"
+    srcs = [CSRC / n for n in BINDING_SOURCES]
+    objs = [OBJ / (src.stem + ".o") for src in srcs]
     cuda_inc = str(Path(_nvcc()).resolve().parent.parent / "include")
     incs = [*ce.include_paths(), sysconfig.get_paths()["include"], cuda_inc]
     cxx = os.environ.get("CXX", "g++")
@@ -151,13 +156,15 @@ def build_bindings(force: bool = False, debug: bool = False) -> Path:
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-Wno-deprecated-declarations"]
     cflags += ["-O0", "-g"] if debug else ["-O2"]
     stamp = _deps_digest(" ".join(cflags) + torch.__version__)
-    if force or _stale(src, obj, stamp):
-        _run([cxx, *cflags, *[f"-I{i}" for i in incs], "-c", str(src), "-o", str(obj)])
+    todo = [(src, obj) for src, obj in zip(srcs, objs) if force or _stale(src, obj, stamp)]
+    with ThreadPoolExecutor(max_workers=max(1, len(todo))) as ex:
+        list(ex.map(lambda j: _run([cxx, *cflags, *[f"-I{i}" for i in incs], "-c", str(j[0]), "-o", str(j[1])]), todo))
+    for src, obj in todo:
         _mark(src, obj, stamp)
         force = True
     if force or not out.exists():
         torch_lib = str(Path(torch.__file__).resolve().parent / "lib")
-        _run([cxx, "-shared", "-o", str(out), str(obj), f"-L{LIB}", "-lumdk_cam", f"-L{torch_lib}", "-lc10", "-ltorch",
+        _run([cxx, "-shared", "-o", str(out), *map(str, objs), f"-L{LIB}", "-lumdk_cam", f"-L{torch_lib}", "-lc10", "-ltorch",
               "-ltorch_cpu", "-ltorch_python", "-lc10_cuda", "-ltorch_cuda", "-Wl,-rpath,$ORIGIN/lib",
               f"-Wl,-rpath,{torch_lib}"])
     return out

@@ -18,6 +18,7 @@
 #include <string>
 
 #include "runtime/cam_runtime.h"
+#include "runtime/expert_ops.h"
 
 namespace {
 
@@ -1023,5 +1024,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         .def("act_s", &Buffer::act_s);
     m.def("set_phase_mask", [](int mask) { g_phase_mask = mask; });
     m.def("get_phase_mask", []() { return g_phase_mask; });
+    // (code, who, block, detail) of the first wait that ran out in a kernel of the operators without a Buffer, on the current device
+    m.def("expert_ops_status", []() {
+        CamStatus st{};
+        CAM_RT(cam_expert_ops_status(&st));
+        return std::make_tuple(st.code, st.who, st.block, st.detail);
+    });
     m.def("status_string", [](int code) { return std::string(cam_status_string(code)); });
 }

@@ -1,0 +1,222 @@
+// PyTorch bindings of the expert-MLP operators that need no Buffer: 4-bit quantisation, grouped products of 4-bit operands.
+// Schemas are added to the library that bindings.cpp defines.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+#include <torch/library.h>
+
+#include "runtime/cam_runtime.h"
+#include "runtime/expert_ops.h"
+
+namespace {
+
+#define CAM_ASSERT(cond, ...) TORCH_CHECK(cond, "umdk_cam_op_lib: ", __VA_ARGS__)
+#define CAM_RT(call) TORCH_CHECK((call) == 0, "umdk_cam_op_lib: ", cam_last_error())
+
+using OptTensor = c10::optional<at::Tensor>;
+
+// Numbers enter messages as text: formatting them through the string streams of TORCH_CHECK crashes in a process whose C++
+// runtime libraries disagree about the locale.
+std::string num(int64_t v) { return std::to_string(v); }
+std::string shape(at::IntArrayRef v) {
+    std::string s = "[";
+    for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + num(v[i]);
+    return s + "]";
+}
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+void check_operand(const at::Tensor& t, const at::Tensor& with, const char* what) {
+    CAM_ASSERT(t.device() == with.device(), what, " must be on ", with.device().str(), ", the device of the rows");
+    CAM_ASSERT(t.is_contiguous(), what, " must be contiguous");
+}
+
+int dtype_of(at::ScalarType t, const char* what) {
+    CAM_ASSERT(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat, what, " must be bfloat16, float16 or float32");
+    return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : 2;
+}
+
+at::ScalarType scale_type(int64_t block) {
+    CAM_ASSERT(block == 16 || block == 32, "block must be 16 (nvfp4) or 32 (mxfp4), got ", num(block));
+    return block == 16 ? at::kFloat8_e4m3fn : at::kFloat8_e8m0fnu;
+}
+
+// Block of a scale tensor, by its type.
+int64_t block_of(const at::Tensor& s, const char* what) {
+    CAM_ASSERT(s.scalar_type() == at::kFloat8_e4m3fn || s.scalar_type() == at::kFloat8_e8m0fnu, what,
+               " must be float8_e4m3fn (nvfp4) or float8_e8m0fnu (mxfp4)");
+    return s.scalar_type() == at::kFloat8_e4m3fn ? 16 : 32;
+}
+
+// Codes [..., K/2] with their scales [..., K/block]; returns K.
+int64_t check_fp4(const at::Tensor& q, const at::Tensor& s, int64_t block, const char* what) {
+    CAM_ASSERT(q.scalar_type() == at::kByte && q.dim() >= 1, what, " codes must be uint8 [..., K / 2]");
+    const int64_t k = q.size(-1) * 2;
+    CAM_ASSERT(k % block == 0, what, ": K ", num(k), " is not a multiple of the block ", num(block));
+    auto want = q.sizes().vec();
+    want.back() = k / block;
+    CAM_ASSERT(s.sizes() == at::IntArrayRef(want), what, " scales must be [..., K / ", num(block), "] for codes [..., K / 2]: got ",
+               shape(s.sizes()), " for ", shape(q.sizes()));
+    return k;
+}
+
+// A global scale: one float, or (where `per` > 0) one for each of `per` experts.  Only nvfp4 has them.
+const float* check_gscale(const OptTensor& g, const at::Tensor& with, int64_t block, int64_t per, const char* what) {
+    if (!given(g)) return nullptr;
+    CAM_ASSERT(block == 16, what, ": mxfp4 has no global scale");
+    check_operand(*g, with, what);
+    CAM_ASSERT(g->scalar_type() == at::kFloat && (per > 0 ? g->numel() == per : g->numel() == 1), what, " must be float32 with ",
+               num(per > 0 ? per : 1), " element(s)");
+    return g->data_ptr<float>();
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_fp4_empty(const at::Tensor& x, int64_t block) {
+    const auto st = scale_type(block);
+    CAM_ASSERT(x.dim() >= 1 && x.size(-1) % block == 0 && x.size(-1) > 0, "quantize_fp4: the last dimension must be a multiple of ", num(block));
+    auto qs = x.sizes().vec(), ss = x.sizes().vec();
+    qs.back() /= 2;
+    ss.back() /= block;
+    return {at::empty(qs, x.options().dtype(at::kByte)), at::empty(ss, x.options().dtype(st))};
+}
+
+// Global scales of a tensor: one, or one per leading index of a 3-D tensor (experts).
+int64_t gscales_of(const OptTensor& g, const at::Tensor& t) { return given(g) && t.dim() == 3 && g->numel() != 1 ? t.size(0) : 0; }
+
+std::tuple<at::Tensor, at::Tensor> quantize_fp4_cuda(const at::Tensor& x, int64_t block, const OptTensor& global_scale) {
+    check_operand(x, x, "x");
+    const int dt = dtype_of(x.scalar_type(), "x");
+    const int64_t per = gscales_of(global_scale, x);
+    const float* g = check_gscale(global_scale, x, block, per, "global_scale");
+    c10::cuda::CUDAGuard guard(x.device());
+    auto out = quantize_fp4_empty(x, block);
+    CAM_RT(cam_quantize_fp4(x.data_ptr(), dt, block == 16 ? 0 : 1, std::get<0>(out).data_ptr(), std::get<1>(out).data_ptr(), x.numel(), g,
+                            per > 0 ? per : 1, at::cuda::getCurrentCUDAStream().stream()));
+    return out;
+}
+
+at::Tensor dequantize_fp4_empty(const at::Tensor& q, c10::optional<at::ScalarType> dtype) {
+    auto shape = q.sizes().vec();
+    shape.back() *= 2;
+    return at::empty(shape, q.options().dtype(dtype.value_or(at::kBFloat16)));
+}
+
+at::Tensor dequantize_fp4_cuda(const at::Tensor& q, const at::Tensor& s, const OptTensor& global_scale, c10::optional<at::ScalarType> dtype) {
+    check_operand(q, q, "q");
+    check_operand(s, q, "s");
+    const int64_t block = block_of(s, "s");
+    check_fp4(q, s, block, "dequantize_fp4:");
+    const int64_t per = gscales_of(global_scale, q);
+    const float* g = check_gscale(global_scale, q, block, per, "global_scale");
+    const int dt = dtype_of(dtype.value_or(at::kBFloat16), "dtype");
+    c10::cuda::CUDAGuard guard(q.device());
+    at::Tensor out = dequantize_fp4_empty(q, dtype);
+    CAM_RT(cam_dequantize_fp4(q.data_ptr(), s.data_ptr(), dt, block == 16 ? 0 : 1, out.data_ptr(), out.numel(), g, per > 0 ? per : 1,
+                              at::cuda::getCurrentCUDAStream().stream()));
+    return out;
+}
+
+struct Fp4Problem {
+    int64_t rows, experts, n, k, block;
+    const float *a_gs, *w_gs;
+};
+
+Fp4Problem check_grouped_fp4(const at::Tensor& a_q, const at::Tensor& a_s, const at::Tensor& w_q, const at::Tensor& w_s,
+                             const at::Tensor& expert_offsets, const OptTensor& a_gs, const OptTensor& w_gs, int64_t n_step) {
+    check_operand(a_q, a_q, "a_q");
+    check_operand(a_s, a_q, "a_s");
+    check_operand(w_q, a_q, "w_q");
+    check_operand(w_s, a_q, "w_s");
+    check_operand(expert_offsets, a_q, "expert_offsets");
+    Fp4Problem p{};
+    p.block = block_of(a_s, "a_s");
+    CAM_ASSERT(block_of(w_s, "w_s") == p.block, "a_s and w_s must be of the same format");
+    CAM_ASSERT(a_q.dim() == 2 && w_q.dim() == 3 && a_q.size(1) == w_q.size(2), "a_q must be [M, K / 2] and w_q [E, N, K / 2]");
+    p.k = check_fp4(a_q, a_s, p.block, "a");
+    check_fp4(w_q, w_s, p.block, "w");
+    p.rows = a_q.size(0);
+    p.experts = w_q.size(0);
+    p.n = w_q.size(1);
+    CAM_ASSERT(p.k % 128 == 0 && p.k > 0, "K ", num(p.k), " must be a multiple of 128");
+    CAM_ASSERT(p.n % n_step == 0 && p.n > 0, "N ", num(p.n), " must be a multiple of ", num(n_step));
+    CAM_ASSERT(p.experts >= 1 && p.rows < (1ll << 31) && p.experts * p.n < (1ll << 31), "M, E and E * N must be below 2^31");
+    CAM_ASSERT(expert_offsets.scalar_type() == at::kInt && expert_offsets.numel() == p.experts + 1, "expert_offsets must be int32 [E+1]");
+    p.a_gs = check_gscale(a_gs, a_q, p.block, 0, "a_global_scale");
+    p.w_gs = check_gscale(w_gs, a_q, p.block, p.experts, "w_global_scale");
+    return p;
+}
+
+at::Tensor grouped_gemm_fp4_cuda(const at::Tensor& a_q, const at::Tensor& a_s, const at::Tensor& w_q, const at::Tensor& w_s,
+                                 const at::Tensor& expert_offsets, const OptTensor& a_gs, const OptTensor& w_gs) {
+    const Fp4Problem p = check_grouped_fp4(a_q, a_s, w_q, w_s, expert_offsets, a_gs, w_gs, 128);
+    c10::cuda::CUDAGuard guard(a_q.device());
+    at::Tensor out = at::empty({p.rows, p.n}, a_q.options().dtype(at::kBFloat16));
+    if (p.rows == 0) return out;
+    CAM_RT(cam_grouped_gemm_fp4(a_q.data_ptr(), a_s.data_ptr(), static_cast<int>(p.rows), w_q.data_ptr(), w_s.data_ptr(),
+                                expert_offsets.data_ptr<int>(), static_cast<int>(p.experts), static_cast<int>(p.n), static_cast<int>(p.k),
+                                p.block == 16 ? 0 : 1, 0, p.a_gs, p.w_gs, nullptr, out.data_ptr(), nullptr,
+                                at::cuda::getCurrentCUDAStream().stream()));
+    return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> grouped_gemm_fp4_swiglu_cuda(const at::Tensor& a_q, const at::Tensor& a_s, const at::Tensor& w_q,
+                                                                const at::Tensor& w_s, const at::Tensor& expert_offsets,
+                                                                const OptTensor& a_gs, const OptTensor& w_gs, const OptTensor& out_gs) {
+    const Fp4Problem p = check_grouped_fp4(a_q, a_s, w_q, w_s, expert_offsets, a_gs, w_gs, 256);
+    const float* og = check_gscale(out_gs, a_q, p.block, 0, "out_global_scale");
+    c10::cuda::CUDAGuard guard(a_q.device());
+    at::Tensor q = at::empty({p.rows, p.n / 4}, a_q.options());
+    at::Tensor s = at::empty({p.rows, p.n / 2 / p.block}, a_s.options());
+    if (p.rows == 0) return {q, s};
+    CAM_RT(cam_grouped_gemm_fp4(a_q.data_ptr(), a_s.data_ptr(), static_cast<int>(p.rows), w_q.data_ptr(), w_s.data_ptr(),
+                                expert_offsets.data_ptr<int>(), static_cast<int>(p.experts), static_cast<int>(p.n), static_cast<int>(p.k),
+                                p.block == 16 ? 0 : 1, 1, p.a_gs, p.w_gs, og, q.data_ptr(), s.data_ptr(),
+                                at::cuda::getCurrentCUDAStream().stream()));
+    return {q, s};
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_fp4_meta(const at::Tensor& x, int64_t block, const OptTensor&) { return quantize_fp4_empty(x, block); }
+at::Tensor dequantize_fp4_meta(const at::Tensor& q, const at::Tensor&, const OptTensor&, c10::optional<at::ScalarType> dtype) {
+    return dequantize_fp4_empty(q, dtype);
+}
+at::Tensor grouped_gemm_fp4_meta(const at::Tensor& a_q, const at::Tensor&, const at::Tensor& w_q, const at::Tensor&, const at::Tensor&,
+                                 const OptTensor&, const OptTensor&) {
+    return at::empty({a_q.size(0), w_q.size(1)}, a_q.options().dtype(at::kBFloat16));
+}
+std::tuple<at::Tensor, at::Tensor> grouped_gemm_fp4_swiglu_meta(const at::Tensor& a_q, const at::Tensor& a_s, const at::Tensor& w_q,
+                                                                const at::Tensor&, const at::Tensor&, const OptTensor&, const OptTensor&,
+                                                                const OptTensor&) {
+    return {at::empty({a_q.size(0), w_q.size(1) / 4}, a_q.options()),
+            at::empty({a_q.size(0), w_q.size(1) / 2 / block_of(a_s, "a_s")}, a_s.options())};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(umdk_cam_op_lib, m) {
+    m.def("quantize_fp4(Tensor x, int block=16, Tensor? global_scale=None) -> (Tensor, Tensor)");
+    m.def("dequantize_fp4(Tensor q, Tensor s, Tensor? global_scale=None, ScalarType? dtype=None) -> Tensor");
+    m.def("grouped_gemm_fp4(Tensor a_q, Tensor a_s, Tensor w_q, Tensor w_s, Tensor expert_offsets, "
+          "Tensor? a_global_scale=None, Tensor? w_global_scale=None) -> Tensor");
+    m.def("grouped_gemm_fp4_swiglu(Tensor a_q, Tensor a_s, Tensor w_q, Tensor w_s, Tensor expert_offsets, "
+          "Tensor? a_global_scale=None, Tensor? w_global_scale=None, Tensor? out_global_scale=None) -> (Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(umdk_cam_op_lib, CUDA, m) {
+    m.impl("quantize_fp4", &quantize_fp4_cuda);
+    m.impl("dequantize_fp4", &dequantize_fp4_cuda);
+    m.impl("grouped_gemm_fp4", &grouped_gemm_fp4_cuda);
+    m.impl("grouped_gemm_fp4_swiglu", &grouped_gemm_fp4_swiglu_cuda);
+}
+
+TORCH_LIBRARY_IMPL(umdk_cam_op_lib, Meta, m) {
+    m.impl("quantize_fp4", &quantize_fp4_meta);
+    m.impl("dequantize_fp4", &dequantize_fp4_meta);
+    m.impl("grouped_gemm_fp4", &grouped_gemm_fp4_meta);
+    m.impl("grouped_gemm_fp4_swiglu", &grouped_gemm_fp4_swiglu_meta);
+}
+
+TORCH_LIBRARY_IMPL(umdk_cam_op_lib, Autograd, m) {
+    m.impl("quantize_fp4", torch::autograd::autogradNotImplementedFallback());
+    m.impl("dequantize_fp4", torch::autograd::autogradNotImplementedFallback());
+    m.impl("grouped_gemm_fp4", torch::autograd::autogradNotImplementedFallback());
+    m.impl("grouped_gemm_fp4_swiglu", torch::autograd::autogradNotImplementedFallback());
+}

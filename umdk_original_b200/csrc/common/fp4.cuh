@@ -1,0 +1,105 @@
+// 4-bit floating point with block scales.
+//   e2m1     values 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives; two to a byte, the even element in the low nibble
+//   nvfp4    blocks of 16: s = e4m3(amax / (6 g)), q = e2m1(x / (s g)), x ~ q s g with one fp32 scale g per tensor or expert
+//   mxfp4    blocks of 32: s = 2^k, the smallest with 2^k >= amax / 6 (k >= -126; an all-zero block has 2^-127), x ~ q s
+// All roundings are to nearest, ties to even.  A NaN anywhere in an nvfp4 block makes its scale NaN (and with it the whole
+// block); an infinity takes the largest scale and saturates to 6.  In mxfp4 NaN gives the scale code 255 (NaN), an
+// infinity the scale 2^127.
+#pragma once
+#include "ptx.cuh"
+
+namespace cam {
+
+constexpr int kFp4Nv = 0, kFp4Mx = 1;  // formats
+__host__ __device__ constexpr int fp4_block(int fmt) { return fmt == kFp4Nv ? 16 : 32; }
+
+// Eight floats (already divided by their scale) to four bytes of e2m1, saturating.
+__device__ __forceinline__ uint32_t pack_e2m1x8(float a0, float a1, float a2, float a3, float a4, float a5, float a6, float a7) {
+    uint32_t r;
+    asm("{\n"
+        ".reg .b8 b0, b1, b2, b3;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n"  // the first source lands in the upper nibble
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n"
+        "mov.b32 %0, {b0, b1, b2, b3};\n"
+        "}\n"
+        : "=r"(r)
+        : "f"(a0), "f"(a1), "f"(a2), "f"(a3), "f"(a4), "f"(a5), "f"(a6), "f"(a7));
+    return r;
+}
+
+// Four bytes of e2m1 to eight halves (every e2m1 value is exact in fp16).
+__device__ __forceinline__ void unpack_e2m1x8(uint32_t w, uint32_t (&h)[4]) {
+    asm("{\n"
+        ".reg .b8 b0, b1, b2, b3;\n"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n"
+        "}\n"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(w));
+}
+
+__device__ __forceinline__ uint32_t e4m3_code(float v) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
+    return r & 0xFFu;
+}
+__device__ __forceinline__ float e4m3_value(uint32_t code) {
+    __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3);
+    return __half2float(*reinterpret_cast<__half*>(&h));
+}
+__device__ __forceinline__ float e8m0_value(uint32_t code) {  // 2^(code - 127); code 255 is NaN
+    return __uint_as_float(code == 0u ? 0x00400000u : code == 255u ? 0x7FC00000u : code << 23);
+}
+
+// The scale of a block from the bits of its largest magnitude: its code, the divisor d and 1 / d rounded to nearest.
+// (The maximum of magnitudes as unsigned integers is the maximum of the values, with NaN above infinity.)
+template <int FMT>
+__device__ __forceinline__ uint32_t fp4_scale(uint32_t amax_bits, float g, float six_g, float& d, float& inv) {
+    const float amax = __uint_as_float(amax_bits);
+    if (FMT == kFp4Nv) {
+        const uint32_t code = e4m3_code(__fdiv_rn(amax, six_g));
+        d = __fmul_rn(e4m3_value(code), g);
+        inv = d > 0.f ? __fdiv_rn(1.f, d) : 0.f;  // d is NaN for a NaN block, whose codes mean nothing
+        return code;
+    }
+    if (amax_bits > 0x7F800000u) {
+        d = amax;
+        inv = 0.f;
+        return 255u;
+    }
+    const uint32_t b = __float_as_uint(__fdiv_rn(amax, 6.f));
+    uint32_t e = (b >> 23) + ((b & 0x7FFFFFu) ? 1u : 0u);
+    e = e > 254u ? 254u : e;
+    d = e8m0_value(e);
+    inv = e == 254u ? __uint_as_float(0x00400000u) : e == 0u ? 0.f : __uint_as_float((254u - e) << 23);
+    return e;
+}
+
+// x / d rounded to nearest.  nvfp4: with y = x inv and inv = 1 / d rounded to nearest, one remainder step
+// y + (x - y d) inv gives the correctly rounded quotient (Markstein, "Computation of elementary functions on the IBM RISC
+// System/6000 processor", 1990), so that a quotient half-way between two e2m1 values is seen as one.  `finite` is false for
+// a block that holds an infinity, where the remainder would be NaN.  mxfp4 divides by a power of two: the product is exact.
+template <int FMT>
+__device__ __forceinline__ float fp4_divide(float x, float d, float inv, bool finite) {
+    const float y = x * inv;
+    if (FMT == kFp4Mx) return y;
+    const float z = __fmaf_rn(__fmaf_rn(-y, d, x), inv, y);
+    return finite ? z : y;
+}
+
+// Sixteen floats to eight bytes of codes.
+template <int FMT>
+__device__ __forceinline__ uint2 fp4_codes16(const float* v, float d, float inv, bool finite) {
+    float y[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = fp4_divide<FMT>(v[i], d, inv, finite);
+    return make_uint2(pack_e2m1x8(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]),
+                      pack_e2m1x8(y[8], y[9], y[10], y[11], y[12], y[13], y[14], y[15]));
+}
+
+}  // namespace cam

@@ -1,0 +1,430 @@
+// Grouped product of 4-bit operands (nvfp4 / mxfp4, ../common/fp4.cuh) on CTA pairs, for the rows of every expert:
+//   y[r, n] = a_g w_g[e] sum_k (a_q a_s)[r, k] (w_q w_s)[e, n, k]
+// and the first product of an expert MLP, whose epilogue forms silu(gate) * up and writes it back as 4-bit rows.
+//
+// The tensor core multiplies e2m1 values and applies the block scales itself (kind::mxf4nvf4 with 16 values per scale,
+// kind::mxf4 with 32), so a tile is a loop over K-blocks of 256 values (128 bytes of a row).  A pair of CTAs computes 256
+// rows x 256 columns: each holds its 128 rows of A and HALF of the weight tile, one CTA issues the MMAs of both.
+//
+// Scales stay in memory as the quantiser wrote them, row by row; the tensor core wants them in tensor memory as
+// [32 lanes][4 words] per 128 rows and 64 values (word j of lane l: row 32 j + l).  Three warps per CTA (its rows, the lower
+// and the upper 128 weight rows) bring them there: lane l copies the 16 bytes of rows l, 32 + l, 64 + l, 96 + l of a K-block
+// into the stage's slot with cp.async, three K-blocks ahead, transposes the 4 x 4 words in place (the slot holds the same
+// four addresses of this lane before and after) and raises the stage's barrier.  The MMA issuer then moves the slot into
+// tensor memory with tcgen05.cp directly in front of the MMAs that read it.
+//
+// Barriers: as in grouped_gemm_mx2.cu, bar_sf counts the 3 + 3 scale warps of the pair.
+#include "../common/fp4.cuh"
+#include "expert_gemm.cuh"
+
+namespace cam {
+
+constexpr int kF4Threads = 768;
+constexpr int kF4EpiThreads = 512;
+constexpr int kF4SfWarp0 = 4, kF4EpiWarp0 = 8;
+constexpr int kF4Stages = 5;
+constexpr int kF4K = 256;                      // values of one K-block
+constexpr int kF4Tile = 128 * 128;             // 128 rows of one K-block, 16 KiB
+constexpr int kF4StageBytes = 2 * kF4Tile;
+constexpr int kF4SfBlock = 4 * 512;            // scales of 128 rows (mxfp4 uses half)
+constexpr int kF4SfStage = 3 * kF4SfBlock;
+constexpr int kF4StgPitch = 272;               // bf16 rows of 128 columns, 16 bytes apart from a multiple of 128
+constexpr int kF4StgBytes = 128 * kF4StgPitch;
+constexpr int kF4Smem = kF4Stages * (kF4StageBytes + kF4SfStage) + kF4StgBytes + 1024;
+static_assert(kF4Smem <= 232448, "exceeds the shared memory of one CTA");
+constexpr int kF4Ahead = 3;                    // K-blocks whose scales are on their way
+static_assert(kF4Ahead <= kF4Stages, "scale copies may not run further ahead than there are stages");
+constexpr uint32_t kF4TmemCols = 512, kF4SfCol0 = 256, kF4SfCols = 48;
+static_assert(kF4SfCol0 + kF4Stages * kF4SfCols <= kF4TmemCols, "tensor memory");
+// setmaxnreg: the shares must not exceed what the CTA was launched with (checked against ptxas by the build)
+constexpr uint32_t kF4LaunchRegs = 80, kF4CtrlRegs = 32, kF4SfRegs = 56, kF4EpiRegs = 96;
+static_assert(128 * kF4CtrlRegs + 128 * kF4SfRegs + kF4EpiThreads * kF4EpiRegs <= kF4LaunchRegs * kF4Threads,
+              "setmaxnreg budget exceeds the registers the CTA owns: the kernel would hang");
+
+static __device__ CamStatus g_fp4_status;
+
+namespace {
+
+// D (+)= (A sfa) (B sfb), e2m1 x e2m1, on the pair; the formats differ in the scales' type and block
+template <int FMT>
+__device__ __forceinline__ void tc_mma_fp4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate, uint32_t sfa_tmem, uint32_t sfb_tmem) {
+    if constexpr (FMT == kFp4Nv) {
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%5], [%6], p;\n"
+            "}\n" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n"
+            "}\n" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+            : "memory");
+    }
+}
+
+// Instruction descriptor of kind::mxf4 / mxf4nvf4: e2m1 (1) at [7,10) and [10,12), N>>3 at [17,23), scale type [23]
+// (0 = e4m3, 1 = e8m0), M>>4 at [24,29), bytes of the scale word for B at [4,6) and for A at [29,31): 0 or 2.
+template <int FMT>
+__device__ __forceinline__ constexpr uint32_t idesc_fp4(uint32_t m, uint32_t n, uint32_t sf_id) {
+    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((FMT == kFp4Mx ? 1u : 0u) << 23) | ((m >> 4) << 24) |
+           (sf_id << 29);
+}
+
+// Shared-memory matrix without swizzle, 16 bytes wide: groups of 8 rows 128 bytes apart (the 512 bytes of one scale tile)
+__device__ __forceinline__ uint64_t desc_scales(uint32_t smem_addr) {
+    return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+
+// 32 rows x 16 bytes of shared memory to 32 lanes x 4 columns of tensor memory, repeated in all four lane quarters, in both CTAs
+__device__ __forceinline__ void tc_copy_scales_pair(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {  // zeros where not `live`
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(live ? BYTES : 0), "n"(BYTES) : "memory");
+}
+
+}  // namespace
+
+template <int FMT, bool SWIGLU>
+__global__ void __launch_bounds__(kF4Threads, 1)
+grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
+                        const __grid_constant__ CUtensorMap tmap_b, const GroupedGemmFp4Params p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 1023u) {  // swizzled TMA tiles need it; the same in both CTAs of a pair
+        if (threadIdx.x == 0) gemm_record_status(&g_fp4_status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
+        return;
+    }
+    constexpr int NS = kF4Stages;
+    constexpr int SFW = FMT == kFp4Nv ? 4 : 2;  // scale words of a row and K-block
+    constexpr int BLK = fp4_block(FMT);
+    uint8_t* sfm = smem + NS * kF4StageBytes;
+    uint8_t* stg = sfm + NS * kF4SfStage;
+    uint8_t* ctrl = stg + kF4StgBytes;
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(ctrl);  // first CTA: TMA bytes of both CTAs' stage have landed
+    uint64_t* bar_sf = bar_full + NS;                        // first CTA: scale slots of both CTAs are ready
+    uint64_t* bar_empty = bar_sf + NS;                       // each CTA: the MMAs that read a stage have retired
+    uint64_t* bar_tfull = bar_empty + NS;                    // each CTA: accumulator of a tile is complete
+    uint64_t* bar_tempty = bar_tfull + 1;                    // first CTA: both accumulators have been drained
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_tempty + 1);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+
+    const int warp = static_cast<int>(threadIdx.x) >> 5;
+    const uint32_t lane = lane_id();
+    const uint32_t cta = cluster_cta_rank();  // 0 = first CTA of the pair (issues the MMAs)
+    const int pair_id = static_cast<int>(blockIdx.x) >> 1;
+    const int num_pairs = static_cast<int>(gridDim.x) >> 1;
+    const int kblocks = (p.k_dim + kF4K - 1) / kF4K;
+    const int half_n = p.n_dim / 2;
+    const int n_tiles = SWIGLU ? half_n / 128 : (p.n_dim + 255) / 256;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&bar_full[s], 1);
+            mbar_init(&bar_sf[s], 6);
+            mbar_init(&bar_empty[s], 1);
+        }
+        mbar_init(bar_tfull, 1);
+        mbar_init(bar_tempty, 2 * (kF4EpiThreads / 32));
+        *abort_flag = 0u;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, kF4TmemCols);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();  // both CTAs' barriers are initialised before anything signals them
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    PairTileWalker w(p.expert_offsets, p.num_experts, n_tiles, p.rows);
+    int e, nt, row0, rows;
+    bool ok = true;
+    // first weight row of the lower / upper half of a tile
+    auto b_row = [&](int half) { return e * p.n_dim + (SWIGLU ? half * half_n + nt * 128 : nt * 256 + half * 128); };
+
+    if (warp < kF4SfWarp0) {
+        reg_dealloc<kF4CtrlRegs>();
+        if (warp == 0 && lane == 0) {
+            // ------------------------------------------------------------ TMA producer (both CTAs)
+            prefetch_tensormap(&tmap_a);
+            prefetch_tensormap(&tmap_a32);
+            prefetch_tensormap(&tmap_b);
+            uint32_t it = 0;
+            // Only 32-row pieces of A that hold rows are loaded; what stays in the other rows of the stage reaches
+            // accumulator rows that nobody reads.
+            auto pieces = [](int r) { return r > 96 ? 4 : r > 0 ? (r + 31) / 32 : 0; };
+            for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows); tile += num_pairs) {
+                const int p0 = pieces(min(rows, BM)), p1 = pieces(rows - BM);
+                const int mine = cta ? p1 : p0;
+                const uint32_t bytes = 2u * kF4Tile + static_cast<uint32_t>(p0 + p1) * 4096u;
+                const int arow = row0 + static_cast<int>(cta) * BM, brow = b_row(static_cast<int>(cta));
+                for (int kb = 0; kb < kblocks; ++kb, ++it) {
+                    const uint32_t s = it % NS, ph = (it / NS) & 1u;
+                    if (!mbar_wait_bounded(&bar_empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
+                    uint8_t* sa = smem + s * kF4StageBytes;
+                    if (cta == 0) mbar_arrive_expect_tx(&bar_full[s], bytes);
+                    const uint32_t full0 = map_to_cta(&bar_full[s], 0);
+                    tma_load_2d_pair(sa + kF4Tile, &tmap_b, full0, kb * 128, brow);
+                    if (mine == 4) tma_load_2d_pair(sa, &tmap_a, full0, kb * 128, arow);
+                    else for (int i = 0; i < mine; ++i) tma_load_2d_pair(sa + i * 4096, &tmap_a32, full0, kb * 128, arow + i * 32);
+                }
+            }
+            if (!ok) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 0, static_cast<int>(it));
+        } else if (warp == 1 && lane == 0 && cta == 0) {
+            // ------------------------------------------------------------ MMA issuer (first CTA only)
+            uint32_t it = 0, tcount = 0;
+            const uint32_t tfull0 = map_to_cta(bar_tfull, 0), tfull1 = map_to_cta(bar_tfull, 1);
+            for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
+                // both epilogues must have drained the previous tile before its columns are overwritten
+                if (!mbar_wait_bounded(bar_tempty, (tcount & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                tc_fence_after_sync();
+                for (int kb = 0; kb < kblocks; ++kb, ++it) {
+                    const uint32_t s = it % NS, ph = (it / NS) & 1u;
+                    if (!mbar_wait_bounded(&bar_sf[s], ph, abort_flag)) { ok = false; break; }
+                    if (!mbar_wait_bounded(&bar_full[s], ph, abort_flag)) { ok = false; break; }
+                    tc_fence_after_sync();
+                    const uint32_t sa = smem_u32(smem + s * kF4StageBytes);
+                    const uint64_t adesc = umma_desc_k_sw128(sa), bdesc = umma_desc_k_sw128(sa + kF4Tile);
+                    const uint32_t sfs = smem_u32(sfm + s * kF4SfStage);
+                    const uint32_t sf = tmem_base + kF4SfCol0 + s * kF4SfCols;  // SFW x (4 columns of A, 8 of B)
+#pragma unroll
+                    for (int k = 0; k < SFW; ++k) {
+                        tc_copy_scales_pair(sf + 12u * k, desc_scales(sfs + k * 512));
+                        tc_copy_scales_pair(sf + 12u * k + 4u, desc_scales(sfs + kF4SfBlock + k * 512));
+                        tc_copy_scales_pair(sf + 12u * k + 8u, desc_scales(sfs + 2 * kF4SfBlock + k * 512));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {  // 64 values = 32 bytes (2 x 16) further along K inside the swizzle atom
+                        const uint32_t c = sf + 12u * (FMT == kFp4Nv ? k : k >> 1);
+                        tc_mma_fp4_pair<FMT>(tmem_base, adesc + 2u * k, bdesc + 2u * k,
+                                             idesc_fp4<FMT>(2 * BM, 256, FMT == kFp4Nv ? 0u : 2u * (k & 1)), (kb | k) ? 1u : 0u, c, c + 4u);
+                    }
+                    // the stage and its scale slot, in both CTAs, are reusable once these have retired
+                    tc_commit_pair(map_to_cta(&bar_empty[s], 0));
+                    tc_commit_pair(map_to_cta(&bar_empty[s], 1));
+                }
+                if (!ok) break;
+                tc_commit_pair(tfull0);
+                tc_commit_pair(tfull1);
+            }
+            if (!ok) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(it));
+        }
+    } else if (warp < kF4EpiWarp0) {
+        reg_dealloc<kF4SfRegs>();
+        // ---------------------------------------------------------------- scale warps: rows, lower and upper weight rows
+        const int what = warp - kF4SfWarp0;
+        if (what < 3) {
+            const int pitch = p.k_dim / BLK;          // bytes of scales of a row
+            const int words = pitch / 4;
+            const uint32_t slot0 = smem_u32(sfm + what * kF4SfBlock) + lane * 16u;
+            const uint8_t* src[4] = {nullptr, nullptr, nullptr, nullptr};
+            const int last_b = p.num_experts * p.n_dim - 1;
+            uint32_t issued = 0, done = 0;
+            int tile = pair_id, kb = 0;
+            bool more = true;
+            while (true) {
+                while (more && issued - done < kF4Ahead) {
+                    if (kb == 0) {
+                        if (!w.locate(tile, e, nt, row0, rows)) { more = false; break; }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int r = 32 * j + static_cast<int>(lane);
+                            if (what == 0) src[j] = p.a_scales + static_cast<size_t>(min(row0 + static_cast<int>(cta) * BM + r, p.rows - 1)) * pitch;
+                            else src[j] = p.b_scales + static_cast<size_t>(min(b_row(what - 1) + r, last_b)) * pitch;
+                        }
+                    }
+                    const uint32_t s = issued % NS;
+                    const bool got = mbar_wait_bounded(&bar_empty[s], ((issued / NS) & 1u) ^ 1u, abort_flag);
+                    if (!__all_sync(0xFFFFFFFFu, got)) { ok = false; break; }
+                    const uint32_t dst = slot0 + s * kF4SfStage;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t d = FMT == kFp4Nv ? dst + j * 512u : dst + (j >> 1) * 512u + (j & 1) * 8u;
+                        const uint8_t* from = src[j] + kb * SFW * 4;
+                        if (p.scale_vec) {
+                            copy_async<SFW * 4>(d, from, true);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < SFW; ++i) {
+                                const bool live = kb * SFW + i < words;
+                                copy_async<4>(d + i * 4u, live ? from + i * 4 : src[j], live);
+                            }
+                        }
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    ++issued;
+                    if (++kb == kblocks) { kb = 0; tile += num_pairs; }
+                }
+                if (!ok || issued == done) break;
+                if (issued - done == kF4Ahead) asm volatile("cp.async.wait_group %0;" ::"n"(kF4Ahead - 1) : "memory");
+                else asm volatile("cp.async.wait_group 0;" ::: "memory");
+                // this lane's words, in place: [row j][K-step i] -> [K-step i][row j]
+                uint8_t* slot = sfm + (done % NS) * kF4SfStage + what * kF4SfBlock + lane * 16u;
+                if constexpr (FMT == kFp4Nv) {
+                    const uint4 a = *reinterpret_cast<uint4*>(slot), b = *reinterpret_cast<uint4*>(slot + 512);
+                    const uint4 c = *reinterpret_cast<uint4*>(slot + 1024), d = *reinterpret_cast<uint4*>(slot + 1536);
+                    *reinterpret_cast<uint4*>(slot) = make_uint4(a.x, b.x, c.x, d.x);
+                    *reinterpret_cast<uint4*>(slot + 512) = make_uint4(a.y, b.y, c.y, d.y);
+                    *reinterpret_cast<uint4*>(slot + 1024) = make_uint4(a.z, b.z, c.z, d.z);
+                    *reinterpret_cast<uint4*>(slot + 1536) = make_uint4(a.w, b.w, c.w, d.w);
+                } else {
+                    const uint4 a = *reinterpret_cast<uint4*>(slot), b = *reinterpret_cast<uint4*>(slot + 512);
+                    *reinterpret_cast<uint4*>(slot) = make_uint4(a.x, a.z, b.x, b.z);
+                    *reinterpret_cast<uint4*>(slot + 512) = make_uint4(a.y, a.w, b.y, b.w);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {  // the first CTA's barrier counts the warps of both CTAs
+                    if (cta == 0) mbar_arrive(&bar_sf[done % NS]);
+                    else mbar_arrive_cluster(map_to_cta(&bar_sf[done % NS], 0));
+                }
+                ++done;
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");  // nothing of this warp is in flight when the CTA ends
+            if (!ok && lane == 0) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 3, static_cast<int>(done));
+        }
+    } else {
+        reg_alloc<kF4EpiRegs>();
+        // ---------------------------------------------------------------- epilogue warps
+        const int ew = warp - kF4EpiWarp0;
+        const int q = warp & 3;   // TMEM lane quarter this warp may read
+        const int cq = ew >> 2;   // which 32-column quarter of each 128-column half
+        const int r = q * 32 + static_cast<int>(lane);
+        const float a_g = p.a_gscale != nullptr ? __ldg(p.a_gscale) : 1.f;
+        const float out_g = p.out_gscale != nullptr ? __ldg(p.out_gscale) : 1.f;
+        uint32_t tcount = 0;
+        for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
+            row0 += static_cast<int>(cta) * BM;
+            rows = max(0, min(BM, rows - static_cast<int>(cta) * BM));
+            const bool valid = r < rows;
+            const size_t grow = static_cast<size_t>(row0 + (valid ? r : 0));
+            const float alpha = p.b_gscale != nullptr ? a_g * __ldg(p.b_gscale + e) : a_g;
+            if (!mbar_wait_bounded(bar_tfull, tcount & 1u, abort_flag, 2000000000ull, 64u)) { ok = false; break; }
+            tc_fence_after_sync();
+            const uint32_t t0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + cq * 32;
+            uint32_t v0[32], v1[32];  // columns cq*32.. of the first 128-column half, same of the second
+            tmem_ld_32x32b_x32(t0, v0);
+            tmem_ld_32x32b_x32(t0 + 128, v1);
+            tc_wait_ld_regs(v0);
+            tc_wait_ld_regs(v1);
+            // the tile now lives in registers: hand the accumulator back to the MMA issuer
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (cta == 0) mbar_arrive(bar_tempty);
+                else mbar_arrive_cluster(map_to_cta(bar_tempty, 0));
+            }
+            if constexpr (SWIGLU) {
+                // silu(gate) * up of 32 columns, then their scales (two blocks of 16 or one of 32) and codes
+                float act[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const float g = __uint_as_float(v0[j]) * alpha;
+                    act[j] = (g / (1.f + expf(-g))) * (__uint_as_float(v1[j]) * alpha);
+                }
+                const float six_g = __fmul_rn(6.f, out_g);
+                uint32_t amax[2] = {0u, 0u};
+#pragma unroll
+                for (int j = 0; j < 32; ++j) amax[j >> 4] = max(amax[j >> 4], __float_as_uint(act[j]) & 0x7FFFFFFFu);
+                if (FMT == kFp4Mx) amax[0] = amax[1] = max(amax[0], amax[1]);
+                uint2 codes[2];
+                uint32_t sc[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float d, inv;
+                    sc[h] = fp4_scale<FMT>(amax[h], out_g, six_g, d, inv);
+                    codes[h] = fp4_codes16<FMT>(act + 16 * h, d, inv, amax[h] < 0x7F800000u);
+                }
+                if (valid) {
+                    const size_t at = grow * (half_n / 32) + nt * 4 + cq;  // in units of 32 columns
+                    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + at * 16) = make_uint4(codes[0].x, codes[0].y, codes[1].x, codes[1].y);
+                    if (FMT == kFp4Nv) *reinterpret_cast<uint16_t*>(p.out_scales + at * 2) = static_cast<uint16_t>(sc[0] | (sc[1] << 8));
+                    else p.out_scales[at] = static_cast<uint8_t>(sc[0]);
+                }
+            } else {
+                // 128 columns at a time go through shared memory as bf16 and leave as one 256-byte bulk copy per row
+                __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) + grow * p.n_dim;
+                auto push_half = [&](const uint32_t (&v)[32], int c0) {
+                    uint8_t* srow = stg + r * kF4StgPitch;
+                    if (cq == 0) bulk_wait_group_read<0>();  // the copies that read this buffer are done with it
+                    named_bar_sync(1, kF4EpiThreads);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                        *reinterpret_cast<uint4*>(srow + cq * 64 + j * 2) =
+                            pack_bf16x8(__uint_as_float(v[j]) * alpha, __uint_as_float(v[j + 1]) * alpha, __uint_as_float(v[j + 2]) * alpha,
+                                        __uint_as_float(v[j + 3]) * alpha, __uint_as_float(v[j + 4]) * alpha, __uint_as_float(v[j + 5]) * alpha,
+                                        __uint_as_float(v[j + 6]) * alpha, __uint_as_float(v[j + 7]) * alpha);
+                    fence_proxy_async_smem();
+                    named_bar_sync(1, kF4EpiThreads);
+                    if (cq == 0) {
+                        if (valid) bulk_store_s2g(orow + c0, srow, 256);
+                        bulk_commit_group();
+                    }
+                };
+                const int c_lo = nt * 256;
+                push_half(v0, c_lo);
+                if (c_lo + 128 < p.n_dim) push_half(v1, c_lo + 128);  // same answer in every thread of the CTA
+            }
+        }
+        if (!SWIGLU && cq == 0) bulk_wait_group<0>();  // every row this thread sent has been written
+        if (!ok) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
+        // rows of no expert
+        const int et = static_cast<int>(threadIdx.x) - kF4EpiWarp0 * 32;
+        if constexpr (SWIGLU) {
+            zero_loose_rows(p.out, half_n / 32, p.expert_offsets, p.num_experts, p.rows, et, kF4EpiThreads);
+            const int head = expert_bound(p.expert_offsets, 0, p.rows), tail = expert_bound(p.expert_offsets, p.num_experts, p.rows);
+            const int64_t sp = half_n / BLK, n0 = head * sp, n1 = (p.rows - tail) * sp;
+            for (int64_t i = static_cast<int64_t>(blockIdx.x) * kF4EpiThreads + et; i < n0 + n1; i += static_cast<int64_t>(gridDim.x) * kF4EpiThreads)
+                p.out_scales[i < n0 ? i : tail * sp + (i - n0)] = 0;
+        } else {
+            zero_loose_rows(p.out, p.n_dim / 8, p.expert_offsets, p.num_experts, p.rows, et, kF4EpiThreads);
+        }
+    }
+
+    // ------------------------------------------------------------------ teardown
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();  // the other CTA may still read this CTA's shared memory or signal its barriers
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem_base, kF4TmemCols);
+    }
+}
+
+}  // namespace cam
+
+namespace {
+
+template <int FMT, bool SWIGLU>
+int launch_fp4(const cam::GroupedGemmFp4Params* p, const CUtensorMap* ta, const CUtensorMap* ta32, const CUtensorMap* tb, cudaStream_t stream) {
+    static cam::PairLimit limit;
+    // at most one row block per expert beyond the full ones
+    const int64_t n_tiles = SWIGLU ? p->n_dim / 256 : (p->n_dim + 255) / 256;
+    const int64_t blocks = p->rows / 256 + (p->rows < p->num_experts ? p->rows : p->num_experts);
+    return cam::launch_pairs(limit, cam::grouped_gemm_fp4_kernel<FMT, SWIGLU>, cam::kF4Threads, cam::kF4Smem, blocks * n_tiles, stream, *ta, *ta32, *tb, *p);
+}
+
+}  // namespace
+
+extern "C" int cam_launch_grouped_gemm_fp4(const cam::GroupedGemmFp4Params* p, int fmt, int swiglu, const CUtensorMap* tmap_a,
+                                           const CUtensorMap* tmap_a32, const CUtensorMap* tmap_b, cudaStream_t stream) {
+    if (fmt == cam::kFp4Nv)
+        return swiglu ? launch_fp4<cam::kFp4Nv, true>(p, tmap_a, tmap_a32, tmap_b, stream) : launch_fp4<cam::kFp4Nv, false>(p, tmap_a, tmap_a32, tmap_b, stream);
+    return swiglu ? launch_fp4<cam::kFp4Mx, true>(p, tmap_a, tmap_a32, tmap_b, stream) : launch_fp4<cam::kFp4Mx, false>(p, tmap_a, tmap_a32, tmap_b, stream);
+}
+
+extern "C" int cam_fp4_status(CamStatus* out) { return static_cast<int>(cudaMemcpyFromSymbol(out, cam::g_fp4_status, sizeof(CamStatus))); }

@@ -17,6 +17,7 @@
 #include <tuple>
 #include <vector>
 
+#include "../kernels/expert_ops.h"
 #include "../kernels/launch.h"
 
 namespace {
@@ -896,6 +897,32 @@ static EncodeTiledFn get_encode_fn() {
     });
     return fn;
 }
+
+extern "C" int cam_encode_tmap(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                               const uint32_t* box) {
+    EncodeTiledFn fn = get_encode_fn();
+    CAM_CHECK(fn != nullptr, "cuTensorMapEncodeTiled is not available from the driver");
+    CAM_CHECK(rank >= 2 && rank <= 5 && (reinterpret_cast<uintptr_t>(base) & 15u) == 0, "tensor map base %p is not 16-byte aligned", base);
+    cuuint64_t d[5], st[4];
+    cuuint32_t bx[5], es[5];
+    for (int i = 0; i < rank; ++i) {
+        CAM_CHECK(dims[i] >= 1, "tensor map: dimension %d is empty", i);
+        d[i] = dims[i];
+        bx[i] = box[i];
+        es[i] = 1;
+        if (i + 1 < rank) {
+            CAM_CHECK(strides[i] % 16 == 0, "tensor map: stride %llu is not a multiple of 16 bytes", static_cast<unsigned long long>(strides[i]));
+            st[i] = strides[i];
+        }
+    }
+    const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, st, bx, es,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CAM_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
+    return 0;
+}
+
+extern "C" int cam_fail(const char* message) { return fail("%s", message); }
 
 constexpr size_t kTmapCacheEntries = 64;
 

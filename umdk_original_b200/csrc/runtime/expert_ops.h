@@ -1,0 +1,32 @@
+// C interface of the expert-MLP operators that need no Buffer.  Like cam_runtime.h: no PyTorch, raw device pointers, 0 on
+// success and cam_last_error() otherwise; nothing here allocates or waits.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../common/cam_types.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+// dtype: 0 bf16, 1 fp16, 2 fp32.  fmt: 0 nvfp4 (e4m3 scale per 16 values), 1 mxfp4 (e8m0 scale per 32).
+// numel is a multiple of the block; gscale: null, or `gscales` floats that each cover numel / gscales values (nvfp4 only).
+int cam_quantize_fp4(const void* x, int dtype, int fmt, void* q, void* s, int64_t numel, const float* gscale, int64_t gscales,
+                     cudaStream_t stream);
+int cam_dequantize_fp4(const void* q, const void* s, int dtype, int fmt, void* out, int64_t numel, const float* gscale,
+                       int64_t gscales, cudaStream_t stream);
+
+// a_q [rows, K/2], a_s [rows, K/block], w_q [E, N, K/2], w_s [E, N, K/block], offsets int32 [E+1] on the device.
+// swiglu 0: out bf16 [rows, N].  swiglu 1: N = 2I (gate rows first), out codes [rows, I/2], out_s [rows, I/block].
+// Rows outside [offsets[0], offsets[E]) are written as zeros.
+int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, const void* w_q, const void* w_s, const int* offsets,
+                         int num_experts, int n_dim, int k_dim, int fmt, int swiglu, const float* a_gscale,
+                         const float* w_gscale, const float* out_gscale, void* out, void* out_s, cudaStream_t stream);
+
+// First wait that ran out in a kernel of these operators on the current device (code 0: none); waits for the device.
+int cam_expert_ops_status(CamStatus* out);
+
+#ifdef __cplusplus
+}
+#endif

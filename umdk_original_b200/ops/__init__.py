@@ -11,3 +11,7 @@ moe_combine_shmem = ops.moe_combine_shmem
 moe_dispatch_prefill_quant = ops.moe_dispatch_prefill_quant
 grouped_gemm_fp8 = ops.grouped_gemm_fp8
 grouped_gemm_fp8_swiglu = ops.grouped_gemm_fp8_swiglu
+quantize_fp4 = ops.quantize_fp4
+dequantize_fp4 = ops.dequantize_fp4
+grouped_gemm_fp4 = ops.grouped_gemm_fp4
+grouped_gemm_fp4_swiglu = ops.grouped_gemm_fp4_swiglu

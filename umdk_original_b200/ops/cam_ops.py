@@ -16,6 +16,7 @@ from typing import List, Optional
 
 import torch
 
+from . import expert_mlp
 from . import reference as ref
 
 _C = None
@@ -52,6 +53,7 @@ SCHEMAS = [
     "grouped_gemm_fp8_swiglu(Tensor a_q, Tensor a_s, Tensor w_q, Tensor w_s, Tensor expert_offsets, "
     "bool ue8m0=False) -> (Tensor, Tensor)",
     "grouped_gemm_w8a8(Tensor a_q, Tensor a_s, Tensor w_q, Tensor w_s, Tensor expert_offsets) -> Tensor",
+    *expert_mlp.SCHEMAS,
 ]
 
 if _C is None:
@@ -318,5 +320,7 @@ def _grouped_gemm_w8a8_cpu(a_q, a_s, w_q, w_s, expert_offsets):
 
 _CPU.impl("grouped_gemm_fp8_swiglu", _grouped_gemm_fp8_swiglu_cpu)
 _CPU.impl("grouped_gemm_w8a8", _grouped_gemm_w8a8_cpu)
+for _name, _fn in expert_mlp.CPU_IMPLS.items():
+    _CPU.impl(_name, _fn)
 
 ops = torch.ops.umdk_cam_op_lib
