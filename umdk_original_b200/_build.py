@@ -48,6 +48,7 @@ KERNEL_SOURCES = [
     "kernels/tp_exchange.cu",
     "kernels/quant_fp4.cu",
     "kernels/grouped_gemm_fp4.cu",
+    "kernels/grouped_mlp.cu",
     "runtime/cam_runtime.cpp",
     "runtime/expert_ops.cpp",
 ]
@@ -131,7 +132,8 @@ def build_kernels(force: bool = False, debug: bool = False) -> Path:
             logs = list(ex.map(lambda j: _run(j[0]), jobs))
         for (_, src, obj), log in zip(jobs, logs):
             if src.name in ("grouped_gemm.cu", "grouped_gemm_mx.cu", "grouped_gemm_mx2.cu", "grouped_gemm_i8.cu",
-                            "grouped_gemm_rows_n_mx.cu", "grouped_gemm_rows_n_i8.cu", "fused_moe_mx.cu", "grouped_gemm_fp4.cu"):
+                            "grouped_gemm_rows_n_mx.cu", "grouped_gemm_rows_n_i8.cu", "fused_moe_mx.cu", "grouped_gemm_fp4.cu",
+                            "grouped_mlp.cu"):
                 _check_gemm_registers(log, src)
             _mark(src, obj, stamp)
     so = LIB / "libumdk_cam.so"

@@ -1,9 +1,13 @@
-// PyTorch bindings of the expert-MLP operators that need no Buffer: 4-bit quantisation, grouped products of 4-bit operands.
+// PyTorch bindings of the expert-MLP operators that need no Buffer: 4-bit quantisation, grouped products of 4-bit operands, the
+// gated feed-forward block of 16-bit experts with its backward pass.
 // Schemas are added to the library that bindings.cpp defines.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 #include <torch/library.h>
+
+#include <string>
+#include <tuple>
 
 #include "runtime/cam_runtime.h"
 #include "runtime/expert_ops.h"
@@ -189,6 +193,144 @@ std::tuple<at::Tensor, at::Tensor> grouped_gemm_fp4_swiglu_meta(const at::Tensor
             at::empty({a_q.size(0), w_q.size(1) / 2 / block_of(a_s, "a_s")}, a_s.options())};
 }
 
+// ------------------------------------------------------------------------------------------------
+// Gated feed-forward block of 16-bit experts
+// ------------------------------------------------------------------------------------------------
+struct MlpProblem {
+    int rows, experts, h, inter, dtype;
+};
+
+MlpProblem check_mlp(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, const at::Tensor& expert_offsets) {
+    check_operand(x, x, "x");
+    check_operand(w1, x, "w1");
+    check_operand(w2, x, "w2");
+    check_operand(expert_offsets, x, "expert_offsets");
+    CAM_ASSERT(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "grouped_mlp: x must be bfloat16 or float16");
+    CAM_ASSERT(w1.scalar_type() == x.scalar_type() && w2.scalar_type() == x.scalar_type(), "grouped_mlp: x, w1 and w2 must be of one type");
+    CAM_ASSERT(x.dim() == 2 && w1.dim() == 3 && w2.dim() == 3, "grouped_mlp: x must be [M, h], w1 [E, 2I, h], w2 [E, h, I]");
+    const int64_t m = x.size(0), h = x.size(1), e = w1.size(0), i = w2.size(2);
+    CAM_ASSERT(w1.size(1) == 2 * i && w1.size(2) == h && w2.size(0) == e && w2.size(1) == h,
+               "grouped_mlp: x must be [M, h], w1 [E, 2I, h], w2 [E, h, I]: got ", shape(x.sizes()), ", ", shape(w1.sizes()), ", ", shape(w2.sizes()));
+    CAM_ASSERT(h > 0 && i > 0 && h % 8 == 0 && i % 8 == 0, "grouped_mlp: h ", num(h), " and I ", num(i), " must be multiples of 8");
+    CAM_ASSERT(e >= 1 && m < (1ll << 31) - 512 && h < (1 << 28) && i < (1 << 28) && e < (1 << 24), "grouped_mlp: sizes out of range");
+    CAM_ASSERT(expert_offsets.scalar_type() == at::kInt && expert_offsets.numel() == e + 1, "expert_offsets must be int32 [E+1]");
+    return {static_cast<int>(m), static_cast<int>(e), static_cast<int>(h), static_cast<int>(i), x.scalar_type() == at::kHalf ? 1 : 0};
+}
+
+// gate_up is kept (fp32 [M, 2I]) for a backward pass, otherwise empty
+std::tuple<at::Tensor, at::Tensor, at::Tensor> mlp_forward(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2,
+                                                           const at::Tensor& expert_offsets, bool keep) {
+    const MlpProblem p = check_mlp(x, w1, w2, expert_offsets);
+    c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor act = at::empty({p.rows, p.inter}, x.options());
+    at::Tensor gu = at::empty({keep ? p.rows : 0, 2 * p.inter}, x.options().dtype(at::kFloat));
+    at::Tensor y = at::empty({p.rows, p.h}, x.options());
+    if (p.rows == 0) return {y, act, gu};
+    const auto stream = at::cuda::getCurrentCUDAStream().stream();
+    const int* off = expert_offsets.data_ptr<int>();
+    CAM_RT(cam_grouped_mlp_up(x.data_ptr(), w1.data_ptr(), off, p.rows, p.experts, p.h, p.inter, p.dtype, act.data_ptr(),
+                              keep ? gu.data_ptr<float>() : nullptr, stream));
+    CAM_RT(cam_grouped_mlp_down(act.data_ptr(), w2.data_ptr(), off, p.rows, p.experts, p.h, p.inter, p.dtype, y.data_ptr(), stream));
+    return {y, act, gu};
+}
+
+at::Tensor grouped_mlp_cuda(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, const at::Tensor& expert_offsets) {
+    return std::get<0>(mlp_forward(x, w1, w2, expert_offsets, false));
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> grouped_mlp_train_cuda(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2,
+                                                                      const at::Tensor& expert_offsets) {
+    return mlp_forward(x, w1, w2, expert_offsets, true);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> mlp_grads_empty(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2,
+                                                               bool need_dx, bool need_dw1, bool need_dw2) {
+    auto like = [](const at::Tensor& t, bool need) { return need ? at::empty_like(t) : at::empty({0}, t.options()); };
+    return {like(x, need_dx), like(w1, need_dw1), like(w2, need_dw2)};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> grouped_mlp_backward_cuda(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w1,
+                                                                         const at::Tensor& w2, const at::Tensor& expert_offsets,
+                                                                         const at::Tensor& act, const at::Tensor& gate_up, bool need_dx,
+                                                                         bool need_dw1, bool need_dw2) {
+    const MlpProblem p = check_mlp(x, w1, w2, expert_offsets);
+    check_operand(dy, x, "dy");
+    check_operand(act, x, "act");
+    check_operand(gate_up, x, "gate_up");
+    CAM_ASSERT(dy.scalar_type() == x.scalar_type() && dy.sizes() == x.sizes(), "grouped_mlp: dy must be like x");
+    CAM_ASSERT(act.scalar_type() == x.scalar_type() && act.dim() == 2 && act.size(0) == p.rows && act.size(1) == p.inter, "grouped_mlp: act must be [M, I]");
+    CAM_ASSERT(gate_up.scalar_type() == at::kFloat && gate_up.dim() == 2 && gate_up.size(0) == p.rows && gate_up.size(1) == 2 * p.inter,
+               "grouped_mlp: gate_up must be float32 [M, 2I]");
+    c10::cuda::CUDAGuard guard(x.device());
+    auto out = mlp_grads_empty(x, w1, w2, need_dx, need_dw1, need_dw2);
+    auto& [dx, dw1, dw2] = out;
+    if (p.rows == 0) {
+        dw1.zero_();
+        dw2.zero_();
+        return out;
+    }
+    const auto stream = at::cuda::getCurrentCUDAStream().stream();
+    const int* off = expert_offsets.data_ptr<int>();
+    if (need_dw2)
+        CAM_RT(cam_grouped_mlp_dw(dy.data_ptr(), act.data_ptr(), off, p.rows, p.experts, p.h, p.inter, p.dtype, dw2.data_ptr(), stream));
+    if (!need_dx && !need_dw1) return out;
+    at::Tensor dgu = at::empty({p.rows, 2 * p.inter}, x.options());
+    CAM_RT(cam_grouped_mlp_dact(dy.data_ptr(), w2.data_ptr(), gate_up.data_ptr<float>(), off, p.rows, p.experts, p.h, p.inter, p.dtype,
+                                dgu.data_ptr(), stream));
+    if (need_dx)
+        CAM_RT(cam_grouped_mlp_dx(dgu.data_ptr(), w1.data_ptr(), off, p.rows, p.experts, p.h, p.inter, p.dtype, dx.data_ptr(), stream));
+    if (need_dw1)
+        CAM_RT(cam_grouped_mlp_dw(dgu.data_ptr(), x.data_ptr(), off, p.rows, p.experts, 2 * p.inter, p.h, p.dtype, dw1.data_ptr(), stream));
+    return out;
+}
+
+at::Tensor grouped_mlp_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, const at::Tensor&) { return at::empty_like(x); }
+std::tuple<at::Tensor, at::Tensor, at::Tensor> grouped_mlp_train_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor& w2, const at::Tensor&) {
+    return {at::empty_like(x), at::empty({x.size(0), w2.size(2)}, x.options()), at::empty({x.size(0), 2 * w2.size(2)}, x.options().dtype(at::kFloat))};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> grouped_mlp_backward_meta(const at::Tensor&, const at::Tensor& x, const at::Tensor& w1,
+                                                                         const at::Tensor& w2, const at::Tensor&, const at::Tensor&,
+                                                                         const at::Tensor&, bool need_dx, bool need_dw1, bool need_dw2) {
+    return mlp_grads_empty(x, w1, w2, need_dx, need_dw1, need_dw2);
+}
+
+using Mlp3 = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
+
+Mlp3 call_mlp_train(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, const at::Tensor& off) {
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("umdk_cam_op_lib::grouped_mlp_train", "")
+                         .typed<Mlp3(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&)>();
+    return op.call(x, w1, w2, off);
+}
+
+struct GroupedMlpFunction : public torch::autograd::Function<GroupedMlpFunction> {
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2,
+                              const at::Tensor& expert_offsets) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto [y, act, gu] = call_mlp_train(x, w1, w2, expert_offsets);
+        ctx->save_for_backward({x, w1, w2, expert_offsets, act, gu});
+        return y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
+        static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("umdk_cam_op_lib::grouped_mlp_backward", "")
+                             .typed<Mlp3(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                         const at::Tensor&, const at::Tensor&, bool, bool, bool)>();
+        const bool need_dx = ctx->needs_input_grad(0), need_dw1 = ctx->needs_input_grad(1), need_dw2 = ctx->needs_input_grad(2);
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        const auto s = ctx->get_saved_variables();
+        auto [dx, dw1, dw2] = op.call(grads[0].contiguous(), s[0], s[1], s[2], s[3], s[4], s[5], need_dx, need_dw1, need_dw2);
+        return {need_dx ? dx : at::Tensor(), need_dw1 ? dw1 : at::Tensor(), need_dw2 ? dw2 : at::Tensor(), at::Tensor()};
+    }
+};
+
+at::Tensor grouped_mlp_autograd(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, const at::Tensor& expert_offsets) {
+    if (at::GradMode::is_enabled() && (x.requires_grad() || w1.requires_grad() || w2.requires_grad()))
+        return GroupedMlpFunction::apply(x, w1, w2, expert_offsets);
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("umdk_cam_op_lib::grouped_mlp", "")
+                         .typed<at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&)>();
+    return op.call(x, w1, w2, expert_offsets);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(umdk_cam_op_lib, m) {
@@ -198,6 +340,10 @@ TORCH_LIBRARY_FRAGMENT(umdk_cam_op_lib, m) {
           "Tensor? a_global_scale=None, Tensor? w_global_scale=None) -> Tensor");
     m.def("grouped_gemm_fp4_swiglu(Tensor a_q, Tensor a_s, Tensor w_q, Tensor w_s, Tensor expert_offsets, "
           "Tensor? a_global_scale=None, Tensor? w_global_scale=None, Tensor? out_global_scale=None) -> (Tensor, Tensor)");
+    m.def("grouped_mlp(Tensor x, Tensor w1, Tensor w2, Tensor expert_offsets) -> Tensor");
+    m.def("grouped_mlp_train(Tensor x, Tensor w1, Tensor w2, Tensor expert_offsets) -> (Tensor, Tensor, Tensor)");
+    m.def("grouped_mlp_backward(Tensor dy, Tensor x, Tensor w1, Tensor w2, Tensor expert_offsets, Tensor act, Tensor gate_up, "
+          "bool need_dx=True, bool need_dw1=True, bool need_dw2=True) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(umdk_cam_op_lib, CUDA, m) {
@@ -205,6 +351,9 @@ TORCH_LIBRARY_IMPL(umdk_cam_op_lib, CUDA, m) {
     m.impl("dequantize_fp4", &dequantize_fp4_cuda);
     m.impl("grouped_gemm_fp4", &grouped_gemm_fp4_cuda);
     m.impl("grouped_gemm_fp4_swiglu", &grouped_gemm_fp4_swiglu_cuda);
+    m.impl("grouped_mlp", &grouped_mlp_cuda);
+    m.impl("grouped_mlp_train", &grouped_mlp_train_cuda);
+    m.impl("grouped_mlp_backward", &grouped_mlp_backward_cuda);
 }
 
 TORCH_LIBRARY_IMPL(umdk_cam_op_lib, Meta, m) {
@@ -212,6 +361,9 @@ TORCH_LIBRARY_IMPL(umdk_cam_op_lib, Meta, m) {
     m.impl("dequantize_fp4", &dequantize_fp4_meta);
     m.impl("grouped_gemm_fp4", &grouped_gemm_fp4_meta);
     m.impl("grouped_gemm_fp4_swiglu", &grouped_gemm_fp4_swiglu_meta);
+    m.impl("grouped_mlp", &grouped_mlp_meta);
+    m.impl("grouped_mlp_train", &grouped_mlp_train_meta);
+    m.impl("grouped_mlp_backward", &grouped_mlp_backward_meta);
 }
 
 TORCH_LIBRARY_IMPL(umdk_cam_op_lib, Autograd, m) {
@@ -219,4 +371,7 @@ TORCH_LIBRARY_IMPL(umdk_cam_op_lib, Autograd, m) {
     m.impl("dequantize_fp4", torch::autograd::autogradNotImplementedFallback());
     m.impl("grouped_gemm_fp4", torch::autograd::autogradNotImplementedFallback());
     m.impl("grouped_gemm_fp4_swiglu", torch::autograd::autogradNotImplementedFallback());
+    m.impl("grouped_mlp", &grouped_mlp_autograd);
+    m.impl("grouped_mlp_train", torch::autograd::autogradNotImplementedFallback());
+    m.impl("grouped_mlp_backward", torch::autograd::autogradNotImplementedFallback());
 }

@@ -25,6 +25,21 @@ struct GroupedGemmFp4Params {
     uint8_t* out_scales;        // SwiGLU form: [rows, I / block]
 };
 
+// Products of the gated feed-forward block in 16 bits (grouped_mlp.cu) and what its epilogue does with them
+constexpr int kMlpUp = 0, kMlpDown = 1, kMlpDact = 2, kMlpDx = 3, kMlpDw = 4;
+constexpr int kMlpPlain = 0, kMlpSwiglu = 1, kMlpSwigluBackward = 2;
+
+struct GroupedMlpParams {
+    const int* expert_offsets;  // [E+1]
+    int num_experts, rows;      // rows of the row operands
+    int m_dim;                  // kMlpDw: rows of an expert's gradient
+    int n_dim;                  // columns of the result (I for kMlpUp and kMlpDact)
+    int k_dim;                  // contraction (not kMlpDw)
+    int fp16;                   // operands and results are fp16, otherwise bf16
+    void* out;                  // [rows, n_dim]; kMlpDact: dgu [rows, 2 n_dim]; kMlpDw: [E, m_dim, n_dim]
+    float* gate_up;             // [rows, 2I] fp32: written by kMlpUp (or null), read by kMlpDact
+};
+
 }  // namespace cam
 
 extern "C" {
@@ -39,5 +54,11 @@ int cam_launch_dequantize_fp4(const void* q, const void* s, int dtype, int fmt, 
 // tmap_a: boxes of 128 rows, tmap_a32: of 32 rows, both on A [rows, K / 2 bytes]; tmap_b: boxes of 128 rows on W [E N, K / 2]
 int cam_launch_grouped_gemm_fp4(const cam::GroupedGemmFp4Params* p, int fmt, int swiglu, const CUtensorMap* tmap_a,
                                 const CUtensorMap* tmap_a32, const CUtensorMap* tmap_b, cudaStream_t stream);
-int cam_fp4_status(CamStatus* out);  // of the current device: the first wait that ran out in any grouped_gemm_fp4 kernel
+// tmap_a: the row operand in boxes of 128 rows (kMlpDw: 64 rows), tmap_a32: in boxes of 32 rows; tmap_b: the weights
+// [E, rows, columns] in boxes of 128 rows, or of 64 where their row is the contraction index (kMlpDact, kMlpDx), or for kMlpDw
+// the second row operand in boxes of 64 rows.  All boxes are 128 bytes wide.
+int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, const CUtensorMap* tmap_a, const CUtensorMap* tmap_a32,
+                           const CUtensorMap* tmap_b, cudaStream_t stream);
+int cam_mlp_status(CamStatus* out);
+int cam_fp4_status(CamStatus* out);  // of the current device: the first wait that ran out in a kernel of that file
 }

@@ -90,7 +90,82 @@ extern "C" int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, 
     return launched(cam_launch_grouped_gemm_fp4(&p, fmt, swiglu, &ta, &ta32, &tb, stream), "grouped_gemm_fp4");
 }
 
+namespace {
+
+// [experts, rows, bytes] with boxes of 128 bytes x box_rows
+int map_3d(CUtensorMap* out, const void* base, uint64_t bytes, uint64_t rows, uint64_t experts, uint32_t box_rows) {
+    const uint64_t dims[3] = {bytes, rows, experts}, strides[2] = {bytes, bytes * rows};
+    const uint32_t box[3] = {128, box_rows, 1};
+    return cam_encode_tmap(out, base, 3, dims, strides, box);
+}
+
+// A product of the rows a [rows, k] with the weights: w [E, w_rows, w_cols], contracted over its columns or (by_rows) its rows.
+int row_product(int form, const char* what, const void* a, int k, const void* w, int w_rows, int w_cols, bool by_rows, int n,
+                const int* offsets, int rows, int num_experts, int dtype, void* out, float* gate_up, cudaStream_t stream) {
+    EXP_CHECK(a && w && offsets && out, "%s: null operand", what);
+    EXP_CHECK(rows >= 1 && num_experts >= 1, "%s: empty problem", what);
+    EXP_CHECK(k >= 8 && n >= 8 && k % 8 == 0 && n % 8 == 0, "%s: sizes %d and %d must be multiples of 8", what, k, n);
+    cam::GroupedMlpParams p{};
+    p.expert_offsets = offsets;
+    p.num_experts = num_experts;
+    p.rows = rows;
+    p.n_dim = n;
+    p.k_dim = k;
+    p.fp16 = dtype == 1;
+    p.out = out;
+    p.gate_up = gate_up;
+    CUtensorMap ta, ta32, tb;
+    if (map_2d(&ta, a, static_cast<uint64_t>(k) * 2, static_cast<uint64_t>(rows), 128) != 0) return -1;
+    if (map_2d(&ta32, a, static_cast<uint64_t>(k) * 2, static_cast<uint64_t>(rows), 32) != 0) return -1;
+    if (map_3d(&tb, w, static_cast<uint64_t>(w_cols) * 2, static_cast<uint64_t>(w_rows), static_cast<uint64_t>(num_experts), by_rows ? 64 : 128) != 0) return -1;
+    return launched(cam_launch_grouped_mlp(&p, form, &ta, &ta32, &tb, stream), what);
+}
+
+}  // namespace
+
+extern "C" int cam_grouped_mlp_up(const void* x, const void* w1, const int* offsets, int rows, int num_experts, int h, int inter,
+                                  int dtype, void* act, float* gate_up, cudaStream_t stream) {
+    return row_product(cam::kMlpUp, "grouped_mlp (gate and up)", x, h, w1, 2 * inter, h, false, inter, offsets, rows, num_experts, dtype, act, gate_up, stream);
+}
+
+extern "C" int cam_grouped_mlp_down(const void* act, const void* w2, const int* offsets, int rows, int num_experts, int h, int inter,
+                                    int dtype, void* y, cudaStream_t stream) {
+    return row_product(cam::kMlpDown, "grouped_mlp (down)", act, inter, w2, h, inter, false, h, offsets, rows, num_experts, dtype, y, nullptr, stream);
+}
+
+extern "C" int cam_grouped_mlp_dact(const void* dy, const void* w2, const float* gate_up, const int* offsets, int rows, int num_experts,
+                                    int h, int inter, int dtype, void* dgu, cudaStream_t stream) {
+    EXP_CHECK(gate_up != nullptr, "grouped_mlp (dact): null operand");
+    return row_product(cam::kMlpDact, "grouped_mlp (dact)", dy, h, w2, h, inter, true, inter, offsets, rows, num_experts, dtype, dgu,
+                       const_cast<float*>(gate_up), stream);
+}
+
+extern "C" int cam_grouped_mlp_dx(const void* dgu, const void* w1, const int* offsets, int rows, int num_experts, int h, int inter,
+                                  int dtype, void* dx, cudaStream_t stream) {
+    return row_product(cam::kMlpDx, "grouped_mlp (dx)", dgu, 2 * inter, w1, 2 * inter, h, true, h, offsets, rows, num_experts, dtype, dx, nullptr, stream);
+}
+
+extern "C" int cam_grouped_mlp_dw(const void* a, const void* b, const int* offsets, int rows, int num_experts, int m_dim, int n_dim,
+                                  int dtype, void* dw, cudaStream_t stream) {
+    EXP_CHECK(a && b && offsets && dw, "grouped_mlp (dw): null operand");
+    EXP_CHECK(rows >= 1 && num_experts >= 1, "grouped_mlp (dw): empty problem");
+    EXP_CHECK(m_dim >= 8 && n_dim >= 8 && m_dim % 8 == 0 && n_dim % 8 == 0, "grouped_mlp (dw): sizes %d and %d must be multiples of 8", m_dim, n_dim);
+    cam::GroupedMlpParams p{};
+    p.expert_offsets = offsets;
+    p.num_experts = num_experts;
+    p.rows = rows;
+    p.m_dim = m_dim;
+    p.n_dim = n_dim;
+    p.fp16 = dtype == 1;
+    p.out = dw;
+    CUtensorMap ta, tb;
+    if (map_2d(&ta, a, static_cast<uint64_t>(m_dim) * 2, static_cast<uint64_t>(rows), 64) != 0) return -1;
+    if (map_2d(&tb, b, static_cast<uint64_t>(n_dim) * 2, static_cast<uint64_t>(rows), 64) != 0) return -1;
+    return launched(cam_launch_grouped_mlp(&p, cam::kMlpDw, &ta, &ta, &tb, stream), "grouped_mlp (dw)");
+}
+
 extern "C" int cam_expert_ops_status(CamStatus* out) {
-    const int rc = cam_fp4_status(out);
+    int rc = cam_fp4_status(out);
+    if (rc == 0 && out->code == 0) rc = cam_mlp_status(out);
     return rc == 0 ? 0 : refuse("expert_ops_status: %s", cudaGetErrorString(static_cast<cudaError_t>(rc)));
 }

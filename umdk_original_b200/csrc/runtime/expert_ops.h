@@ -24,6 +24,21 @@ int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, const void*
                          int num_experts, int n_dim, int k_dim, int fmt, int swiglu, const float* a_gscale,
                          const float* w_gscale, const float* out_gscale, void* out, void* out_s, cudaStream_t stream);
 
+// Gated feed-forward block of 16-bit experts (kernels/grouped_mlp.cu), dtype 0 bf16 or 1 fp16.  x, y, dy, dx [rows, h], w1, dw1
+// [E, 2I, h] (gate rows first), w2, dw2 [E, h, I], act [rows, I]; gate_up [rows, 2I] fp32 (null: not kept), dgu [rows, 2I].
+// Rows outside [offsets[0], offsets[E]) of y and dx, and gradients of experts without rows, are written as zeros.
+int cam_grouped_mlp_up(const void* x, const void* w1, const int* offsets, int rows, int num_experts, int h, int inter, int dtype,
+                       void* act, float* gate_up, cudaStream_t stream);
+int cam_grouped_mlp_down(const void* act, const void* w2, const int* offsets, int rows, int num_experts, int h, int inter, int dtype,
+                         void* y, cudaStream_t stream);
+int cam_grouped_mlp_dact(const void* dy, const void* w2, const float* gate_up, const int* offsets, int rows, int num_experts, int h,
+                         int inter, int dtype, void* dgu, cudaStream_t stream);
+int cam_grouped_mlp_dx(const void* dgu, const void* w1, const int* offsets, int rows, int num_experts, int h, int inter, int dtype,
+                       void* dx, cudaStream_t stream);
+// dw[e] = a[rows of e]^T b[rows of e]: a [rows, m_dim], b [rows, n_dim], dw [E, m_dim, n_dim]
+int cam_grouped_mlp_dw(const void* a, const void* b, const int* offsets, int rows, int num_experts, int m_dim, int n_dim, int dtype,
+                       void* dw, cudaStream_t stream);
+
 // First wait that ran out in a kernel of these operators on the current device (code 0: none); waits for the device.
 int cam_expert_ops_status(CamStatus* out);
 

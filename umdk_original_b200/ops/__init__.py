@@ -11,7 +11,14 @@ moe_combine_shmem = ops.moe_combine_shmem
 moe_dispatch_prefill_quant = ops.moe_dispatch_prefill_quant
 grouped_gemm_fp8 = ops.grouped_gemm_fp8
 grouped_gemm_fp8_swiglu = ops.grouped_gemm_fp8_swiglu
-quantize_fp4 = ops.quantize_fp4
-dequantize_fp4 = ops.dequantize_fp4
-grouped_gemm_fp4 = ops.grouped_gemm_fp4
-grouped_gemm_fp4_swiglu = ops.grouped_gemm_fp4_swiglu
+
+# The operators that need no Buffer are looked up when they are first used: the package, and with it the build, can be
+# imported beside an extension that was built before they existed.
+_EXPERT_OPS = ("quantize_fp4", "dequantize_fp4", "grouped_gemm_fp4", "grouped_gemm_fp4_swiglu", "grouped_mlp",
+               "grouped_mlp_train", "grouped_mlp_backward")
+
+
+def __getattr__(name):
+    if name in _EXPERT_OPS:
+        return getattr(ops, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -3,6 +3,10 @@
 ``quantize_fp4`` / ``dequantize_fp4`` / ``grouped_gemm_fp4`` / ``grouped_gemm_fp4_swiglu``: 4-bit floating point with block
 scales (the formats are described in csrc/common/fp4.cuh).  The CUDA implementations live in csrc/bindings_expert.cpp; the CPU
 ones here follow the same contracts in fp32, expert by expert.
+
+``grouped_mlp``: the gated feed-forward block of 16-bit experts, differentiable in the rows and both weights.  Its parts,
+``grouped_mlp_train`` (also returns what the backward pass needs) and ``grouped_mlp_backward``, can be called by programs that
+keep their own graph of derivatives.
 """
 from __future__ import annotations
 
@@ -17,6 +21,10 @@ SCHEMAS = [
     "Tensor? a_global_scale=None, Tensor? w_global_scale=None) -> Tensor",
     "grouped_gemm_fp4_swiglu(Tensor a_q, Tensor a_s, Tensor w_q, Tensor w_s, Tensor expert_offsets, "
     "Tensor? a_global_scale=None, Tensor? w_global_scale=None, Tensor? out_global_scale=None) -> (Tensor, Tensor)",
+    "grouped_mlp(Tensor x, Tensor w1, Tensor w2, Tensor expert_offsets) -> Tensor",
+    "grouped_mlp_train(Tensor x, Tensor w1, Tensor w2, Tensor expert_offsets) -> (Tensor, Tensor, Tensor)",
+    "grouped_mlp_backward(Tensor dy, Tensor x, Tensor w1, Tensor w2, Tensor expert_offsets, Tensor act, Tensor gate_up, "
+    "bool need_dx=True, bool need_dw1=True, bool need_dw2=True) -> (Tensor, Tensor, Tensor)",
 ]
 
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
@@ -139,9 +147,60 @@ def grouped_gemm_fp4_swiglu_cpu(a_q, a_s, w_q, w_s, expert_offsets, a_global_sca
     return quantize_fp4_cpu((torch.nn.functional.silu(gate) * up).contiguous(), block, out_global_scale)
 
 
+def _check_mlp(x, w1, w2, expert_offsets):
+    for t, what in ((x, "x"), (w1, "w1"), (w2, "w2"), (expert_offsets, "expert_offsets")):
+        _check(t.is_contiguous(), f"{what} must be contiguous")
+    _check(x.dtype in (torch.bfloat16, torch.float16), "grouped_mlp: x must be bfloat16 or float16")
+    _check(w1.dtype == x.dtype and w2.dtype == x.dtype, "grouped_mlp: x, w1 and w2 must be of one type")
+    _check(x.dim() == 2 and w1.dim() == 3 and w2.dim() == 3, "grouped_mlp: x must be [M, h], w1 [E, 2I, h], w2 [E, h, I]")
+    h, e, i = x.shape[1], w1.shape[0], w2.shape[2]
+    _check(tuple(w1.shape) == (e, 2 * i, h) and tuple(w2.shape) == (e, h, i), "grouped_mlp: x must be [M, h], w1 [E, 2I, h], w2 [E, h, I]")
+    _check(h > 0 and i > 0 and h % 8 == 0 and i % 8 == 0, f"grouped_mlp: h {h} and I {i} must be multiples of 8")
+    _check(expert_offsets.dtype == torch.int32 and expert_offsets.numel() == e + 1, "expert_offsets must be int32 [E+1]")
+
+
+def grouped_mlp_train_cpu(x, w1, w2, expert_offsets):
+    _check_mlp(x, w1, w2, expert_offsets)
+    m, i = x.shape[0], w2.shape[2]
+    y, act, gu = torch.zeros_like(x), torch.zeros(m, i, dtype=x.dtype), torch.zeros(m, 2 * i)
+    for e, lo, hi in _spans(expert_offsets, m):
+        gu[lo:hi] = x[lo:hi].float() @ w1[e].float().t()
+        gate, up = gu[lo:hi].chunk(2, -1)
+        act[lo:hi] = (torch.nn.functional.silu(gate) * up).to(x.dtype)
+        y[lo:hi] = (act[lo:hi].float() @ w2[e].float().t()).to(x.dtype)
+    return y, act, gu
+
+
+def grouped_mlp_cpu(x, w1, w2, expert_offsets):
+    return grouped_mlp_train_cpu(x, w1, w2, expert_offsets)[0]
+
+
+def grouped_mlp_backward_cpu(dy, x, w1, w2, expert_offsets, act, gate_up, need_dx=True, need_dw1=True, need_dw2=True):
+    _check_mlp(x, w1, w2, expert_offsets)
+    _check(dy.dtype == x.dtype and dy.shape == x.shape and dy.is_contiguous(), "grouped_mlp: dy must be like x")
+    _check(act.dtype == x.dtype and tuple(act.shape) == (x.shape[0], w2.shape[2]), "grouped_mlp: act must be [M, I]")
+    _check(gate_up.dtype == torch.float32 and tuple(gate_up.shape) == (x.shape[0], 2 * w2.shape[2]), "grouped_mlp: gate_up must be float32 [M, 2I]")
+    dx, dw1, dw2 = (torch.zeros_like(t) if need else t.new_empty(0) for t, need in ((x, need_dx), (w1, need_dw1), (w2, need_dw2)))
+    for e, lo, hi in _spans(expert_offsets, x.shape[0]):
+        g, u = gate_up[lo:hi].chunk(2, -1)
+        d = dy[lo:hi].float()
+        da, s = d @ w2[e].float(), torch.sigmoid(g)
+        dgu = torch.cat([da * u * s * (1 + g * (1 - s)), da * g * s], -1).to(x.dtype).float()
+        if need_dx:
+            dx[lo:hi] = (dgu @ w1[e].float()).to(x.dtype)
+        if need_dw1:
+            dw1[e] = (dgu.t() @ x[lo:hi].float()).to(x.dtype)
+        if need_dw2:
+            dw2[e] = (d.t() @ act[lo:hi].float()).to(x.dtype)
+    return dx, dw1, dw2
+
+
 CPU_IMPLS = {
     "quantize_fp4": quantize_fp4_cpu,
     "dequantize_fp4": dequantize_fp4_cpu,
     "grouped_gemm_fp4": grouped_gemm_fp4_cpu,
     "grouped_gemm_fp4_swiglu": grouped_gemm_fp4_swiglu_cpu,
+    "grouped_mlp": grouped_mlp_cpu,
+    "grouped_mlp_train": grouped_mlp_train_cpu,
+    "grouped_mlp_backward": grouped_mlp_backward_cpu,
 }
