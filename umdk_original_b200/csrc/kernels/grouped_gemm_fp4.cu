@@ -7,13 +7,13 @@
 // rows x 256 columns: each holds its 128 rows of A and HALF of the weight tile, one CTA issues the MMAs of both.
 //
 // Scales stay in memory as the quantiser wrote them, row by row; the tensor core wants them in tensor memory as
-// [32 lanes][4 words] per 128 rows and 64 values (word j of lane l: row 32 j + l).  Three warps per CTA (its rows, the lower
-// and the upper 128 weight rows) bring them there: lane l copies the 16 bytes of rows l, 32 + l, 64 + l, 96 + l of a K-block
-// into the stage's slot with cp.async, three K-blocks ahead, transposes the 4 x 4 words in place (the slot holds the same
-// four addresses of this lane before and after) and raises the stage's barrier.  The MMA issuer then moves the slot into
-// tensor memory with tcgen05.cp directly in front of the MMAs that read it.
+// [32 lanes][4 words] per 128 rows and 64 values (word j of lane l: row 32 j + l).  Four warps per CTA bring them there, each
+// for every fourth K-block: lane l copies the 16 bytes of rows l, 32 + l, 64 + l, 96 + l of each 128 rows into the stage's slot
+// with cp.async, transposes the 4 x 4 words in place (the slot holds the same four addresses of this lane before and after) and
+// raises the stage's barrier.  The MMA issuer then moves the slot into tensor memory with tcgen05.cp directly in front of the
+// MMAs that read it.
 //
-// Barriers: as in grouped_gemm_mx2.cu, bar_sf counts the 3 + 3 scale warps of the pair.
+// Barriers: as in grouped_gemm_mx2.cu, bar_sf counts one scale warp of each CTA.
 #include "../common/fp4.cuh"
 #include "expert_gemm.cuh"
 
@@ -32,8 +32,6 @@ constexpr int kF4StgPitch = 272;               // bf16 rows of 128 columns, 16 b
 constexpr int kF4StgBytes = 128 * kF4StgPitch;
 constexpr int kF4Smem = kF4Stages * (kF4StageBytes + kF4SfStage) + kF4StgBytes + 1024;
 static_assert(kF4Smem <= 232448, "exceeds the shared memory of one CTA");
-constexpr int kF4Ahead = 3;                    // K-blocks whose scales are on their way
-static_assert(kF4Ahead <= kF4Stages, "scale copies may not run further ahead than there are stages");
 constexpr uint32_t kF4TmemCols = 512, kF4SfCol0 = 256, kF4SfCols = 48;
 static_assert(kF4SfCol0 + kF4Stages * kF4SfCols <= kF4TmemCols, "tensor memory");
 // setmaxnreg: the shares must not exceed what the CTA was launched with (checked against ptxas by the build)
@@ -91,9 +89,9 @@ __device__ __forceinline__ void tc_copy_scales_pair(uint32_t taddr, uint64_t des
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {  // zeros where not `live`
     if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
     else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(live ? BYTES : 0), "n"(BYTES) : "memory");
+        asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(live ? BYTES : 0), "n"(BYTES) : "memory");
 }
 
 }  // namespace
@@ -133,7 +131,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&bar_full[s], 1);
-            mbar_init(&bar_sf[s], 6);
+            mbar_init(&bar_sf[s], 2);
             mbar_init(&bar_empty[s], 1);
         }
         mbar_init(bar_tfull, 1);
@@ -225,78 +223,72 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         }
     } else if (warp < kF4EpiWarp0) {
         reg_dealloc<kF4SfRegs>();
-        // ---------------------------------------------------------------- scale warps: rows, lower and upper weight rows
-        const int what = warp - kF4SfWarp0;
-        if (what < 3) {
-            const int pitch = p.k_dim / BLK;          // bytes of scales of a row
-            const int words = pitch / 4;
-            const uint32_t slot0 = smem_u32(sfm + what * kF4SfBlock) + lane * 16u;
-            const uint8_t* src[4] = {nullptr, nullptr, nullptr, nullptr};
-            const int last_b = p.num_experts * p.n_dim - 1;
-            uint32_t issued = 0, done = 0;
-            int tile = pair_id, kb = 0;
-            bool more = true;
-            while (true) {
-                while (more && issued - done < kF4Ahead) {
-                    if (kb == 0) {
-                        if (!w.locate(tile, e, nt, row0, rows)) { more = false; break; }
+        // ---------------------------------------------------------------- scale warps: each takes every fourth K-block
+        const uint32_t mine = static_cast<uint32_t>(warp - kF4SfWarp0);
+        const int pitch = p.k_dim / BLK;          // bytes of scales of a row
+        const int words = pitch / 4;
+        const int last_b = p.num_experts * p.n_dim - 1;
+        uint32_t it = 0;
+        for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows); tile += num_pairs) {
+            const uint8_t* src[12];  // rows 32 j + lane of this CTA's rows, of the lower and of the upper weight rows
+            // Past the tile's rows nothing is loaded: those accumulator rows are not read.  (Loading some row there instead
+            // made all SMs ask one L2 slice for the same bytes: 8 rows of 8 experts, 4096 x 7168, 231 us.)
+            const int a_first = row0 + static_cast<int>(cta) * BM, a_rows = rows - static_cast<int>(cta) * BM;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int r = 32 * j + static_cast<int>(lane);
-                            if (what == 0) src[j] = p.a_scales + static_cast<size_t>(min(row0 + static_cast<int>(cta) * BM + r, p.rows - 1)) * pitch;
-                            else src[j] = p.b_scales + static_cast<size_t>(min(b_row(what - 1) + r, last_b)) * pitch;
+            for (int j = 0; j < 4; ++j) {
+                const int r = 32 * j + static_cast<int>(lane);
+                src[j] = p.a_scales + static_cast<size_t>(min(a_first + r, p.rows - 1)) * pitch;
+                src[4 + j] = p.b_scales + static_cast<size_t>(min(b_row(0) + r, last_b)) * pitch;
+                src[8 + j] = p.b_scales + static_cast<size_t>(min(b_row(1) + r, last_b)) * pitch;
+            }
+            for (int kb = 0; kb < kblocks; ++kb, ++it) {
+                if ((it & 3u) != mine) continue;
+                const uint32_t s = it % NS;
+                const bool got = mbar_wait_bounded(&bar_empty[s], ((it / NS) & 1u) ^ 1u, abort_flag);
+                if (!__all_sync(0xFFFFFFFFu, got)) { ok = false; break; }
+                uint8_t* slot = sfm + s * kF4SfStage + lane * 16u;
+                const uint32_t dst = smem_u32(slot);
+#pragma unroll
+                for (int j = 0; j < 12; ++j) {
+                    if (j < 4 && 32 * j + static_cast<int>(lane) >= a_rows) continue;
+                    const uint32_t d = dst + (j >> 2) * kF4SfBlock + (FMT == kFp4Nv ? (j & 3) * 512u : ((j >> 1) & 1) * 512u + (j & 1) * 8u);
+                    const uint8_t* from = src[j] + kb * SFW * 4;
+                    if (p.scale_vec) {
+                        copy_async<SFW * 4>(d, from, true);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < SFW; ++i) {
+                            const bool live = kb * SFW + i < words;
+                            copy_async<4>(d + i * 4u, live ? from + i * 4 : src[j], live);
                         }
                     }
-                    const uint32_t s = issued % NS;
-                    const bool got = mbar_wait_bounded(&bar_empty[s], ((issued / NS) & 1u) ^ 1u, abort_flag);
-                    if (!__all_sync(0xFFFFFFFFu, got)) { ok = false; break; }
-                    const uint32_t dst = slot0 + s * kF4SfStage;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t d = FMT == kFp4Nv ? dst + j * 512u : dst + (j >> 1) * 512u + (j & 1) * 8u;
-                        const uint8_t* from = src[j] + kb * SFW * 4;
-                        if (p.scale_vec) {
-                            copy_async<SFW * 4>(d, from, true);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < SFW; ++i) {
-                                const bool live = kb * SFW + i < words;
-                                copy_async<4>(d + i * 4u, live ? from + i * 4 : src[j], live);
-                            }
-                        }
-                    }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    ++issued;
-                    if (++kb == kblocks) { kb = 0; tile += num_pairs; }
                 }
-                if (!ok || issued == done) break;
-                if (issued - done == kF4Ahead) asm volatile("cp.async.wait_group %0;" ::"n"(kF4Ahead - 1) : "memory");
-                else asm volatile("cp.async.wait_group 0;" ::: "memory");
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 // this lane's words, in place: [row j][K-step i] -> [K-step i][row j]
-                uint8_t* slot = sfm + (done % NS) * kF4SfStage + what * kF4SfBlock + lane * 16u;
-                if constexpr (FMT == kFp4Nv) {
-                    const uint4 a = *reinterpret_cast<uint4*>(slot), b = *reinterpret_cast<uint4*>(slot + 512);
-                    const uint4 c = *reinterpret_cast<uint4*>(slot + 1024), d = *reinterpret_cast<uint4*>(slot + 1536);
-                    *reinterpret_cast<uint4*>(slot) = make_uint4(a.x, b.x, c.x, d.x);
-                    *reinterpret_cast<uint4*>(slot + 512) = make_uint4(a.y, b.y, c.y, d.y);
-                    *reinterpret_cast<uint4*>(slot + 1024) = make_uint4(a.z, b.z, c.z, d.z);
-                    *reinterpret_cast<uint4*>(slot + 1536) = make_uint4(a.w, b.w, c.w, d.w);
-                } else {
-                    const uint4 a = *reinterpret_cast<uint4*>(slot), b = *reinterpret_cast<uint4*>(slot + 512);
-                    *reinterpret_cast<uint4*>(slot) = make_uint4(a.x, a.z, b.x, b.z);
-                    *reinterpret_cast<uint4*>(slot + 512) = make_uint4(a.y, a.w, b.y, b.w);
+#pragma unroll
+                for (int blk = 0; blk < 3; ++blk, slot += kF4SfBlock) {
+                    if constexpr (FMT == kFp4Nv) {
+                        const uint4 a = *reinterpret_cast<uint4*>(slot), b = *reinterpret_cast<uint4*>(slot + 512);
+                        const uint4 c = *reinterpret_cast<uint4*>(slot + 1024), d = *reinterpret_cast<uint4*>(slot + 1536);
+                        *reinterpret_cast<uint4*>(slot) = make_uint4(a.x, b.x, c.x, d.x);
+                        *reinterpret_cast<uint4*>(slot + 512) = make_uint4(a.y, b.y, c.y, d.y);
+                        *reinterpret_cast<uint4*>(slot + 1024) = make_uint4(a.z, b.z, c.z, d.z);
+                        *reinterpret_cast<uint4*>(slot + 1536) = make_uint4(a.w, b.w, c.w, d.w);
+                    } else {
+                        const uint4 a = *reinterpret_cast<uint4*>(slot), b = *reinterpret_cast<uint4*>(slot + 512);
+                        *reinterpret_cast<uint4*>(slot) = make_uint4(a.x, a.z, b.x, b.z);
+                        *reinterpret_cast<uint4*>(slot + 512) = make_uint4(a.y, a.w, b.y, b.w);
+                    }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) {  // the first CTA's barrier counts the warps of both CTAs
-                    if (cta == 0) mbar_arrive(&bar_sf[done % NS]);
-                    else mbar_arrive_cluster(map_to_cta(&bar_sf[done % NS], 0));
+                if (lane == 0) {  // the first CTA's barrier counts both CTAs
+                    if (cta == 0) mbar_arrive(&bar_sf[s]);
+                    else mbar_arrive_cluster(map_to_cta(&bar_sf[s], 0));
                 }
-                ++done;
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");  // nothing of this warp is in flight when the CTA ends
-            if (!ok && lane == 0) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 3, static_cast<int>(done));
         }
+        if (!ok && lane == 0) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 3, static_cast<int>(it));
     } else {
         reg_alloc<kF4EpiRegs>();
         // ---------------------------------------------------------------- epilogue warps
