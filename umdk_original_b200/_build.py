@@ -49,6 +49,7 @@ KERNEL_SOURCES = [
     "kernels/quant_fp4.cu",
     "kernels/grouped_gemm_fp4.cu",
     "kernels/grouped_mlp.cu",
+    "kernels/expert_gemm_narrow.cu",
     "runtime/cam_runtime.cpp",
     "runtime/expert_ops.cpp",
 ]

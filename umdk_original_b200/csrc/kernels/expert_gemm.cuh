@@ -1,6 +1,7 @@
 // What the grouped products of the stand-alone expert-MLP operators share: the walker over the tiles of ragged experts, the
 // zero fill of rows that belong to no expert, the epilogue's staging of 16-bit rows and the launch on CTA pairs.
 #pragma once
+#include "../common/fp4.cuh"
 #include "expert_ops.h"
 #include "gemm_common.cuh"
 
@@ -9,22 +10,23 @@ namespace cam {
 // Offsets are data on the device: whatever they hold, first and last row of an expert stay inside [0, rows].
 __device__ __forceinline__ int expert_bound(const int* off, int i, int rows) { return min(max(__ldg(off + i), 0), rows); }
 
-// Tiles of 256 rows x n_tiles columns of every expert, expert by expert; the columns of a row block are neighbours.
-struct PairTileWalker {
+// Tiles of TM rows x n_tiles columns of every expert, expert by expert; the columns of a row block are neighbours.
+template <int TM>
+struct RowWalker {
     const int* off;
     int num_experts, n_tiles, rows_total;
     int e = 0, base = 0;
-    __device__ PairTileWalker(const int* o, int ne, int nt, int rt) : off(o), num_experts(ne), n_tiles(nt), rows_total(rt) {}
+    __device__ RowWalker(const int* o, int ne, int nt, int rt) : off(o), num_experts(ne), n_tiles(nt), rows_total(rt) {}
     __device__ bool locate(int tile, int& e_out, int& nt, int& row0, int& rows) {
         while (e < num_experts) {
             const int first = expert_bound(off, e, rows_total);
             const int cnt = max(expert_bound(off, e + 1, rows_total) - first, 0);
-            const int tiles = ((cnt + 2 * BM - 1) / (2 * BM)) * n_tiles;
+            const int tiles = ((cnt + TM - 1) / TM) * n_tiles;
             if (tile < base + tiles) {
                 const int local = tile - base, mt = local / n_tiles;
                 nt = local - mt * n_tiles;
-                row0 = first + mt * 2 * BM;
-                rows = min(2 * BM, cnt - mt * 2 * BM);
+                row0 = first + mt * TM;
+                rows = min(TM, cnt - mt * TM);
                 e_out = e;
                 return true;
             }
@@ -34,6 +36,8 @@ struct PairTileWalker {
         return false;
     }
 };
+
+using PairTileWalker = RowWalker<2 * BM>;
 
 // Rows before the first and past the last expert get zeros (16-byte units, `pitch16` of them per row); called by `threads`
 // threads of every CTA, `t` their index.
@@ -81,6 +85,92 @@ int launch_pairs(PairLimit& limit, Kernel kernel, int threads, int smem_bytes, i
     if (pairs > n) pairs = n;
     cfg.gridDim = dim3(static_cast<unsigned>(2 * (pairs < 1 ? 1 : pairs)));
     return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
+// Instruction descriptor of kind::mxf4 / mxf4nvf4: e2m1 (1) at [7,10) and [10,12), N>>3 at [17,23), scale type [23]
+// (0 = e4m3, 1 = e8m0), M>>4 at [24,29), bytes of the scale word for B at [4,6) and for A at [29,31): 0 or 2.
+template <int FMT>
+__device__ __forceinline__ constexpr uint32_t idesc_fp4(uint32_t m, uint32_t n, uint32_t sf_id) {
+    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((FMT == kFp4Mx ? 1u : 0u) << 23) | ((m >> 4) << 24) |
+           (sf_id << 29);
+}
+
+// Shared-memory matrix without swizzle, 16 bytes wide: groups of 8 rows 128 bytes apart (the 512 bytes of one scale tile)
+__device__ __forceinline__ uint64_t desc_scales(uint32_t smem_addr) {
+    return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {  // zeros where not `live`
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(live ? BYTES : 0), "n"(BYTES) : "memory");
+}
+
+// The scale words of rows l, 32 + l, 64 + l, 96 + l that lane l copied to `slot` (its 16 bytes of every 512), in place:
+// [row j][K-step i] -> [K-step i][row j], what tcgen05.cp takes to tensor memory.
+template <int FMT>
+__device__ __forceinline__ void fp4_transpose_scales(uint8_t* slot) {
+    if constexpr (FMT == kFp4Nv) {
+        const uint4 a = *reinterpret_cast<uint4*>(slot), b = *reinterpret_cast<uint4*>(slot + 512);
+        const uint4 c = *reinterpret_cast<uint4*>(slot + 1024), d = *reinterpret_cast<uint4*>(slot + 1536);
+        *reinterpret_cast<uint4*>(slot) = make_uint4(a.x, b.x, c.x, d.x);
+        *reinterpret_cast<uint4*>(slot + 512) = make_uint4(a.y, b.y, c.y, d.y);
+        *reinterpret_cast<uint4*>(slot + 1024) = make_uint4(a.z, b.z, c.z, d.z);
+        *reinterpret_cast<uint4*>(slot + 1536) = make_uint4(a.w, b.w, c.w, d.w);
+    } else {
+        const uint4 a = *reinterpret_cast<uint4*>(slot), b = *reinterpret_cast<uint4*>(slot + 512);
+        *reinterpret_cast<uint4*>(slot) = make_uint4(a.x, a.z, b.x, b.z);
+        *reinterpret_cast<uint4*>(slot + 512) = make_uint4(a.y, a.w, b.y, b.w);
+    }
+}
+// Where the words of row block j of lane l start before that, beyond the lane's 16 bytes
+template <int FMT>
+__device__ __forceinline__ uint32_t fp4_scale_at(int j) {
+    return FMT == kFp4Nv ? static_cast<uint32_t>(j) * 512u : static_cast<uint32_t>(j >> 1) * 512u + static_cast<uint32_t>(j & 1) * 8u;
+}
+
+// silu(gate) * up of 32 columns, then scales (two blocks of 16 or one of 32) and codes; `gate` and `up` are raw accumulators.
+template <int FMT>
+__device__ __forceinline__ void fp4_swiglu32(const uint32_t* gate, const uint32_t* up, float alpha, float out_g, uint4& codes, uint32_t& scales) {
+    float act[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        const float g = __uint_as_float(gate[j]) * alpha;
+        act[j] = (g / (1.f + expf(-g))) * (__uint_as_float(up[j]) * alpha);
+    }
+    uint32_t amax[2] = {0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 32; ++j) amax[j >> 4] = max(amax[j >> 4], __float_as_uint(act[j]) & 0x7FFFFFFFu);
+    if (FMT == kFp4Mx) amax[0] = amax[1] = max(amax[0], amax[1]);
+    uint2 c[2];
+    uint32_t sc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float d, inv;
+        sc[h] = fp4_scale<FMT>(amax[h], out_g, __fmul_rn(6.f, out_g), d, inv);
+        c[h] = fp4_codes16<FMT>(act + 16 * h, d, inv, amax[h] < 0x7F800000u);
+    }
+    codes = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
+    scales = sc[0] | (sc[1] << 8);
+}
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, bool fp16) {
+    if (fp16) {
+        const __half2 t = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    }
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+// Rows of scales of no expert, byte by byte (see zero_loose_rows)
+__device__ __forceinline__ void zero_loose_scales(uint8_t* s, int64_t pitch, const int* off, int num_experts, int rows, int t, int threads) {
+    const int head = expert_bound(off, 0, rows), tail = expert_bound(off, num_experts, rows);
+    const int64_t n0 = head * pitch, n1 = (rows - tail) * pitch;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * threads + t; i < n0 + n1; i += static_cast<int64_t>(gridDim.x) * threads)
+        s[i < n0 ? i : tail * pitch + (i - n0)] = 0;
 }
 
 }  // namespace cam

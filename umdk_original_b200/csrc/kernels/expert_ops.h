@@ -40,6 +40,26 @@ struct GroupedMlpParams {
     float* gate_up;             // [rows, 2I] fp32: written by kMlpUp (or null), read by kMlpDact
 };
 
+// One-CTA form of the row products for experts with few rows (expert_gemm_narrow.cu): tiles of 128 rows x `width` columns.
+constexpr int kNarrow16 = 2;  // beside the formats of fp4.cuh: 16-bit operands
+struct NarrowParams {
+    const int* expert_offsets;
+    int num_experts, rows;
+    int n_dim;                  // columns of the result; with SwiGLU: I, the weights have 2I rows
+    int kblocks;                // 128-byte blocks of a row
+    int width;                  // columns of the product per tile: 32 (not fp4), 64 or 128
+    int slot_rows;              // rows of A a stage has room for: 32, 64 or 128 (at least the rows of any expert's tile)
+    int stages, stage_bytes;
+    int fp16;
+    void* out;                  // 16-bit [rows, n_dim], or fp4 SwiGLU: codes [rows, I/2]
+    float* gate_up;             // 16-bit SwiGLU: null or fp32 [rows, 2I]
+    // fp4
+    const uint8_t *a_scales, *b_scales;
+    int scale_pitch, scale_vec;
+    const float *a_gscale, *b_gscale, *out_gscale;
+    uint8_t* out_scales;
+};
+
 }  // namespace cam
 
 extern "C" {
@@ -59,6 +79,12 @@ int cam_launch_grouped_gemm_fp4(const cam::GroupedGemmFp4Params* p, int fmt, int
 // the second row operand in boxes of 64 rows.  All boxes are 128 bytes wide.
 int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, const CUtensorMap* tmap_a, const CUtensorMap* tmap_a32,
                            const CUtensorMap* tmap_b, cudaStream_t stream);
+// kind: kFp4Nv, kFp4Mx or kNarrow16.  tmap_a: rows in boxes of 32; tmap_b: weights [E, rows, bytes] in boxes of `width` rows, or
+// of width / 2 with SwiGLU.
+int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int swiglu, int64_t tiles, const CUtensorMap* tmap_a,
+                                  const CUtensorMap* tmap_b, cudaStream_t stream);
+int cam_expert_narrow_max_stages(int kind);
+int cam_narrow_status(CamStatus* out);
 int cam_mlp_status(CamStatus* out);
 int cam_fp4_status(CamStatus* out);  // of the current device: the first wait that ran out in a kernel of that file
 }

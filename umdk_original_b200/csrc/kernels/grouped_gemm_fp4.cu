@@ -68,30 +68,9 @@ __device__ __forceinline__ void tc_mma_fp4_pair(uint32_t d_tmem, uint64_t a_desc
     }
 }
 
-// Instruction descriptor of kind::mxf4 / mxf4nvf4: e2m1 (1) at [7,10) and [10,12), N>>3 at [17,23), scale type [23]
-// (0 = e4m3, 1 = e8m0), M>>4 at [24,29), bytes of the scale word for B at [4,6) and for A at [29,31): 0 or 2.
-template <int FMT>
-__device__ __forceinline__ constexpr uint32_t idesc_fp4(uint32_t m, uint32_t n, uint32_t sf_id) {
-    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((FMT == kFp4Mx ? 1u : 0u) << 23) | ((m >> 4) << 24) |
-           (sf_id << 29);
-}
-
-// Shared-memory matrix without swizzle, 16 bytes wide: groups of 8 rows 128 bytes apart (the 512 bytes of one scale tile)
-__device__ __forceinline__ uint64_t desc_scales(uint32_t smem_addr) {
-    return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
-}
-
 // 32 rows x 16 bytes of shared memory to 32 lanes x 4 columns of tensor memory, repeated in all four lane quarters, in both CTAs
 __device__ __forceinline__ void tc_copy_scales_pair(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {  // zeros where not `live`
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(live ? BYTES : 0), "n"(BYTES) : "memory");
 }
 
 }  // namespace
@@ -251,7 +230,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
 #pragma unroll
                 for (int j = 0; j < 12; ++j) {
                     if (j < 4 && 32 * j + static_cast<int>(lane) >= a_rows) continue;
-                    const uint32_t d = dst + (j >> 2) * kF4SfBlock + (FMT == kFp4Nv ? (j & 3) * 512u : ((j >> 1) & 1) * 512u + (j & 1) * 8u);
+                    const uint32_t d = dst + (j >> 2) * kF4SfBlock + fp4_scale_at<FMT>(j & 3);
                     const uint8_t* from = src[j] + kb * SFW * 4;
                     if (p.scale_vec) {
                         copy_async<SFW * 4>(d, from, true);
@@ -264,22 +243,8 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                     }
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
-                // this lane's words, in place: [row j][K-step i] -> [K-step i][row j]
 #pragma unroll
-                for (int blk = 0; blk < 3; ++blk, slot += kF4SfBlock) {
-                    if constexpr (FMT == kFp4Nv) {
-                        const uint4 a = *reinterpret_cast<uint4*>(slot), b = *reinterpret_cast<uint4*>(slot + 512);
-                        const uint4 c = *reinterpret_cast<uint4*>(slot + 1024), d = *reinterpret_cast<uint4*>(slot + 1536);
-                        *reinterpret_cast<uint4*>(slot) = make_uint4(a.x, b.x, c.x, d.x);
-                        *reinterpret_cast<uint4*>(slot + 512) = make_uint4(a.y, b.y, c.y, d.y);
-                        *reinterpret_cast<uint4*>(slot + 1024) = make_uint4(a.z, b.z, c.z, d.z);
-                        *reinterpret_cast<uint4*>(slot + 1536) = make_uint4(a.w, b.w, c.w, d.w);
-                    } else {
-                        const uint4 a = *reinterpret_cast<uint4*>(slot), b = *reinterpret_cast<uint4*>(slot + 512);
-                        *reinterpret_cast<uint4*>(slot) = make_uint4(a.x, a.z, b.x, b.z);
-                        *reinterpret_cast<uint4*>(slot + 512) = make_uint4(a.y, a.w, b.y, b.w);
-                    }
-                }
+                for (int blk = 0; blk < 3; ++blk) fp4_transpose_scales<FMT>(slot + blk * kF4SfBlock);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {  // the first CTA's barrier counts both CTAs
@@ -321,31 +286,14 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                 else mbar_arrive_cluster(map_to_cta(bar_tempty, 0));
             }
             if constexpr (SWIGLU) {
-                // silu(gate) * up of 32 columns, then their scales (two blocks of 16 or one of 32) and codes
-                float act[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float g = __uint_as_float(v0[j]) * alpha;
-                    act[j] = (g / (1.f + expf(-g))) * (__uint_as_float(v1[j]) * alpha);
-                }
-                const float six_g = __fmul_rn(6.f, out_g);
-                uint32_t amax[2] = {0u, 0u};
-#pragma unroll
-                for (int j = 0; j < 32; ++j) amax[j >> 4] = max(amax[j >> 4], __float_as_uint(act[j]) & 0x7FFFFFFFu);
-                if (FMT == kFp4Mx) amax[0] = amax[1] = max(amax[0], amax[1]);
-                uint2 codes[2];
-                uint32_t sc[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float d, inv;
-                    sc[h] = fp4_scale<FMT>(amax[h], out_g, six_g, d, inv);
-                    codes[h] = fp4_codes16<FMT>(act + 16 * h, d, inv, amax[h] < 0x7F800000u);
-                }
+                uint4 codes;
+                uint32_t scales;
+                fp4_swiglu32<FMT>(v0, v1, alpha, out_g, codes, scales);
                 if (valid) {
                     const size_t at = grow * (half_n / 32) + nt * 4 + cq;  // in units of 32 columns
-                    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + at * 16) = make_uint4(codes[0].x, codes[0].y, codes[1].x, codes[1].y);
-                    if (FMT == kFp4Nv) *reinterpret_cast<uint16_t*>(p.out_scales + at * 2) = static_cast<uint16_t>(sc[0] | (sc[1] << 8));
-                    else p.out_scales[at] = static_cast<uint8_t>(sc[0]);
+                    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + at * 16) = codes;
+                    if (FMT == kFp4Nv) *reinterpret_cast<uint16_t*>(p.out_scales + at * 2) = static_cast<uint16_t>(scales);
+                    else p.out_scales[at] = static_cast<uint8_t>(scales);
                 }
             } else {
                 // 128 columns at a time go through shared memory as bf16 and leave as one 256-byte bulk copy per row
@@ -378,10 +326,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         const int et = static_cast<int>(threadIdx.x) - kF4EpiWarp0 * 32;
         if constexpr (SWIGLU) {
             zero_loose_rows(p.out, half_n / 32, p.expert_offsets, p.num_experts, p.rows, et, kF4EpiThreads);
-            const int head = expert_bound(p.expert_offsets, 0, p.rows), tail = expert_bound(p.expert_offsets, p.num_experts, p.rows);
-            const int64_t sp = half_n / BLK, n0 = head * sp, n1 = (p.rows - tail) * sp;
-            for (int64_t i = static_cast<int64_t>(blockIdx.x) * kF4EpiThreads + et; i < n0 + n1; i += static_cast<int64_t>(gridDim.x) * kF4EpiThreads)
-                p.out_scales[i < n0 ? i : tail * sp + (i - n0)] = 0;
+            zero_loose_scales(p.out_scales, half_n / BLK, p.expert_offsets, p.num_experts, p.rows, et, kF4EpiThreads);
         } else {
             zero_loose_rows(p.out, p.n_dim / 8, p.expert_offsets, p.num_experts, p.rows, et, kF4EpiThreads);
         }

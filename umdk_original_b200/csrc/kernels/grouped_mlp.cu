@@ -86,15 +86,6 @@ struct GradTileWalker {
     }
 };
 
-__device__ __forceinline__ uint32_t pack16(float a, float b, bool fp16) {
-    if (fp16) {
-        const __half2 t = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&t);
-    }
-    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&t);
-}
-
 }  // namespace
 
 // A_MN / B_MN: the operand's contraction index is its row index in memory.  A_MN is the weight-gradient form.

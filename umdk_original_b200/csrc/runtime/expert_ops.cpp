@@ -3,8 +3,10 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 
 #include "../kernels/expert_ops.h"
+#include "../kernels/launch.h"
 
 namespace {
 
@@ -31,8 +33,56 @@ int map_2d(CUtensorMap* out, const void* base, uint64_t bytes, uint64_t rows, ui
     return cam_encode_tmap(out, base, 2, dims, strides, box);
 }
 
+// [experts, rows, bytes] with boxes of 128 bytes x box_rows
+int map_3d(CUtensorMap* out, const void* base, uint64_t bytes, uint64_t rows, uint64_t experts, uint32_t box_rows) {
+    const uint64_t dims[3] = {bytes, rows, experts}, strides[2] = {bytes, bytes * rows};
+    const uint32_t box[3] = {128, box_rows, 1};
+    return cam_encode_tmap(out, base, 3, dims, strides, box);
+}
+
 int launched(int rc, const char* what) {
     return rc == 0 ? 0 : refuse("%s: launch failed: %s", what, cudaGetErrorString(static_cast<cudaError_t>(rc)));
+}
+
+// Environment switch: -1 unset, otherwise its number.
+int env_switch(const char* name) {
+    const char* v = std::getenv(name);
+    return v != nullptr && *v != 0 ? std::atoi(v) : -1;
+}
+
+// One-CTA tiles of 128 rows (expert_gemm_narrow.cu) or CTA pairs with tiles of 256 x 256?
+bool narrow_pays(int rows, int num_experts) {
+    const int sw = env_switch("UMDK_CAM_EXPERT_NARROW");
+    if (sw >= 0) return sw != 0;
+    return static_cast<int64_t>(rows) <= 128ll * num_experts;
+}
+
+// Tile width, stages and number of tiles of the one-CTA form for `n` result columns.
+void narrow_plan(cam::NarrowParams* p, int kind, bool swiglu, int64_t* tiles) {
+    const bool fp4 = kind != cam::kNarrow16;
+    const int sms = cam::sm_count_of_current_device();
+    const int64_t blocks = p->rows <= p->num_experts ? p->rows
+                                                     : static_cast<int64_t>(p->num_experts) * (((p->rows + p->num_experts - 1) / p->num_experts + 127) / 128);
+    const int forced = env_switch("UMDK_CAM_EXPERT_WIDTH");
+    int64_t best = -1;
+    for (int width = 128; width >= (fp4 ? 64 : 32); width /= 2) {
+        const int step = swiglu ? width / 2 : width;
+        const int64_t t = blocks * ((p->n_dim + step - 1) / step);
+        // turns of the SMs x time of a tile; a tile costs its weights and a fixed part
+        const int64_t cost = ((t + sms - 1) / sms) * (width + 16);
+        if (forced > 0 ? width == forced : best < 0 || cost < best) {
+            best = cost;
+            p->width = width;
+        }
+    }
+    const int step = swiglu ? p->width / 2 : p->width;
+    const int64_t upper = p->rows / 128 + (p->rows < p->num_experts ? p->rows : p->num_experts);  // row blocks there can be
+    *tiles = upper * ((p->n_dim + step - 1) / step);
+    p->slot_rows = p->rows <= 32 ? 32 : p->rows <= 64 ? 64 : 128;
+    p->stage_bytes = (p->slot_rows + p->width) * 128 + (fp4 ? 4096 : 0);
+    const int pad = p->stage_bytes < 16384 ? 16384 - p->stage_bytes : 0;
+    const int fit = (232448 - 1024 - pad) / p->stage_bytes, most = cam_expert_narrow_max_stages(kind);
+    p->stages = fit < most ? fit : most;
 }
 
 }  // namespace
@@ -68,6 +118,31 @@ extern "C" int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, 
     EXP_CHECK(n_dim >= 128 && n_dim % (swiglu ? 256 : 128) == 0, "grouped_gemm_fp4: N %d must be a multiple of %d", n_dim, swiglu ? 256 : 128);
     EXP_CHECK(static_cast<int64_t>(num_experts) * n_dim < (1ll << 31), "grouped_gemm_fp4: weight rows overflow");
     EXP_CHECK(aligned(a_s, 4) && aligned(w_s, 4), "grouped_gemm_fp4: scales must be 4-byte aligned");
+    if (narrow_pays(rows, num_experts)) {
+        cam::NarrowParams p{};
+        p.expert_offsets = offsets;
+        p.num_experts = num_experts;
+        p.rows = rows;
+        p.n_dim = swiglu ? n_dim / 2 : n_dim;
+        p.kblocks = (k_dim + 255) / 256;
+        p.out = out;
+        p.a_scales = static_cast<const uint8_t*>(a_s);
+        p.b_scales = static_cast<const uint8_t*>(w_s);
+        p.scale_pitch = k_dim / (fmt == 0 ? 16 : 32);
+        p.scale_vec = k_dim % 256 == 0 && aligned(a_s, 16) && aligned(w_s, 16);
+        p.a_gscale = a_gscale;
+        p.b_gscale = w_gscale;
+        p.out_gscale = out_gscale;
+        p.out_scales = static_cast<uint8_t*>(out_s);
+        int64_t tiles = 0;
+        narrow_plan(&p, fmt, swiglu != 0, &tiles);
+        CUtensorMap ta, tb;
+        if (map_2d(&ta, a_q, static_cast<uint64_t>(k_dim) / 2, static_cast<uint64_t>(rows), 32) != 0) return -1;
+        if (map_3d(&tb, w_q, static_cast<uint64_t>(k_dim) / 2, static_cast<uint64_t>(n_dim), static_cast<uint64_t>(num_experts),
+                   static_cast<uint32_t>(swiglu ? p.width / 2 : p.width)) != 0)
+            return -1;
+        return launched(cam_launch_expert_gemm_narrow(&p, fmt, swiglu, tiles, &ta, &tb, stream), "grouped_gemm_fp4");
+    }
     cam::GroupedGemmFp4Params p{};
     p.expert_offsets = offsets;
     p.num_experts = num_experts;
@@ -92,19 +167,32 @@ extern "C" int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, 
 
 namespace {
 
-// [experts, rows, bytes] with boxes of 128 bytes x box_rows
-int map_3d(CUtensorMap* out, const void* base, uint64_t bytes, uint64_t rows, uint64_t experts, uint32_t box_rows) {
-    const uint64_t dims[3] = {bytes, rows, experts}, strides[2] = {bytes, bytes * rows};
-    const uint32_t box[3] = {128, box_rows, 1};
-    return cam_encode_tmap(out, base, 3, dims, strides, box);
-}
-
 // A product of the rows a [rows, k] with the weights: w [E, w_rows, w_cols], contracted over its columns or (by_rows) its rows.
 int row_product(int form, const char* what, const void* a, int k, const void* w, int w_rows, int w_cols, bool by_rows, int n,
                 const int* offsets, int rows, int num_experts, int dtype, void* out, float* gate_up, cudaStream_t stream) {
     EXP_CHECK(a && w && offsets && out, "%s: null operand", what);
     EXP_CHECK(rows >= 1 && num_experts >= 1, "%s: empty problem", what);
     EXP_CHECK(k >= 8 && n >= 8 && k % 8 == 0 && n % 8 == 0, "%s: sizes %d and %d must be multiples of 8", what, k, n);
+    if (!by_rows && narrow_pays(rows, num_experts)) {
+        const bool swiglu = form == cam::kMlpUp;
+        cam::NarrowParams p{};
+        p.expert_offsets = offsets;
+        p.num_experts = num_experts;
+        p.rows = rows;
+        p.n_dim = n;
+        p.kblocks = (k + 63) / 64;
+        p.fp16 = dtype == 1;
+        p.out = out;
+        p.gate_up = gate_up;
+        int64_t tiles = 0;
+        narrow_plan(&p, cam::kNarrow16, swiglu, &tiles);
+        CUtensorMap ta, tb;
+        if (map_2d(&ta, a, static_cast<uint64_t>(k) * 2, static_cast<uint64_t>(rows), 32) != 0) return -1;
+        if (map_3d(&tb, w, static_cast<uint64_t>(w_cols) * 2, static_cast<uint64_t>(w_rows), static_cast<uint64_t>(num_experts),
+                   static_cast<uint32_t>(swiglu ? p.width / 2 : p.width)) != 0)
+            return -1;
+        return launched(cam_launch_expert_gemm_narrow(&p, cam::kNarrow16, swiglu, tiles, &ta, &tb, stream), what);
+    }
     cam::GroupedMlpParams p{};
     p.expert_offsets = offsets;
     p.num_experts = num_experts;
@@ -167,5 +255,6 @@ extern "C" int cam_grouped_mlp_dw(const void* a, const void* b, const int* offse
 extern "C" int cam_expert_ops_status(CamStatus* out) {
     int rc = cam_fp4_status(out);
     if (rc == 0 && out->code == 0) rc = cam_mlp_status(out);
+    if (rc == 0 && out->code == 0) rc = cam_narrow_status(out);
     return rc == 0 ? 0 : refuse("expert_ops_status: %s", cudaGetErrorString(static_cast<cudaError_t>(rc)));
 }
