@@ -201,6 +201,41 @@ def test_swiglu(ops, fmt, k, inter, counts):
     assert (q[~live] == 0).all() and (s.view(torch.uint8)[~live] == 0).all()
 
 
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("m,e,k,n,swiglu", [
+    (8, 32, 7168, 4096, True), (8, 32, 2048, 7168, False),        # a token's eight experts
+    (40, 4, 1024, 512, True), (40, 4, 1024, 512, False),          # up to 64 rows in all
+    (768, 32, 4096, 2048, True), (768, 32, 1024, 4096, False),    # many experts, narrow tiles beside room for 128 rows
+    (100, 1, 512, 256, True), (200, 2, 640, 384, False),          # few tiles
+    (300, 3, 4096, 1024, True),
+])
+def test_few_rows(ops, fmt, m, e, k, n, swiglu):
+    """The forms for few rows per expert, at the sizes where their tiles, stages and row slots differ."""
+    gen = torch.Generator().manual_seed(m + e)
+    cnt = torch.bincount(torch.randint(0, e, (m,), generator=gen), minlength=e).tolist()
+    aq, as_ = random_fp4((m, k), fmt, gen)
+    wq, ws = random_fp4((e, n, k), fmt, gen)
+    ag, wg = (torch.full((1,), 0.002), torch.rand(e, generator=gen) * 0.02) if fmt == "nvfp4" else (None, None)
+    off = offsets_of(cnt)
+    if not swiglu:
+        got = ops.grouped_gemm_fp4(*_dev(aq, as_, wq, ws, off, ag, wg))
+        want, mag = _product64(values64(*_dev(aq, as_, ag)), values64(*_dev(wq, ws, wg)), off, m)
+        assert ((got.double() - want).abs() <= want.abs() * 2.0 ** -8 + mag * _acc_tol(k)).all()
+        return
+    # gate and up from the plain product; the SwiGLU form has to agree with it through its own definition
+    gu = ops.grouped_gemm_fp4(*_dev(aq, as_, wq, ws, off, ag, wg)).double()
+    q, s = ops.grouped_gemm_fp4_swiglu(*_dev(aq, as_, wq, ws, off, ag, wg))
+    g, u = gu.chunk(2, -1)
+    act = g * torch.sigmoid(g) * u
+    # gu was rounded to bf16 (2^-8 relative in each factor, |silu'| <= 1.1 of the gate) on top of the 4-bit rounding: half a
+    # step (a step is at most a third of the value, or half of the scale) and what is cut off above 6 scales (a sixteenth)
+    val = values64(q, s)
+    d = (s.double() if fmt == "nvfp4" else torch.exp2(s.view(torch.uint8).double() - 127)).repeat_interleave(16 if fmt == "nvfp4" else 32, -1)
+    slack = 2.0 ** -8 * (1.1 * g.abs() * u.abs() + act.abs()) * 1.01 + act.abs() * 2.0 ** -12
+    cut = torch.where(d <= 2.0 ** -8, act.abs(), act.abs() / 16)  # scales near the smallest e4m3 are rounded by up to half of themselves
+    assert ((val - act).abs() <= torch.maximum(0.25 * d, act.abs() / 6) + cut + slack).all()
+
+
 def test_status_is_clean(ops):
     from umdk_original_b200.ops import cam_ops
     assert cam_ops.native_module().expert_ops_status()[0] == 0

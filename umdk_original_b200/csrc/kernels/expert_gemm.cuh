@@ -7,6 +7,59 @@
 
 namespace cam {
 
+// ----------------------------------------------------------------------------------------
+// Waits of the single-lane roles (TMA producer, MMA issuer).  The whole warp walks the loop and one elected lane issues, so
+// that descriptors and counters stay uniform.  A look at an mbarrier takes about 130 cycles even when the phase is complete,
+// a quarter of a K-block: the roles therefore look at the next stage's barrier before they issue the present one's work
+// (mbar_test), and come back to it only if it was not complete then (mbar_wait_warp).
+// ----------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok;
+}
+// Bounded: after kWaitPolls polls (each of which the hardware may itself hold for a while), or once another role has given up,
+// it returns with *abort set; the pipeline then runs to its end without waiting and its results mean nothing.
+constexpr uint32_t kWaitPolls = 1u << 23;
+__device__ __forceinline__ void mbar_wait_warp(uint32_t bar, uint32_t parity, uint32_t abort) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        ".reg .b32 n, f;\n"
+        "mov.u32 n, 0;\n"
+        "POLL:\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n"
+        "@p bra DONE;\n"
+        "add.u32 n, n, 1;\n"
+        "and.b32 f, n, 255;\n"
+        "setp.ne.u32 q, f, 0;\n"
+        "@q bra POLL;\n"
+        "ld.volatile.shared.u32 f, [%2];\n"
+        "setp.ne.u32 q, f, 0;\n"
+        "@q bra DONE;\n"
+        "setp.lt.u32 q, n, %3;\n"
+        "@q bra POLL;\n"
+        "st.volatile.shared.u32 [%2], 1;\n"
+        "DONE:\n"
+        "}\n" ::"r"(bar), "r"(parity), "r"(abort), "n"(kWaitPolls)
+        : "memory");
+}
+// Position in a ring of stages: stage and the parity of its current turn
+struct Ring {
+    uint32_t s = 0, ph = 0;
+    __device__ __forceinline__ void next(uint32_t n) {
+        if (++s == n) { s = 0; ph ^= 1u; }
+    }
+};
+
 // Offsets are data on the device: whatever they hold, first and last row of an expert stay inside [0, rows].
 __device__ __forceinline__ int expert_bound(const int* off, int i, int rows) { return min(max(__ldg(off + i), 0), rows); }
 
@@ -59,7 +112,7 @@ int launch_pairs(PairLimit& limit, Kernel kernel, int threads, int smem_bytes, i
     cudaError_t err = limit.smem.ensure(kernel, smem_bytes);
     if (err != cudaSuccess) return static_cast<int>(err);
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3(2);
     cfg.blockDim = dim3(static_cast<unsigned>(threads));
     cfg.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
@@ -68,6 +121,7 @@ int launch_pairs(PairLimit& limit, Kernel kernel, int threads, int smem_bytes, i
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1] = pdl_attribute();
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int dev = 0;
@@ -84,6 +138,7 @@ int launch_pairs(PairLimit& limit, Kernel kernel, int threads, int smem_bytes, i
     }
     if (pairs > n) pairs = n;
     cfg.gridDim = dim3(static_cast<unsigned>(2 * (pairs < 1 ? 1 : pairs)));
+    cfg.numAttrs = 2;
     return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 

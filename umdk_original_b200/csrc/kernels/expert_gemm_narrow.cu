@@ -4,8 +4,11 @@
 // What bounds these calls is the stream of weights, so the form differs from the CTA pairs (grouped_gemm_fp4.cu,
 // grouped_mlp.cu) in what it keeps small:
 //   * A tile is narrow enough that there are several for every SM, even where one expert has one row.
-//   * The ring of K-blocks is cut for the rows there can be: a stage holds 32, 64 or 128 rows of A beside the weights, and there
+//   * The ring of stages is cut for the rows there can be: a stage holds 32, 64 or 128 rows of A beside the weights, and there
 //     are as many stages as shared memory holds, so that the weights in flight cover the latency of memory.
+//   * A stage of a narrow tile is several K-blocks (128 bytes of every row; `chunks` of them), 16 KiB of weights in all, brought
+//     by one TMA instruction: the turn of a stage (two waits, an arrive, a commit) costs each role about 300 cycles, more than
+//     the 4 KiB of one K-block of 32 columns take at this SM's share of the memory bandwidth.
 //   * No staging: a thread stores 32 columns of its row (64 bytes) from registers.
 //   * Scale factors (4-bit): only rows that exist and the tile's own weight rows are brought to tensor memory; with CTA pairs
 //     both CTAs need those of all 256 columns.
@@ -17,10 +20,11 @@ namespace cam {
 
 constexpr int kNwEpiWarps = 8;
 constexpr int kNwMaxStages = 24;
-constexpr int kNwMaxStagesFp4 = 8;      // as many as there are scale slots in tensor memory
+constexpr int kNwScaleWarps = 4;
+constexpr int kNwScaleSlots = 8;        // K-blocks whose scales tensor memory has room for
 constexpr int kNwSfBlock = 4 * 512;     // scales of 128 rows of a K-block
 constexpr uint32_t kNwTmemCols = 512, kNwSfCol0 = 256, kNwSfCols = 32;
-static_assert(kNwSfCol0 + kNwMaxStagesFp4 * kNwSfCols <= kNwTmemCols, "tensor memory");
+static_assert(kNwSfCol0 + kNwScaleSlots * kNwSfCols <= kNwTmemCols, "tensor memory");
 constexpr int kNwCtrlBytes = 1024;
 static_assert((3 * kNwMaxStages + 4) * 8 + 16 <= kNwCtrlBytes, "barriers");
 
@@ -58,20 +62,18 @@ __device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-__device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, uint64_t* bar, int32_t c0, int32_t c1, int32_t c2) {
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const void* tmap, uint32_t bar, int32_t c0, int32_t c1, int32_t c2) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
-
-// Position in the ring: stage and the parity of its current turn
-struct Ring {
-    uint32_t s = 0, ph = 0;
-    __device__ __forceinline__ void next(uint32_t n) {
-        if (++s == n) { s = 0; ph ^= 1u; }
-    }
-};
+__device__ __forceinline__ void tma_load_5d(uint32_t smem_dst, const void* tmap, uint32_t bar, int32_t c0, int32_t c1, int32_t c2, int32_t c3, int32_t c4) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+        : "memory");
+}
 
 __host__ __device__ constexpr int narrow_epi_warp0(int kind) { return kind == kNarrow16 ? 4 : 8; }
 __host__ __device__ constexpr int narrow_threads(int kind) { return (narrow_epi_warp0(kind) + kNwEpiWarps) * 32; }
@@ -91,9 +93,12 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     constexpr int EPI0 = narrow_epi_warp0(KIND);
     const uint32_t ns = static_cast<uint32_t>(p.stages);
     const int width = p.width;
-    const int a_bytes = p.slot_rows * 128, b_bytes = width * 128;
+    const int chunks = p.chunks;
+    const int a_bytes = p.slot_rows * 128, b_bytes = width * 128;  // of one K-block
+    const int a_all = a_bytes * chunks, b_all = b_bytes * chunks;
+    const int nstages = (p.kblocks + chunks - 1) / chunks;         // of a tile
     uint8_t* ctrl = smem;
-    uint8_t* ring = smem + kNwCtrlBytes;  // stages: rows of A | weight rows | scales of A | scales of the weights
+    uint8_t* ring = smem + kNwCtrlBytes;  // stages, each [chunk] rows of A | [chunk] weight rows | [chunk] scales of A, scales of the weights
     uint64_t* bar_full = reinterpret_cast<uint64_t*>(ctrl);
     uint64_t* bar_sf = bar_full + kNwMaxStages;
     uint64_t* bar_empty = bar_sf + kNwMaxStages;
@@ -128,87 +133,126 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
+    pdl_wait();
+    pdl_release();
     RowWalker<BM> w(p.expert_offsets, p.num_experts, n_tiles, p.rows);
     int e, nt, row0, rows;
     bool ok = true;
     const int tile0 = static_cast<int>(blockIdx.x), tiles_step = static_cast<int>(gridDim.x);
 
+    const uint32_t abort_at = smem_u32(tmem_slot + 1), ring_at = smem_u32(ring);
+    const uint32_t full_at = smem_u32(bar_full), sf_at = smem_u32(bar_sf), empty_at = smem_u32(bar_empty);
     if (warp == 0) {
-        if (lane == 0) {
-            // ------------------------------------------------------------ TMA producer
+        // ---------------------------------------------------------------- TMA producer
+        const bool leader = elect_one();
+        if (leader) {
             prefetch_tensormap(&tmap_a);
             prefetch_tensormap(&tmap_b);
-            Ring r;
-            for (int tile = tile0; ok && w.locate(tile, e, nt, row0, rows); tile += tiles_step) {
-                const int pieces = min((rows + 31) / 32, p.slot_rows / 32);
-                const uint32_t bytes = static_cast<uint32_t>(pieces * 4096 + b_bytes);
-                for (int kb = 0; kb < p.kblocks; ++kb, r.next(ns)) {
-                    if (!mbar_wait_bounded(&bar_empty[r.s], r.ph ^ 1u, abort_flag)) { ok = false; break; }
-                    uint8_t* sa = ring + r.s * static_cast<uint32_t>(p.stage_bytes);
-                    uint8_t* sb = sa + a_bytes;
-                    mbar_arrive_expect_tx(&bar_full[r.s], bytes);
-                    tma_load_3d(sb, &tmap_b, &bar_full[r.s], kb * 128, nt * step, e);
-                    if (SWIGLU) tma_load_3d(sb + b_bytes / 2, &tmap_b, &bar_full[r.s], kb * 128, p.n_dim + nt * step, e);
-                    for (int i = 0; i < pieces; ++i) tma_load_2d(sa + i * 4096, &tmap_a, &bar_full[r.s], kb * 128, row0 + i * 32);
-                }
-            }
-            if (!ok) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 0, 0);
         }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            // ------------------------------------------------------------ MMA issuer
-            const uint32_t n = static_cast<uint32_t>(width);
-            uint32_t idesc[2];
-            if constexpr (FP4) {
-                idesc[0] = idesc_fp4<KIND>(BM, 0, 0u) | ((n >> 3) << 17);
-                idesc[1] = KIND == kFp4Mx ? idesc_fp4<KIND>(BM, 0, 2u) | ((n >> 3) << 17) : idesc[0];
-            } else {
-                idesc[0] = idesc[1] = umma_idesc(BM, 0, 1u, p.fp16 ? 0u : 1u) | ((n >> 3) << 17);
+        Ring r;
+        uint32_t ready = 1u;  // the first turn of every stage is free
+        for (int tile = tile0; w.locate(tile, e, nt, row0, rows); tile += tiles_step) {
+            // with several chunks a stage's rows come in one box; otherwise in pieces of 32 rows, those that exist
+            const int pieces = chunks > 1 ? 1 : min((rows + 31) / 32, p.slot_rows / 32);
+            const uint32_t bytes = static_cast<uint32_t>((chunks > 1 ? a_all : pieces * 4096) + b_all);
+            for (int kb = 0; kb < nstages; ++kb) {
+                const uint32_t bar = full_at + 8u * r.s, sa = ring_at + r.s * static_cast<uint32_t>(p.stage_bytes);
+                if (!ready) mbar_wait_warp(empty_at + 8u * r.s, r.ph ^ 1u, abort_at);
+                uint64_t* full = &bar_full[r.s];
+                r.next(ns);
+                ready = mbar_test(empty_at + 8u * r.s, r.ph ^ 1u);
+                if (leader) {
+                    mbar_arrive_expect_tx(full, bytes);
+                    const int c0 = p.chunked ? 0 : kb * 128, c3 = p.chunked ? kb * chunks : 0;
+                    tma_load_5d(sa + static_cast<uint32_t>(a_all), &tmap_b, bar, c0, nt * step, 0, c3, e);
+                    for (int i = 0; i < pieces; ++i) tma_load_3d(sa + static_cast<uint32_t>(i) * 4096u, &tmap_a, bar, c0, row0 + i * 32, c3);
+                }
+                __syncwarp();
             }
-            Ring r;
-            uint32_t tcount = 0;
-            for (int tile = tile0; ok && w.locate(tile, e, nt, row0, rows); tile += tiles_step, ++tcount) {
-                const uint32_t b = tcount & 1u;
-                if (!mbar_wait_bounded(&bar_tempty[b], ((tcount >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+        }
+        if (leader && *abort_flag) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 0, 0);
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issuer
+        const bool leader = elect_one();
+        const uint32_t n = static_cast<uint32_t>(width);
+        uint32_t idesc[2];
+        if constexpr (FP4) {
+            idesc[0] = idesc_fp4<KIND>(BM, 0, 0u) | ((n >> 3) << 17);
+            idesc[1] = KIND == kFp4Mx ? idesc_fp4<KIND>(BM, 0, 2u) | ((n >> 3) << 17) : idesc[0];
+        } else {
+            idesc[0] = idesc[1] = umma_idesc(BM, 0, 1u, p.fp16 ? 0u : 1u) | ((n >> 3) << 17);
+        }
+        Ring r;
+        uint32_t tcount = 0, ready = 0u;
+        for (int tile = tile0; w.locate(tile, e, nt, row0, rows); tile += tiles_step, ++tcount) {
+            const uint32_t b = tcount & 1u;
+            mbar_wait_warp(smem_u32(&bar_tempty[b]), ((tcount >> 1) & 1u) ^ 1u, abort_at);
+            for (int kb = 0; kb < nstages; ++kb) {
+                if (!ready) {
+                    if (FP4) mbar_wait_warp(sf_at + 8u * r.s, r.ph, abort_at);
+                    mbar_wait_warp(full_at + 8u * r.s, r.ph, abort_at);
+                }
                 tc_fence_after_sync();
-                for (int kb = 0; kb < p.kblocks; ++kb, r.next(ns)) {
-                    if (FP4 && !mbar_wait_bounded(&bar_sf[r.s], r.ph, abort_flag)) { ok = false; break; }
-                    if (!mbar_wait_bounded(&bar_full[r.s], r.ph, abort_flag)) { ok = false; break; }
-                    tc_fence_after_sync();
-                    const uint32_t sa = smem_u32(ring + r.s * static_cast<uint32_t>(p.stage_bytes)), sb = sa + static_cast<uint32_t>(a_bytes);
-                    const uint64_t adesc = umma_desc_k_sw128(sa), bdesc = umma_desc_k_sw128(sb);
-                    const uint32_t sf = tmem_base + kNwSfCol0 + r.s * kNwSfCols;
-                    if constexpr (FP4) {
-                        const uint32_t sfs = sb + static_cast<uint32_t>(b_bytes);
+                const uint32_t s = r.s, sa = ring_at + s * static_cast<uint32_t>(p.stage_bytes), sb = sa + static_cast<uint32_t>(a_all);
+                r.next(ns);
+                ready = mbar_test(full_at + 8u * r.s, r.ph);
+                if (FP4) ready &= mbar_test(sf_at + 8u * r.s, r.ph);
+                const int live = min(chunks, p.kblocks - kb * chunks);
+                if (leader) {
+                    for (int c = 0; c < live; ++c) {
+                        const uint64_t adesc = umma_desc_k_sw128(sa + static_cast<uint32_t>(c * a_bytes));
+                        const uint64_t bdesc = umma_desc_k_sw128(sb + static_cast<uint32_t>(c * b_bytes));
+                        const uint32_t sf = tmem_base + kNwSfCol0 + (s * static_cast<uint32_t>(chunks) + static_cast<uint32_t>(c)) * kNwSfCols;
+                        if constexpr (FP4) {
+                            const uint32_t sfs = sb + static_cast<uint32_t>(b_all + c * 2 * kNwSfBlock);
 #pragma unroll
-                        for (int k = 0; k < SFW; ++k) {
-                            tc_copy_scales(sf + 8u * k, desc_scales(sfs + k * 512));
-                            tc_copy_scales(sf + 8u * k + 4u, desc_scales(sfs + kNwSfBlock + k * 512));
+                            for (int k = 0; k < SFW; ++k) {
+                                tc_copy_scales(sf + 8u * k, desc_scales(sfs + k * 512));
+                                tc_copy_scales(sf + 8u * k + 4u, desc_scales(sfs + kNwSfBlock + k * 512));
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t cs = sf + 8u * (KIND == kFp4Mx ? k >> 1 : k);
+                            narrow_mma<KIND>(tmem_base + b * 128u, adesc + 2u * k, bdesc + 2u * k, idesc[k & 1], (kb | c | k) ? 1u : 0u, cs, cs + 4u);
                         }
                     }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t c = sf + 8u * (KIND == kFp4Mx ? k >> 1 : k);
-                        narrow_mma<KIND>(tmem_base + b * 128u, adesc + 2u * k, bdesc + 2u * k, idesc[k & 1], (kb | k) ? 1u : 0u, c, c + 4u);
-                    }
-                    tc_commit(&bar_empty[r.s]);
+                    tc_commit(&bar_empty[s]);
                 }
-                if (!ok) break;
-                tc_commit(&bar_tfull[b]);
+                __syncwarp();
             }
-            if (!ok) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
+            if (leader) tc_commit(&bar_tfull[b]);
+            __syncwarp();
         }
+        if (leader && *abort_flag) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
     } else if (warp < EPI0) {
         if constexpr (FP4) {
         if (warp >= 4) {
-            // ------------------------------------------------------------ scale warps: each takes every fourth K-block
+            // ------------------------------------------------------------ scale warps: each takes every fourth stage
+            // A warp does not see every turn of a stage.  With at least as many stages as scale warps the wait for its last
+            // one (turn i - 4, free once the MMAs of i - 4 - stages were done) still tells that the turn before the one it
+            // waits for now (i - 2 stages) is over, which a wait by parity has to know.
             const uint32_t mine = static_cast<uint32_t>(warp - 4);
             const int words = p.scale_pitch / 4;
             const int w_rows = SWIGLU ? 2 * p.n_dim : p.n_dim;
             const int last_b = p.num_experts * w_rows - 1;
             Ring r;
             uint32_t it = 0;
+            // The K-block's scales are small pieces of many rows, and a warp waits for them before it can take its next stage:
+            // they are brought to L2 a whole tile ahead, so that this wait is one of L2 and not of memory.
+            RowWalker<BM> wn(p.expert_offsets, p.num_experts, n_tiles, p.rows);
+            auto prefetch_tile = [&](int tile) {
+                int pe, pnt, prow0, prows;
+                if (!wn.locate(tile, pe, pnt, prow0, prows)) return;
+                for (int t = static_cast<int>(threadIdx.x) - 128; t < width; t += 128) {
+                    const int wr = SWIGLU ? (t < step ? pnt * step + t : p.n_dim + pnt * step + t - step) : pnt * step + t;
+                    const uint8_t* row = p.b_scales + static_cast<size_t>(min(pe * w_rows + wr, last_b)) * p.scale_pitch;
+                    for (int c = 0; c < p.scale_pitch; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
+                }
+            };
+            prefetch_tile(tile0);
             for (int tile = tile0; ok && w.locate(tile, e, nt, row0, rows); tile += tiles_step) {
+                prefetch_tile(tile + tiles_step);
                 const uint8_t* src[8];  // rows 32 j + lane of the tile, then weight rows 32 j + lane
                 bool live[8];
 #pragma unroll
@@ -220,30 +264,33 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                     live[4 + j] = t < width;
                     src[4 + j] = p.b_scales + static_cast<size_t>(min(e * w_rows + wr, last_b)) * p.scale_pitch;
                 }
-                for (int kb = 0; kb < p.kblocks; ++kb, ++it, r.next(ns)) {
+                for (int kb = 0; kb < nstages; ++kb, ++it, r.next(ns)) {
                     if ((it & 3u) != mine) continue;
                     const bool got = mbar_wait_bounded(&bar_empty[r.s], r.ph ^ 1u, abort_flag);
                     if (!__all_sync(0xFFFFFFFFu, got)) { ok = false; break; }
-                    uint8_t* slot = ring + r.s * static_cast<uint32_t>(p.stage_bytes) + a_bytes + b_bytes + lane * 16u;
+                    uint8_t* slot = ring + r.s * static_cast<uint32_t>(p.stage_bytes) + a_all + b_all + lane * 16u;
                     const uint32_t dst = smem_u32(slot);
+                    const int live_chunks = min(chunks, p.kblocks - kb * chunks);
+                    for (int c = 0; c < live_chunks; ++c) {
+                        const int word0 = (kb * chunks + c) * SFW;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        if (!live[j]) continue;
-                        const uint32_t d = dst + (j >> 2) * kNwSfBlock + fp4_scale_at<KIND>(j & 3);
-                        const uint8_t* from = src[j] + kb * SFW * 4;
-                        if (p.scale_vec) {
-                            copy_async<SFW * 4>(d, from, true);
-                        } else {
+                        for (int j = 0; j < 8; ++j) {
+                            if (!live[j]) continue;
+                            const uint32_t d = dst + static_cast<uint32_t>(c * 2 * kNwSfBlock) + (j >> 2) * kNwSfBlock + fp4_scale_at<KIND>(j & 3);
+                            const uint8_t* from = src[j] + word0 * 4;
+                            if (p.scale_vec) {
+                                copy_async<SFW * 4>(d, from, true);
+                            } else {
 #pragma unroll
-                            for (int i = 0; i < SFW; ++i) {
-                                const bool in = kb * SFW + i < words;
-                                copy_async<4>(d + i * 4u, in ? from + i * 4 : src[j], in);
+                                for (int i = 0; i < SFW; ++i) {
+                                    const bool in = word0 + i < words;
+                                    copy_async<4>(d + i * 4u, in ? from + i * 4 : src[j], in);
+                                }
                             }
                         }
                     }
                     asm volatile("cp.async.wait_all;" ::: "memory");
-                    fp4_transpose_scales<KIND>(slot);
-                    fp4_transpose_scales<KIND>(slot + kNwSfBlock);
+                    for (int c = 0; c < 2 * live_chunks; ++c) fp4_transpose_scales<KIND>(slot + c * kNwSfBlock);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bar_sf[r.s]);
@@ -278,6 +325,13 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             const uint32_t t0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 128u;
             const bool some = q * 32 < rows;  // the same in all lanes: no row of this quarter exists otherwise
             const int groups = (step + 31) / 32;  // groups of 32 result columns
+            bool held = true;
+            auto hand_back = [&]() {  // what this warp needs of the accumulator is in registers
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_tempty[b]);
+                held = false;
+            };
             for (int g = cg; some && g < groups; g += 2) {
                 __syncwarp();
                 const int c = nt * step + g * 32;
@@ -294,6 +348,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                         for (int j = 0; j < 16; ++j) v1[j] = v0[16 + j];
                     }
                 }
+                if (g + 2 >= groups) hand_back();
                 if (!valid) continue;
                 if constexpr (FP4 && SWIGLU) {
                     uint4 codes;
@@ -338,9 +393,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                     }
                 }
             }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar_tempty[b]);
+            if (held) hand_back();
         }
         if (!ok) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
         const int et = static_cast<int>(threadIdx.x) - EPI0 * 32;
@@ -365,7 +418,7 @@ namespace {
 // The MMA reads 128 rows of A from a stage whatever the stage has room for: behind a short one lie weights and scales, and behind
 // the last stage this padding.  What it reads there ends in accumulator rows that nobody reads.
 int narrow_smem(const cam::NarrowParams* p) {
-    const int over = cam::BM * 128 - p->stage_bytes;
+    const int over = (cam::BM - p->slot_rows) * 128 - (p->stage_bytes - p->slot_rows * 128 * p->chunks);  // from the last chunk's rows
     return cam::kNwCtrlBytes + p->stages * p->stage_bytes + (over > 0 ? over : 0);
 }
 
@@ -377,21 +430,29 @@ int launch_narrow(const cam::NarrowParams* p, int64_t tiles, const CUtensorMap* 
     if (err != cudaSuccess) return static_cast<int>(err);
     const int64_t sms = cam::sm_count_of_current_device();
     const unsigned grid = static_cast<unsigned>(tiles < 1 ? 1 : tiles < sms ? tiles : sms);
-    cam::expert_narrow_kernel<KIND, SWIGLU><<<grid, cam::narrow_threads(KIND), static_cast<size_t>(smem), stream>>>(*ta, *tb, *p);
-    return static_cast<int>(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1] = {cam::pdl_attribute()};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(static_cast<unsigned>(cam::narrow_threads(KIND)));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, cam::expert_narrow_kernel<KIND, SWIGLU>, *ta, *tb, *p));
 }
 
 }  // namespace
 
 extern "C" int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int swiglu, int64_t tiles, const CUtensorMap* ta,
                                              const CUtensorMap* tb, cudaStream_t stream) {
-    if (p->stages < 2 || p->stages > cam_expert_narrow_max_stages(kind) || narrow_smem(p) > 232448 || p->stage_bytes % 1024 != 0)
+    const int least = kind == cam::kNarrow16 ? 2 : cam::kNwScaleWarps;
+    if (p->chunks < 1 || p->stages < least || p->stages > cam_expert_narrow_max_stages(kind, p->chunks) || narrow_smem(p) > 232448 || p->stage_bytes % 1024 != 0)
         return static_cast<int>(cudaErrorInvalidValue);
     if (kind == cam::kFp4Nv) return swiglu ? launch_narrow<cam::kFp4Nv, true>(p, tiles, ta, tb, stream) : launch_narrow<cam::kFp4Nv, false>(p, tiles, ta, tb, stream);
     if (kind == cam::kFp4Mx) return swiglu ? launch_narrow<cam::kFp4Mx, true>(p, tiles, ta, tb, stream) : launch_narrow<cam::kFp4Mx, false>(p, tiles, ta, tb, stream);
     return swiglu ? launch_narrow<cam::kNarrow16, true>(p, tiles, ta, tb, stream) : launch_narrow<cam::kNarrow16, false>(p, tiles, ta, tb, stream);
 }
 
-extern "C" int cam_expert_narrow_max_stages(int kind) { return kind == cam::kNarrow16 ? cam::kNwMaxStages : cam::kNwMaxStagesFp4; }
+extern "C" int cam_expert_narrow_max_stages(int kind, int chunks) { return kind == cam::kNarrow16 ? cam::kNwMaxStages : cam::kNwScaleSlots / chunks; }
 
 extern "C" int cam_narrow_status(CamStatus* out) { return static_cast<int>(cudaMemcpyFromSymbol(out, cam::g_narrow_status, sizeof(CamStatus))); }

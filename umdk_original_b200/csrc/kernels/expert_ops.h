@@ -9,6 +9,21 @@
 
 namespace cam {
 
+// Programmatic dependent launch.  The kernels of these operators follow one another closely (quantise, gate and up, down; the
+// products of a backward pass), each takes microseconds, and the start of one (launch, barriers, tensor memory) can overlap the
+// end of the one before: a kernel waits for its predecessor's results only before its first access to memory (pdl_wait), and
+// allows its successor to start once it runs itself (pdl_release).
+#ifdef __CUDACC__
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+#endif
+inline cudaLaunchAttribute pdl_attribute() {
+    cudaLaunchAttribute a = {};
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    return a;
+}
+
 constexpr int kDtBf16 = 0, kDtFp16 = 1, kDtFp32 = 2;
 
 struct GroupedGemmFp4Params {
@@ -49,6 +64,8 @@ struct NarrowParams {
     int kblocks;                // 128-byte blocks of a row
     int width;                  // columns of the product per tile: 32 (not fp4), 64 or 128
     int slot_rows;              // rows of A a stage has room for: 32, 64 or 128 (at least the rows of any expert's tile)
+    int chunks;                 // K-blocks of a stage; 4-bit: stages * chunks <= 8
+    int chunked;                // the maps split rows into 128-byte K-blocks (rows of whole blocks only; needed for chunks > 1)
     int stages, stage_bytes;
     int fp16;
     void* out;                  // 16-bit [rows, n_dim], or fp4 SwiGLU: codes [rows, I/2]
@@ -79,11 +96,12 @@ int cam_launch_grouped_gemm_fp4(const cam::GroupedGemmFp4Params* p, int fmt, int
 // the second row operand in boxes of 64 rows.  All boxes are 128 bytes wide.
 int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, const CUtensorMap* tmap_a, const CUtensorMap* tmap_a32,
                            const CUtensorMap* tmap_b, cudaStream_t stream);
-// kind: kFp4Nv, kFp4Mx or kNarrow16.  tmap_a: rows in boxes of 32; tmap_b: weights [E, rows, bytes] in boxes of `width` rows, or
-// of width / 2 with SwiGLU.
+// kind: kFp4Nv, kFp4Mx or kNarrow16.  The maps, innermost first; with `chunked` a row is (K-block, 128 bytes), otherwise all of
+// its bytes and one K-block: tmap_a {bytes, rows, K-blocks} in boxes {128, slot_rows (32 without chunks), chunks}; tmap_b {bytes,
+// rows, halves, K-blocks, experts} in boxes {128, step, halves, chunks, 1} with SwiGLU's gate and up rows as two halves.
 int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int swiglu, int64_t tiles, const CUtensorMap* tmap_a,
                                   const CUtensorMap* tmap_b, cudaStream_t stream);
-int cam_expert_narrow_max_stages(int kind);
+int cam_expert_narrow_max_stages(int kind, int chunks);
 int cam_narrow_status(CamStatus* out);
 int cam_mlp_status(CamStatus* out);
 int cam_fp4_status(CamStatus* out);  // of the current device: the first wait that ran out in a kernel of that file

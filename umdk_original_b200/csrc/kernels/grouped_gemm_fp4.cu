@@ -127,6 +127,8 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     cluster_sync_all();  // both CTAs' barriers are initialised before anything signals them
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
+    pdl_wait();
+    pdl_release();
     PairTileWalker w(p.expert_offsets, p.num_experts, n_tiles, p.rows);
     int e, nt, row0, rows;
     bool ok = true;
@@ -203,6 +205,8 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     } else if (warp < kF4EpiWarp0) {
         reg_dealloc<kF4SfRegs>();
         // ---------------------------------------------------------------- scale warps: each takes every fourth K-block
+        // (a warp does not see every turn of a stage: at least as many stages as warps keep its waits by parity unambiguous)
+        static_assert(NS >= 4, "scale warps could run a whole turn ahead");
         const uint32_t mine = static_cast<uint32_t>(warp - kF4SfWarp0);
         const int pitch = p.k_dim / BLK;          // bytes of scales of a row
         const int words = pitch / 4;

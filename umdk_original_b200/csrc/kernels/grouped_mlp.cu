@@ -140,6 +140,8 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     cluster_sync_all();  // both CTAs' barriers are initialised before anything signals them
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
+    pdl_wait();
+    pdl_release();
     PairTileWalker wr(p.expert_offsets, p.num_experts, n_tiles, p.rows);
     const GradTileWalker wg(p.expert_offsets, p.num_experts, (p.m_dim + 255) / 256, n_tiles, p.rows);
     int e, mt = 0, nt, row0, rows;

@@ -43,12 +43,28 @@ __device__ __forceinline__ void widen(const Raw16<DT>& r, float (&f)[16]) {
     }
 }
 
+template <class Kernel, class... Args>
+int launch_flat(Kernel kernel, int64_t groups, cudaStream_t stream, Args... args) {
+    const int64_t per = kQThreads * kQPer, grid = (groups + per - 1) / per;
+    if (grid > 0x7FFFFFFF) return static_cast<int>(cudaErrorInvalidValue);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1] = {pdl_attribute()};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(kQThreads);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
 template <int FMT, int DT>
 __global__ void __launch_bounds__(kQThreads)
 quantize_fp4_kernel(const uint4* __restrict__ x, uint2* __restrict__ q, uint8_t* __restrict__ s, int64_t groups,
                     const float* __restrict__ gscale, int64_t groups_per_scale) {
     constexpr int V = DT == kDtFp32 ? 4 : 2;  // 16-byte loads of a group
     const int64_t base = static_cast<int64_t>(blockIdx.x) * (kQThreads * kQPer) + threadIdx.x;
+    pdl_wait();
+    pdl_release();
     Raw16<DT> r[kQPer];
 #pragma unroll
     for (int u = 0; u < kQPer; ++u) {
@@ -82,6 +98,8 @@ dequantize_fp4_kernel(const uint2* __restrict__ q, const uint8_t* __restrict__ s
                       const float* __restrict__ gscale, int64_t groups_per_scale) {
     constexpr int V = DT == kDtFp32 ? 4 : 2;
     const int64_t base = static_cast<int64_t>(blockIdx.x) * (kQThreads * kQPer) + threadIdx.x;
+    pdl_wait();
+    pdl_release();
     uint2 c[kQPer];
     uint32_t sc[kQPer];
 #pragma unroll
@@ -129,42 +147,22 @@ extern "C" int cam_launch_quantize_fp4(const void* x, int dtype, int fmt, void* 
                                        const float* gscale, int64_t groups_per_scale, cudaStream_t stream) {
     using namespace cam;
     if (groups <= 0) return 0;
-    const int64_t per = kQThreads * kQPer, grid = (groups + per - 1) / per;
-    if (grid > 0x7FFFFFFF) return static_cast<int>(cudaErrorInvalidValue);
     auto go = [&](auto kernel) {
-        kernel<<<static_cast<unsigned>(grid), kQThreads, 0, stream>>>(static_cast<const uint4*>(x), static_cast<uint2*>(q),
-                                                                      static_cast<uint8_t*>(s), groups, gscale, groups_per_scale);
+        return launch_flat(kernel, groups, stream, static_cast<const uint4*>(x), static_cast<uint2*>(q), static_cast<uint8_t*>(s), groups, gscale, groups_per_scale);
     };
-    if (fmt == kFp4Nv) {
-        if (dtype == kDtBf16) go(quantize_fp4_kernel<kFp4Nv, kDtBf16>);
-        else if (dtype == kDtFp16) go(quantize_fp4_kernel<kFp4Nv, kDtFp16>);
-        else go(quantize_fp4_kernel<kFp4Nv, kDtFp32>);
-    } else {
-        if (dtype == kDtBf16) go(quantize_fp4_kernel<kFp4Mx, kDtBf16>);
-        else if (dtype == kDtFp16) go(quantize_fp4_kernel<kFp4Mx, kDtFp16>);
-        else go(quantize_fp4_kernel<kFp4Mx, kDtFp32>);
-    }
-    return static_cast<int>(cudaGetLastError());
+    if (fmt == kFp4Nv)
+        return dtype == kDtBf16 ? go(quantize_fp4_kernel<kFp4Nv, kDtBf16>) : dtype == kDtFp16 ? go(quantize_fp4_kernel<kFp4Nv, kDtFp16>) : go(quantize_fp4_kernel<kFp4Nv, kDtFp32>);
+    return dtype == kDtBf16 ? go(quantize_fp4_kernel<kFp4Mx, kDtBf16>) : dtype == kDtFp16 ? go(quantize_fp4_kernel<kFp4Mx, kDtFp16>) : go(quantize_fp4_kernel<kFp4Mx, kDtFp32>);
 }
 
 extern "C" int cam_launch_dequantize_fp4(const void* q, const void* s, int dtype, int fmt, void* out, int64_t groups,
                                          const float* gscale, int64_t groups_per_scale, cudaStream_t stream) {
     using namespace cam;
     if (groups <= 0) return 0;
-    const int64_t per = kQThreads * kQPer, grid = (groups + per - 1) / per;
-    if (grid > 0x7FFFFFFF) return static_cast<int>(cudaErrorInvalidValue);
     auto go = [&](auto kernel) {
-        kernel<<<static_cast<unsigned>(grid), kQThreads, 0, stream>>>(static_cast<const uint2*>(q), static_cast<const uint8_t*>(s),
-                                                                      static_cast<uint4*>(out), groups, gscale, groups_per_scale);
+        return launch_flat(kernel, groups, stream, static_cast<const uint2*>(q), static_cast<const uint8_t*>(s), static_cast<uint4*>(out), groups, gscale, groups_per_scale);
     };
-    if (fmt == kFp4Nv) {
-        if (dtype == kDtBf16) go(dequantize_fp4_kernel<kFp4Nv, kDtBf16>);
-        else if (dtype == kDtFp16) go(dequantize_fp4_kernel<kFp4Nv, kDtFp16>);
-        else go(dequantize_fp4_kernel<kFp4Nv, kDtFp32>);
-    } else {
-        if (dtype == kDtBf16) go(dequantize_fp4_kernel<kFp4Mx, kDtBf16>);
-        else if (dtype == kDtFp16) go(dequantize_fp4_kernel<kFp4Mx, kDtFp16>);
-        else go(dequantize_fp4_kernel<kFp4Mx, kDtFp32>);
-    }
-    return static_cast<int>(cudaGetLastError());
+    if (fmt == kFp4Nv)
+        return dtype == kDtBf16 ? go(dequantize_fp4_kernel<kFp4Nv, kDtBf16>) : dtype == kDtFp16 ? go(dequantize_fp4_kernel<kFp4Nv, kDtFp16>) : go(dequantize_fp4_kernel<kFp4Nv, kDtFp32>);
+    return dtype == kDtBf16 ? go(dequantize_fp4_kernel<kFp4Mx, kDtBf16>) : dtype == kDtFp16 ? go(dequantize_fp4_kernel<kFp4Mx, kDtFp16>) : go(dequantize_fp4_kernel<kFp4Mx, kDtFp32>);
 }

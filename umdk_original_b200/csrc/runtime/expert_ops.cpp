@@ -57,8 +57,9 @@ bool narrow_pays(int rows, int num_experts) {
     return static_cast<int64_t>(rows) <= 128ll * num_experts;
 }
 
-// Tile width, stages and number of tiles of the one-CTA form for `n` result columns.
-void narrow_plan(cam::NarrowParams* p, int kind, bool swiglu, int64_t* tiles) {
+// The one-CTA form: tile width, stages, maps, launch.  `row_bytes` of the row operand and of the weights' rows; n_dim, the
+// operands' scales and outputs are set.
+int launch_narrow(cam::NarrowParams* p, int kind, bool swiglu, const void* a, const void* w, int row_bytes, const char* what, cudaStream_t stream) {
     const bool fp4 = kind != cam::kNarrow16;
     const int sms = cam::sm_count_of_current_device();
     const int64_t blocks = p->rows <= p->num_experts ? p->rows
@@ -77,12 +78,26 @@ void narrow_plan(cam::NarrowParams* p, int kind, bool swiglu, int64_t* tiles) {
     }
     const int step = swiglu ? p->width / 2 : p->width;
     const int64_t upper = p->rows / 128 + (p->rows < p->num_experts ? p->rows : p->num_experts);  // row blocks there can be
-    *tiles = upper * ((p->n_dim + step - 1) / step);
+    p->kblocks = (row_bytes + 127) / 128;
+    p->chunked = row_bytes % 128 == 0;
     p->slot_rows = p->rows <= 32 ? 32 : p->rows <= 64 ? 64 : 128;
-    p->stage_bytes = (p->slot_rows + p->width) * 128 + (fp4 ? 4096 : 0);
-    const int pad = p->stage_bytes < 16384 ? 16384 - p->stage_bytes : 0;
-    const int fit = (232448 - 1024 - pad) / p->stage_bytes, most = cam_expert_narrow_max_stages(kind);
+    // 16 KiB of weights in a stage, as long as four stages fit (4-bit needs as many as it has scale warps)
+    const int per_chunk = (p->slot_rows + p->width) * 128 + (fp4 ? 4096 : 0);
+    p->chunks = p->chunked ? 128 / p->width : 1;
+    while (p->chunks > 1 && (4 * p->chunks * per_chunk > 232448 - 1024 - 16384 || p->chunks > p->kblocks)) p->chunks /= 2;
+    p->stage_bytes = p->chunks * per_chunk;
+    const int fit = (232448 - 1024 - 16384) / p->stage_bytes, most = cam_expert_narrow_max_stages(kind, p->chunks);
     p->stages = fit < most ? fit : most;
+    const uint64_t bytes = p->chunked ? 128 : static_cast<uint64_t>(row_bytes), blocks_k = p->chunked ? static_cast<uint64_t>(p->kblocks) : 1;
+    const uint64_t pitch = static_cast<uint64_t>(row_bytes), halves = swiglu ? 2 : 1, n = static_cast<uint64_t>(p->n_dim);
+    CUtensorMap ta, tb;
+    const uint64_t da[3] = {bytes, static_cast<uint64_t>(p->rows), blocks_k}, sa[2] = {pitch, 128};
+    const uint32_t ba[3] = {128, p->chunks > 1 ? static_cast<uint32_t>(p->slot_rows) : 32u, static_cast<uint32_t>(p->chunks)};
+    if (cam_encode_tmap(&ta, a, 3, da, sa, ba) != 0) return -1;
+    const uint64_t db[5] = {bytes, n, halves, blocks_k, static_cast<uint64_t>(p->num_experts)}, sb[4] = {pitch, pitch * n, 128, pitch * n * halves};
+    const uint32_t bb[5] = {128, static_cast<uint32_t>(step), static_cast<uint32_t>(halves), static_cast<uint32_t>(p->chunks), 1};
+    if (cam_encode_tmap(&tb, w, 5, db, sb, bb) != 0) return -1;
+    return launched(cam_launch_expert_gemm_narrow(p, kind, swiglu, upper * ((p->n_dim + step - 1) / step), &ta, &tb, stream), what);
 }
 
 }  // namespace
@@ -124,7 +139,6 @@ extern "C" int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, 
         p.num_experts = num_experts;
         p.rows = rows;
         p.n_dim = swiglu ? n_dim / 2 : n_dim;
-        p.kblocks = (k_dim + 255) / 256;
         p.out = out;
         p.a_scales = static_cast<const uint8_t*>(a_s);
         p.b_scales = static_cast<const uint8_t*>(w_s);
@@ -134,14 +148,7 @@ extern "C" int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, 
         p.b_gscale = w_gscale;
         p.out_gscale = out_gscale;
         p.out_scales = static_cast<uint8_t*>(out_s);
-        int64_t tiles = 0;
-        narrow_plan(&p, fmt, swiglu != 0, &tiles);
-        CUtensorMap ta, tb;
-        if (map_2d(&ta, a_q, static_cast<uint64_t>(k_dim) / 2, static_cast<uint64_t>(rows), 32) != 0) return -1;
-        if (map_3d(&tb, w_q, static_cast<uint64_t>(k_dim) / 2, static_cast<uint64_t>(n_dim), static_cast<uint64_t>(num_experts),
-                   static_cast<uint32_t>(swiglu ? p.width / 2 : p.width)) != 0)
-            return -1;
-        return launched(cam_launch_expert_gemm_narrow(&p, fmt, swiglu, tiles, &ta, &tb, stream), "grouped_gemm_fp4");
+        return launch_narrow(&p, fmt, swiglu != 0, a_q, w_q, k_dim / 2, "grouped_gemm_fp4", stream);
     }
     cam::GroupedGemmFp4Params p{};
     p.expert_offsets = offsets;
@@ -180,18 +187,10 @@ int row_product(int form, const char* what, const void* a, int k, const void* w,
         p.num_experts = num_experts;
         p.rows = rows;
         p.n_dim = n;
-        p.kblocks = (k + 63) / 64;
         p.fp16 = dtype == 1;
         p.out = out;
         p.gate_up = gate_up;
-        int64_t tiles = 0;
-        narrow_plan(&p, cam::kNarrow16, swiglu, &tiles);
-        CUtensorMap ta, tb;
-        if (map_2d(&ta, a, static_cast<uint64_t>(k) * 2, static_cast<uint64_t>(rows), 32) != 0) return -1;
-        if (map_3d(&tb, w, static_cast<uint64_t>(w_cols) * 2, static_cast<uint64_t>(w_rows), static_cast<uint64_t>(num_experts),
-                   static_cast<uint32_t>(swiglu ? p.width / 2 : p.width)) != 0)
-            return -1;
-        return launched(cam_launch_expert_gemm_narrow(&p, cam::kNarrow16, swiglu, tiles, &ta, &tb, stream), what);
+        return launch_narrow(&p, cam::kNarrow16, swiglu, a, w, k * 2, what, stream);
     }
     cam::GroupedMlpParams p{};
     p.expert_offsets = offsets;
