@@ -52,6 +52,13 @@ __device__ __forceinline__ void mbar_wait_warp(uint32_t bar, uint32_t parity, ui
         "}\n" ::"r"(bar), "r"(parity), "r"(abort), "n"(kWaitPolls)
         : "memory");
 }
+// Arrive on the barrier at this shared-memory offset in BOTH CTAs of the pair once every MMA issued so far by this thread has
+// completed: one instruction instead of two.
+__device__ __forceinline__ void tc_commit_both(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
+}
 // Position in a ring of stages: stage and the parity of its current turn
 struct Ring {
     uint32_t s = 0, ph = 0;
@@ -186,6 +193,10 @@ __device__ __forceinline__ uint32_t fp4_scale_at(int j) {
     return FMT == kFp4Nv ? static_cast<uint32_t>(j) * 512u : static_cast<uint32_t>(j >> 1) * 512u + static_cast<uint32_t>(j & 1) * 8u;
 }
 
+// 1 / (1 + e^-x) from the fast exponential and division: a few units of 2^-22 of the result for |x| up to 16 (the products it
+// enters carry more), 0 where e^-x overflows.
+__device__ __forceinline__ float sigmoid_fast(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
 // silu(gate) * up of 32 columns, then scales (two blocks of 16 or one of 32) and codes; `gate` and `up` are raw accumulators.
 template <int FMT>
 __device__ __forceinline__ void fp4_swiglu32(const uint32_t* gate, const uint32_t* up, float alpha, float out_g, uint4& codes, uint32_t& scales) {
@@ -193,7 +204,7 @@ __device__ __forceinline__ void fp4_swiglu32(const uint32_t* gate, const uint32_
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
         const float g = __uint_as_float(gate[j]) * alpha;
-        act[j] = (g / (1.f + expf(-g))) * (__uint_as_float(up[j]) * alpha);
+        act[j] = g * sigmoid_fast(g) * (__uint_as_float(up[j]) * alpha);
     }
     uint32_t amax[2] = {0u, 0u};
 #pragma unroll
@@ -209,6 +220,14 @@ __device__ __forceinline__ void fp4_swiglu32(const uint32_t* gate, const uint32_
     }
     codes = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
     scales = sc[0] | (sc[1] << 8);
+}
+
+// Where the fp32 gate and up values of a row lie in the tensor that the forward pass keeps for the backward pass.  The rows of an
+// expert form groups of 32 (the last one of `n` < 32): a group's 2 I n values are [gate, up][32 columns][4 columns][row][4], so
+// that a warp with a row per lane writes and reads whole lines.  Returns the place of column `col` (a multiple of 32) of the
+// gate; four columns on are 4 n floats further, the up values I n floats.
+__device__ __forceinline__ size_t gate_up_at(size_t group_row, int n, int row_in_group, int inter, int col) {
+    return group_row * (2 * static_cast<size_t>(inter)) + static_cast<size_t>(col) * n + row_in_group * 4;
 }
 
 __device__ __forceinline__ uint32_t pack16(float a, float b, bool fp16) {

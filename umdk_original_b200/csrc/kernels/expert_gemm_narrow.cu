@@ -364,19 +364,22 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                     const int cols = min(min(32, step), p.n_dim - c);  // a multiple of 8
                     if constexpr (SWIGLU) {
                         if (p.gate_up != nullptr) {
-                            float* gu = p.gate_up + grow * (2 * static_cast<size_t>(p.n_dim)) + c;
+                            const int in_group = min(32, rows - q * 32);
+                            // columns c.. are 32-aligned, or half of such a block (width 32)
+                            float* gu = p.gate_up + gate_up_at(static_cast<size_t>(row0 + q * 32), in_group, static_cast<int>(lane), p.n_dim, c & ~31) + (c & 31) * in_group;
+                            const size_t up = static_cast<size_t>(p.n_dim) * in_group;
 #pragma unroll
                             for (int j = 0; j < 32; j += 4) {
                                 if (j < cols) {
-                                    *reinterpret_cast<uint4*>(gu + j) = make_uint4(v0[j], v0[j + 1], v0[j + 2], v0[j + 3]);
-                                    *reinterpret_cast<uint4*>(gu + p.n_dim + j) = make_uint4(v1[j], v1[j + 1], v1[j + 2], v1[j + 3]);
+                                    *reinterpret_cast<uint4*>(gu + j * in_group) = make_uint4(v0[j], v0[j + 1], v0[j + 2], v0[j + 3]);
+                                    *reinterpret_cast<uint4*>(gu + up + j * in_group) = make_uint4(v1[j], v1[j + 1], v1[j + 2], v1[j + 3]);
                                 }
                             }
                         }
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
                             const float x = __uint_as_float(v0[j]);
-                            v0[j] = __float_as_uint((x / (1.f + expf(-x))) * __uint_as_float(v1[j]));
+                            v0[j] = __float_as_uint(x * sigmoid_fast(x) * __uint_as_float(v1[j]));
                         }
                     }
                     uint8_t* out = static_cast<uint8_t*>(p.out) + (grow * p.n_dim + c) * 2;

@@ -52,7 +52,7 @@ struct GroupedMlpParams {
     int k_dim;                  // contraction (not kMlpDw)
     int fp16;                   // operands and results are fp16, otherwise bf16
     void* out;                  // [rows, n_dim]; kMlpDact: dgu [rows, 2 n_dim]; kMlpDw: [E, m_dim, n_dim]
-    float* gate_up;             // [rows, 2I] fp32: written by kMlpUp (or null), read by kMlpDact
+    float* gate_up;             // rows x 2I fp32 in the order of gate_up_at (expert_gemm.cuh): written by kMlpUp (or null), read by kMlpDact
 };
 
 // One-CTA form of the row products for experts with few rows (expert_gemm_narrow.cu): tiles of 128 rows x `width` columns.
@@ -69,7 +69,7 @@ struct NarrowParams {
     int stages, stage_bytes;
     int fp16;
     void* out;                  // 16-bit [rows, n_dim], or fp4 SwiGLU: codes [rows, I/2]
-    float* gate_up;             // 16-bit SwiGLU: null or fp32 [rows, 2I]
+    float* gate_up;             // 16-bit SwiGLU: null or fp32, see GroupedMlpParams
     // fp4
     const uint8_t *a_scales, *b_scales;
     int scale_pitch, scale_vec;

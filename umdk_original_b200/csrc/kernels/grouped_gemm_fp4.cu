@@ -137,70 +137,88 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
 
     if (warp < kF4SfWarp0) {
         reg_dealloc<kF4CtrlRegs>();
-        if (warp == 0 && lane == 0) {
+        const uint32_t abort_at = smem_u32(tmem_slot + 1);
+        const uint32_t full_at = smem_u32(bar_full), sf_at = smem_u32(bar_sf), empty_at = smem_u32(bar_empty);
+        if (warp == 0) {
             // ------------------------------------------------------------ TMA producer (both CTAs)
-            prefetch_tensormap(&tmap_a);
-            prefetch_tensormap(&tmap_a32);
-            prefetch_tensormap(&tmap_b);
-            uint32_t it = 0;
+            const bool leader = elect_one();
+            if (leader) {
+                prefetch_tensormap(&tmap_a);
+                prefetch_tensormap(&tmap_a32);
+                prefetch_tensormap(&tmap_b);
+            }
+            Ring ring;
+            uint32_t ready = 1u;  // the first turn of every stage is free
+            const uint32_t full0 = map_to_cta(bar_full, 0);
             // Only 32-row pieces of A that hold rows are loaded; what stays in the other rows of the stage reaches
             // accumulator rows that nobody reads.
             auto pieces = [](int r) { return r > 96 ? 4 : r > 0 ? (r + 31) / 32 : 0; };
-            for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows); tile += num_pairs) {
+            for (int tile = pair_id; w.locate(tile, e, nt, row0, rows); tile += num_pairs) {
                 const int p0 = pieces(min(rows, BM)), p1 = pieces(rows - BM);
                 const int mine = cta ? p1 : p0;
                 const uint32_t bytes = 2u * kF4Tile + static_cast<uint32_t>(p0 + p1) * 4096u;
                 const int arow = row0 + static_cast<int>(cta) * BM, brow = b_row(static_cast<int>(cta));
-                for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                    const uint32_t s = it % NS, ph = (it / NS) & 1u;
-                    if (!mbar_wait_bounded(&bar_empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
-                    uint8_t* sa = smem + s * kF4StageBytes;
-                    if (cta == 0) mbar_arrive_expect_tx(&bar_full[s], bytes);
-                    const uint32_t full0 = map_to_cta(&bar_full[s], 0);
-                    tma_load_2d_pair(sa + kF4Tile, &tmap_b, full0, kb * 128, brow);
-                    if (mine == 4) tma_load_2d_pair(sa, &tmap_a, full0, kb * 128, arow);
-                    else for (int i = 0; i < mine; ++i) tma_load_2d_pair(sa + i * 4096, &tmap_a32, full0, kb * 128, arow + i * 32);
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    const uint32_t s = ring.s;
+                    if (!ready) mbar_wait_warp(empty_at + 8u * s, ring.ph ^ 1u, abort_at);
+                    ring.next(NS);
+                    ready = mbar_test(empty_at + 8u * ring.s, ring.ph ^ 1u);
+                    if (leader) {
+                        uint8_t* sa = smem + s * kF4StageBytes;
+                        const uint32_t bar = full0 + 8u * s;
+                        if (cta == 0) mbar_arrive_expect_tx(&bar_full[s], bytes);
+                        tma_load_2d_pair(sa + kF4Tile, &tmap_b, bar, kb * 128, brow);
+                        if (mine == 4) tma_load_2d_pair(sa, &tmap_a, bar, kb * 128, arow);
+                        else for (int i = 0; i < mine; ++i) tma_load_2d_pair(sa + i * 4096, &tmap_a32, bar, kb * 128, arow + i * 32);
+                    }
+                    __syncwarp();
                 }
             }
-            if (!ok) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 0, static_cast<int>(it));
-        } else if (warp == 1 && lane == 0 && cta == 0) {
+            if (leader && *abort_flag) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 0, 0);
+        } else if (warp == 1 && cta == 0) {
             // ------------------------------------------------------------ MMA issuer (first CTA only)
-            uint32_t it = 0, tcount = 0;
-            const uint32_t tfull0 = map_to_cta(bar_tfull, 0), tfull1 = map_to_cta(bar_tfull, 1);
-            for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
+            const bool leader = elect_one();
+            Ring ring;
+            uint32_t tcount = 0, ready = 0u;
+            for (int tile = pair_id; w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
                 // both epilogues must have drained the previous tile before its columns are overwritten
-                if (!mbar_wait_bounded(bar_tempty, (tcount & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                mbar_wait_warp(smem_u32(bar_tempty), (tcount & 1u) ^ 1u, abort_at);
                 tc_fence_after_sync();
-                for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                    const uint32_t s = it % NS, ph = (it / NS) & 1u;
-                    if (!mbar_wait_bounded(&bar_sf[s], ph, abort_flag)) { ok = false; break; }
-                    if (!mbar_wait_bounded(&bar_full[s], ph, abort_flag)) { ok = false; break; }
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    const uint32_t s = ring.s;
+                    if (!ready) {
+                        mbar_wait_warp(sf_at + 8u * s, ring.ph, abort_at);
+                        mbar_wait_warp(full_at + 8u * s, ring.ph, abort_at);
+                    }
                     tc_fence_after_sync();
-                    const uint32_t sa = smem_u32(smem + s * kF4StageBytes);
+                    ring.next(NS);
+                    ready = mbar_test(full_at + 8u * ring.s, ring.ph) & mbar_test(sf_at + 8u * ring.s, ring.ph);
+                    const uint32_t sa = smem_u32(smem) + s * kF4StageBytes;
                     const uint64_t adesc = umma_desc_k_sw128(sa), bdesc = umma_desc_k_sw128(sa + kF4Tile);
-                    const uint32_t sfs = smem_u32(sfm + s * kF4SfStage);
+                    const uint32_t sfs = smem_u32(sfm) + s * kF4SfStage;
                     const uint32_t sf = tmem_base + kF4SfCol0 + s * kF4SfCols;  // SFW x (4 columns of A, 8 of B)
+                    if (leader) {
 #pragma unroll
-                    for (int k = 0; k < SFW; ++k) {
-                        tc_copy_scales_pair(sf + 12u * k, desc_scales(sfs + k * 512));
-                        tc_copy_scales_pair(sf + 12u * k + 4u, desc_scales(sfs + kF4SfBlock + k * 512));
-                        tc_copy_scales_pair(sf + 12u * k + 8u, desc_scales(sfs + 2 * kF4SfBlock + k * 512));
-                    }
+                        for (int k = 0; k < SFW; ++k) {
+                            tc_copy_scales_pair(sf + 12u * k, desc_scales(sfs + k * 512));
+                            tc_copy_scales_pair(sf + 12u * k + 4u, desc_scales(sfs + kF4SfBlock + k * 512));
+                            tc_copy_scales_pair(sf + 12u * k + 8u, desc_scales(sfs + 2 * kF4SfBlock + k * 512));
+                        }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {  // 64 values = 32 bytes (2 x 16) further along K inside the swizzle atom
-                        const uint32_t c = sf + 12u * (FMT == kFp4Nv ? k : k >> 1);
-                        tc_mma_fp4_pair<FMT>(tmem_base, adesc + 2u * k, bdesc + 2u * k,
-                                             idesc_fp4<FMT>(2 * BM, 256, FMT == kFp4Nv ? 0u : 2u * (k & 1)), (kb | k) ? 1u : 0u, c, c + 4u);
+                        for (int k = 0; k < 4; ++k) {  // 64 values = 32 bytes (2 x 16) further along K inside the swizzle atom
+                            const uint32_t c = sf + 12u * (FMT == kFp4Nv ? k : k >> 1);
+                            tc_mma_fp4_pair<FMT>(tmem_base, adesc + 2u * k, bdesc + 2u * k,
+                                                 idesc_fp4<FMT>(2 * BM, 256, FMT == kFp4Nv ? 0u : 2u * (k & 1)), (kb | k) ? 1u : 0u, c, c + 4u);
+                        }
+                        // the stage and its scale slot, in both CTAs, are reusable once these have retired
+                        tc_commit_both(empty_at + 8u * s);
                     }
-                    // the stage and its scale slot, in both CTAs, are reusable once these have retired
-                    tc_commit_pair(map_to_cta(&bar_empty[s], 0));
-                    tc_commit_pair(map_to_cta(&bar_empty[s], 1));
+                    __syncwarp();
                 }
-                if (!ok) break;
-                tc_commit_pair(tfull0);
-                tc_commit_pair(tfull1);
+                if (leader) tc_commit_both(smem_u32(bar_tfull));
+                __syncwarp();
             }
-            if (!ok) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(it));
+            if (leader && *abort_flag) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
         }
     } else if (warp < kF4EpiWarp0) {
         reg_dealloc<kF4SfRegs>();

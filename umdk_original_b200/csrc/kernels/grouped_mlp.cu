@@ -68,6 +68,11 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr) {
            (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 
+__device__ __forceinline__ float4 ld_nc_f4(const float* p) {
+    const uint4 v = ld_nc_v4(p);
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+
 // Tiles of the weight gradients: 256 x 256 of every expert's [m_dim, n_dim]; `rows` are the rows summed over.
 struct GradTileWalker {
     const int* off;
@@ -151,84 +156,101 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 
     if (warp < kEmEpiWarp0) {
         reg_dealloc<kEmCtrlRegs>();
-        if (warp == 0 && lane == 0) {
+        const uint32_t abort_at = smem_u32(tmem_slot + 1);
+        const uint32_t full_at = smem_u32(bar_full), empty_at = smem_u32(bar_empty);
+        if (warp == 0) {
             // ------------------------------------------------------------ TMA producer (both CTAs)
-            prefetch_tensormap(&tmap_a);
-            prefetch_tensormap(&tmap_a32);
-            prefetch_tensormap(&tmap_b);
-            uint32_t it = 0;
+            const bool leader = elect_one();
+            if (leader) {
+                prefetch_tensormap(&tmap_a);
+                prefetch_tensormap(&tmap_a32);
+                prefetch_tensormap(&tmap_b);
+            }
+            Ring ring;
+            uint32_t ready = 1u;  // the first turn of every stage is free
+            const uint32_t full0 = map_to_cta(bar_full, 0), tail_own = map_to_cta(bar_tail, cta);
             // row forms: only 32-row pieces of A that hold rows are loaded; what stays in the other rows of the stage reaches
             // accumulator rows that nobody reads
             auto pieces = [](int r) { return r > 96 ? 4 : r > 0 ? (r + 31) / 32 : 0; };
-            for (int tile = pair_id; ok && locate(tile); tile += num_pairs) {
+            for (int tile = pair_id; locate(tile); tile += num_pairs) {
                 const int kblocks = kblocks_of();
                 const int p0 = pieces(min(rows, BM)), p1 = pieces(rows - BM), mine = cta ? p1 : p0;
                 const uint32_t bytes = WGRAD ? 2u * kEmStageBytes : 2u * kEmTile + static_cast<uint32_t>(p0 + p1) * 4096u;
                 const int half = static_cast<int>(cta);
-                for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                    const uint32_t s = it % NS, ph = (it / NS) & 1u;
-                    if (!mbar_wait_bounded(&bar_empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
-                    uint8_t* sa = smem + s * kEmStageBytes;
-                    uint8_t* sb = sa + kEmTile;
-                    uint32_t bar = map_to_cta(&bar_full[s], 0);
-                    if (WGRAD && kb == kblocks - 1 && (rows & 63) != 0) {
-                        bar = map_to_cta(&bar_tail[s], cta);
-                        mbar_arrive_expect_tx(&bar_tail[s], kEmStageBytes);
-                    } else if (cta == 0) {
-                        mbar_arrive_expect_tx(&bar_full[s], bytes);
-                    } else if (WGRAD) {
-                        mbar_arrive_cluster(bar);
-                    }
-                    if constexpr (WGRAD) {
-                        const int r = row0 + kb * 64, ca = (mt * 256 + half * 128) * 2, cb = (nt * 256 + half * 128) * 2;
-                        tma_load_2d_pair(sa, &tmap_a, bar, ca, r);
-                        tma_load_2d_pair(sa + 8192, &tmap_a, bar, ca + 128, r);
-                        tma_load_2d_pair(sb, &tmap_b, bar, cb, r);
-                        tma_load_2d_pair(sb + 8192, &tmap_b, bar, cb + 128, r);
-                    } else {
-                        if constexpr (B_MN) {
-                            const int cb = (nt * 256 + half * 128) * 2;
-                            tma_load_3d_pair(sb, &tmap_b, bar, cb, kb * 64, e);
-                            tma_load_3d_pair(sb + 8192, &tmap_b, bar, cb + 128, kb * 64, e);
-                        } else {
-                            tma_load_3d_pair(sb, &tmap_b, bar, kb * 128, SWIGLU ? half * p.n_dim + nt * 128 : nt * 256 + half * 128, e);
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    const uint32_t s = ring.s;
+                    if (!ready) mbar_wait_warp(empty_at + 8u * s, ring.ph ^ 1u, abort_at);
+                    ring.next(NS);
+                    ready = mbar_test(empty_at + 8u * ring.s, ring.ph ^ 1u);
+                    if (leader) {
+                        uint8_t* sa = smem + s * kEmStageBytes;
+                        uint8_t* sb = sa + kEmTile;
+                        uint32_t bar = full0 + 8u * s;
+                        if (WGRAD && kb == kblocks - 1 && (rows & 63) != 0) {
+                            bar = tail_own + 8u * s;
+                            mbar_arrive_expect_tx(&bar_tail[s], kEmStageBytes);
+                        } else if (cta == 0) {
+                            mbar_arrive_expect_tx(&bar_full[s], bytes);
+                        } else if (WGRAD) {
+                            mbar_arrive_cluster(bar);
                         }
-                        const int arow = row0 + half * BM;
-                        if (mine == 4) tma_load_2d_pair(sa, &tmap_a, bar, kb * 128, arow);
-                        else for (int i = 0; i < mine; ++i) tma_load_2d_pair(sa + i * 4096, &tmap_a32, bar, kb * 128, arow + i * 32);
+                        if constexpr (WGRAD) {
+                            const int r = row0 + kb * 64, ca = (mt * 256 + half * 128) * 2, cb = (nt * 256 + half * 128) * 2;
+                            tma_load_2d_pair(sa, &tmap_a, bar, ca, r);
+                            tma_load_2d_pair(sa + 8192, &tmap_a, bar, ca + 128, r);
+                            tma_load_2d_pair(sb, &tmap_b, bar, cb, r);
+                            tma_load_2d_pair(sb + 8192, &tmap_b, bar, cb + 128, r);
+                        } else {
+                            if constexpr (B_MN) {
+                                const int cb = (nt * 256 + half * 128) * 2;
+                                tma_load_3d_pair(sb, &tmap_b, bar, cb, kb * 64, e);
+                                tma_load_3d_pair(sb + 8192, &tmap_b, bar, cb + 128, kb * 64, e);
+                            } else {
+                                tma_load_3d_pair(sb, &tmap_b, bar, kb * 128, SWIGLU ? half * p.n_dim + nt * 128 : nt * 256 + half * 128, e);
+                            }
+                            const int arow = row0 + half * BM;
+                            if (mine == 4) tma_load_2d_pair(sa, &tmap_a, bar, kb * 128, arow);
+                            else for (int i = 0; i < mine; ++i) tma_load_2d_pair(sa + i * 4096, &tmap_a32, bar, kb * 128, arow + i * 32);
+                        }
                     }
+                    __syncwarp();
                 }
             }
-            if (!ok) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 0, static_cast<int>(it));
-        } else if (warp == 1 && lane == 0 && cta == 0) {
+            if (leader && *abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 0, 0);
+        } else if (warp == 1 && cta == 0) {
             // ------------------------------------------------------------ MMA issuer (first CTA only)
+            const bool leader = elect_one();
             // fp32 accumulator; a_major / b_major (bits 15, 16) = 1 for MN-major operands
             const uint32_t idesc = umma_idesc(2 * BM, 256, 1u, p.fp16 ? 0u : 1u) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
-            uint32_t it = 0, tcount = 0;
-            for (int tile = pair_id; ok && locate(tile); tile += num_pairs, ++tcount) {
+            Ring ring;
+            uint32_t tcount = 0, ready = 0u;
+            for (int tile = pair_id; locate(tile); tile += num_pairs, ++tcount) {
                 const int kblocks = kblocks_of();
                 const uint32_t b = tcount & 1u;
                 // both epilogues must have drained this accumulator's previous tile
-                if (!mbar_wait_bounded(&bar_tempty[b], ((tcount >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                mbar_wait_warp(smem_u32(&bar_tempty[b]), ((tcount >> 1) & 1u) ^ 1u, abort_at);
                 tc_fence_after_sync();
-                for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                    const uint32_t s = it % NS, ph = (it / NS) & 1u;
-                    if (!mbar_wait_bounded(&bar_full[s], ph, abort_flag)) { ok = false; break; }
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    const uint32_t s = ring.s;
+                    if (!ready) mbar_wait_warp(full_at + 8u * s, ring.ph, abort_at);
                     tc_fence_after_sync();
-                    const uint32_t sa = smem_u32(smem + s * kEmStageBytes);
+                    ring.next(NS);
+                    ready = mbar_test(full_at + 8u * ring.s, ring.ph);
+                    const uint32_t sa = smem_u32(smem) + s * kEmStageBytes;
                     const uint64_t adesc = A_MN ? umma_desc_mn_sw128(sa) : umma_desc_k_sw128(sa);
                     const uint64_t bdesc = B_MN ? umma_desc_mn_sw128(sa + kEmTile) : umma_desc_k_sw128(sa + kEmTile);
+                    if (leader) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)  // 16 of the contraction: 32 bytes of a row, or 16 rows of 128 bytes
-                        tc_mma_16_pair(tmem_base + b * 256u, adesc + (A_MN ? 128u : 2u) * k, bdesc + (B_MN ? 128u : 2u) * k, idesc, (kb | k) ? 1u : 0u);
-                    tc_commit_pair(map_to_cta(&bar_empty[s], 0));
-                    tc_commit_pair(map_to_cta(&bar_empty[s], 1));
+                        for (int k = 0; k < 4; ++k)  // 16 of the contraction: 32 bytes of a row, or 16 rows of 128 bytes
+                            tc_mma_16_pair(tmem_base + b * 256u, adesc + (A_MN ? 128u : 2u) * k, bdesc + (B_MN ? 128u : 2u) * k, idesc, (kb | k) ? 1u : 0u);
+                        tc_commit_both(empty_at + 8u * s);
+                    }
+                    __syncwarp();
                 }
-                if (!ok) break;
-                tc_commit_pair(map_to_cta(&bar_tfull[b], 0));
-                tc_commit_pair(map_to_cta(&bar_tfull[b], 1));
+                if (leader) tc_commit_both(smem_u32(&bar_tfull[b]));
+                __syncwarp();
             }
-            if (!ok) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(it));
+            if (leader && *abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
         } else if (WGRAD && warp == 2) {
             // ------------------------------------------------------------ zeros behind the last row (both CTAs)
             uint32_t it = 0, phases = 0;  // bit s: parity of stage s's next ragged block
@@ -284,73 +306,117 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             const bool valid = first + r < (WGRAD ? p.m_dim : rows);
             const size_t orow_i = WGRAD ? static_cast<size_t>(e) * p.m_dim + first + r : static_cast<size_t>(row0 + first + r);
             const bool empty = WGRAD && rows == 0;
+            if constexpr (DSWIGLU) {
+                // this tile's gate and up come from memory while its MMAs run: a line per lane of each block of 32 rows x 32 columns
+                const int left = rows - (first + q * 32);
+                if (left > 0) {
+                    const int n = min(32, left);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int c = nt * 256 + h * 128 + cq * 32;
+                        const float* gu = p.gate_up + gate_up_at(static_cast<size_t>(row0 + first + q * 32), n, 0, p.n_dim, c);
+                        if (static_cast<int>(lane) < n && c + 32 <= p.n_dim) {
+                            asm volatile("prefetch.global.L2 [%0];" ::"l"(gu + lane * 32u));
+                            asm volatile("prefetch.global.L2 [%0];" ::"l"(gu + static_cast<size_t>(p.n_dim) * n + lane * 32u));
+                        }
+                    }
+                }
+            }
+            const uint32_t t0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 256u + cq * 32;
+            auto hand_back = [&]() {  // what this warp needs of the accumulator is in registers
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if (cta == 0) mbar_arrive(&bar_tempty[b]);
+                    else mbar_arrive_cluster(map_to_cta(&bar_tempty[b], 0));
+                }
+            };
+            if constexpr (DSWIGLU) {
+                // n_dim = I columns of da; dgu [rows, 2I].  16 columns at a time: their gate and up values are asked for before
+                // the accumulator is waited for, or while the 16 before them are worked on.
+                const int n = max(1, min(32, rows - (first + q * 32)));
+                const float* gu0 = p.gate_up + gate_up_at(static_cast<size_t>(row0 + first + q * 32), n, static_cast<int>(lane), p.n_dim, nt * 256 + cq * 32);
+                const size_t up = static_cast<size_t>(p.n_dim) * n;
+                float4 g4[4], u4[4];
+                auto load = [&](int part) {  // part 0..3: half part / 2, columns 16 (part % 2)
+                    const int off = (part >> 1) * 128 + (part & 1) * 16;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool in = valid && nt * 256 + cq * 32 + off + 4 * i < p.n_dim;
+                        const float* at = gu0 + (off + 4 * i) * n;
+                        g4[i] = in ? ld_nc_f4(at) : make_float4(0, 0, 0, 0);
+                        u4[i] = in ? ld_nc_f4(at + up) : make_float4(0, 0, 0, 0);
+                    }
+                };
+                load(0);
+                if (!mbar_wait_bounded(&bar_tfull[b], (tcount >> 1) & 1u, abort_flag, 2000000000ull, 64u)) { ok = false; break; }
+                tc_fence_after_sync();
+                uint8_t* orow = valid ? static_cast<uint8_t*>(p.out) + orow_i * (4 * static_cast<size_t>(p.n_dim)) : nullptr;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t v[32];
+                    tmem_ld_32x32b_x32(t0 + h * 128, v);
+                    tc_wait_ld_regs(v);
+                    if (h == 1) hand_back();
+                    const int c0 = nt * 256 + h * 128;
+                    uint32_t du[16];
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float gg[4] = {g4[i].x, g4[i].y, g4[i].z, g4[i].w}, uu[4] = {u4[i].x, u4[i].y, u4[i].z, u4[i].w};
+                            float a[4], d[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float da = __uint_as_float(v[part * 16 + 4 * i + k]);
+                                const float s = sigmoid_fast(gg[k]);
+                                a[k] = da * uu[k] * (s * (1.f + gg[k] * (1.f - s)));
+                                d[k] = da * (gg[k] * s);
+                            }
+                            v[part * 8 + 2 * i] = pack16(a[0], a[1], fp16);  // words 0..15: dg; their da has been used
+                            v[part * 8 + 2 * i + 1] = pack16(a[2], a[3], fp16);
+                            du[part * 8 + 2 * i] = pack16(d[0], d[1], fp16);
+                            du[part * 8 + 2 * i + 1] = pack16(d[2], d[3], fp16);
+                        }
+                        if (2 * h + part < 3) load(2 * h + part + 1);
+                    }
+                    if (c0 < p.n_dim) {  // the same in every thread of the CTA
+                        push(v, orow, c0, p.n_dim);
+                        push(du, orow != nullptr ? orow + static_cast<size_t>(p.n_dim) * 2 : nullptr, c0, p.n_dim);
+                    }
+                }
+                continue;
+            }
             if (!mbar_wait_bounded(&bar_tfull[b], (tcount >> 1) & 1u, abort_flag, 2000000000ull, 64u)) { ok = false; break; }
             tc_fence_after_sync();
-            const uint32_t t0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 256u + cq * 32;
             uint32_t v0[32], v1[32];  // columns cq*32.. of the first 128-column half, same of the second
             tmem_ld_32x32b_x32(t0, v0);
             tmem_ld_32x32b_x32(t0 + 128, v1);
             tc_wait_ld_regs(v0);
             tc_wait_ld_regs(v1);
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                if (cta == 0) mbar_arrive(&bar_tempty[b]);
-                else mbar_arrive_cluster(map_to_cta(&bar_tempty[b], 0));
-            }
+            hand_back();
             uint8_t* out = static_cast<uint8_t*>(p.out);
             if constexpr (SWIGLU) {
                 const int c0 = nt * 128 + cq * 32;
                 if (p.gate_up != nullptr && valid) {
-                    float* gu = p.gate_up + orow_i * (2 * static_cast<size_t>(p.n_dim)) + c0;
+                    const int n = min(32, rows - (first + q * 32));
+                    float* gu = p.gate_up + gate_up_at(static_cast<size_t>(row0 + first + q * 32), n, static_cast<int>(lane), p.n_dim, c0);
+                    const size_t up = static_cast<size_t>(p.n_dim) * n;
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
                         if (c0 + j < p.n_dim) {  // n_dim is a multiple of 8
-                            *reinterpret_cast<uint4*>(gu + j) = make_uint4(v0[j], v0[j + 1], v0[j + 2], v0[j + 3]);
-                            *reinterpret_cast<uint4*>(gu + p.n_dim + j) = make_uint4(v1[j], v1[j + 1], v1[j + 2], v1[j + 3]);
+                            *reinterpret_cast<uint4*>(gu + j * n) = make_uint4(v0[j], v0[j + 1], v0[j + 2], v0[j + 3]);
+                            *reinterpret_cast<uint4*>(gu + up + j * n) = make_uint4(v1[j], v1[j + 1], v1[j + 2], v1[j + 3]);
                         }
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
                     const float g0 = __uint_as_float(v0[j]), g1 = __uint_as_float(v0[j + 1]);
-                    v0[j >> 1] = pack16((g0 / (1.f + expf(-g0))) * __uint_as_float(v1[j]),
-                                        (g1 / (1.f + expf(-g1))) * __uint_as_float(v1[j + 1]), fp16);
+                    v0[j >> 1] = pack16(g0 * sigmoid_fast(g0) * __uint_as_float(v1[j]),
+                                        g1 * sigmoid_fast(g1) * __uint_as_float(v1[j + 1]), fp16);
                 }
                 push(v0, valid ? out + orow_i * p.n_dim * 2 : nullptr, nt * 128, p.n_dim);
-            } else if constexpr (DSWIGLU) {
-                // n_dim = I columns of da; dgu [rows, 2I]
-                auto half = [&](uint32_t (&v)[32], int h) {
-                    const int c0 = nt * 256 + h * 128;
-                    if (c0 >= p.n_dim) return;  // the same in every thread of the CTA
-                    const int c = c0 + cq * 32;
-                    const float* gu = p.gate_up + orow_i * (2 * static_cast<size_t>(p.n_dim)) + c;
-                    uint32_t dg[16], du[16];
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const bool in = valid && c + j < p.n_dim;
-                        const float4 g4 = in ? __ldg(reinterpret_cast<const float4*>(gu + j)) : make_float4(0, 0, 0, 0);
-                        const float4 u4 = in ? __ldg(reinterpret_cast<const float4*>(gu + p.n_dim + j)) : make_float4(0, 0, 0, 0);
-                        const float gg[4] = {g4.x, g4.y, g4.z, g4.w}, uu[4] = {u4.x, u4.y, u4.z, u4.w};
-                        float a[4], d[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float da = __uint_as_float(v[j + i]);
-                            const float s = 1.f / (1.f + expf(-gg[i]));
-                            a[i] = da * uu[i] * (s * (1.f + gg[i] * (1.f - s)));
-                            d[i] = da * (gg[i] * s);
-                        }
-                        dg[j >> 1] = pack16(a[0], a[1], fp16);
-                        dg[(j >> 1) + 1] = pack16(a[2], a[3], fp16);
-                        du[j >> 1] = pack16(d[0], d[1], fp16);
-                        du[(j >> 1) + 1] = pack16(d[2], d[3], fp16);
-                    }
-                    uint8_t* orow = valid ? out + orow_i * (4 * static_cast<size_t>(p.n_dim)) : nullptr;
-                    push(dg, orow, c0, p.n_dim);
-                    push(du, orow != nullptr ? orow + static_cast<size_t>(p.n_dim) * 2 : nullptr, c0, p.n_dim);
-                };
-                half(v0, 0);
-                half(v1, 1);
             } else {
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
