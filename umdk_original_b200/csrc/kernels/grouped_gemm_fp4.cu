@@ -7,13 +7,15 @@
 // rows x 256 columns: each holds its 128 rows of A and HALF of the weight tile, one CTA issues the MMAs of both.
 //
 // Scales stay in memory as the quantiser wrote them, row by row; the tensor core wants them in tensor memory as
-// [32 lanes][4 words] per 128 rows and 64 values (word j of lane l: row 32 j + l).  Four warps per CTA bring them there, each
-// for every fourth K-block: lane l copies the 16 bytes of rows l, 32 + l, 64 + l, 96 + l of each 128 rows into the stage's slot
-// with cp.async, transposes the 4 x 4 words in place (the slot holds the same four addresses of this lane before and after) and
-// raises the stage's barrier.  The MMA issuer then moves the slot into tensor memory with tcgen05.cp directly in front of the
-// MMAs that read it.
+// [32 lanes][4 words] per 128 rows and 64 values (word j of lane l: row 32 j + l).  Three warps per CTA (its rows, the lower and
+// the upper 128 weight rows) bring them there, four K-blocks at a time: 64 bytes of a row are copied by four lanes with cp.async,
+// each to the slot of its K-block, then lane l transposes the 4 x 4 words of rows l, 32 + l, 64 + l, 96 + l of each K-block in
+// place and the warp raises the group's barrier.  The MMA issuer moves a slot into tensor memory with tcgen05.cp directly in
+// front of the MMAs that read it.  What sets the pace of these warps is the number of rows they touch, not the bytes: one K-block
+// at a time (16 bytes of every row) took 1070 cycles per K-block where the MMAs take 512.
 //
-// Barriers: as in grouped_gemm_mx2.cu, bar_sf counts one scale warp of each CTA.
+// Barriers: as in grouped_gemm_mx2.cu, bar_sf counts the three scale warps of each CTA;
+// bar_sfe[group], in each CTA, tells that tensor memory has the scales of the group's K-blocks.
 #include "../common/fp4.cuh"
 #include "expert_gemm.cuh"
 
@@ -22,18 +24,23 @@ namespace cam {
 constexpr int kF4Threads = 768;
 constexpr int kF4EpiThreads = 512;
 constexpr int kF4SfWarp0 = 4, kF4EpiWarp0 = 8;
-constexpr int kF4Stages = 5;
 constexpr int kF4K = 256;                      // values of one K-block
 constexpr int kF4Tile = 128 * 128;             // 128 rows of one K-block, 16 KiB
 constexpr int kF4StageBytes = 2 * kF4Tile;
 constexpr int kF4SfBlock = 4 * 512;            // scales of 128 rows (mxfp4 uses half)
 constexpr int kF4SfStage = 3 * kF4SfBlock;
+constexpr int kF4SfGroup = 4;                  // K-blocks whose scales travel together
+constexpr int kF4SfSlots = 2 * kF4SfGroup;     // two groups
 constexpr int kF4StgPitch = 272;               // bf16 rows of 128 columns, 16 bytes apart from a multiple of 128
 constexpr int kF4StgBytes = 128 * kF4StgPitch;
-constexpr int kF4Smem = kF4Stages * (kF4StageBytes + kF4SfStage) + kF4StgBytes + 1024;
-static_assert(kF4Smem <= 232448, "exceeds the shared memory of one CTA");
+// the plain form gives up a stage for the staging of its rows
+__host__ __device__ constexpr int fp4_stages(bool swiglu) { return swiglu ? 5 : 4; }
+__host__ __device__ constexpr int fp4_smem(bool swiglu) {
+    return fp4_stages(swiglu) * kF4StageBytes + kF4SfSlots * kF4SfStage + (swiglu ? 0 : kF4StgBytes) + 1024;
+}
+static_assert(fp4_smem(true) <= 232448 && fp4_smem(false) <= 232448, "exceeds the shared memory of one CTA");
 constexpr uint32_t kF4TmemCols = 512, kF4SfCol0 = 256, kF4SfCols = 48;
-static_assert(kF4SfCol0 + kF4Stages * kF4SfCols <= kF4TmemCols, "tensor memory");
+static_assert(kF4SfCol0 + fp4_stages(true) * kF4SfCols <= kF4TmemCols, "tensor memory");
 // setmaxnreg: the shares must not exceed what the CTA was launched with (checked against ptxas by the build)
 constexpr uint32_t kF4LaunchRegs = 80, kF4CtrlRegs = 32, kF4SfRegs = 56, kF4EpiRegs = 96;
 static_assert(128 * kF4CtrlRegs + 128 * kF4SfRegs + kF4EpiThreads * kF4EpiRegs <= kF4LaunchRegs * kF4Threads,
@@ -84,15 +91,16 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         if (threadIdx.x == 0) gemm_record_status(&g_fp4_status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
         return;
     }
-    constexpr int NS = kF4Stages;
+    constexpr int NS = fp4_stages(SWIGLU);
     constexpr int SFW = FMT == kFp4Nv ? 4 : 2;  // scale words of a row and K-block
     constexpr int BLK = fp4_block(FMT);
     uint8_t* sfm = smem + NS * kF4StageBytes;
-    uint8_t* stg = sfm + NS * kF4SfStage;
-    uint8_t* ctrl = stg + kF4StgBytes;
+    uint8_t* stg = sfm + kF4SfSlots * kF4SfStage;
+    uint8_t* ctrl = stg + (SWIGLU ? 0 : kF4StgBytes);
     uint64_t* bar_full = reinterpret_cast<uint64_t*>(ctrl);  // first CTA: TMA bytes of both CTAs' stage have landed
-    uint64_t* bar_sf = bar_full + NS;                        // first CTA: scale slots of both CTAs are ready
-    uint64_t* bar_empty = bar_sf + NS;                       // each CTA: the MMAs that read a stage have retired
+    uint64_t* bar_sf = bar_full + NS;                        // first CTA: a group of scale slots of both CTAs is ready
+    uint64_t* bar_sfe = bar_sf + 2;                          // each CTA: a group of scale slots has been copied to tensor memory
+    uint64_t* bar_empty = bar_sfe + 2;                       // each CTA: the MMAs that read a stage have retired
     uint64_t* bar_tfull = bar_empty + NS;                    // each CTA: accumulator of a tile is complete
     uint64_t* bar_tempty = bar_tfull + 1;                    // first CTA: both accumulators have been drained
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_tempty + 1);
@@ -110,8 +118,11 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&bar_full[s], 1);
-            mbar_init(&bar_sf[s], 2);
             mbar_init(&bar_empty[s], 1);
+        }
+        for (int j = 0; j < 2; ++j) {
+            mbar_init(&bar_sf[j], 6);
+            mbar_init(&bar_sfe[j], 1);
         }
         mbar_init(bar_tfull, 1);
         mbar_init(bar_tempty, 2 * (kF4EpiThreads / 32));
@@ -138,7 +149,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     if (warp < kF4SfWarp0) {
         reg_dealloc<kF4CtrlRegs>();
         const uint32_t abort_at = smem_u32(tmem_slot + 1);
-        const uint32_t full_at = smem_u32(bar_full), sf_at = smem_u32(bar_sf), empty_at = smem_u32(bar_empty);
+        const uint32_t full_at = smem_u32(bar_full), sf_at = smem_u32(bar_sf), sfe_at = smem_u32(bar_sfe), empty_at = smem_u32(bar_empty);
         if (warp == 0) {
             // ------------------------------------------------------------ TMA producer (both CTAs)
             const bool leader = elect_one();
@@ -178,24 +189,24 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         } else if (warp == 1 && cta == 0) {
             // ------------------------------------------------------------ MMA issuer (first CTA only)
             const bool leader = elect_one();
-            Ring ring;
+            Ring ring, groups;
             uint32_t tcount = 0, ready = 0u;
             for (int tile = pair_id; w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
                 // both epilogues must have drained the previous tile before its columns are overwritten
                 mbar_wait_warp(smem_u32(bar_tempty), (tcount & 1u) ^ 1u, abort_at);
                 tc_fence_after_sync();
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    const uint32_t s = ring.s;
-                    if (!ready) {
-                        mbar_wait_warp(sf_at + 8u * s, ring.ph, abort_at);
-                        mbar_wait_warp(full_at + 8u * s, ring.ph, abort_at);
-                    }
+                    const uint32_t s = ring.s, gr = groups.s, in_group = static_cast<uint32_t>(kb) % kF4SfGroup;
+                    const bool group_ends = in_group == kF4SfGroup - 1 || kb == kblocks - 1;
+                    if (in_group == 0) mbar_wait_warp(sf_at + 8u * gr, groups.ph, abort_at);
+                    if (!ready) mbar_wait_warp(full_at + 8u * s, ring.ph, abort_at);
                     tc_fence_after_sync();
                     ring.next(NS);
-                    ready = mbar_test(full_at + 8u * ring.s, ring.ph) & mbar_test(sf_at + 8u * ring.s, ring.ph);
+                    if (group_ends) groups.next(2);
+                    ready = mbar_test(full_at + 8u * ring.s, ring.ph);
                     const uint32_t sa = smem_u32(smem) + s * kF4StageBytes;
                     const uint64_t adesc = umma_desc_k_sw128(sa), bdesc = umma_desc_k_sw128(sa + kF4Tile);
-                    const uint32_t sfs = smem_u32(sfm) + s * kF4SfStage;
+                    const uint32_t sfs = smem_u32(sfm) + (gr * kF4SfGroup + in_group) * kF4SfStage;
                     const uint32_t sf = tmem_base + kF4SfCol0 + s * kF4SfCols;  // SFW x (4 columns of A, 8 of B)
                     if (leader) {
 #pragma unroll
@@ -204,14 +215,14 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                             tc_copy_scales_pair(sf + 12u * k + 4u, desc_scales(sfs + kF4SfBlock + k * 512));
                             tc_copy_scales_pair(sf + 12u * k + 8u, desc_scales(sfs + 2 * kF4SfBlock + k * 512));
                         }
+                        if (group_ends) tc_commit_both(sfe_at + 8u * gr);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {  // 64 values = 32 bytes (2 x 16) further along K inside the swizzle atom
                             const uint32_t c = sf + 12u * (FMT == kFp4Nv ? k : k >> 1);
                             tc_mma_fp4_pair<FMT>(tmem_base, adesc + 2u * k, bdesc + 2u * k,
                                                  idesc_fp4<FMT>(2 * BM, 256, FMT == kFp4Nv ? 0u : 2u * (k & 1)), (kb | k) ? 1u : 0u, c, c + 4u);
                         }
-                        // the stage and its scale slot, in both CTAs, are reusable once these have retired
-                        tc_commit_both(empty_at + 8u * s);
+                        tc_commit_both(empty_at + 8u * s);  // the stage, in both CTAs, is reusable once these have retired
                     }
                     __syncwarp();
                 }
@@ -222,60 +233,59 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         }
     } else if (warp < kF4EpiWarp0) {
         reg_dealloc<kF4SfRegs>();
-        // ---------------------------------------------------------------- scale warps: each takes every fourth K-block
-        // (a warp does not see every turn of a stage: at least as many stages as warps keep its waits by parity unambiguous)
-        static_assert(NS >= 4, "scale warps could run a whole turn ahead");
-        const uint32_t mine = static_cast<uint32_t>(warp - kF4SfWarp0);
-        const int pitch = p.k_dim / BLK;          // bytes of scales of a row
-        const int words = pitch / 4;
-        const int last_b = p.num_experts * p.n_dim - 1;
-        uint32_t it = 0;
-        for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows); tile += num_pairs) {
-            const uint8_t* src[12];  // rows 32 j + lane of this CTA's rows, of the lower and of the upper weight rows
-            // Past the tile's rows nothing is loaded: those accumulator rows are not read.  (Loading some row there instead
-            // made all SMs ask one L2 slice for the same bytes: 8 rows of 8 experts, 4096 x 7168, 231 us.)
-            const int a_first = row0 + static_cast<int>(cta) * BM, a_rows = rows - static_cast<int>(cta) * BM;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = 32 * j + static_cast<int>(lane);
-                src[j] = p.a_scales + static_cast<size_t>(min(a_first + r, p.rows - 1)) * pitch;
-                src[4 + j] = p.b_scales + static_cast<size_t>(min(b_row(0) + r, last_b)) * pitch;
-                src[8 + j] = p.b_scales + static_cast<size_t>(min(b_row(1) + r, last_b)) * pitch;
-            }
-            for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                if ((it & 3u) != mine) continue;
-                const uint32_t s = it % NS;
-                const bool got = mbar_wait_bounded(&bar_empty[s], ((it / NS) & 1u) ^ 1u, abort_flag);
-                if (!__all_sync(0xFFFFFFFFu, got)) { ok = false; break; }
-                uint8_t* slot = sfm + s * kF4SfStage + lane * 16u;
-                const uint32_t dst = smem_u32(slot);
-#pragma unroll
-                for (int j = 0; j < 12; ++j) {
-                    if (j < 4 && 32 * j + static_cast<int>(lane) >= a_rows) continue;
-                    const uint32_t d = dst + (j >> 2) * kF4SfBlock + fp4_scale_at<FMT>(j & 3);
-                    const uint8_t* from = src[j] + kb * SFW * 4;
+        // ---------------------------------------------------------------- scale warps: rows, lower and upper weight rows
+        const int what = warp - kF4SfWarp0;
+        if (what < 3) {
+            const int pitch = p.k_dim / BLK;          // bytes of scales of a row
+            const int words = pitch / 4;
+            const int last_b = p.num_experts * p.n_dim - 1;
+            const int sub = static_cast<int>(lane) >> 2, piece = static_cast<int>(lane) & 3;  // row of 8, K-block of the group
+            uint8_t* block = sfm + what * kF4SfBlock;
+            Ring groups;
+            for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows); tile += num_pairs) {
+                // Past the tile's rows nothing is loaded: those accumulator rows are not read.  (Loading some row there instead
+                // made all SMs ask one L2 slice for the same bytes: 8 rows of 8 experts, 4096 x 7168, 231 us.)
+                // A block of weight rows past the last one (its columns are not stored either) is left out.
+                const int first = what == 0 ? row0 + static_cast<int>(cta) * BM : b_row(what - 1);
+                const int live = what == 0 ? rows - static_cast<int>(cta) * BM : first < last_b ? 128 : 0;
+                const uint8_t* from = (what == 0 ? p.a_scales : p.b_scales) + static_cast<size_t>(first + sub) * pitch + piece * (SFW * 4);
+                for (int kb = 0; kb < kblocks; kb += kF4SfGroup, groups.next(2)) {
+                    const bool got = mbar_wait_bounded(&bar_sfe[groups.s], groups.ph ^ 1u, abort_flag);
+                    if (!__all_sync(0xFFFFFFFFu, got)) { ok = false; break; }
+                    uint8_t* slots = block + groups.s * (kF4SfGroup * kF4SfStage);
+                    const uint32_t dst = smem_u32(slots) + static_cast<uint32_t>(piece) * kF4SfStage + static_cast<uint32_t>(sub) * 16u;
+                    const int left = words - (kb + piece) * SFW;  // words of the row that this lane's piece can have
                     if (p.scale_vec) {
-                        copy_async<SFW * 4>(d, from, true);
-                    } else {
+                        if (left > 0) {
+                            const uint8_t* at = from;
 #pragma unroll
-                        for (int i = 0; i < SFW; ++i) {
-                            const bool live = kb * SFW + i < words;
-                            copy_async<4>(d + i * 4u, live ? from + i * 4 : src[j], live);
+                            for (int i = 0; i < 16; ++i, at += 8 * pitch)  // rows 8 i + sub
+                                if (8 * i + sub < live) copy_async<SFW * 4>(dst + fp4_scale_at<FMT>(i >> 2) + (i & 3) * 128u, at, true);
+                        }
+                    } else {
+                        for (int i = 0; i < 16; ++i) {
+                            if (8 * i + sub >= live) break;
+                            const uint8_t* at = from + static_cast<size_t>(8 * i) * pitch;
+#pragma unroll
+                            for (int j = 0; j < SFW; ++j)
+                                copy_async<4>(dst + fp4_scale_at<FMT>(i >> 2) + (i & 3) * 128u + j * 4u, j < left ? at + j * 4 : p.a_scales, j < left);
                         }
                     }
-                }
-                asm volatile("cp.async.wait_all;" ::: "memory");
+                    from += kF4SfGroup * SFW * 4;
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    __syncwarp();  // the words a lane transposes were copied by others
 #pragma unroll
-                for (int blk = 0; blk < 3; ++blk) fp4_transpose_scales<FMT>(slot + blk * kF4SfBlock);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {  // the first CTA's barrier counts both CTAs
-                    if (cta == 0) mbar_arrive(&bar_sf[s]);
-                    else mbar_arrive_cluster(map_to_cta(&bar_sf[s], 0));
+                    for (int c = 0; c < kF4SfGroup; ++c) fp4_transpose_scales<FMT>(slots + c * kF4SfStage + lane * 16u);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {  // the first CTA's barrier counts the warps of both CTAs
+                        if (cta == 0) mbar_arrive(&bar_sf[groups.s]);
+                        else mbar_arrive_cluster(map_to_cta(&bar_sf[groups.s], 0));
+                    }
                 }
             }
+            if (!ok && lane == 0) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 3, static_cast<int>(groups.s));
         }
-        if (!ok && lane == 0) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 3, static_cast<int>(it));
     } else {
         reg_alloc<kF4EpiRegs>();
         // ---------------------------------------------------------------- epilogue warps
@@ -318,7 +328,8 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                     else p.out_scales[at] = static_cast<uint8_t>(scales);
                 }
             } else {
-                // 128 columns at a time go through shared memory as bf16 and leave as one 256-byte bulk copy per row
+                // 128 columns at a time go through shared memory as bf16 and leave as one 256-byte bulk copy per row.  (Stores of
+                // 64 bytes per thread straight from registers: 16 x 1024 rows, K 2048, N 7168 167 -> 231 us.)
                 __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) + grow * p.n_dim;
                 auto push_half = [&](const uint32_t (&v)[32], int c0) {
                     uint8_t* srow = stg + r * kF4StgPitch;
@@ -374,7 +385,7 @@ int launch_fp4(const cam::GroupedGemmFp4Params* p, const CUtensorMap* ta, const 
     // at most one row block per expert beyond the full ones
     const int64_t n_tiles = SWIGLU ? p->n_dim / 256 : (p->n_dim + 255) / 256;
     const int64_t blocks = p->rows / 256 + (p->rows < p->num_experts ? p->rows : p->num_experts);
-    return cam::launch_pairs(limit, cam::grouped_gemm_fp4_kernel<FMT, SWIGLU>, cam::kF4Threads, cam::kF4Smem, blocks * n_tiles, stream, *ta, *ta32, *tb, *p);
+    return cam::launch_pairs(limit, cam::grouped_gemm_fp4_kernel<FMT, SWIGLU>, cam::kF4Threads, cam::fp4_smem(SWIGLU), blocks * n_tiles, stream, *ta, *ta32, *tb, *p);
 }
 
 }  // namespace
