@@ -20,13 +20,14 @@ namespace cam {
 
 constexpr int kNwEpiWarps = 8;
 constexpr int kNwMaxStages = 24;
-constexpr int kNwScaleWarps = 4;
-constexpr int kNwScaleSlots = 8;        // K-blocks whose scales tensor memory has room for
+constexpr int kNwSfGroup = 4;           // K-blocks whose scales travel together (see grouped_gemm_fp4.cu)
+constexpr int kNwScaleSlots = 2 * kNwSfGroup;
 constexpr int kNwSfBlock = 4 * 512;     // scales of 128 rows of a K-block
+constexpr int kNwSfSlot = 2 * kNwSfBlock;  // of the tile's rows and its weight rows
 constexpr uint32_t kNwTmemCols = 512, kNwSfCol0 = 256, kNwSfCols = 32;
 static_assert(kNwSfCol0 + kNwScaleSlots * kNwSfCols <= kNwTmemCols, "tensor memory");
 constexpr int kNwCtrlBytes = 1024;
-static_assert((3 * kNwMaxStages + 4) * 8 + 16 <= kNwCtrlBytes, "barriers");
+static_assert((2 * kNwMaxStages + 8) * 8 + 16 <= kNwCtrlBytes, "barriers");
 
 static __device__ CamStatus g_narrow_status;
 
@@ -98,11 +99,13 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     const int a_all = a_bytes * chunks, b_all = b_bytes * chunks;
     const int nstages = (p.kblocks + chunks - 1) / chunks;         // of a tile
     uint8_t* ctrl = smem;
-    uint8_t* ring = smem + kNwCtrlBytes;  // stages, each [chunk] rows of A | [chunk] weight rows | [chunk] scales of A, scales of the weights
+    uint8_t* ring = smem + kNwCtrlBytes;  // stages, each [chunk] rows of A | [chunk] weight rows; behind the last one the scale slots
+    uint8_t* sfm = ring + p.stages * p.stage_bytes;
     uint64_t* bar_full = reinterpret_cast<uint64_t*>(ctrl);
-    uint64_t* bar_sf = bar_full + kNwMaxStages;
-    uint64_t* bar_empty = bar_sf + kNwMaxStages;
-    uint64_t* bar_tfull = bar_empty + kNwMaxStages;
+    uint64_t* bar_empty = bar_full + kNwMaxStages;
+    uint64_t* bar_sf = bar_empty + kNwMaxStages;   // [2]: a group of scale slots is ready
+    uint64_t* bar_sfe = bar_sf + 2;                // [2]: the MMAs that read a group's scales have retired
+    uint64_t* bar_tfull = bar_sfe + 2;
     uint64_t* bar_tempty = bar_tfull + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_tempty + 2);
     volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -115,10 +118,11 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < ns; ++s) {
             mbar_init(&bar_full[s], 1);
-            mbar_init(&bar_sf[s], 1);
             mbar_init(&bar_empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
+            mbar_init(&bar_sf[b], 2);
+            mbar_init(&bar_sfe[b], 1);
             mbar_init(&bar_tfull[b], 1);
             mbar_init(&bar_tempty[b], kNwEpiWarps);
         }
@@ -141,7 +145,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     const int tile0 = static_cast<int>(blockIdx.x), tiles_step = static_cast<int>(gridDim.x);
 
     const uint32_t abort_at = smem_u32(tmem_slot + 1), ring_at = smem_u32(ring);
-    const uint32_t full_at = smem_u32(bar_full), sf_at = smem_u32(bar_sf), empty_at = smem_u32(bar_empty);
+    const uint32_t full_at = smem_u32(bar_full), sf_at = smem_u32(bar_sf), sfe_at = smem_u32(bar_sfe), empty_at = smem_u32(bar_empty);
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer
         const bool leader = elect_one();
@@ -182,29 +186,31 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         } else {
             idesc[0] = idesc[1] = umma_idesc(BM, 0, 1u, p.fp16 ? 0u : 1u) | ((n >> 3) << 17);
         }
-        Ring r;
+        Ring r, groups;
         uint32_t tcount = 0, ready = 0u;
         for (int tile = tile0; w.locate(tile, e, nt, row0, rows); tile += tiles_step, ++tcount) {
             const uint32_t b = tcount & 1u;
             mbar_wait_warp(smem_u32(&bar_tempty[b]), ((tcount >> 1) & 1u) ^ 1u, abort_at);
             for (int kb = 0; kb < nstages; ++kb) {
-                if (!ready) {
-                    if (FP4) mbar_wait_warp(sf_at + 8u * r.s, r.ph, abort_at);
-                    mbar_wait_warp(full_at + 8u * r.s, r.ph, abort_at);
-                }
+                // a stage is one or two K-blocks, a group of scales four
+                const int k0 = kb * chunks, in_group = k0 % kNwSfGroup;
+                const bool group_ends = FP4 && (in_group + chunks == kNwSfGroup || kb == nstages - 1);
+                const uint32_t gr = groups.s;
+                if (FP4 && in_group == 0) mbar_wait_warp(sf_at + 8u * gr, groups.ph, abort_at);
+                if (!ready) mbar_wait_warp(full_at + 8u * r.s, r.ph, abort_at);
                 tc_fence_after_sync();
                 const uint32_t s = r.s, sa = ring_at + s * static_cast<uint32_t>(p.stage_bytes), sb = sa + static_cast<uint32_t>(a_all);
                 r.next(ns);
                 ready = mbar_test(full_at + 8u * r.s, r.ph);
-                if (FP4) ready &= mbar_test(sf_at + 8u * r.s, r.ph);
-                const int live = min(chunks, p.kblocks - kb * chunks);
+                if (group_ends) groups.next(2);
+                const int live = min(chunks, p.kblocks - k0);
                 if (leader) {
                     for (int c = 0; c < live; ++c) {
                         const uint64_t adesc = umma_desc_k_sw128(sa + static_cast<uint32_t>(c * a_bytes));
                         const uint64_t bdesc = umma_desc_k_sw128(sb + static_cast<uint32_t>(c * b_bytes));
-                        const uint32_t sf = tmem_base + kNwSfCol0 + (s * static_cast<uint32_t>(chunks) + static_cast<uint32_t>(c)) * kNwSfCols;
+                        const uint32_t slot = gr * kNwSfGroup + static_cast<uint32_t>(in_group + c), sf = tmem_base + kNwSfCol0 + slot * kNwSfCols;
                         if constexpr (FP4) {
-                            const uint32_t sfs = sb + static_cast<uint32_t>(b_all + c * 2 * kNwSfBlock);
+                            const uint32_t sfs = smem_u32(sfm) + slot * kNwSfSlot;
 #pragma unroll
                             for (int k = 0; k < SFW; ++k) {
                                 tc_copy_scales(sf + 8u * k, desc_scales(sfs + k * 512));
@@ -218,6 +224,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                         }
                     }
                     tc_commit(&bar_empty[s]);
+                    if (group_ends) tc_commit(&bar_sfe[gr]);  // shared and tensor memory of the group's scales are free
                 }
                 __syncwarp();
             }
@@ -228,75 +235,55 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     } else if (warp < EPI0) {
         if constexpr (FP4) {
         if (warp >= 4) {
-            // ------------------------------------------------------------ scale warps: each takes every fourth stage
-            // A warp does not see every turn of a stage.  With at least as many stages as scale warps the wait for its last
-            // one (turn i - 4, free once the MMAs of i - 4 - stages were done) still tells that the turn before the one it
-            // waits for now (i - 2 stages) is over, which a wait by parity has to know.
-            const uint32_t mine = static_cast<uint32_t>(warp - 4);
+            // ------------------------------------------------------------ scale warps
+            // Two for the tile's rows, two for its weight rows, each pair taking groups of four K-blocks in turn; a warp
+            // therefore always fills the same half of the slots and sees every turn of it.
+            const int weights = warp & 1;
+            const uint32_t mine = static_cast<uint32_t>(warp >> 1) & 1u;
             const int words = p.scale_pitch / 4;
             const int w_rows = SWIGLU ? 2 * p.n_dim : p.n_dim;
-            const int last_b = p.num_experts * w_rows - 1;
-            Ring r;
-            uint32_t it = 0;
-            // The K-block's scales are small pieces of many rows, and a warp waits for them before it can take its next stage:
-            // they are brought to L2 a whole tile ahead, so that this wait is one of L2 and not of memory.
-            RowWalker<BM> wn(p.expert_offsets, p.num_experts, n_tiles, p.rows);
-            auto prefetch_tile = [&](int tile) {
-                int pe, pnt, prow0, prows;
-                if (!wn.locate(tile, pe, pnt, prow0, prows)) return;
-                for (int t = static_cast<int>(threadIdx.x) - 128; t < width; t += 128) {
-                    const int wr = SWIGLU ? (t < step ? pnt * step + t : p.n_dim + pnt * step + t - step) : pnt * step + t;
-                    const uint8_t* row = p.b_scales + static_cast<size_t>(min(pe * w_rows + wr, last_b)) * p.scale_pitch;
-                    for (int c = 0; c < p.scale_pitch; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
-                }
-            };
-            prefetch_tile(tile0);
+            const int sub = static_cast<int>(lane) >> 2, piece = static_cast<int>(lane) & 3;  // row of 8, K-block of the group
+            uint8_t* slots = sfm + mine * (kNwSfGroup * kNwSfSlot) + weights * kNwSfBlock;
+            const uint32_t dst = smem_u32(slots) + static_cast<uint32_t>(piece) * kNwSfSlot + static_cast<uint32_t>(sub) * 16u;
+            const int ngroups = (p.kblocks + kNwSfGroup - 1) / kNwSfGroup;
+            const int64_t to_up = SWIGLU ? static_cast<int64_t>(p.n_dim - step) * p.scale_pitch : 0;  // from gate row t to up row t - step
+            uint32_t count = 0, ph = 0;
             for (int tile = tile0; ok && w.locate(tile, e, nt, row0, rows); tile += tiles_step) {
-                prefetch_tile(tile + tiles_step);
-                const uint8_t* src[8];  // rows 32 j + lane of the tile, then weight rows 32 j + lane
-                bool live[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int t = 32 * j + static_cast<int>(lane);
-                    live[j] = t < rows;
-                    src[j] = p.a_scales + static_cast<size_t>(min(row0 + t, p.rows - 1)) * p.scale_pitch;
-                    const int wr = SWIGLU ? (t < step ? nt * step + t : p.n_dim + nt * step + t - step) : nt * step + t;
-                    live[4 + j] = t < width;
-                    src[4 + j] = p.b_scales + static_cast<size_t>(min(e * w_rows + wr, last_b)) * p.scale_pitch;
-                }
-                for (int kb = 0; kb < nstages; ++kb, ++it, r.next(ns)) {
-                    if ((it & 3u) != mine) continue;
-                    const bool got = mbar_wait_bounded(&bar_empty[r.s], r.ph ^ 1u, abort_flag);
+                const int first = weights ? e * w_rows + nt * step : row0, live = weights ? width : rows;
+                const uint8_t* row = (weights ? p.b_scales : p.a_scales) + static_cast<size_t>(first + sub) * p.scale_pitch + piece * (SFW * 4);
+                const int64_t jump = weights ? to_up : 0;
+                for (int g = 0; g < ngroups; ++g, ++count) {
+                    if ((count & 1u) != mine) continue;
+                    const bool got = mbar_wait_bounded(&bar_sfe[mine], ph ^ 1u, abort_flag);
                     if (!__all_sync(0xFFFFFFFFu, got)) { ok = false; break; }
-                    uint8_t* slot = ring + r.s * static_cast<uint32_t>(p.stage_bytes) + a_all + b_all + lane * 16u;
-                    const uint32_t dst = smem_u32(slot);
-                    const int live_chunks = min(chunks, p.kblocks - kb * chunks);
-                    for (int c = 0; c < live_chunks; ++c) {
-                        const int word0 = (kb * chunks + c) * SFW;
+                    ph ^= 1u;
+                    const uint8_t* from = row + static_cast<size_t>(g) * (kNwSfGroup * SFW * 4);
+                    const int left = words - (g * kNwSfGroup + piece) * SFW;  // words of the row that this lane's piece can have
+                    if (p.scale_vec) {
+                        if (left > 0) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (!live[j]) continue;
-                            const uint32_t d = dst + static_cast<uint32_t>(c * 2 * kNwSfBlock) + (j >> 2) * kNwSfBlock + fp4_scale_at<KIND>(j & 3);
-                            const uint8_t* from = src[j] + word0 * 4;
-                            if (p.scale_vec) {
-                                copy_async<SFW * 4>(d, from, true);
-                            } else {
+                            for (int i = 0; i < 16; ++i, from += 8 * p.scale_pitch)  // rows 8 i + sub
+                                if (8 * i + sub < live) copy_async<SFW * 4>(dst + fp4_scale_at<KIND>(i >> 2) + (i & 3) * 128u, from + (8 * i >= step ? jump : 0), true);
+                        }
+                    } else {
+                        for (int i = 0; i < 16; ++i, from += 8 * p.scale_pitch) {
+                            if (8 * i + sub >= live) break;
+                            const uint8_t* at = from + (8 * i >= step ? jump : 0);
 #pragma unroll
-                                for (int i = 0; i < SFW; ++i) {
-                                    const bool in = word0 + i < words;
-                                    copy_async<4>(d + i * 4u, in ? from + i * 4 : src[j], in);
-                                }
-                            }
+                            for (int j = 0; j < SFW; ++j)
+                                copy_async<4>(dst + fp4_scale_at<KIND>(i >> 2) + (i & 3) * 128u + j * 4u, j < left ? at + j * 4 : p.a_scales, j < left);
                         }
                     }
                     asm volatile("cp.async.wait_all;" ::: "memory");
-                    for (int c = 0; c < 2 * live_chunks; ++c) fp4_transpose_scales<KIND>(slot + c * kNwSfBlock);
+                    __syncwarp();  // the words a lane transposes were copied by others
+#pragma unroll
+                    for (int c = 0; c < kNwSfGroup; ++c) fp4_transpose_scales<KIND>(slots + c * kNwSfSlot + lane * 16u);
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&bar_sf[r.s]);
+                    if (lane == 0) mbar_arrive(&bar_sf[mine]);
                 }
             }
-            if (!ok && lane == 0) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 3, static_cast<int>(it));
+            if (!ok && lane == 0) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 3, static_cast<int>(count));
         }
         }
     } else {
@@ -420,15 +407,16 @@ namespace {
 
 // The MMA reads 128 rows of A from a stage whatever the stage has room for: behind a short one lie weights and scales, and behind
 // the last stage this padding.  What it reads there ends in accumulator rows that nobody reads.
-int narrow_smem(const cam::NarrowParams* p) {
-    const int over = (cam::BM - p->slot_rows) * 128 - (p->stage_bytes - p->slot_rows * 128 * p->chunks);  // from the last chunk's rows
-    return cam::kNwCtrlBytes + p->stages * p->stage_bytes + (over > 0 ? over : 0);
+int narrow_smem(const cam::NarrowParams* p, bool fp4) {
+    const int scales = fp4 ? cam::kNwScaleSlots * cam::kNwSfSlot : 0;
+    const int over = (cam::BM - p->slot_rows) * 128 - (p->stage_bytes - p->slot_rows * 128 * p->chunks) - scales;  // from the last chunk's rows
+    return cam::kNwCtrlBytes + p->stages * p->stage_bytes + scales + (over > 0 ? over : 0);
 }
 
 template <int KIND, bool SWIGLU>
 int launch_narrow(const cam::NarrowParams* p, int64_t tiles, const CUtensorMap* ta, const CUtensorMap* tb, cudaStream_t stream) {
     static cam::SmemLimitCache limit;
-    const int smem = narrow_smem(p);
+    const int smem = narrow_smem(p, KIND != cam::kNarrow16);
     const cudaError_t err = limit.ensure(cam::expert_narrow_kernel<KIND, SWIGLU>, smem);
     if (err != cudaSuccess) return static_cast<int>(err);
     const int64_t sms = cam::sm_count_of_current_device();
@@ -448,14 +436,15 @@ int launch_narrow(const cam::NarrowParams* p, int64_t tiles, const CUtensorMap* 
 
 extern "C" int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int swiglu, int64_t tiles, const CUtensorMap* ta,
                                              const CUtensorMap* tb, cudaStream_t stream) {
-    const int least = kind == cam::kNarrow16 ? 2 : cam::kNwScaleWarps;
-    if (p->chunks < 1 || p->stages < least || p->stages > cam_expert_narrow_max_stages(kind, p->chunks) || narrow_smem(p) > 232448 || p->stage_bytes % 1024 != 0)
+    const bool fp4 = kind != cam::kNarrow16;
+    if (p->chunks < 1 || (fp4 && p->chunks > 2) || p->stages < 2 || p->stages > cam::kNwMaxStages || narrow_smem(p, fp4) > 232448 ||
+        p->stage_bytes % 1024 != 0)
         return static_cast<int>(cudaErrorInvalidValue);
     if (kind == cam::kFp4Nv) return swiglu ? launch_narrow<cam::kFp4Nv, true>(p, tiles, ta, tb, stream) : launch_narrow<cam::kFp4Nv, false>(p, tiles, ta, tb, stream);
     if (kind == cam::kFp4Mx) return swiglu ? launch_narrow<cam::kFp4Mx, true>(p, tiles, ta, tb, stream) : launch_narrow<cam::kFp4Mx, false>(p, tiles, ta, tb, stream);
     return swiglu ? launch_narrow<cam::kNarrow16, true>(p, tiles, ta, tb, stream) : launch_narrow<cam::kNarrow16, false>(p, tiles, ta, tb, stream);
 }
 
-extern "C" int cam_expert_narrow_max_stages(int kind, int chunks) { return kind == cam::kNarrow16 ? cam::kNwMaxStages : cam::kNwScaleSlots / chunks; }
+extern "C" int cam_expert_narrow_max_stages(void) { return cam::kNwMaxStages; }
 
 extern "C" int cam_narrow_status(CamStatus* out) { return static_cast<int>(cudaMemcpyFromSymbol(out, cam::g_narrow_status, sizeof(CamStatus))); }

@@ -64,7 +64,7 @@ struct NarrowParams {
     int kblocks;                // 128-byte blocks of a row
     int width;                  // columns of the product per tile: 32 (not fp4), 64 or 128
     int slot_rows;              // rows of A a stage has room for: 32, 64 or 128 (at least the rows of any expert's tile)
-    int chunks;                 // K-blocks of a stage; 4-bit: stages * chunks <= 8
+    int chunks;                 // K-blocks of a stage; 4-bit: 1 or 2
     int chunked;                // the maps split rows into 128-byte K-blocks (rows of whole blocks only; needed for chunks > 1)
     int stages, stage_bytes;
     int fp16;
@@ -101,7 +101,7 @@ int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, const CUten
 // rows, halves, K-blocks, experts} in boxes {128, step, halves, chunks, 1} with SwiGLU's gate and up rows as two halves.
 int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int swiglu, int64_t tiles, const CUtensorMap* tmap_a,
                                   const CUtensorMap* tmap_b, cudaStream_t stream);
-int cam_expert_narrow_max_stages(int kind, int chunks);
+int cam_expert_narrow_max_stages(void);
 int cam_narrow_status(CamStatus* out);
 int cam_mlp_status(CamStatus* out);
 int cam_fp4_status(CamStatus* out);  // of the current device: the first wait that ran out in a kernel of that file

@@ -69,8 +69,9 @@ int launch_narrow(cam::NarrowParams* p, int kind, bool swiglu, const void* a, co
     for (int width = 128; width >= (fp4 ? 64 : 32); width /= 2) {
         const int step = swiglu ? width / 2 : width;
         const int64_t t = blocks * ((p->n_dim + step - 1) / step);
-        // turns of the SMs x time of a tile; a tile costs its weights and a fixed part
-        const int64_t cost = ((t + sms - 1) / sms) * (width + 16);
+        // turns of the SMs x cycles of a tile: its weights at an SM's share of the memory bandwidth (22 bytes a cycle), or
+        // the four MMAs of a K-block (67 cycles each, however narrow), and a fixed part
+        const int64_t cost = ((t + sms - 1) / sms) * ((row_bytes + 127) / 128 * (width * 6 < 280 ? 280 : width * 6) + 2000);
         if (forced > 0 ? width == forced : best < 0 || cost < best) {
             best = cost;
             p->width = width;
@@ -81,12 +82,12 @@ int launch_narrow(cam::NarrowParams* p, int kind, bool swiglu, const void* a, co
     p->kblocks = (row_bytes + 127) / 128;
     p->chunked = row_bytes % 128 == 0;
     p->slot_rows = p->rows <= 32 ? 32 : p->rows <= 64 ? 64 : 128;
-    // 16 KiB of weights in a stage, as long as four stages fit (4-bit needs as many as it has scale warps)
-    const int per_chunk = (p->slot_rows + p->width) * 128 + (fp4 ? 4096 : 0);
+    // 16 KiB of weights in a stage, as long as three stages fit
+    const int per_chunk = (p->slot_rows + p->width) * 128, room = 232448 - 1024 - (fp4 ? 32768 : 16384);
     p->chunks = p->chunked ? 128 / p->width : 1;
-    while (p->chunks > 1 && (4 * p->chunks * per_chunk > 232448 - 1024 - 16384 || p->chunks > p->kblocks)) p->chunks /= 2;
+    while (p->chunks > 1 && (3 * p->chunks * per_chunk > room || p->chunks > p->kblocks)) p->chunks /= 2;
     p->stage_bytes = p->chunks * per_chunk;
-    const int fit = (232448 - 1024 - 16384) / p->stage_bytes, most = cam_expert_narrow_max_stages(kind, p->chunks);
+    const int fit = room / p->stage_bytes, most = cam_expert_narrow_max_stages();
     p->stages = fit < most ? fit : most;
     const uint64_t bytes = p->chunked ? 128 : static_cast<uint64_t>(row_bytes), blocks_k = p->chunked ? static_cast<uint64_t>(p->kblocks) : 1;
     const uint64_t pitch = static_cast<uint64_t>(row_bytes), halves = swiglu ? 2 : 1, n = static_cast<uint64_t>(p->n_dim);
