@@ -55,17 +55,17 @@ struct GroupedMlpParams {
     float* gate_up;             // rows x 2I fp32 in the order of gate_up_at (expert_gemm.cuh): written by kMlpUp (or null), read by kMlpDact
 };
 
-// One-CTA form of the row products for experts with few rows (expert_gemm_narrow.cu): tiles of 128 rows x `width` columns.
+// Form of the row products for experts with few rows (expert_gemm_narrow.cu): tiles of 128 weight rows x slot_rows rows.
 constexpr int kNarrow16 = 2;  // beside the formats of fp4.cuh: 16-bit operands
 struct NarrowParams {
     const int* expert_offsets;
     int num_experts, rows;
     int n_dim;                  // columns of the result; with SwiGLU: I, the weights have 2I rows
     int kblocks;                // 128-byte blocks of a row
-    int width;                  // columns of the product per tile: 32 (not fp4), 64 or 128
-    int slot_rows;              // rows of A a stage has room for: 32, 64 or 128 (at least the rows of any expert's tile)
-    int chunks;                 // K-blocks of a stage; 4-bit: 1 or 2
-    int chunked;                // the maps split rows into 128-byte K-blocks (rows of whole blocks only; needed for chunks > 1)
+    int slot_rows;              // rows of a tile at most: 32, 64 or 128
+    int split;                  // CTAs of a cluster that share the K-blocks of a tile: 1, 2 or 4
+    int chunks;                 // K-blocks of a stage: 1 or 2
+    int chunked;                // the maps split rows into 128-byte K-blocks (rows of whole blocks only; needed for 2 chunks)
     int stages, stage_bytes;
     int fp16;
     void* out;                  // 16-bit [rows, n_dim], or fp4 SwiGLU: codes [rows, I/2]
@@ -98,10 +98,11 @@ int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, const CUten
                            const CUtensorMap* tmap_b, cudaStream_t stream);
 // kind: kFp4Nv, kFp4Mx or kNarrow16.  The maps, innermost first; with `chunked` a row is (K-block, 128 bytes), otherwise all of
 // its bytes and one K-block: tmap_a {bytes, rows, K-blocks} in boxes {128, slot_rows (32 without chunks), chunks}; tmap_b {bytes,
-// rows, halves, K-blocks, experts} in boxes {128, step, halves, chunks, 1} with SwiGLU's gate and up rows as two halves.
+// rows, halves, K-blocks, experts} in boxes {128, 128 / halves, halves, chunks, 1} with SwiGLU's gate and up rows as two halves.
 int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int swiglu, int64_t tiles, const CUtensorMap* tmap_a,
                                   const CUtensorMap* tmap_b, cudaStream_t stream);
 int cam_expert_narrow_max_stages(void);
+int cam_expert_narrow_fixed_smem(int fp4, int slot_rows);  // shared memory beside the stages
 int cam_narrow_status(CamStatus* out);
 int cam_mlp_status(CamStatus* out);
 int cam_fp4_status(CamStatus* out);  // of the current device: the first wait that ran out in a kernel of that file

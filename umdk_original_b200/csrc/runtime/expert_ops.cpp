@@ -50,45 +50,49 @@ int env_switch(const char* name) {
     return v != nullptr && *v != 0 ? std::atoi(v) : -1;
 }
 
-// One-CTA tiles of 128 rows (expert_gemm_narrow.cu) or CTA pairs with tiles of 256 x 256?
-bool narrow_pays(int rows, int num_experts) {
+// The form for few rows per expert (expert_gemm_narrow.cu), or CTA pairs with tiles of 256 x 256?  Up to 128 rows per expert the
+// first takes 0.77 - 1.0 of the time of the second (16 experts of 4096 x 1024, 4 of 7168 x 2048, one of either; 16 and 4 bits), at
+// 160 it computes two tiles where the pairs compute one: 1.2 - 2.0.  With fewer than 32 pair tiles most SMs would stand still, while
+// the form for few rows divides a tile's K-blocks: one expert of 7168 x 2048, 256 rows 0.82 - 0.95, of 2048 x 1024, 768 rows 0.9 - 1.0.
+bool narrow_pays(int rows, int num_experts, int n_dim, bool swiglu) {
     const int sw = env_switch("UMDK_CAM_EXPERT_NARROW");
     if (sw >= 0) return sw != 0;
-    return static_cast<int64_t>(rows) <= 128ll * num_experts;
+    const int64_t mean = (static_cast<int64_t>(rows) + num_experts - 1) / num_experts;
+    return mean <= 128 || (mean + 255) / 256 * num_experts * ((n_dim + (swiglu ? 127 : 255)) / (swiglu ? 128 : 256)) < 32;
 }
 
-// The one-CTA form: tile width, stages, maps, launch.  `row_bytes` of the row operand and of the weights' rows; n_dim, the
-// operands' scales and outputs are set.
+// The form for few rows: rows of a tile, stages, clusters, maps, launch.  `row_bytes` of the row operand and of the weights'
+// rows; n_dim, the operands' scales and outputs are set.
 int launch_narrow(cam::NarrowParams* p, int kind, bool swiglu, const void* a, const void* w, int row_bytes, const char* what, cudaStream_t stream) {
     const bool fp4 = kind != cam::kNarrow16;
     const int sms = cam::sm_count_of_current_device();
-    const int64_t blocks = p->rows <= p->num_experts ? p->rows
-                                                     : static_cast<int64_t>(p->num_experts) * (((p->rows + p->num_experts - 1) / p->num_experts + 127) / 128);
-    const int forced = env_switch("UMDK_CAM_EXPERT_WIDTH");
-    int64_t best = -1;
-    for (int width = 128; width >= (fp4 ? 64 : 32); width /= 2) {
-        const int step = swiglu ? width / 2 : width;
-        const int64_t t = blocks * ((p->n_dim + step - 1) / step);
-        // turns of the SMs x cycles of a tile: its weights at an SM's share of the memory bandwidth (22 bytes a cycle), or
-        // the four MMAs of a K-block (67 cycles each, however narrow), and a fixed part
-        const int64_t cost = ((t + sms - 1) / sms) * ((row_bytes + 127) / 128 * (width * 6 < 280 ? 280 : width * 6) + 2000);
-        if (forced > 0 ? width == forced : best < 0 || cost < best) {
-            best = cost;
-            p->width = width;
-        }
-    }
-    const int step = swiglu ? p->width / 2 : p->width;
-    const int64_t upper = p->rows / 128 + (p->rows < p->num_experts ? p->rows : p->num_experts);  // row blocks there can be
+    const int step = swiglu ? 64 : 128;
+    const int64_t n_tiles = (p->n_dim + step - 1) / step;
+    // Room for twice the mean rows per expert: larger experts are cut, and their weights come from L2 for the further tiles.
+    const int64_t mean = (p->rows + p->num_experts - 1) / p->num_experts;
+    p->slot_rows = p->rows <= 32 || mean <= 16 ? 32 : p->rows <= 64 || mean <= 40 ? 64 : 128;
+    const int64_t blocks = p->rows <= p->num_experts ? p->rows : static_cast<int64_t>(p->num_experts) * ((mean + p->slot_rows - 1) / p->slot_rows);
+    const int64_t upper = p->rows / p->slot_rows + (p->rows < p->num_experts ? p->rows : p->num_experts);  // row blocks there can be
     p->kblocks = (row_bytes + 127) / 128;
     p->chunked = row_bytes % 128 == 0;
-    p->slot_rows = p->rows <= 32 ? 32 : p->rows <= 64 ? 64 : 128;
-    // 16 KiB of weights in a stage, as long as three stages fit
-    const int per_chunk = (p->slot_rows + p->width) * 128, room = 232448 - 1024 - (fp4 ? 32768 : 16384);
-    p->chunks = p->chunked ? 128 / p->width : 1;
-    while (p->chunks > 1 && (3 * p->chunks * per_chunk > room || p->chunks > p->kblocks)) p->chunks /= 2;
+    const int per_chunk = (p->slot_rows + 128) * 128, room = 232448 - cam_expert_narrow_fixed_smem(fp4, p->slot_rows);
+    p->chunks = p->chunked && p->kblocks > 1 && room / (2 * per_chunk) >= 3 ? 2 : 1;
     p->stage_bytes = p->chunks * per_chunk;
     const int fit = room / p->stage_bytes, most = cam_expert_narrow_max_stages();
     p->stages = fit < most ? fit : most;
+    // CTAs per tile: turns of the SMs x cycles of a turn (a K-block at an SM's share of the memory bandwidth, a fixed part, the
+    // exchange inside the cluster)
+    const int unit = fp4 ? 4 : p->chunks, units = (p->kblocks + unit - 1) / unit;
+    const int forced = env_switch("UMDK_CAM_EXPERT_SPLIT");
+    int64_t best = -1;
+    for (int split = 1; split <= 4 && split <= units; split *= 2) {  // clusters of 8 find too few places at once
+        const int64_t turns = (blocks * n_tiles + sms / split - 1) / (sms / split);
+        const int64_t cost = turns * (static_cast<int64_t>((units + split - 1) / split) * unit * 770 + 1500 + (split > 1 ? 2000 : 0));
+        if (forced > 0 ? split <= forced : best < 0 || cost < best) {
+            best = cost;
+            p->split = split;
+        }
+    }
     const uint64_t bytes = p->chunked ? 128 : static_cast<uint64_t>(row_bytes), blocks_k = p->chunked ? static_cast<uint64_t>(p->kblocks) : 1;
     const uint64_t pitch = static_cast<uint64_t>(row_bytes), halves = swiglu ? 2 : 1, n = static_cast<uint64_t>(p->n_dim);
     CUtensorMap ta, tb;
@@ -98,7 +102,7 @@ int launch_narrow(cam::NarrowParams* p, int kind, bool swiglu, const void* a, co
     const uint64_t db[5] = {bytes, n, halves, blocks_k, static_cast<uint64_t>(p->num_experts)}, sb[4] = {pitch, pitch * n, 128, pitch * n * halves};
     const uint32_t bb[5] = {128, static_cast<uint32_t>(step), static_cast<uint32_t>(halves), static_cast<uint32_t>(p->chunks), 1};
     if (cam_encode_tmap(&tb, w, 5, db, sb, bb) != 0) return -1;
-    return launched(cam_launch_expert_gemm_narrow(p, kind, swiglu, upper * ((p->n_dim + step - 1) / step), &ta, &tb, stream), what);
+    return launched(cam_launch_expert_gemm_narrow(p, kind, swiglu, upper * n_tiles, &ta, &tb, stream), what);
 }
 
 }  // namespace
@@ -134,7 +138,7 @@ extern "C" int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, 
     EXP_CHECK(n_dim >= 128 && n_dim % (swiglu ? 256 : 128) == 0, "grouped_gemm_fp4: N %d must be a multiple of %d", n_dim, swiglu ? 256 : 128);
     EXP_CHECK(static_cast<int64_t>(num_experts) * n_dim < (1ll << 31), "grouped_gemm_fp4: weight rows overflow");
     EXP_CHECK(aligned(a_s, 4) && aligned(w_s, 4), "grouped_gemm_fp4: scales must be 4-byte aligned");
-    if (narrow_pays(rows, num_experts)) {
+    if (narrow_pays(rows, num_experts, swiglu ? n_dim / 2 : n_dim, swiglu != 0)) {
         cam::NarrowParams p{};
         p.expert_offsets = offsets;
         p.num_experts = num_experts;
@@ -181,7 +185,7 @@ int row_product(int form, const char* what, const void* a, int k, const void* w,
     EXP_CHECK(a && w && offsets && out, "%s: null operand", what);
     EXP_CHECK(rows >= 1 && num_experts >= 1, "%s: empty problem", what);
     EXP_CHECK(k >= 8 && n >= 8 && k % 8 == 0 && n % 8 == 0, "%s: sizes %d and %d must be multiples of 8", what, k, n);
-    if (!by_rows && narrow_pays(rows, num_experts)) {
+    if (!by_rows && narrow_pays(rows, num_experts, n, form == cam::kMlpUp)) {
         const bool swiglu = form == cam::kMlpUp;
         cam::NarrowParams p{};
         p.expert_offsets = offsets;
