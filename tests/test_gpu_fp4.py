@@ -136,7 +136,10 @@ def _acc_tol(k):
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("k,n", [(128, 128), (384, 256), (512, 640), (2048, 384)])
 @pytest.mark.parametrize("counts", list(COUNTS))
-def test_product(ops, fmt, k, n, counts):
+@pytest.mark.parametrize("form", ["chosen", "pairs"])
+def test_product(ops, fmt, k, n, counts, form, monkeypatch):
+    if form == "pairs":  # the form for many rows per expert, at all sizes
+        monkeypatch.setenv("UMDK_CAM_EXPERT_NARROW", "0")
     cnt, head, tail = COUNTS[counts]
     gen = torch.Generator().manual_seed(k + n)
     e, m = len(cnt), head + sum(cnt) + tail
@@ -156,7 +159,10 @@ def test_product(ops, fmt, k, n, counts):
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("k,inter", [(128, 128), (384, 256), (1024, 384)])
 @pytest.mark.parametrize("counts", list(COUNTS))
-def test_swiglu(ops, fmt, k, inter, counts):
+@pytest.mark.parametrize("form", ["chosen", "pairs"])
+def test_swiglu(ops, fmt, k, inter, counts, form, monkeypatch):
+    if form == "pairs":
+        monkeypatch.setenv("UMDK_CAM_EXPERT_NARROW", "0")
     cnt, head, tail = COUNTS[counts]
     block = 16 if fmt == "nvfp4" else 32
     gen = torch.Generator().manual_seed(k + inter)

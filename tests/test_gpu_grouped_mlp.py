@@ -100,7 +100,10 @@ def check(got, want, tol, tiny, scale=1.0):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("h,inter", [(8, 8), (136, 72), (256, 128), (1000, 344), (512, 640)])
 @pytest.mark.parametrize("counts", list(COUNTS))
-def test_forward_and_gradients(ops, dtype, h, inter, counts):
+@pytest.mark.parametrize("form", ["chosen", "pairs"])
+def test_forward_and_gradients(ops, dtype, h, inter, counts, form, monkeypatch):
+    if form == "pairs":  # the form for many rows per expert, at all sizes
+        monkeypatch.setenv("UMDK_CAM_EXPERT_NARROW", "0")
     x, w1, w2, dy, off = make(dtype, h, inter, counts)
     half, tiny = bounds(dtype)
     want, tol = formula64(x, w1, w2, dy, off, half, acc)

@@ -13,6 +13,18 @@ namespace {
 constexpr int kQThreads = 256;
 constexpr int kQPer = 2;  // groups of 16 values per thread, loads of all in flight together
 
+// 32 bytes per thread at a time: a warp's accesses are whole sectors
+__device__ __forceinline__ void load32(uint4* v, const uint4* p) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0].x), "=r"(v[0].y), "=r"(v[0].z), "=r"(v[0].w), "=r"(v[1].x), "=r"(v[1].y), "=r"(v[1].z), "=r"(v[1].w)
+                 : "l"(p));
+}
+__device__ __forceinline__ void store32(uint4* p, const uint32_t* v) {
+    asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
 template <int DT>
 struct Raw16;  // sixteen values as loaded
 template <>
@@ -70,7 +82,10 @@ quantize_fp4_kernel(const uint4* __restrict__ x, uint2* __restrict__ q, uint8_t*
     for (int u = 0; u < kQPer; ++u) {
         const int64_t i = base + u * kQThreads;
 #pragma unroll
-        for (int j = 0; j < V; ++j) r[u].v[j] = i < groups ? ld_nc_v4(x + i * V + j) : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < V; j += 2) {
+            if (i < groups) load32(r[u].v + j, x + i * V + j);
+            else r[u].v[j] = r[u].v[j + 1] = make_uint4(0, 0, 0, 0);
+        }
     }
 #pragma unroll
     for (int u = 0; u < kQPer; ++u) {
@@ -134,7 +149,7 @@ dequantize_fp4_kernel(const uint2* __restrict__ q, const uint8_t* __restrict__ s
             }
         }
 #pragma unroll
-        for (int j = 0; j < V; ++j) st_na_v4(out + i * V + j, make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
+        for (int j = 0; j < V; j += 2) store32(out + i * V + j, o + 4 * j);
     }
 }
 

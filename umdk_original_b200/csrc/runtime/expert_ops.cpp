@@ -112,7 +112,7 @@ extern "C" int cam_quantize_fp4(const void* x, int dtype, int fmt, void* q, void
     if (numel == 0) return 0;
     EXP_CHECK(x && q && s, "quantize_fp4: null operand");
     EXP_CHECK(numel > 0 && numel % (fmt == 0 ? 16 : 32) == 0, "quantize_fp4: %lld values are not whole blocks", static_cast<long long>(numel));
-    EXP_CHECK(aligned(x, 16) && aligned(q, 8), "quantize_fp4: operands must be 16-byte aligned");
+    EXP_CHECK(aligned(x, 32) && aligned(q, 8), "quantize_fp4: x must be 32-byte aligned");
     const int64_t groups = numel / 16;
     EXP_CHECK(gscale == nullptr || (gscales >= 1 && groups % gscales == 0), "quantize_fp4: %lld global scales", static_cast<long long>(gscales));
     return launched(cam_launch_quantize_fp4(x, dtype, fmt, q, s, groups, gscale, gscale && gscales > 1 ? groups / gscales : 0, stream), "quantize_fp4");
@@ -123,7 +123,7 @@ extern "C" int cam_dequantize_fp4(const void* q, const void* s, int dtype, int f
     if (numel == 0) return 0;
     EXP_CHECK(q && s && out, "dequantize_fp4: null operand");
     EXP_CHECK(numel > 0 && numel % (fmt == 0 ? 16 : 32) == 0, "dequantize_fp4: %lld values are not whole blocks", static_cast<long long>(numel));
-    EXP_CHECK(aligned(q, 8) && aligned(out, 16), "dequantize_fp4: operands must be 8-byte aligned");
+    EXP_CHECK(aligned(q, 8) && aligned(out, 32), "dequantize_fp4: q must be 8-byte aligned");
     const int64_t groups = numel / 16;
     EXP_CHECK(gscale == nullptr || (gscales >= 1 && groups % gscales == 0), "dequantize_fp4: %lld global scales", static_cast<long long>(gscales));
     return launched(cam_launch_dequantize_fp4(q, s, dtype, fmt, out, groups, gscale, gscale && gscales > 1 ? groups / gscales : 0, stream), "dequantize_fp4");
