@@ -307,3 +307,40 @@ def test_graph_and_streams(ops):
     offs.copy_(off2)
     g.replay()
     assert torch.equal(y, layer(x2, off2))
+
+
+def test_offsets_past_32_bits(ops):
+    """Weights of more than 2^31 bytes of codes: the last expert's; rows behind 2^31 values."""
+    e, n, k = 70, 8192, 8192
+    gen = torch.Generator().manual_seed(11)
+    wq = torch.zeros(e, n, k // 2, dtype=torch.uint8, device=DEV)
+    ws = torch.zeros(e, n, k // 16, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    assert wq.numel() > 2 ** 31
+    q, s = random_fp4((n, k), "nvfp4", gen, DEV)
+    wq[-1] = q
+    ws.view(torch.uint8)[-1] = s.view(torch.uint8)
+    aq, as_ = random_fp4((33, k), "nvfp4", gen, DEV)
+    off = torch.tensor([0] * e + [33], dtype=torch.int32, device=DEV)
+    want, mag = _product64(values64(aq, as_), values64(q, s)[None], torch.tensor([0, 33]), 33)
+    got = ops.grouped_gemm_fp4(aq, as_, wq, ws, off)
+    assert ((got.double() - want).abs() <= want.abs() * 2.0 ** -8 + mag * _acc_tol(k)).all()
+    del wq, ws
+    x = torch.zeros(2 ** 31 // 4096 + 3, 4096, dtype=torch.bfloat16, device=DEV)
+    x[-2:] = torch.randn(2, 4096, generator=gen).to(DEV)
+    q, s = ops.quantize_fp4(x, 32)
+    wq2, ws2 = ops.quantize_fp4(x[-2:].contiguous(), 32)
+    assert torch.equal(q[-2:], wq2) and torch.equal(s[-2:].view(torch.uint8), ws2.view(torch.uint8))
+    assert (ops.dequantize_fp4(q, s)[-2:] != 0).any()
+
+
+def test_wild_offsets_stay_inside(ops):
+    from umdk_original_b200.ops import cam_ops
+    gen = torch.Generator().manual_seed(12)
+    aq, as_ = random_fp4((50, 256), "mxfp4", gen, DEV)
+    wq, ws = random_fp4((3, 256, 256), "mxfp4", gen, DEV)
+    for off in ([40, -7, 60, 10], [2 ** 31 - 1] * 4, [0, 0, 0, 10 ** 9]):
+        o = torch.tensor(off, dtype=torch.int32, device=DEV)
+        ops.grouped_gemm_fp4(aq, as_, wq, ws, o)
+        ops.grouped_gemm_fp4_swiglu(aq, as_, wq, ws, o)
+        torch.cuda.synchronize()
+        assert cam_ops.native_module().expert_ops_status()[0] == 0

@@ -127,3 +127,219 @@ def test_forward_and_gradients(ops, dtype, h, inter, counts, form, monkeypatch):
 def test_status_is_clean(ops):
     from umdk_original_b200.ops import cam_ops
     assert cam_ops.native_module().expert_ops_status()[0] == 0
+
+
+@pytest.mark.parametrize("m,e,h,inter", [(1, 1, 512, 256), (3, 2, 4096, 64), (40, 8, 264, 1024), (640, 1, 1024, 256), (130, 1, 2048, 136)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_few_rows(ops, dtype, m, e, h, inter):
+    """Sizes at which the form for few rows divides a product among several CTAs, or has room for 32, 64 or 128 rows."""
+    gen = torch.Generator(device=DEV).manual_seed(m + h)
+    x = torch.randn(m, h, device=DEV, generator=gen).to(dtype)
+    w1 = (torch.randn(e, 2 * inter, h, device=DEV, generator=gen) * h ** -0.5).to(dtype)
+    w2 = (torch.randn(e, h, inter, device=DEV, generator=gen) * inter ** -0.5).to(dtype)
+    dy = torch.randn(m, h, device=DEV, generator=gen).to(dtype)
+    cnt = torch.bincount(torch.randint(0, e, (m,), generator=torch.Generator().manual_seed(m)), minlength=e).tolist()
+    off = offsets_of(cnt, 0, DEV)
+    half, tiny = bounds(dtype)
+    want, tol = formula64(x, w1, w2, dy, off, half, acc)
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+    y = ops.grouped_mlp(*leaves, off)
+    dx, dw1, dw2 = torch.autograd.grad(y, leaves, dy)
+    check({"y": y.detach(), "dx": dx, "dw1": dw1, "dw2": dw2}, want, tol, tiny * (m + 2 * inter + h))
+
+
+def test_two_runs_give_the_same_bits(ops):
+    x, w1, w2, dy, off = make(torch.bfloat16, 1000, 344, "block borders")
+    runs = []
+    for _ in range(2):
+        leaves = [t.clone().requires_grad_() for t in (x, w1, w2)]
+        y = ops.grouped_mlp(*leaves, off)
+        runs.append((y, *torch.autograd.grad(y, leaves, dy)))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("form", ["chosen", "pairs"])
+def test_nan_stays_with_its_expert(ops, form, monkeypatch):
+    """Rows and weights of one expert, and rows of none, are NaN and infinities; the others' results are as without them."""
+    if form == "pairs":
+        monkeypatch.setenv("UMDK_CAM_EXPERT_NARROW", "0")
+    x, w1, w2, dy, off = make(torch.bfloat16, 136, 72, "head and tail")  # experts of 40, 0 and 200 rows behind 7 and before 260
+    cnt = [40, 100, 100]
+    off = offsets_of(cnt, 7, DEV)
+    clean = [t.clone().requires_grad_() for t in (x, w1, w2)]
+    y0 = ops.grouped_mlp(*clean, off)
+    g0 = torch.autograd.grad(y0, clean, dy)
+    bad = [t.clone() for t in (x, w1, w2, dy)]
+    bad[0][:7], bad[0][247:], bad[0][47:147] = float("nan"), float("inf"), float("nan")
+    bad[1][1], bad[2][1] = float("nan"), float("inf")
+    bad[3][:7], bad[3][247:], bad[3][47:147] = float("inf"), float("nan"), float("-inf")
+    leaves = [t.requires_grad_() for t in bad[:3]]
+    y = ops.grouped_mlp(*leaves, off)
+    g = torch.autograd.grad(y, leaves, bad[3])
+    keep = torch.ones(x.shape[0], dtype=torch.bool, device=DEV)
+    keep[47:147] = False
+    assert torch.equal(y[keep], y0[keep]) and torch.equal(g[0][keep], g0[0][keep])
+    for i in (1, 2):
+        assert torch.equal(g[i][0], g0[i][0]) and torch.equal(g[i][2], g0[i][2])
+        assert not g[i][1].isfinite().all()
+
+
+def test_offsets_past_32_bits(ops):
+    """Weights of more than 2^32 bytes: the last expert's."""
+    e, h, inter = 66, 8192, 2048
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    w1 = torch.empty(e, 2 * inter, h, device=DEV, dtype=torch.bfloat16)
+    w2 = torch.empty(e, h, inter, device=DEV, dtype=torch.bfloat16)
+    assert w1.numel() * 2 > 2 ** 32
+    w1[-1] = torch.randn(2 * inter, h, device=DEV, generator=gen) * h ** -0.5
+    w2[-1] = torch.randn(h, inter, device=DEV, generator=gen) * inter ** -0.5
+    x = torch.randn(70, h, device=DEV, generator=gen).to(torch.bfloat16)
+    dy = torch.randn(70, h, device=DEV, generator=gen).to(torch.bfloat16)
+    off = torch.tensor([0] * e + [70], dtype=torch.int32, device=DEV)
+    want, tol = formula64(x, w1[-1:], w2[-1:], dy, torch.tensor([0, 70]), *[bounds(torch.bfloat16)[0], acc])
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+    y = ops.grouped_mlp(*leaves, off)
+    dx, dw1, dw2 = torch.autograd.grad(y, leaves, dy)
+    check({"y": y.detach(), "dx": dx, "dw1": dw1[-1:], "dw2": dw2[-1:]}, want, tol, 0.0)
+    assert (dw1[:-1] == 0).all() and (dw2[:-1] == 0).all()
+
+
+def test_wild_offsets_stay_inside(ops):
+    """Offsets that make no sense (decreasing, negative, past the rows) are clamped; what they select is computed, nothing else is
+    touched and no wait runs out."""
+    from umdk_original_b200.ops import cam_ops
+    x, w1, w2, dy, _ = make(torch.bfloat16, 136, 72, "holes")
+    for off in ([5, -3, 2 ** 31 - 1, 7, 7, 0, 10, 3], [0, 0, 0, 0, 0, 0, 0, 10 ** 9], [79, 79, 79, 79, 79, 79, 79, -5]):
+        o = torch.tensor(off, dtype=torch.int32, device=DEV)
+        leaves = [t.clone().requires_grad_() for t in (x, w1, w2)]
+        y = ops.grouped_mlp(*leaves, o)
+        torch.autograd.grad(y, leaves, dy)
+        torch.cuda.synchronize()
+        assert cam_ops.native_module().expert_ops_status()[0] == 0
+
+
+def test_capture_and_replay(ops):
+    """Forward and backward in one CUDA graph, replayed with other rows, weights and offsets; and a side stream."""
+    x, w1, w2, dy, off = make(torch.bfloat16, 256, 128, "holes")
+    leaves = [t.clone().requires_grad_() for t in (x, w1, w2)]
+    d, o = dy.clone(), off.clone()
+
+    def step():
+        y = ops.grouped_mlp(*leaves, o)
+        return (y.detach(), *torch.autograd.grad(y, leaves, d))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = step()
+    torch.cuda.current_stream().wait_stream(side)
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(first, want))
+    del first
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    x2, w12, w22, dy2, _ = make(torch.bfloat16, 256, 128, "holes", seed=9)
+    with torch.no_grad():
+        for a, b in zip(leaves, (x2, w12, w22)):
+            a.copy_(b)
+    d.copy_(dy2)
+    o.copy_(offsets_of([10, 0, 0, 30, 1, 2, 3], 2, DEV))
+    g.replay()
+    got = [t.clone() for t in out]
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_capture_beside_an_eager_graph_is_refused(ops):
+    x, w1, w2, dy, off = make(torch.bfloat16, 256, 128, "holes")
+    w1.requires_grad_()
+    eager = ops.grouped_mlp(x, w1, w2, off)  # holds w1's accumulation node
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="let go of its outputs"):
+        with torch.cuda.graph(g):
+            ops.grouped_mlp(x, w1, w2, off)
+    del eager
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ops.grouped_mlp(x, w1, w2, off)
+        dw, = torch.autograd.grad(y, w1, dy)
+    g.replay()
+    y2 = ops.grouped_mlp(x, w1, w2, off)
+    assert torch.equal(y, y2) and torch.equal(dw, torch.autograd.grad(y2, w1, dy)[0])
+
+
+def test_refusals(ops):
+    from test_grouped_mlp_cpu import refusals
+    for call in refusals(DEV):
+        with pytest.raises(RuntimeError, match="umdk_cam_op_lib"):
+            call()
+    x, w1, w2, dy, off = make(torch.bfloat16, 256, 128, "holes")
+    with pytest.raises(RuntimeError, match="device"):
+        ops.grouped_mlp(x, w1, w2, off.cpu())
+    shifted = torch.empty(x.numel() + 1, device=DEV, dtype=x.dtype)[1:].view_as(x)
+    with pytest.raises(RuntimeError, match="aligned"):
+        ops.grouped_mlp(shifted, w1, w2, off)
+
+
+def test_training_with_accumulated_gradients(ops):
+    """.backward() twice accumulates; gradients of an expanded scalar; weights that do not want a gradient."""
+    x, w1, w2, dy, off = make(torch.float16, 136, 72, "block borders")
+    w1.requires_grad_()
+    ops.grouped_mlp(x, w1, w2, off).float().sum().backward()
+    once = w1.grad.clone()
+    ops.grouped_mlp(x, w1, w2, off).float().sum().backward()
+    assert torch.equal(w1.grad, (once.float() * 2).half())
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "nvfp4", "mxfp4"])
+def test_dispatch_experts_combine(ops, fmt):
+    """The operators as they are used: rows from a dispatch, the experts' MLP, the weighted sum of the combine."""
+    from umdk_original_b200 import Buffer, CamConfig
+    from umdk_original_b200.models import ExpertMLP, offsets_from_counts
+    t, h, inter, e, k = 64, 256, 128, 8, 2
+    gen = torch.Generator().manual_seed(7)
+    x = torch.randn(t, h, generator=gen).to(torch.bfloat16).to(DEV)
+    idx = torch.stack([torch.randperm(e, generator=gen)[:k] for _ in range(t)]).to(DEV)
+    wt = torch.rand(t, k, generator=gen).to(DEV)
+    buf = Buffer(None, CamConfig(num_experts=e, max_tokens=t, hidden=h, topk=k, timeout_ms=2000.0), name="expert_mlp_" + fmt,
+                 device=torch.device(DEV, 0), rank=0, num_ranks=1)
+    mlp = ExpertMLP(e, h, inter, device=DEV, seed=1)
+    layer = mlp if fmt == "bf16" else mlp.quantized(fmt)
+    with torch.no_grad():
+        # a receive buffer of fixed size: rows past the last expert belong to none
+        rx, src, cnt, per_e, _ = ops.moe_dispatch_prefill_quant(x, idx, wt, buf.capacity, buf.name, 0, 1, 0)
+        off = offsets_from_counts(per_e)
+        y = layer(rx, off)
+        out = ops.moe_combine_prefill(y, idx, wt, src, cnt, buf.name, 0, 1)
+    buf.check()
+    if fmt == "bf16":
+        w1, w2 = mlp.w1.detach().double(), mlp.w2.detach().double()
+    else:
+        w1 = ops.dequantize_fp4(layer.w1_q, layer.w1_s, layer.w1_gs, torch.float32).double()
+        w2 = ops.dequantize_fp4(layer.w2_q, layer.w2_s, layer.w2_gs, torch.float32).double()
+
+    def rows64(v):
+        if fmt == "bf16":
+            return v
+        q, s = ops.quantize_fp4(v.float().contiguous(), layer.block)
+        return ops.dequantize_fp4(q, s, None, torch.float32).double()
+    want = torch.zeros(t, h, dtype=torch.float64, device=DEV)
+    for j in range(k):
+        g, u = torch.einsum("th,tih->ti", rows64(x.double()), w1[idx[:, j]]).chunk(2, -1)
+        act = rows64(g * torch.sigmoid(g) * u)
+        want += torch.einsum("ti,thi->th", act, w2[idx[:, j]]) * wt[:, j: j + 1].double()
+    # bf16: act, expert output and result are rounded (half a step, 2^-8, each); 4 bits: a value of act near the middle between two
+    # points may round to the other one, which moves few values by a third at most
+    err = (out.double() - want).norm() / want.norm()
+    assert err < (3 * 2.0 ** -8 if fmt == "bf16" else 0.02)
+    if fmt == "bf16":
+        y = mlp(rx.clone(), off)
+        dw1, dw2 = torch.autograd.grad(y.float().square().sum(), (mlp.w1, mlp.w2))
+        assert dw1.isfinite().all() and dw2.isfinite().all() and dw1.abs().sum() > 0
+    buf.destroy()
+
+
+def test_status_after_everything(ops):
+    from umdk_original_b200.ops import cam_ops
+    assert cam_ops.native_module().expert_ops_status()[0] == 0

@@ -2,6 +2,7 @@
 // gated feed-forward block of 16-bit experts with its backward pass.
 // Schemas are added to the library that bindings.cpp defines.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 #include <torch/library.h>
@@ -322,9 +323,29 @@ struct GroupedMlpFunction : public torch::autograd::Function<GroupedMlpFunction>
     }
 };
 
+// A captured backward pass that accumulates into a leaf whose accumulation node belongs to an eager graph (another stream) makes
+// the autograd engine synchronise a stream that is not captured, which ends the process.  Refused while it can still be.
+void check_capture(const at::Tensor& t, const char* what) {
+    if (!t.requires_grad() || !t.is_leaf() || !t.is_cuda()) return;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (accumulator == nullptr) return;
+    const auto stream = accumulator->stream();
+    CAM_ASSERT(!stream.has_value() || *stream == at::cuda::getCurrentCUDAStream(t.device().index()).unwrap(), "grouped_mlp is captured into a CUDA graph while a graph of derivatives that was recorded outside the capture still holds ",
+               what, "; let go of its outputs before the capture");
+}
+
 at::Tensor grouped_mlp_autograd(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, const at::Tensor& expert_offsets) {
-    if (at::GradMode::is_enabled() && (x.requires_grad() || w1.requires_grad() || w2.requires_grad()))
+    if (at::GradMode::is_enabled() && (x.requires_grad() || w1.requires_grad() || w2.requires_grad())) {
+        if (x.is_cuda()) {
+            c10::cuda::CUDAGuard guard(x.device());
+            if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+                check_capture(x, "x");
+                check_capture(w1, "w1");
+                check_capture(w2, "w2");
+            }
+        }
         return GroupedMlpFunction::apply(x, w1, w2, expert_offsets);
+    }
     at::AutoDispatchBelowADInplaceOrView guard;
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("umdk_cam_op_lib::grouped_mlp", "")
                          .typed<at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&)>();
