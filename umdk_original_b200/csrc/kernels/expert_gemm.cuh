@@ -27,7 +27,8 @@ __device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity) {
     return ok;
 }
 // Bounded: after kWaitPolls polls (each of which the hardware may itself hold for a while), or once another role has given up,
-// it returns with *abort set; the pipeline then runs to its end without waiting and its results mean nothing.
+// it returns with *abort set; the pipeline then runs to the end of its tile without waiting, its results mean nothing, and the CTA
+// lets the copies in flight land (abort_drain) before it leaves.
 constexpr uint32_t kWaitPolls = 1u << 23;
 __device__ __forceinline__ void mbar_wait_warp(uint32_t bar, uint32_t parity, uint32_t abort) {
     asm volatile(
@@ -58,6 +59,15 @@ __device__ __forceinline__ void tc_commit_both(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
                  "h"(static_cast<uint16_t>(3))
                  : "memory");
+}
+// The same answer in all lanes of a converged warp
+__device__ __forceinline__ bool aborted(const volatile uint32_t* abort_flag) { return __any_sync(0xFFFFFFFFu, *abort_flag != 0u); }
+// After a wait that ran out copies may still be on their way to this CTA's shared memory: two milliseconds, where they take
+// microseconds, before the memory is given up.
+__device__ __forceinline__ void abort_drain(const volatile uint32_t* abort_flag) {
+    if (*abort_flag == 0u) return;
+    const uint64_t t0 = globaltimer_ns();
+    for (int i = 0; i < 4000 && globaltimer_ns() - t0 < 2000000ull; ++i) __nanosleep(1000);
 }
 // Position in a ring of stages: stage and the parity of its current turn
 struct Ring {

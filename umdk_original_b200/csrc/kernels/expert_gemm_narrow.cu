@@ -216,7 +216,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         }
         Ring r;
         uint32_t ready = 1u;  // the first turn of every stage is free
-        for (int tile = tile0; w.locate(tile, e, nt, row0, rows); tile += tiles_step) {
+        for (int tile = tile0; !aborted(abort_flag) && w.locate(tile, e, nt, row0, rows); tile += tiles_step) {
             // with two chunks a stage's rows come in one box; otherwise in pieces of 32 rows, those that exist
             const int pieces = chunks > 1 ? 1 : (rows + 31) / 32;
             const uint32_t bytes = static_cast<uint32_t>((chunks > 1 ? a_all : pieces * 4096) + kWBytes * chunks);
@@ -243,7 +243,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         const bool leader = elect_one();
         Ring r, groups;
         uint32_t tcount = 0, ready = 0u;
-        for (int tile = tile0; w.locate(tile, e, nt, row0, rows); tile += tiles_step, ++tcount) {
+        for (int tile = tile0; !aborted(abort_flag) && w.locate(tile, e, nt, row0, rows); tile += tiles_step, ++tcount) {
             const uint32_t n = static_cast<uint32_t>((rows + 15) & ~15);
             uint32_t idesc[2];
             if constexpr (FP4) {
@@ -484,6 +484,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     }
 
     // ------------------------------------------------------------------ teardown
+    abort_drain(abort_flag);
     tc_fence_before_sync();
     __syncthreads();
     if (split > 1) cluster_sync_all();  // another CTA may still read this one's staging area or signal its barriers

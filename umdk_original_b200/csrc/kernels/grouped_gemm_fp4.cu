@@ -164,7 +164,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             // Only 32-row pieces of A that hold rows are loaded; what stays in the other rows of the stage reaches
             // accumulator rows that nobody reads.
             auto pieces = [](int r) { return r > 96 ? 4 : r > 0 ? (r + 31) / 32 : 0; };
-            for (int tile = pair_id; w.locate(tile, e, nt, row0, rows); tile += num_pairs) {
+            for (int tile = pair_id; !aborted(abort_flag) && w.locate(tile, e, nt, row0, rows); tile += num_pairs) {
                 const int p0 = pieces(min(rows, BM)), p1 = pieces(rows - BM);
                 const int mine = cta ? p1 : p0;
                 const uint32_t bytes = 2u * kF4Tile + static_cast<uint32_t>(p0 + p1) * 4096u;
@@ -191,7 +191,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             const bool leader = elect_one();
             Ring ring, groups;
             uint32_t tcount = 0, ready = 0u;
-            for (int tile = pair_id; w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
+            for (int tile = pair_id; !aborted(abort_flag) && w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
                 // both epilogues must have drained the previous tile before its columns are overwritten
                 mbar_wait_warp(smem_u32(bar_tempty), (tcount & 1u) ^ 1u, abort_at);
                 tc_fence_after_sync();
@@ -366,6 +366,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     }
 
     // ------------------------------------------------------------------ teardown
+    abort_drain(abort_flag);
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync_all();  // the other CTA may still read this CTA's shared memory or signal its barriers

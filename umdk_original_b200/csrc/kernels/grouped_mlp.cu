@@ -172,7 +172,7 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             // row forms: only 32-row pieces of A that hold rows are loaded; what stays in the other rows of the stage reaches
             // accumulator rows that nobody reads
             auto pieces = [](int r) { return r > 96 ? 4 : r > 0 ? (r + 31) / 32 : 0; };
-            for (int tile = pair_id; locate(tile); tile += num_pairs) {
+            for (int tile = pair_id; !aborted(abort_flag) && locate(tile); tile += num_pairs) {
                 const int kblocks = kblocks_of();
                 const int p0 = pieces(min(rows, BM)), p1 = pieces(rows - BM), mine = cta ? p1 : p0;
                 const uint32_t bytes = WGRAD ? 2u * kEmStageBytes : 2u * kEmTile + static_cast<uint32_t>(p0 + p1) * 4096u;
@@ -224,7 +224,7 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             const uint32_t idesc = umma_idesc(2 * BM, 256, 1u, p.fp16 ? 0u : 1u) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
             Ring ring;
             uint32_t tcount = 0, ready = 0u;
-            for (int tile = pair_id; locate(tile); tile += num_pairs, ++tcount) {
+            for (int tile = pair_id; !aborted(abort_flag) && locate(tile); tile += num_pairs, ++tcount) {
                 const int kblocks = kblocks_of();
                 const uint32_t b = tcount & 1u;
                 // both epilogues must have drained this accumulator's previous tile
@@ -436,6 +436,7 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     }
 
     // ------------------------------------------------------------------ teardown
+    abort_drain(abort_flag);
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync_all();  // the other CTA may still read this CTA's shared memory or signal its barriers
