@@ -232,14 +232,6 @@ __device__ __forceinline__ void fp4_swiglu32(const uint32_t* gate, const uint32_
     scales = sc[0] | (sc[1] << 8);
 }
 
-// Where the fp32 gate and up values of a row lie in the tensor that the forward pass keeps for the backward pass.  The rows of an
-// expert form groups of 32 (the last one of `n` < 32): a group's 2 I n values are [gate, up][32 columns][4 columns][row][4], so
-// that a warp with a row per lane writes and reads whole lines.  Returns the place of column `col` (a multiple of 32) of the
-// gate; four columns on are 4 n floats further, the up values I n floats.
-__device__ __forceinline__ size_t gate_up_at(size_t group_row, int n, int row_in_group, int inter, int col) {
-    return group_row * (2 * static_cast<size_t>(inter)) + static_cast<size_t>(col) * n + row_in_group * 4;
-}
-
 __device__ __forceinline__ uint32_t pack16(float a, float b, bool fp16) {
     if (fp16) {
         const __half2 t = __floats2half2_rn(a, b);

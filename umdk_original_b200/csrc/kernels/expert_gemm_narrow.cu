@@ -452,13 +452,11 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                         float u[8];
                         gather(u, 2, t, 64 + ch * 8);
                         if (p.gate_up != nullptr) {
-                            const int n = min(32, rows - (t & ~31));
-                            float* gu = p.gate_up + gate_up_at(static_cast<size_t>(row0 + (t & ~31)), n, t & 31, p.n_dim, c & ~31) + (c & 31) * n;
-                            const size_t up = static_cast<size_t>(p.n_dim) * n;
+                            float* gu = p.gate_up + static_cast<size_t>(row0 + t) * (2 * static_cast<size_t>(p.n_dim)) + c;
 #pragma unroll
                             for (int j = 0; j < 8; j += 4) {
-                                *reinterpret_cast<float4*>(gu + j * n) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                                *reinterpret_cast<float4*>(gu + up + j * n) = make_float4(u[j], u[j + 1], u[j + 2], u[j + 3]);
+                                *reinterpret_cast<float4*>(gu + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                                *reinterpret_cast<float4*>(gu + p.n_dim + j) = make_float4(u[j], u[j + 1], u[j + 2], u[j + 3]);
                             }
                         }
 #pragma unroll

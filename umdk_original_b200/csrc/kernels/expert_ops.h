@@ -40,9 +40,8 @@ struct GroupedGemmFp4Params {
     uint8_t* out_scales;        // SwiGLU form: [rows, I / block]
 };
 
-// Products of the gated feed-forward block in 16 bits (grouped_mlp.cu) and what its epilogue does with them
+// Products of the gated feed-forward block in 16 bits (grouped_mlp.cu)
 constexpr int kMlpUp = 0, kMlpDown = 1, kMlpDact = 2, kMlpDx = 3, kMlpDw = 4;
-constexpr int kMlpPlain = 0, kMlpSwiglu = 1, kMlpSwigluBackward = 2;
 
 struct GroupedMlpParams {
     const int* expert_offsets;  // [E+1]
@@ -52,7 +51,7 @@ struct GroupedMlpParams {
     int k_dim;                  // contraction (not kMlpDw)
     int fp16;                   // operands and results are fp16, otherwise bf16
     void* out;                  // [rows, n_dim]; kMlpDact: dgu [rows, 2 n_dim]; kMlpDw: [E, m_dim, n_dim]
-    float* gate_up;             // rows x 2I fp32 in the order of gate_up_at (expert_gemm.cuh): written by kMlpUp (or null), read by kMlpDact
+    float* gate_up;             // [rows, 2I] fp32: written by kMlpUp (or null), read by kMlpDact
 };
 
 // Form of the row products for experts with few rows (expert_gemm_narrow.cu): tiles of 128 weight rows x slot_rows rows.
@@ -69,7 +68,7 @@ struct NarrowParams {
     int stages, stage_bytes;
     int fp16;
     void* out;                  // 16-bit [rows, n_dim], or fp4 SwiGLU: codes [rows, I/2]
-    float* gate_up;             // 16-bit SwiGLU: null or fp32, see GroupedMlpParams
+    float* gate_up;             // 16-bit SwiGLU: null or fp32 [rows, 2I]
     // fp4
     const uint8_t *a_scales, *b_scales;
     int scale_pitch, scale_vec;

@@ -9,11 +9,22 @@
 // kept in fp32 for the backward pass and da stays in the accumulator, so that no result is more than one rounding of an
 // operand and its own away from the formula.
 //
-// One pipeline for all five: K-blocks of 64 values (128 bytes) come by TMA into a ring of six stages, each CTA of the pair
-// holds 128 rows of A and half of the 256-column B tile, one CTA issues tcgen05.mma.cta_group::2, and the accumulator (256
-// columns of tensor memory) is one of two, so that the epilogue of a tile overlaps the MMAs of the next.  An operand whose
-// contraction index is not its contiguous one (w2 and w1 of dact and dx, both operands of dw) is loaded as [64 of the
-// contraction][64 values] boxes and read by the tensor core in its MN-major form; nothing is transposed in memory.
+// up, down and dx (grouped_gemm_16_rows_kernel): the weights are the M operand of the tensor core, the rows of the expert its N
+// operand in steps of 32, so that the tensor time, and at the power limit the energy, follow the rows present: an expert of 375
+// rows is two tiles of 192, where tiles of 256 rows as M operand compute 512.  A pair of CTAs computes 512 weight rows (each CTA two
+// blocks of 128: the gate and the up block of the same features, or neighbouring blocks) x up to 256 rows, of which each CTA loads
+// half; a K-block of 64 values brings 96 KiB to the pair for 1024 cycles of MMAs, three quarters of what tiles of 256 x 256 need.
+// The accumulators fill tensor memory, so the epilogue takes them to registers at once, rounded, and hands them back before it
+// stores.  Against 256 x 256 tiles in a steady loop: 24 uneven experts of 375 rows, 4096 x 1024 294 -> 278 us, 16 of 375 rows, 4096
+// x 2048 370 -> 337, 8 of 512 rows, 7168 x 2048 397 -> 378.
+//
+// dact and dw (grouped_gemm_16_square_kernel): tiles of 256 x 256 and two accumulators in turn.  dact reads 8 bytes of gate and up
+// for every value of da, and its epilogue is what takes long: with an accumulator to spare it runs beside the MMAs of the next tile
+// (16 x 1024 rows, 4096 x 2048: 225 us, with 512 x 256 tiles 288).
+//
+// K-blocks of 64 values (128 bytes) come by TMA.  An operand whose contraction index is not its contiguous one (w2 of dact, w1 of dx,
+// both operands of dw) is loaded as [64 of the contraction][64 values] boxes and read by the tensor core in its MN-major form;
+// nothing is transposed in memory.
 //
 // The sum of dw runs over a ragged number of rows.  The last K-block of an expert then holds rows of the next one: its loads
 // complete on a barrier of their own, a warp overwrites those rows with zeros in shared memory (in both operands: a NaN times
@@ -68,9 +79,11 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr) {
            (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 
-__device__ __forceinline__ float4 ld_nc_f4(const float* p) {
-    const uint4 v = ld_nc_v4(p);
-    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+// 32 bytes that are read once: a whole sector per thread
+__device__ __forceinline__ void ld_nc_f8(const float* p, float* v) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "l"(p));
 }
 
 // Tiles of the weight gradients: 256 x 256 of every expert's [m_dim, n_dim]; `rows` are the rows summed over.
@@ -93,10 +106,11 @@ struct GradTileWalker {
 
 }  // namespace
 
-// A_MN / B_MN: the operand's contraction index is its row index in memory.  A_MN is the weight-gradient form.
-template <bool A_MN, bool B_MN, int EPI>
+// Tiles of 256 x 256 with two accumulators in turn.  DW: weight gradients (contraction over an expert's rows, both operands
+// MN-major).  Otherwise dact: 256 rows x 256 columns of da, the weights MN-major.
+template <bool DW>
 __global__ void __launch_bounds__(kEmThreads, 1)
-grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
+grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
                        const __grid_constant__ CUtensorMap tmap_b, const GroupedMlpParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {  // swizzled TMA tiles need it; the same in both CTAs of a pair
@@ -104,8 +118,6 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
         return;
     }
     constexpr int NS = kEmStages;
-    constexpr bool WGRAD = A_MN, SWIGLU = EPI == kMlpSwiglu, DSWIGLU = EPI == kMlpSwigluBackward;
-    static_assert(!A_MN || B_MN, "not a form that is used");
     uint8_t* stg = smem + NS * kEmStageBytes;
     uint8_t* ctrl = stg + kEmStgBytes;
     uint64_t* bar_full = reinterpret_cast<uint64_t*>(ctrl);  // first CTA: bytes of both CTAs' stage have landed
@@ -121,11 +133,11 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     const uint32_t cta = cluster_cta_rank();  // 0 = first CTA of the pair (issues the MMAs)
     const int pair_id = static_cast<int>(blockIdx.x) >> 1;
     const int num_pairs = static_cast<int>(gridDim.x) >> 1;
-    const int n_tiles = SWIGLU ? (p.n_dim + 127) / 128 : (p.n_dim + 255) / 256;
+    const int n_tiles = (p.n_dim + 255) / 256;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
-            mbar_init(&bar_full[s], WGRAD ? 2 : 1);
+            mbar_init(&bar_full[s], DW ? 2 : 1);
             mbar_init(&bar_empty[s], 1);
             mbar_init(&bar_tail[s], 1);
         }
@@ -151,8 +163,8 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     const GradTileWalker wg(p.expert_offsets, p.num_experts, (p.m_dim + 255) / 256, n_tiles, p.rows);
     int e, mt = 0, nt, row0, rows;
     bool ok = true;
-    auto locate = [&](int tile) { return WGRAD ? wg.locate(tile, e, mt, nt, row0, rows) : wr.locate(tile, e, nt, row0, rows); };
-    auto kblocks_of = [&]() { return ((WGRAD ? rows : p.k_dim) + 63) / 64; };
+    auto locate = [&](int tile) { return DW ? wg.locate(tile, e, mt, nt, row0, rows) : wr.locate(tile, e, nt, row0, rows); };
+    auto kblocks_of = [&]() { return ((DW ? rows : p.k_dim) + 63) / 64; };
 
     if (warp < kEmEpiWarp0) {
         reg_dealloc<kEmCtrlRegs>();
@@ -169,13 +181,13 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             Ring ring;
             uint32_t ready = 1u;  // the first turn of every stage is free
             const uint32_t full0 = map_to_cta(bar_full, 0), tail_own = map_to_cta(bar_tail, cta);
-            // row forms: only 32-row pieces of A that hold rows are loaded; what stays in the other rows of the stage reaches
+            // dact: only 32-row pieces of A that hold rows are loaded; what stays in the other rows of the stage reaches
             // accumulator rows that nobody reads
             auto pieces = [](int r) { return r > 96 ? 4 : r > 0 ? (r + 31) / 32 : 0; };
             for (int tile = pair_id; !aborted(abort_flag) && locate(tile); tile += num_pairs) {
                 const int kblocks = kblocks_of();
                 const int p0 = pieces(min(rows, BM)), p1 = pieces(rows - BM), mine = cta ? p1 : p0;
-                const uint32_t bytes = WGRAD ? 2u * kEmStageBytes : 2u * kEmTile + static_cast<uint32_t>(p0 + p1) * 4096u;
+                const uint32_t bytes = DW ? 2u * kEmStageBytes : 2u * kEmTile + static_cast<uint32_t>(p0 + p1) * 4096u;
                 const int half = static_cast<int>(cta);
                 for (int kb = 0; kb < kblocks; ++kb) {
                     const uint32_t s = ring.s;
@@ -186,28 +198,24 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                         uint8_t* sa = smem + s * kEmStageBytes;
                         uint8_t* sb = sa + kEmTile;
                         uint32_t bar = full0 + 8u * s;
-                        if (WGRAD && kb == kblocks - 1 && (rows & 63) != 0) {
+                        if (DW && kb == kblocks - 1 && (rows & 63) != 0) {
                             bar = tail_own + 8u * s;
                             mbar_arrive_expect_tx(&bar_tail[s], kEmStageBytes);
                         } else if (cta == 0) {
                             mbar_arrive_expect_tx(&bar_full[s], bytes);
-                        } else if (WGRAD) {
+                        } else if (DW) {
                             mbar_arrive_cluster(bar);
                         }
-                        if constexpr (WGRAD) {
+                        if constexpr (DW) {
                             const int r = row0 + kb * 64, ca = (mt * 256 + half * 128) * 2, cb = (nt * 256 + half * 128) * 2;
                             tma_load_2d_pair(sa, &tmap_a, bar, ca, r);
                             tma_load_2d_pair(sa + 8192, &tmap_a, bar, ca + 128, r);
                             tma_load_2d_pair(sb, &tmap_b, bar, cb, r);
                             tma_load_2d_pair(sb + 8192, &tmap_b, bar, cb + 128, r);
                         } else {
-                            if constexpr (B_MN) {
-                                const int cb = (nt * 256 + half * 128) * 2;
-                                tma_load_3d_pair(sb, &tmap_b, bar, cb, kb * 64, e);
-                                tma_load_3d_pair(sb + 8192, &tmap_b, bar, cb + 128, kb * 64, e);
-                            } else {
-                                tma_load_3d_pair(sb, &tmap_b, bar, kb * 128, SWIGLU ? half * p.n_dim + nt * 128 : nt * 256 + half * 128, e);
-                            }
+                            const int cb = (nt * 256 + half * 128) * 2;
+                            tma_load_3d_pair(sb, &tmap_b, bar, cb, kb * 64, e);
+                            tma_load_3d_pair(sb + 8192, &tmap_b, bar, cb + 128, kb * 64, e);
                             const int arow = row0 + half * BM;
                             if (mine == 4) tma_load_2d_pair(sa, &tmap_a, bar, kb * 128, arow);
                             else for (int i = 0; i < mine; ++i) tma_load_2d_pair(sa + i * 4096, &tmap_a32, bar, kb * 128, arow + i * 32);
@@ -221,7 +229,7 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             // ------------------------------------------------------------ MMA issuer (first CTA only)
             const bool leader = elect_one();
             // fp32 accumulator; a_major / b_major (bits 15, 16) = 1 for MN-major operands
-            const uint32_t idesc = umma_idesc(2 * BM, 256, 1u, p.fp16 ? 0u : 1u) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+            const uint32_t idesc = umma_idesc(2 * BM, 256, 1u, p.fp16 ? 0u : 1u) | (DW ? 1u << 15 : 0u) | (1u << 16);
             Ring ring;
             uint32_t tcount = 0, ready = 0u;
             for (int tile = pair_id; !aborted(abort_flag) && locate(tile); tile += num_pairs, ++tcount) {
@@ -237,12 +245,12 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     ring.next(NS);
                     ready = mbar_test(full_at + 8u * ring.s, ring.ph);
                     const uint32_t sa = smem_u32(smem) + s * kEmStageBytes;
-                    const uint64_t adesc = A_MN ? umma_desc_mn_sw128(sa) : umma_desc_k_sw128(sa);
-                    const uint64_t bdesc = B_MN ? umma_desc_mn_sw128(sa + kEmTile) : umma_desc_k_sw128(sa + kEmTile);
+                    const uint64_t adesc = DW ? umma_desc_mn_sw128(sa) : umma_desc_k_sw128(sa);
+                    const uint64_t bdesc = umma_desc_mn_sw128(sa + kEmTile);
                     if (leader) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)  // 16 of the contraction: 32 bytes of a row, or 16 rows of 128 bytes
-                            tc_mma_16_pair(tmem_base + b * 256u, adesc + (A_MN ? 128u : 2u) * k, bdesc + (B_MN ? 128u : 2u) * k, idesc, (kb | k) ? 1u : 0u);
+                            tc_mma_16_pair(tmem_base + b * 256u, adesc + (DW ? 128u : 2u) * k, bdesc + 128u * k, idesc, (kb | k) ? 1u : 0u);
                         tc_commit_both(empty_at + 8u * s);
                     }
                     __syncwarp();
@@ -251,7 +259,7 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                 __syncwarp();
             }
             if (leader && *abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
-        } else if (WGRAD && warp == 2) {
+        } else if (DW && warp == 2) {
             // ------------------------------------------------------------ zeros behind the last row (both CTAs)
             uint32_t it = 0, phases = 0;  // bit s: parity of stage s's next ragged block
             for (int tile = pair_id; ok && locate(tile); tile += num_pairs) {
@@ -302,26 +310,10 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
         };
         for (int tile = pair_id; ok && locate(tile); tile += num_pairs, ++tcount) {
             const uint32_t b = tcount & 1u;
-            const int first = (WGRAD ? mt * 256 : 0) + static_cast<int>(cta) * BM;  // of this CTA's rows of the tile
-            const bool valid = first + r < (WGRAD ? p.m_dim : rows);
-            const size_t orow_i = WGRAD ? static_cast<size_t>(e) * p.m_dim + first + r : static_cast<size_t>(row0 + first + r);
-            const bool empty = WGRAD && rows == 0;
-            if constexpr (DSWIGLU) {
-                // this tile's gate and up come from memory while its MMAs run: a line per lane of each block of 32 rows x 32 columns
-                const int left = rows - (first + q * 32);
-                if (left > 0) {
-                    const int n = min(32, left);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int c = nt * 256 + h * 128 + cq * 32;
-                        const float* gu = p.gate_up + gate_up_at(static_cast<size_t>(row0 + first + q * 32), n, 0, p.n_dim, c);
-                        if (static_cast<int>(lane) < n && c + 32 <= p.n_dim) {
-                            asm volatile("prefetch.global.L2 [%0];" ::"l"(gu + lane * 32u));
-                            asm volatile("prefetch.global.L2 [%0];" ::"l"(gu + static_cast<size_t>(p.n_dim) * n + lane * 32u));
-                        }
-                    }
-                }
-            }
+            const int first = (DW ? mt * 256 : 0) + static_cast<int>(cta) * BM;  // of this CTA's rows of the tile
+            const bool valid = first + r < (DW ? p.m_dim : rows);
+            const size_t orow_i = DW ? static_cast<size_t>(e) * p.m_dim + first + r : static_cast<size_t>(row0 + first + r);
+            const bool empty = DW && rows == 0;
             const uint32_t t0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 256u + cq * 32;
             auto hand_back = [&]() {  // what this warp needs of the accumulator is in registers
                 tc_fence_before_sync();
@@ -331,21 +323,22 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     else mbar_arrive_cluster(map_to_cta(&bar_tempty[b], 0));
                 }
             };
-            if constexpr (DSWIGLU) {
+            if constexpr (!DW) {
                 // n_dim = I columns of da; dgu [rows, 2I].  16 columns at a time: their gate and up values are asked for before
                 // the accumulator is waited for, or while the 16 before them are worked on.
-                const int n = max(1, min(32, rows - (first + q * 32)));
-                const float* gu0 = p.gate_up + gate_up_at(static_cast<size_t>(row0 + first + q * 32), n, static_cast<int>(lane), p.n_dim, nt * 256 + cq * 32);
-                const size_t up = static_cast<size_t>(p.n_dim) * n;
-                float4 g4[4], u4[4];
+                const float* gu0 = p.gate_up + orow_i * (2 * static_cast<size_t>(p.n_dim)) + nt * 256 + cq * 32;
+                float g[16], u[16];
                 auto load = [&](int part) {  // part 0..3: half part / 2, columns 16 (part % 2)
                     const int off = (part >> 1) * 128 + (part & 1) * 16;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bool in = valid && nt * 256 + cq * 32 + off + 4 * i < p.n_dim;
-                        const float* at = gu0 + (off + 4 * i) * n;
-                        g4[i] = in ? ld_nc_f4(at) : make_float4(0, 0, 0, 0);
-                        u4[i] = in ? ld_nc_f4(at + up) : make_float4(0, 0, 0, 0);
+                    for (int i = 0; i < 16; i += 8) {
+                        if (valid && nt * 256 + cq * 32 + off + i < p.n_dim) {  // n_dim is a multiple of 8
+                            ld_nc_f8(gu0 + off + i, g + i);
+                            ld_nc_f8(gu0 + off + i + p.n_dim, u + i);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) g[i + j] = u[i + j] = 0.f;
+                        }
                     }
                 };
                 load(0);
@@ -364,14 +357,13 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     for (int part = 0; part < 2; ++part) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float gg[4] = {g4[i].x, g4[i].y, g4[i].z, g4[i].w}, uu[4] = {u4[i].x, u4[i].y, u4[i].z, u4[i].w};
                             float a[4], d[4];
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 const float da = __uint_as_float(v[part * 16 + 4 * i + k]);
-                                const float s = sigmoid_fast(gg[k]);
-                                a[k] = da * uu[k] * (s * (1.f + gg[k] * (1.f - s)));
-                                d[k] = da * (gg[k] * s);
+                                const float gg = g[4 * i + k], s = sigmoid_fast(gg);
+                                a[k] = da * u[4 * i + k] * (s * (1.f + gg * (1.f - s)));
+                                d[k] = da * (gg * s);
                             }
                             v[part * 8 + 2 * i] = pack16(a[0], a[1], fp16);  // words 0..15: dg; their da has been used
                             v[part * 8 + 2 * i + 1] = pack16(a[2], a[3], fp16);
@@ -396,28 +388,7 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             tc_wait_ld_regs(v1);
             hand_back();
             uint8_t* out = static_cast<uint8_t*>(p.out);
-            if constexpr (SWIGLU) {
-                const int c0 = nt * 128 + cq * 32;
-                if (p.gate_up != nullptr && valid) {
-                    const int n = min(32, rows - (first + q * 32));
-                    float* gu = p.gate_up + gate_up_at(static_cast<size_t>(row0 + first + q * 32), n, static_cast<int>(lane), p.n_dim, c0);
-                    const size_t up = static_cast<size_t>(p.n_dim) * n;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        if (c0 + j < p.n_dim) {  // n_dim is a multiple of 8
-                            *reinterpret_cast<uint4*>(gu + j * n) = make_uint4(v0[j], v0[j + 1], v0[j + 2], v0[j + 3]);
-                            *reinterpret_cast<uint4*>(gu + up + j * n) = make_uint4(v1[j], v1[j + 1], v1[j + 2], v1[j + 3]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    const float g0 = __uint_as_float(v0[j]), g1 = __uint_as_float(v0[j + 1]);
-                    v0[j >> 1] = pack16(g0 * sigmoid_fast(g0) * __uint_as_float(v1[j]),
-                                        g1 * sigmoid_fast(g1) * __uint_as_float(v1[j + 1]), fp16);
-                }
-                push(v0, valid ? out + orow_i * p.n_dim * 2 : nullptr, nt * 128, p.n_dim);
-            } else {
+            {
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
                     v0[j >> 1] = empty ? 0u : pack16(__uint_as_float(v0[j]), __uint_as_float(v0[j + 1]), fp16);
@@ -431,7 +402,292 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
         }
         if (cq == 0) bulk_wait_group<0>();  // every row this thread sent has been written
         if (!ok) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
-        if (EPI == kMlpPlain && !WGRAD)  // rows of no expert; act and dgu of such rows are read by nothing
+    }
+
+    // ------------------------------------------------------------------ teardown
+    abort_drain(abort_flag);
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();  // the other CTA may still read this CTA's shared memory or signal its barriers
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem_base, kEmTmemCols);
+    }
+}
+
+// One CTA pair, rows as N operand.  W_MN: the weights' contraction index is their row index in memory.
+constexpr int kErStages = 4;
+constexpr int kErStageBytes = 3 * kEmTile;  // two blocks of 128 weight rows, half of the rows
+constexpr int kErSmem = kErStages * kErStageBytes + kEmStgBytes + 1024;
+static_assert(kErSmem <= 232448, "exceeds the shared memory of one CTA");
+
+// Tiles of (expert, rows, weight rows): the rows of an expert in ceil(rows / 256) equal parts of whole 32s.
+struct PartWalker {
+    const int* off;
+    int num_experts, n_tiles, rows_total;
+    int e = 0, base = 0;
+    __device__ PartWalker(const int* o, int ne, int nt, int rt) : off(o), num_experts(ne), n_tiles(nt), rows_total(rt) {}
+    __device__ bool locate(int tile, int& e_out, int& nt, int& row0, int& rows) {
+        while (e < num_experts) {
+            const int first = expert_bound(off, e, rows_total);
+            const int cnt = max(expert_bound(off, e + 1, rows_total) - first, 0);
+            const int parts0 = max(1, (cnt + 255) / 256);
+            const int part = ((cnt + parts0 - 1) / parts0 + 31) & ~31;
+            const int tiles = cnt > 0 ? ((cnt + part - 1) / part) * n_tiles : 0;
+            if (tile < base + tiles) {
+                const int local = tile - base, mt = local / n_tiles;
+                nt = local - mt * n_tiles;
+                row0 = first + mt * part;
+                rows = min(part, cnt - mt * part);
+                e_out = e;
+                return true;
+            }
+            base += tiles;
+            ++e;
+        }
+        return false;
+    }
+};
+
+template <bool W_MN, bool SWIGLU>
+__global__ void __launch_bounds__(kEmThreads, 1)
+grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
+                            const __grid_constant__ CUtensorMap tmap_b, const GroupedMlpParams p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 1023u) {  // swizzled TMA tiles need it; the same in both CTAs of a pair
+        if (threadIdx.x == 0) gemm_record_status(&g_mlp_status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
+        return;
+    }
+    constexpr int NS = kErStages;
+    uint8_t* stg = smem + NS * kErStageBytes;
+    uint8_t* ctrl = stg + kEmStgBytes;
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(ctrl);  // first CTA: bytes of both CTAs' stage have landed
+    uint64_t* bar_empty = bar_full + NS;                     // each CTA: the MMAs that read a stage have retired
+    uint64_t* bar_tfull = bar_empty + NS;                    // each CTA: the accumulators of a tile are complete
+    uint64_t* bar_tempty = bar_tfull + 1;                    // first CTA: both CTAs have drained them
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_tempty + 1);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+
+    const int warp = static_cast<int>(threadIdx.x) >> 5;
+    const uint32_t lane = lane_id();
+    const uint32_t cta = cluster_cta_rank();  // 0 = first CTA of the pair (issues the MMAs)
+    const int pair_id = static_cast<int>(blockIdx.x) >> 1;
+    const int num_pairs = static_cast<int>(gridDim.x) >> 1;
+    const int nblk = (p.n_dim + 127) / 128;                             // blocks of result columns
+    const int n_tiles = SWIGLU ? (nblk + 1) / 2 : (nblk + 3) / 4;
+    const int kblocks = (p.k_dim + 63) / 64;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&bar_full[s], 1);
+            mbar_init(&bar_empty[s], 1);
+        }
+        mbar_init(bar_tfull, 1);
+        mbar_init(bar_tempty, 2 * (kEmEpiThreads / 32));
+        *abort_flag = 0u;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, kEmTmemCols);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();  // both CTAs' barriers are initialised before anything signals them
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    pdl_wait();
+    pdl_release();
+    PartWalker w(p.expert_offsets, p.num_experts, n_tiles, p.rows);
+    int e, nt, row0, rows;
+    bool ok = true;
+    // result columns of this CTA's two blocks; past the last block nothing is loaded that exists (zeros) and nothing is stored
+    auto col_lo = [&]() { return SWIGLU ? (2 * nt + static_cast<int>(cta)) * 128 : (4 * nt + 2 * static_cast<int>(cta)) * 128; };
+
+    if (warp < kEmEpiWarp0) {
+        reg_dealloc<kEmCtrlRegs>();
+        const uint32_t abort_at = smem_u32(tmem_slot + 1);
+        const uint32_t full_at = smem_u32(bar_full), empty_at = smem_u32(bar_empty);
+        if (warp == 0) {
+            // ------------------------------------------------------------ TMA producer (both CTAs)
+            const bool leader = elect_one();
+            if (leader) {
+                prefetch_tensormap(&tmap_a);
+                prefetch_tensormap(&tmap_a32);
+                prefetch_tensormap(&tmap_b);
+            }
+            Ring ring;
+            uint32_t ready = 1u;  // the first turn of every stage is free
+            const uint32_t full0 = map_to_cta(bar_full, 0);
+            for (int tile = pair_id; !aborted(abort_flag) && w.locate(tile, e, nt, row0, rows); tile += num_pairs) {
+                const int half = ((rows + 31) & ~31) / 2;  // rows of the tile in each CTA
+                const int pieces = (half + 31) / 32;
+                const uint32_t bytes = 2u * (2u * kEmTile + static_cast<uint32_t>(pieces) * 4096u);
+                const int my_row = row0 + static_cast<int>(cta) * half, lo = col_lo();
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    const uint32_t s = ring.s;
+                    if (!ready) mbar_wait_warp(empty_at + 8u * s, ring.ph ^ 1u, abort_at);
+                    ring.next(NS);
+                    ready = mbar_test(empty_at + 8u * ring.s, ring.ph ^ 1u);
+                    if (leader) {
+                        uint8_t* sw = smem + s * kErStageBytes;
+                        uint8_t* sr = sw + 2 * kEmTile;
+                        const uint32_t bar = full0 + 8u * s;
+                        if (cta == 0) mbar_arrive_expect_tx(&bar_full[s], bytes);
+                        if constexpr (W_MN) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) tma_load_3d_pair(sw + i * 8192, &tmap_b, bar, lo * 2 + i * 128, kb * 64, e);
+                        } else {
+                            tma_load_3d_pair(sw, &tmap_b, bar, kb * 128, lo, e);
+                            tma_load_3d_pair(sw + kEmTile, &tmap_b, bar, kb * 128, SWIGLU ? p.n_dim + lo : lo + 128, e);
+                        }
+                        if (pieces == 4) tma_load_2d_pair(sr, &tmap_a, bar, kb * 128, my_row);
+                        else for (int i = 0; i < pieces; ++i) tma_load_2d_pair(sr + i * 4096, &tmap_a32, bar, kb * 128, my_row + i * 32);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (leader && *abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 0, 1);
+        } else if (warp == 1 && cta == 0) {
+            // ------------------------------------------------------------ MMA issuer (first CTA only)
+            const bool leader = elect_one();
+            Ring ring;
+            uint32_t tcount = 0, ready = 0u;
+            for (int tile = pair_id; !aborted(abort_flag) && w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
+                const uint32_t n = static_cast<uint32_t>((rows + 31) & ~31);
+                const uint32_t idesc = umma_idesc(2 * BM, 0, 1u, p.fp16 ? 0u : 1u) | ((n >> 3) << 17) | (W_MN ? 1u << 15 : 0u);
+                // both epilogues must have drained the accumulators
+                mbar_wait_warp(smem_u32(bar_tempty), (tcount & 1u) ^ 1u, abort_at);
+                tc_fence_after_sync();
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    const uint32_t s = ring.s;
+                    if (!ready) mbar_wait_warp(full_at + 8u * s, ring.ph, abort_at);
+                    tc_fence_after_sync();
+                    ring.next(NS);
+                    ready = mbar_test(full_at + 8u * ring.s, ring.ph);
+                    const uint32_t sw = smem_u32(smem) + s * kErStageBytes;
+                    const uint64_t lo = W_MN ? umma_desc_mn_sw128(sw) : umma_desc_k_sw128(sw);
+                    const uint64_t hi = W_MN ? umma_desc_mn_sw128(sw + kEmTile) : umma_desc_k_sw128(sw + kEmTile);
+                    const uint64_t rd = umma_desc_k_sw128(sw + 2 * kEmTile);
+                    if (leader) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {  // 16 of the contraction: 32 bytes of a row, or 16 rows of 128 bytes
+                            tc_mma_16_pair(tmem_base, lo + (W_MN ? 128u : 2u) * k, rd + 2u * k, idesc, (kb | k) ? 1u : 0u);
+                            tc_mma_16_pair(tmem_base + 256u, hi + (W_MN ? 128u : 2u) * k, rd + 2u * k, idesc, (kb | k) ? 1u : 0u);
+                        }
+                        tc_commit_both(empty_at + 8u * s);
+                    }
+                    __syncwarp();
+                }
+                if (leader) tc_commit_both(smem_u32(bar_tfull));
+                __syncwarp();
+            }
+            if (leader && *abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
+        }
+    } else {
+        reg_alloc<kEmEpiRegs>();
+        // ---------------------------------------------------------------- epilogue warps: a result column per lane
+        const int ew = warp - kEmEpiWarp0;
+        const int q = warp & 3;   // TMEM lane quarter this warp may read
+        const int cq = ew >> 2;   // which 32 rows of each 128
+        const int f = q * 32 + static_cast<int>(lane);  // column inside a block of 128
+        const bool fp16 = p.fp16 != 0;
+        uint8_t* out = static_cast<uint8_t*>(p.out);
+        // 128 rows x 128 columns go through shared memory and leave as one bulk copy per row: w16 holds rows (2 i, 2 i + 1) of this
+        // thread's 32; the rows start at row r0 of the tile, the columns at column c of a matrix `width` wide with rows `pitch` apart
+        auto push = [&](const uint32_t* w16, int r0, uint8_t* base, size_t pitch, int c, int width) {
+            if (cq == 0) bulk_wait_group_read<0>();  // the copies that read this buffer are done with it
+            named_bar_sync(1, kEmEpiThreads);
+            if (r0 + cq * 32 < rows) {
+                uint8_t* at = stg + (cq * 32) * kEmStgPitch + f * 2;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    *reinterpret_cast<uint16_t*>(at + (2 * j) * kEmStgPitch) = static_cast<uint16_t>(w16[j]);
+                    *reinterpret_cast<uint16_t*>(at + (2 * j + 1) * kEmStgPitch) = static_cast<uint16_t>(w16[j] >> 16);
+                }
+            }
+            fence_proxy_async_smem();
+            named_bar_sync(1, kEmEpiThreads);
+            if (cq == 0) {
+                if (r0 + f < rows)
+                    bulk_store_s2g(base + static_cast<size_t>(row0 + r0 + f) * pitch + static_cast<size_t>(c) * 2, stg + f * kEmStgPitch,
+                                   static_cast<uint32_t>(min(128, width - c)) * 2u);
+                bulk_commit_group();
+            }
+        };
+        uint32_t tcount = 0;
+        for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
+            const uint32_t t0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(cq * 32);
+            const int c_lo = col_lo();
+            const bool two = rows > 128;  // a second 128 rows: the same in every thread of the CTA
+            const bool has[2] = {cq * 32 < rows, 128 + cq * 32 < rows};  // columns past the tile's rows were not written
+            auto hand_back = [&]() {  // what this warp needs of the accumulators is in registers
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if (cta == 0) mbar_arrive(bar_tempty);
+                    else mbar_arrive_cluster(map_to_cta(bar_tempty, 0));
+                }
+            };
+            if (!mbar_wait_bounded(bar_tfull, tcount & 1u, abort_flag, 2000000000ull, 64u)) { ok = false; break; }
+            tc_fence_after_sync();
+            if constexpr (SWIGLU) {
+                uint32_t act[2][16];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (has[h]) {
+                        uint32_t v0[32], v1[32];
+                        tmem_ld_32x32b_x32(t0 + h * 128u, v0);
+                        tmem_ld_32x32b_x32(t0 + h * 128u + 256u, v1);
+                        tc_wait_ld_regs(v0);
+                        tc_wait_ld_regs(v1);
+                        if (p.gate_up != nullptr && c_lo + f < p.n_dim) {
+                            const size_t pitch = 2 * static_cast<size_t>(p.n_dim);
+                            const int left = rows - (h * 128 + cq * 32);
+                            float* gu = p.gate_up + static_cast<size_t>(row0 + h * 128 + cq * 32) * pitch + c_lo + f;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                if (j < left) {
+                                    gu[j * pitch] = __uint_as_float(v0[j]);
+                                    gu[j * pitch + p.n_dim] = __uint_as_float(v1[j]);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            const float g0 = __uint_as_float(v0[j]), g1 = __uint_as_float(v0[j + 1]);
+                            act[h][j >> 1] = pack16(g0 * sigmoid_fast(g0) * __uint_as_float(v1[j]), g1 * sigmoid_fast(g1) * __uint_as_float(v1[j + 1]), fp16);
+                        }
+                    }
+                }
+                hand_back();
+                if (c_lo < p.n_dim) {  // the same in every thread of the CTA
+                    push(act[0], 0, out, static_cast<size_t>(p.n_dim) * 2, c_lo, p.n_dim);
+                    if (two) push(act[1], 128, out, static_cast<size_t>(p.n_dim) * 2, c_lo, p.n_dim);
+                }
+            } else {
+                uint32_t res[4][16];  // [128 rows][block]
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (has[i >> 1]) {
+                        uint32_t v[32];
+                        tmem_ld_32x32b_x32(t0 + (i >> 1) * 128u + (i & 1) * 256u, v);
+                        tc_wait_ld_regs(v);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) res[i][j >> 1] = pack16(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), fp16);
+                    }
+                }
+                hand_back();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = c_lo + (i & 1) * 128;
+                    if (c < p.n_dim && (i < 2 || two)) push(res[i], (i >> 1) * 128, out, static_cast<size_t>(p.n_dim) * 2, c, p.n_dim);
+                }
+            }
+        }
+        if (cq == 0) bulk_wait_group<0>();  // every row this thread sent has been written
+        if (!ok) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
+        if (!SWIGLU)  // rows of no expert; act and dgu of such rows are read by nothing
             zero_loose_rows(p.out, p.n_dim / 8, p.expert_offsets, p.num_experts, p.rows, static_cast<int>(threadIdx.x) - kEmEpiWarp0 * 32, kEmEpiThreads);
     }
 
@@ -450,14 +706,21 @@ grouped_gemm_16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 
 namespace {
 
-template <bool A_MN, bool B_MN, int EPI>
-int launch_16(const cam::GroupedMlpParams* p, const CUtensorMap* ta, const CUtensorMap* ta32, const CUtensorMap* tb, cudaStream_t stream) {
+template <bool W_MN, bool SWIGLU>
+int launch_rows(const cam::GroupedMlpParams* p, const CUtensorMap* ta, const CUtensorMap* ta32, const CUtensorMap* tb, cudaStream_t stream) {
     static cam::PairLimit limit;
-    const int64_t n_tiles = EPI == cam::kMlpSwiglu ? (p->n_dim + 127) / 128 : (p->n_dim + 255) / 256;
-    // row blocks: at most one per expert beyond the full ones
-    const int64_t blocks = A_MN ? static_cast<int64_t>(p->num_experts) * ((p->m_dim + 255) / 256)
-                                : p->rows / 256 + (p->rows < p->num_experts ? p->rows : p->num_experts);
-    return cam::launch_pairs(limit, cam::grouped_gemm_16_kernel<A_MN, B_MN, EPI>, cam::kEmThreads, cam::kEmSmem, blocks * n_tiles, stream, *ta, *ta32, *tb, *p);
+    const int64_t nblk = (p->n_dim + 127) / 128, n_tiles = SWIGLU ? (nblk + 1) / 2 : (nblk + 3) / 4;
+    // parts of an expert's rows: at most one beyond the full ones
+    const int64_t parts = p->rows / 256 + (p->rows < p->num_experts ? p->rows : p->num_experts);
+    return cam::launch_pairs(limit, cam::grouped_gemm_16_rows_kernel<W_MN, SWIGLU>, cam::kEmThreads, cam::kErSmem, parts * n_tiles, stream, *ta, *ta32, *tb, *p);
+}
+
+template <bool DW>
+int launch_square(const cam::GroupedMlpParams* p, const CUtensorMap* ta, const CUtensorMap* ta32, const CUtensorMap* tb, cudaStream_t stream) {
+    static cam::PairLimit limit;
+    const int64_t blocks = DW ? static_cast<int64_t>(p->num_experts) * ((p->m_dim + 255) / 256)
+                              : p->rows / 256 + (p->rows < p->num_experts ? p->rows : p->num_experts);
+    return cam::launch_pairs(limit, cam::grouped_gemm_16_square_kernel<DW>, cam::kEmThreads, cam::kEmSmem, blocks * ((p->n_dim + 255) / 256), stream, *ta, *ta32, *tb, *p);
 }
 
 }  // namespace
@@ -465,11 +728,11 @@ int launch_16(const cam::GroupedMlpParams* p, const CUtensorMap* ta, const CUten
 extern "C" int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, const CUtensorMap* tmap_a, const CUtensorMap* tmap_a32,
                                       const CUtensorMap* tmap_b, cudaStream_t stream) {
     switch (form) {
-        case cam::kMlpUp: return launch_16<false, false, cam::kMlpSwiglu>(p, tmap_a, tmap_a32, tmap_b, stream);
-        case cam::kMlpDown: return launch_16<false, false, cam::kMlpPlain>(p, tmap_a, tmap_a32, tmap_b, stream);
-        case cam::kMlpDact: return launch_16<false, true, cam::kMlpSwigluBackward>(p, tmap_a, tmap_a32, tmap_b, stream);
-        case cam::kMlpDx: return launch_16<false, true, cam::kMlpPlain>(p, tmap_a, tmap_a32, tmap_b, stream);
-        case cam::kMlpDw: return launch_16<true, true, cam::kMlpPlain>(p, tmap_a, tmap_a, tmap_b, stream);
+        case cam::kMlpUp: return launch_rows<false, true>(p, tmap_a, tmap_a32, tmap_b, stream);
+        case cam::kMlpDown: return launch_rows<false, false>(p, tmap_a, tmap_a32, tmap_b, stream);
+        case cam::kMlpDact: return launch_square<false>(p, tmap_a, tmap_a32, tmap_b, stream);
+        case cam::kMlpDx: return launch_rows<true, false>(p, tmap_a, tmap_a32, tmap_b, stream);
+        case cam::kMlpDw: return launch_square<true>(p, tmap_a, tmap_a, tmap_b, stream);
     }
     return static_cast<int>(cudaErrorInvalidValue);
 }

@@ -228,6 +228,7 @@ extern "C" int cam_grouped_mlp_down(const void* act, const void* w2, const int* 
 extern "C" int cam_grouped_mlp_dact(const void* dy, const void* w2, const float* gate_up, const int* offsets, int rows, int num_experts,
                                     int h, int inter, int dtype, void* dgu, cudaStream_t stream) {
     EXP_CHECK(gate_up != nullptr, "grouped_mlp (dact): null operand");
+    EXP_CHECK(aligned(gate_up, 32), "grouped_mlp (dact): gate_up must be 32-byte aligned");
     return row_product(cam::kMlpDact, "grouped_mlp (dact)", dy, h, w2, h, inter, true, inter, offsets, rows, num_experts, dtype, dgu,
                        const_cast<float*>(gate_up), stream);
 }

@@ -25,8 +25,7 @@ int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, const void*
                          const float* w_gscale, const float* out_gscale, void* out, void* out_s, cudaStream_t stream);
 
 // Gated feed-forward block of 16-bit experts (kernels/grouped_mlp.cu), dtype 0 bf16 or 1 fp16.  x, y, dy, dx [rows, h], w1, dw1
-// [E, 2I, h] (gate rows first), w2, dw2 [E, h, I], act [rows, I]; gate_up rows x 2I fp32 in an order of its own
-// (null: not kept), dgu [rows, 2I].
+// [E, 2I, h] (gate rows first), w2, dw2 [E, h, I], act [rows, I]; gate_up [rows, 2I] fp32 (null: not kept), dgu [rows, 2I].
 // Rows outside [offsets[0], offsets[E]) of y and dx, and gradients of experts without rows, are written as zeros.
 int cam_grouped_mlp_up(const void* x, const void* w1, const int* offsets, int rows, int num_experts, int h, int inter, int dtype,
                        void* act, float* gate_up, cudaStream_t stream);
