@@ -340,6 +340,84 @@ def test_dispatch_experts_combine(ops, fmt):
     buf.destroy()
 
 
+def test_backward_after_the_next_dispatch(ops):
+    """Two layers share a Buffer: the second dispatch overwrites the rows that the first layer's experts saw, before backward runs."""
+    from umdk_original_b200 import Buffer, CamConfig
+    from umdk_original_b200.models import ExpertMLP, offsets_from_counts
+    t, h, inter, e, k = 32, 128, 64, 4, 2
+    gen = torch.Generator().manual_seed(11)
+    idx = torch.stack([torch.randperm(e, generator=gen)[:k] for _ in range(t)]).to(DEV)
+    wt = torch.rand(t, k, generator=gen).to(DEV)
+    buf = Buffer(None, CamConfig(num_experts=e, max_tokens=t, hidden=h, topk=k, timeout_ms=2000.0), name="expert_mlp_two_layers",
+                 device=torch.device(DEV, 0), rank=0, num_ranks=1)
+    layers = [ExpertMLP(e, h, inter, device=DEV, seed=s) for s in (1, 2)]
+    loss, rows = 0.0, []
+    for layer in layers:
+        x = torch.randn(t, h, generator=gen).to(torch.bfloat16).to(DEV)
+        rx, _, _, per_e, _ = ops.moe_dispatch_prefill_quant(x, idx, wt, buf.capacity, buf.name, 0, 1, 0)
+        off = offsets_from_counts(per_e)
+        rows.append((rx, rx.clone(), off))
+        loss = loss + layer(rx, off).float().square().sum()
+    assert not torch.equal(rows[0][0], rows[0][1])  # overwritten
+    got = torch.autograd.grad(loss, [p for layer in layers for p in (layer.w1, layer.w2)])
+    want = []
+    for layer, (_, rx, off) in zip(layers, rows):
+        want += torch.autograd.grad(layer(rx, off).float().square().sum(), (layer.w1, layer.w2))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    buf.check()
+    buf.destroy()
+
+
+def test_waits_for_another_stream(ops):
+    """The kernels may start before the one ahead of them on their stream has finished, but not before an event they wait for."""
+    x, w1, w2, dy, off = make(torch.bfloat16, 256, 128, "holes")
+    want = ops.grouped_mlp(x, w1, w2, off)
+    late = torch.zeros_like(w1)
+    side = torch.cuda.Stream()
+
+    def run():
+        side.wait_stream(torch.cuda.current_stream())
+        y = ops.grouped_mlp(x, w1, w2, off)  # the kernel ahead on this stream
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(2_000_000)  # about a millisecond
+            late.copy_(w1)
+        torch.cuda.current_stream().wait_stream(side)
+        return y, ops.grouped_mlp(x, late, w2, off)
+
+    assert all(torch.equal(y, want) for y in run())
+    late.zero_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run()
+    late.zero_()
+    g.replay()
+    assert all(torch.equal(y, want) for y in out)
+
+
+def test_calls_from_two_host_threads(ops):
+    import threading
+    x, w1, w2, dy, off = make(torch.bfloat16, 264, 136, "holes")
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            leaves = [t.clone().requires_grad_() for t in (x, w1, w2)]
+            for _ in range(20):
+                y = ops.grouped_mlp(*leaves, off)
+                got[i] = (y.detach(), *torch.autograd.grad(y, leaves, dy))
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    leaves = [t.clone().requires_grad_() for t in (x, w1, w2)]
+    y = ops.grouped_mlp(*leaves, off)
+    want = (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    for one in got:
+        assert all(torch.equal(a, b) for a, b in zip(one, want))
+
+
 def test_status_after_everything(ops):
     from umdk_original_b200.ops import cam_ops
     assert cam_ops.native_module().expert_ops_status()[0] == 0

@@ -303,12 +303,20 @@ Mlp3 call_mlp_train(const at::Tensor& x, const at::Tensor& w1, const at::Tensor&
     return op.call(x, w1, w2, off);
 }
 
+// What the backward pass will read of an input.  The rows of a dispatch are views of memory that the next dispatch on that Buffer
+// overwrites, behind the back of autograd's version counters, and a program of several layers dispatches again before it runs
+// backward: such memory (any that PyTorch's allocators do not own) is copied.
+at::Tensor kept_for_backward(const at::Tensor& t) {
+    return t.storage().unsafeGetStorageImpl()->resizable() ? t : t.clone();
+}
+
 struct GroupedMlpFunction : public torch::autograd::Function<GroupedMlpFunction> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2,
                               const at::Tensor& expert_offsets) {
         at::AutoDispatchBelowADInplaceOrView guard;
         auto [y, act, gu] = call_mlp_train(x, w1, w2, expert_offsets);
-        ctx->save_for_backward({x, w1, w2, expert_offsets, act, gu});
+        // x itself enters the gradient of w1 only
+        ctx->save_for_backward({w1.requires_grad() ? kept_for_backward(x) : x, w1, w2, kept_for_backward(expert_offsets), act, gu});
         return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {

@@ -5,7 +5,9 @@ scales (the formats are described in csrc/common/fp4.cuh).  The CUDA implementat
 ones here follow the same contracts in fp32, expert by expert.
 
 ``grouped_mlp``: the gated feed-forward block of 16-bit experts, differentiable in the rows and both weights.  Its parts,
-``grouped_mlp_train`` (also returns what the backward pass needs: act, and the gate and up values in fp32) and ``grouped_mlp_backward``, can be called by programs that keep their own graph of derivatives.
+``grouped_mlp_train`` (also returns what the backward pass needs: act, and the gate and up values in fp32) and
+``grouped_mlp_backward``, can be called by programs that keep their own graph of derivatives.  Rows of no expert hold nothing
+defined in act and in the gate and up values; the backward pass reads none of them.
 """
 from __future__ import annotations
 
