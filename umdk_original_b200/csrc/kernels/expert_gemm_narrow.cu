@@ -12,6 +12,12 @@
 //     in the staging area of the CTA that finishes the row (distributed shared memory), which adds them up in the CTAs' order.
 // The accumulator has a weight row per lane and a row of the expert per column; it goes through shared memory as fp32, and the
 // threads that pick it up again own 8 or 16 neighbouring columns of a row each.
+//
+// Measured (one call, L2 cold, launch included): 32 experts of 32 rows, nvfp4, 7168 -> 2 x 2048 with SwiGLU 111 us (4.9 TB/s), 29 of 35
+// rows, 2048 -> 7168 62 us (4.2 TB/s); mxfp4 100 and 57 us; 8 experts of one row 43 and 29 us; 16 experts of 32 rows in 16 bits, 4096 -> 2
+// x 1024 50 us, 1024 -> 4096 28 us.  Left out one at a time, the weights, the scales and the MMAs each save 10 to 15 %, all three half:
+// no single unit is saturated, the short tiles (8 to 28 K-blocks) leave the turns of the stages, the start and the last wave.
+// Scales stored to tensor memory from registers, loaded a group ahead: no faster (62 us), and 10 % slower for one row per expert.
 #include "expert_gemm.cuh"
 
 namespace cam {

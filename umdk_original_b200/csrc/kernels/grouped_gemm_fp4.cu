@@ -11,8 +11,17 @@
 // the upper 128 weight rows) bring them there, four K-blocks at a time: 64 bytes of a row are copied by four lanes with cp.async,
 // each to the slot of its K-block, then lane l transposes the 4 x 4 words of rows l, 32 + l, 64 + l, 96 + l of each K-block in
 // place and the warp raises the group's barrier.  The MMA issuer moves a slot into tensor memory with tcgen05.cp directly in
-// front of the MMAs that read it.  What sets the pace of these warps is the number of rows they touch, not the bytes: one K-block
-// at a time (16 bytes of every row) took 1070 cycles per K-block where the MMAs take 512.
+// front of the MMAs that read it.  Four K-blocks at a time, because these warps are paced by the rows
+// they touch: one K-block at a time (16 bytes of every row) took them 1070 cycles where the MMAs take 512.
+//
+// Measured (one call, L2 cold): 16 experts of 1024 rows, 7168 -> 2 x 2048 with SwiGLU: nvfp4 240 us (4.0 PFLOP/s), mxfp4 184 us (5.2);
+// 32 of 1024 rows, 2048 -> 7168: 287 us (3.4) and 240 us (4.0).  Under back-to-back calls the power limit takes a third of that.
+// What bounds it is the work in shared memory: a K-block brings 32 KiB per CTA by TMA, the MMAs read as much, and the nvfp4 scales
+// are written, transposed and copied on, 24 KiB more; half of that for mxfp4, which is what it is faster by.
+// Tried in place of this arrangement (nvfp4 / mxfp4 us for the first of these sizes, 240 / 184 as it is):
+//   two sets of scale warps that take groups in turn               248 / 188   the copies' latency is hidden already
+//   stages of two K-blocks, half as many barrier turns             237 / 213   less lookahead
+//   scales stored to tensor memory from registers, no transpose    268 / 217   four warps, one per lane quarter, read every word
 //
 // Barriers: as in grouped_gemm_mx2.cu, bar_sf counts the three scale warps of each CTA;
 // bar_sfe[group], in each CTA, tells that tensor memory has the scales of the group's K-blocks.

@@ -50,49 +50,90 @@ int env_switch(const char* name) {
     return v != nullptr && *v != 0 ? std::atoi(v) : -1;
 }
 
-// The form for few rows per expert (expert_gemm_narrow.cu), or CTA pairs with tiles of 256 x 256?  Up to 128 rows per expert the
-// first takes 0.77 - 1.0 of the time of the second (16 experts of 4096 x 1024, 4 of 7168 x 2048, one of either; 16 and 4 bits), at
-// 160 it computes two tiles where the pairs compute one: 1.2 - 2.0.  With fewer than 32 pair tiles most SMs would stand still, while
-// the form for few rows divides a tile's K-blocks: one expert of 7168 x 2048, 256 rows 0.82 - 0.95, of 2048 x 1024, 768 rows 0.9 - 1.0.
-bool narrow_pays(int rows, int num_experts, int n_dim, bool swiglu) {
+// Shape of a product in the form for few rows (expert_gemm_narrow.cu)
+struct FewRows {
+    int slot_rows, kblocks, chunked, chunks, stages, split;
+    int64_t upper;   // row blocks there can be
+    int64_t cycles;  // estimate
+};
+
+FewRows plan_few_rows(int rows, int num_experts, int64_t n_tiles, int row_bytes, bool fp4) {
+    FewRows f{};
+    const int sms = cam::sm_count_of_current_device();
+    // Room for twice the mean rows per expert: larger experts are cut, and their weights come from L2 for the further tiles.
+    const int64_t mean = (static_cast<int64_t>(rows) + num_experts - 1) / num_experts;
+    f.slot_rows = rows <= 32 || mean <= 16 ? 32 : rows <= 64 || mean <= 40 ? 64 : 128;
+    const int64_t blocks = rows <= num_experts ? rows : static_cast<int64_t>(num_experts) * ((mean + f.slot_rows - 1) / f.slot_rows);
+    f.upper = rows / f.slot_rows + (rows < num_experts ? rows : num_experts);
+    f.kblocks = (row_bytes + 127) / 128;
+    f.chunked = row_bytes % 128 == 0;
+    const int per_chunk = (f.slot_rows + 128) * 128, room = 232448 - cam_expert_narrow_fixed_smem(fp4, f.slot_rows);
+    f.chunks = f.chunked && f.kblocks > 1 && room / (2 * per_chunk) >= 3 ? 2 : 1;
+    const int fit = room / (f.chunks * per_chunk), most = cam_expert_narrow_max_stages();
+    f.stages = fit < most ? fit : most;
+    // CTAs per tile: turns of the SMs x cycles of a turn (a K-block at an SM's share of the memory bandwidth, a fixed part, the
+    // exchange inside the cluster)
+    const int unit = fp4 ? 4 : f.chunks, units = (f.kblocks + unit - 1) / unit;
+    const int forced = env_switch("UMDK_CAM_EXPERT_SPLIT");
+    int64_t best = -1;
+    for (int split = 1; split <= 4 && split <= units; split *= 2) {  // clusters of 8 find too few places at once
+        const int64_t turns = (blocks * n_tiles + sms / split - 1) / (sms / split);
+        const int64_t blocks_k = static_cast<int64_t>((units + split - 1) / split) * unit, fixed = 1500 + (split > 1 ? 2000 : 0);
+        const int64_t cost = turns * (blocks_k * 770 + fixed);
+        if (forced > 0 ? split <= forced : best < 0 || cost < best) {
+            best = cost;
+            f.split = split;
+            f.cycles = turns * (blocks_k * (770 + f.slot_rows) + fixed);  // tall tiles also take their rows from L2
+        }
+    }
+    return f;
+}
+
+// That form, or CTA pairs?  Up to 128 rows per expert it takes 0.5 - 1.02 of the time of the pairs (1 to 64 experts of 2048 x 768 to
+// 7168 x 2048, 16 to 128 rows, 16 and 4 bits).
+//
+// 4 bits above that: at 160 rows it computes two tiles where the pairs compute one, 1.0 - 1.3.  With fewer than 32 tiles of 256 x 256
+// most SMs would stand still in pairs, while this form divides a tile's K-blocks: one expert of 7168 x 2048, 160 - 512 rows, or of 2048 x
+// 1024, 160 - 768 rows: 0.75 - 1.15.
+bool few_rows_pay_fp4(int rows, int num_experts, int n_dim, bool swiglu) {
     const int sw = env_switch("UMDK_CAM_EXPERT_NARROW");
     if (sw >= 0) return sw != 0;
     const int64_t mean = (static_cast<int64_t>(rows) + num_experts - 1) / num_experts;
     return mean <= 128 || (mean + 255) / 256 * num_experts * ((n_dim + (swiglu ? 127 : 255)) / (swiglu ? 128 : 256)) < 32;
 }
 
-// The form for few rows: rows of a tile, stages, clusters, maps, launch.  `row_bytes` of the row operand and of the weights'
-// rows; n_dim, the operands' scales and outputs are set.
+// 16 bits above that: the pairs' tiles are larger still, 512 weight rows x 256, and the smaller of two estimates decides.  Pairs: turns
+// of the SMs x (K-blocks of 700 + 3 per row cycles, or the memory's time for their weights, and 18000 for a tile's start and end).
+// One expert of 7168 x 2048, 512 rows 112 (pairs) / 77 us; 8 of 2048 x 1024, 256 rows 66 / 56, 384 rows 65 / 71; 4 of 7168 x 2048, 160
+// rows 110 / 196.  Over 66 sizes (these, 16 of 4096 x 1024, 64 of 2048 x 768; 16 - 768 rows) the choice is at most 2 % behind the better
+// form, over 24 others 4 %.
+bool few_rows_pay_16(int rows, int num_experts, int n_dim, bool swiglu, int k) {
+    const int sw = env_switch("UMDK_CAM_EXPERT_NARROW");
+    if (sw >= 0) return sw != 0;
+    const int64_t mean = (static_cast<int64_t>(rows) + num_experts - 1) / num_experts;
+    if (mean <= 128) return true;
+    const int step = swiglu ? 64 : 128, wide = swiglu ? 256 : 512;
+    const int64_t parts = (mean + 255) / 256, cols = ((mean + parts - 1) / parts + 31) / 32 * 32;
+    const int64_t most = cam::sm_count_of_current_device() / 2;
+    const int64_t tiles = num_experts * parts * ((n_dim + wide - 1) / wide), busy = tiles < most ? tiles : most;
+    const int64_t turns = (tiles + most - 1) / most, work = 700 + 3 * cols, memory = 1420 * busy / most;
+    const FewRows f = plan_few_rows(rows, num_experts, (n_dim + step - 1) / step, k * 2, false);
+    return f.cycles < turns * (f.kblocks * (work > memory ? work : memory) + 18000);
+}
+
+// The form for few rows: maps and launch.  `row_bytes` of the row operand and of the weights' rows; n_dim, the operands' scales and
+// outputs are set.
 int launch_narrow(cam::NarrowParams* p, int kind, bool swiglu, const void* a, const void* w, int row_bytes, const char* what, cudaStream_t stream) {
-    const bool fp4 = kind != cam::kNarrow16;
-    const int sms = cam::sm_count_of_current_device();
     const int step = swiglu ? 64 : 128;
     const int64_t n_tiles = (p->n_dim + step - 1) / step;
-    // Room for twice the mean rows per expert: larger experts are cut, and their weights come from L2 for the further tiles.
-    const int64_t mean = (p->rows + p->num_experts - 1) / p->num_experts;
-    p->slot_rows = p->rows <= 32 || mean <= 16 ? 32 : p->rows <= 64 || mean <= 40 ? 64 : 128;
-    const int64_t blocks = p->rows <= p->num_experts ? p->rows : static_cast<int64_t>(p->num_experts) * ((mean + p->slot_rows - 1) / p->slot_rows);
-    const int64_t upper = p->rows / p->slot_rows + (p->rows < p->num_experts ? p->rows : p->num_experts);  // row blocks there can be
-    p->kblocks = (row_bytes + 127) / 128;
-    p->chunked = row_bytes % 128 == 0;
-    const int per_chunk = (p->slot_rows + 128) * 128, room = 232448 - cam_expert_narrow_fixed_smem(fp4, p->slot_rows);
-    p->chunks = p->chunked && p->kblocks > 1 && room / (2 * per_chunk) >= 3 ? 2 : 1;
-    p->stage_bytes = p->chunks * per_chunk;
-    const int fit = room / p->stage_bytes, most = cam_expert_narrow_max_stages();
-    p->stages = fit < most ? fit : most;
-    // CTAs per tile: turns of the SMs x cycles of a turn (a K-block at an SM's share of the memory bandwidth, a fixed part, the
-    // exchange inside the cluster)
-    const int unit = fp4 ? 4 : p->chunks, units = (p->kblocks + unit - 1) / unit;
-    const int forced = env_switch("UMDK_CAM_EXPERT_SPLIT");
-    int64_t best = -1;
-    for (int split = 1; split <= 4 && split <= units; split *= 2) {  // clusters of 8 find too few places at once
-        const int64_t turns = (blocks * n_tiles + sms / split - 1) / (sms / split);
-        const int64_t cost = turns * (static_cast<int64_t>((units + split - 1) / split) * unit * 770 + 1500 + (split > 1 ? 2000 : 0));
-        if (forced > 0 ? split <= forced : best < 0 || cost < best) {
-            best = cost;
-            p->split = split;
-        }
-    }
+    const FewRows f = plan_few_rows(p->rows, p->num_experts, n_tiles, row_bytes, kind != cam::kNarrow16);
+    p->slot_rows = f.slot_rows;
+    p->kblocks = f.kblocks;
+    p->chunked = f.chunked;
+    p->chunks = f.chunks;
+    p->stages = f.stages;
+    p->stage_bytes = f.chunks * (f.slot_rows + 128) * 128;
+    p->split = f.split;
     const uint64_t bytes = p->chunked ? 128 : static_cast<uint64_t>(row_bytes), blocks_k = p->chunked ? static_cast<uint64_t>(p->kblocks) : 1;
     const uint64_t pitch = static_cast<uint64_t>(row_bytes), halves = swiglu ? 2 : 1, n = static_cast<uint64_t>(p->n_dim);
     CUtensorMap ta, tb;
@@ -102,7 +143,7 @@ int launch_narrow(cam::NarrowParams* p, int kind, bool swiglu, const void* a, co
     const uint64_t db[5] = {bytes, n, halves, blocks_k, static_cast<uint64_t>(p->num_experts)}, sb[4] = {pitch, pitch * n, 128, pitch * n * halves};
     const uint32_t bb[5] = {128, static_cast<uint32_t>(step), static_cast<uint32_t>(halves), static_cast<uint32_t>(p->chunks), 1};
     if (cam_encode_tmap(&tb, w, 5, db, sb, bb) != 0) return -1;
-    return launched(cam_launch_expert_gemm_narrow(p, kind, swiglu, upper * n_tiles, &ta, &tb, stream), what);
+    return launched(cam_launch_expert_gemm_narrow(p, kind, swiglu, f.upper * n_tiles, &ta, &tb, stream), what);
 }
 
 }  // namespace
@@ -138,7 +179,7 @@ extern "C" int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, 
     EXP_CHECK(n_dim >= 128 && n_dim % (swiglu ? 256 : 128) == 0, "grouped_gemm_fp4: N %d must be a multiple of %d", n_dim, swiglu ? 256 : 128);
     EXP_CHECK(static_cast<int64_t>(num_experts) * n_dim < (1ll << 31), "grouped_gemm_fp4: weight rows overflow");
     EXP_CHECK(aligned(a_s, 4) && aligned(w_s, 4), "grouped_gemm_fp4: scales must be 4-byte aligned");
-    if (narrow_pays(rows, num_experts, swiglu ? n_dim / 2 : n_dim, swiglu != 0)) {
+    if (few_rows_pay_fp4(rows, num_experts, swiglu ? n_dim / 2 : n_dim, swiglu != 0)) {
         cam::NarrowParams p{};
         p.expert_offsets = offsets;
         p.num_experts = num_experts;
@@ -185,7 +226,7 @@ int row_product(int form, const char* what, const void* a, int k, const void* w,
     EXP_CHECK(a && w && offsets && out, "%s: null operand", what);
     EXP_CHECK(rows >= 1 && num_experts >= 1, "%s: empty problem", what);
     EXP_CHECK(k >= 8 && n >= 8 && k % 8 == 0 && n % 8 == 0, "%s: sizes %d and %d must be multiples of 8", what, k, n);
-    if (!by_rows && narrow_pays(rows, num_experts, n, form == cam::kMlpUp)) {
+    if (!by_rows && few_rows_pay_16(rows, num_experts, n, form == cam::kMlpUp, k)) {
         const bool swiglu = form == cam::kMlpUp;
         cam::NarrowParams p{};
         p.expert_offsets = offsets;
