@@ -207,6 +207,27 @@ __device__ __forceinline__ uint32_t fp4_scale_at(int j) {
 // enters carry more), 0 where e^-x overflows.
 __device__ __forceinline__ float sigmoid_fast(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
+// act = silu(g) u with the gradient da of act: dg = da u s (1 + g (1 - s)), du = da g s, s = 1 / (1 + e^-g)
+__device__ __forceinline__ void gated_gradients(float da, float g, float u, float& dg, float& du) {
+    const float s = sigmoid_fast(g);
+    dg = da * u * (s * (1.f + g * (1.f - s)));
+    du = da * (g * s);
+}
+
+// MN-major tile with 128-byte swizzle: chunks of 64 values along M (or N), each [64 of the contraction][128 bytes]; chunks are
+// 8192 bytes apart (leading byte offset), groups of 8 of the contraction 1024 bytes (stride byte offset).
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr) {
+    return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(8192 >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+           (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+
+// 32 bytes that are read once: a whole sector per thread
+__device__ __forceinline__ void ld_nc_f8(const float* p, float* v) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "l"(p));
+}
+
 // silu(gate) * up of 32 columns, then scales (two blocks of 16 or one of 32) and codes; `gate` and `up` are raw accumulators.
 template <int FMT>
 __device__ __forceinline__ void fp4_swiglu32(const uint32_t* gate, const uint32_t* up, float alpha, float out_g, uint4& codes, uint32_t& scales) {

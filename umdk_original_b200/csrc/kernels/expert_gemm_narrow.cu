@@ -138,7 +138,7 @@ struct TallWalker {
 
 }  // namespace
 
-template <int KIND, bool SWIGLU>
+template <int KIND, int FORM>
 __global__ void __launch_bounds__(narrow_threads(KIND), 1)
 expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const NarrowParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -146,7 +146,8 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         if (threadIdx.x == 0) gemm_record_status(&g_narrow_status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
         return;
     }
-    constexpr bool FP4 = KIND != kNarrow16;
+    constexpr bool FP4 = KIND != kNarrow16, SWIGLU = FORM == kNarrowSwiglu, DACT = FORM == kNarrowDact;
+    constexpr bool W_MN = DACT || FORM == kNarrowByRows;  // the weights' contraction index is their row index in memory
     constexpr int SFW = KIND == kFp4Nv ? 4 : 2;  // scale words of a row and K-block
     constexpr int EPI0 = narrow_epi_warp0(KIND);
     constexpr int STEP = SWIGLU ? 64 : 128;      // result columns of a tile: 64 gate and 64 up rows, or 128 rows
@@ -236,7 +237,12 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                     const int k = k_lo + st * chunks;
                     mbar_arrive_expect_tx(full, bytes);
                     const int c0 = p.chunked ? 0 : k * 128, c3 = p.chunked ? k : 0;
-                    tma_load_5d(sw, &tmap_b, bar, c0, nt * STEP, 0, c3, e);
+                    if constexpr (W_MN) {
+                        for (int i = 0; i < 2 * chunks; ++i)  // [64 of the contraction][64 values]; what lies outside comes as zeros
+                            tma_load_3d(sw + static_cast<uint32_t>(i) * 8192u, &tmap_b, bar, (nt * STEP + (i & 1) * 64) * 2, (k + (i >> 1)) * 64, e);
+                    } else {
+                        tma_load_5d(sw, &tmap_b, bar, c0, nt * STEP, 0, c3, e);
+                    }
                     const uint32_t sr = sw + static_cast<uint32_t>(kWBytes * chunks);
                     for (int i = 0; i < pieces; ++i) tma_load_3d(sr + static_cast<uint32_t>(i) * 4096u, &tmap_a, bar, c0, row0 + i * 32, c3);
                 }
@@ -256,7 +262,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                 idesc[0] = idesc_fp4<KIND>(BM, 0, 0u) | ((n >> 3) << 17);
                 idesc[1] = KIND == kFp4Mx ? idesc_fp4<KIND>(BM, 0, 2u) | ((n >> 3) << 17) : idesc[0];
             } else {
-                idesc[0] = idesc[1] = umma_idesc(BM, 0, 1u, p.fp16 ? 0u : 1u) | ((n >> 3) << 17);
+                idesc[0] = idesc[1] = umma_idesc(BM, 0, 1u, p.fp16 ? 0u : 1u) | ((n >> 3) << 17) | (W_MN ? 1u << 15 : 0u);
             }
             const uint32_t b = tcount & 1u;
             mbar_wait_warp(smem_u32(&bar_tempty[b]), ((tcount >> 1) & 1u) ^ 1u, abort_at);
@@ -275,7 +281,8 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                 const int live = min(chunks, k_hi - k_lo - st * chunks);
                 if (leader) {
                     for (int c = 0; c < live; ++c) {
-                        const uint64_t wdesc = umma_desc_k_sw128(sw + static_cast<uint32_t>(c * kWBytes));
+                        const uint32_t wat = sw + static_cast<uint32_t>(c * kWBytes);
+                        const uint64_t wdesc = W_MN ? umma_desc_mn_sw128(wat) : umma_desc_k_sw128(wat);
                         const uint64_t rdesc = umma_desc_k_sw128(sr + static_cast<uint32_t>(c * a_bytes));
                         const uint32_t slot = gr * kNwSfGroup + static_cast<uint32_t>(in_group + c), sf = tmem_base + kNwSfCol0 + slot * kNwSfCols;
                         if constexpr (FP4) {
@@ -289,7 +296,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const uint32_t cs = sf + 8u * (KIND == kFp4Mx ? k >> 1 : k);
-                            narrow_mma<KIND>(tmem_base + b * 128u, wdesc + 2u * k, rdesc + 2u * k, idesc[k & 1], (st | c | k) ? 1u : 0u, cs, cs + 4u);
+                            narrow_mma<KIND>(tmem_base + b * 128u, wdesc + (W_MN ? 128u : 2u) * k, rdesc + 2u * k, idesc[k & 1], (st | c | k) ? 1u : 0u, cs, cs + 4u);
                         }
                     }
                     tc_commit(&bar_empty[s]);
@@ -454,6 +461,18 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                     if (c >= p.n_dim) continue;  // n_dim is a multiple of 8
                     float v[8];
                     gather(v, 2, t, ch * 8);
+                    if constexpr (DACT) {
+                        const size_t at = static_cast<size_t>(row0 + t) * (2 * static_cast<size_t>(p.n_dim)) + c;
+                        float g[8], u[8], dg[8], du[8];
+                        ld_nc_f8(p.gate_up + at, g);
+                        ld_nc_f8(p.gate_up + at + p.n_dim, u);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) gated_gradients(v[j], g[j], u[j], dg[j], du[j]);
+                        uint16_t* o = static_cast<uint16_t*>(p.out) + at;
+                        *reinterpret_cast<uint4*>(o) = make_uint4(pack16(dg[0], dg[1], fp16), pack16(dg[2], dg[3], fp16), pack16(dg[4], dg[5], fp16), pack16(dg[6], dg[7], fp16));
+                        *reinterpret_cast<uint4*>(o + p.n_dim) = make_uint4(pack16(du[0], du[1], fp16), pack16(du[2], du[3], fp16), pack16(du[4], du[5], fp16), pack16(du[6], du[7], fp16));
+                        continue;
+                    }
                     if constexpr (SWIGLU) {
                         float u[8];
                         gather(u, 2, t, 64 + ch * 8);
@@ -482,7 +501,8 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             }
         }
         if (!ok && te == 0) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
-        zero_loose_rows(p.out, (FP4 && SWIGLU) ? p.n_dim / 32 : p.n_dim / 8, p.expert_offsets, p.num_experts, p.rows, te, kNwEpiThreads);
+        if constexpr (!DACT)  // dgu of rows of no expert is read by nothing
+            zero_loose_rows(p.out, (FP4 && SWIGLU) ? p.n_dim / 32 : p.n_dim / 8, p.expert_offsets, p.num_experts, p.rows, te, kNwEpiThreads);
         if constexpr (FP4 && SWIGLU)
             zero_loose_scales(p.out_scales, p.n_dim / fp4_block(KIND), p.expert_offsets, p.num_experts, p.rows, te, kNwEpiThreads);
     }
@@ -506,11 +526,11 @@ int narrow_smem(const cam::NarrowParams* p, bool fp4) {
     return cam::kNwCtrlBytes + p->stages * p->stage_bytes + (fp4 ? cam::kNwScaleSlots * cam::kNwSfSlot : 0) + p->slot_rows * cam::kNwPitch * 4;
 }
 
-template <int KIND, bool SWIGLU>
+template <int KIND, int FORM>
 int launch_narrow(const cam::NarrowParams* p, int64_t tiles, const CUtensorMap* ta, const CUtensorMap* tb, cudaStream_t stream) {
     static cam::SmemLimitCache limit;
     const int smem = narrow_smem(p, KIND != cam::kNarrow16);
-    const cudaError_t err = limit.ensure(cam::expert_narrow_kernel<KIND, SWIGLU>, smem);
+    const cudaError_t err = limit.ensure(cam::expert_narrow_kernel<KIND, FORM>, smem);
     if (err != cudaSuccess) return static_cast<int>(err);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2] = {cam::pdl_attribute(), {}};
@@ -525,21 +545,29 @@ int launch_narrow(const cam::NarrowParams* p, int64_t tiles, const CUtensorMap* 
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = p->split > 1 ? 2 : 1;
-    return static_cast<int>(cudaLaunchKernelEx(&cfg, cam::expert_narrow_kernel<KIND, SWIGLU>, *ta, *tb, *p));
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, cam::expert_narrow_kernel<KIND, FORM>, *ta, *tb, *p));
 }
 
 }  // namespace
 
-extern "C" int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int swiglu, int64_t tiles, const CUtensorMap* ta,
+extern "C" int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int form, int64_t tiles, const CUtensorMap* ta,
                                              const CUtensorMap* tb, cudaStream_t stream) {
     const bool fp4 = kind != cam::kNarrow16;
     const int unit = fp4 ? cam::kNwSfGroup : p->chunks;
     if (p->chunks < 1 || p->chunks > 2 || p->stages < 2 || p->stages > cam::kNwMaxStages || narrow_smem(p, fp4) > 232448 ||
         p->stage_bytes % 1024 != 0 || (p->split != 1 && p->split != 2 && p->split != 4) || p->split > (p->kblocks + unit - 1) / unit)
         return static_cast<int>(cudaErrorInvalidValue);
-    if (kind == cam::kFp4Nv) return swiglu ? launch_narrow<cam::kFp4Nv, true>(p, tiles, ta, tb, stream) : launch_narrow<cam::kFp4Nv, false>(p, tiles, ta, tb, stream);
-    if (kind == cam::kFp4Mx) return swiglu ? launch_narrow<cam::kFp4Mx, true>(p, tiles, ta, tb, stream) : launch_narrow<cam::kFp4Mx, false>(p, tiles, ta, tb, stream);
-    return swiglu ? launch_narrow<cam::kNarrow16, true>(p, tiles, ta, tb, stream) : launch_narrow<cam::kNarrow16, false>(p, tiles, ta, tb, stream);
+    switch (kind * 4 + form) {
+        case cam::kFp4Nv * 4 + cam::kNarrowPlain: return launch_narrow<cam::kFp4Nv, cam::kNarrowPlain>(p, tiles, ta, tb, stream);
+        case cam::kFp4Nv * 4 + cam::kNarrowSwiglu: return launch_narrow<cam::kFp4Nv, cam::kNarrowSwiglu>(p, tiles, ta, tb, stream);
+        case cam::kFp4Mx * 4 + cam::kNarrowPlain: return launch_narrow<cam::kFp4Mx, cam::kNarrowPlain>(p, tiles, ta, tb, stream);
+        case cam::kFp4Mx * 4 + cam::kNarrowSwiglu: return launch_narrow<cam::kFp4Mx, cam::kNarrowSwiglu>(p, tiles, ta, tb, stream);
+        case cam::kNarrow16 * 4 + cam::kNarrowPlain: return launch_narrow<cam::kNarrow16, cam::kNarrowPlain>(p, tiles, ta, tb, stream);
+        case cam::kNarrow16 * 4 + cam::kNarrowSwiglu: return launch_narrow<cam::kNarrow16, cam::kNarrowSwiglu>(p, tiles, ta, tb, stream);
+        case cam::kNarrow16 * 4 + cam::kNarrowDact: return launch_narrow<cam::kNarrow16, cam::kNarrowDact>(p, tiles, ta, tb, stream);
+        case cam::kNarrow16 * 4 + cam::kNarrowByRows: return launch_narrow<cam::kNarrow16, cam::kNarrowByRows>(p, tiles, ta, tb, stream);
+    }
+    return static_cast<int>(cudaErrorInvalidValue);
 }
 
 extern "C" int cam_expert_narrow_max_stages(void) { return cam::kNwMaxStages; }

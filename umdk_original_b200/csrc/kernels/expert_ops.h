@@ -56,6 +56,8 @@ struct GroupedMlpParams {
 
 // Form of the row products for experts with few rows (expert_gemm_narrow.cu): tiles of 128 weight rows x slot_rows rows.
 constexpr int kNarrow16 = 2;  // beside the formats of fp4.cuh: 16-bit operands
+// Weights contracted over their columns, plain or with SwiGLU; over their rows (16 bits): the gradient of the activation, or plain
+constexpr int kNarrowPlain = 0, kNarrowSwiglu = 1, kNarrowDact = 2, kNarrowByRows = 3;
 struct NarrowParams {
     const int* expert_offsets;
     int num_experts, rows;
@@ -68,7 +70,7 @@ struct NarrowParams {
     int stages, stage_bytes;
     int fp16;
     void* out;                  // 16-bit [rows, n_dim], or fp4 SwiGLU: codes [rows, I/2]
-    float* gate_up;             // 16-bit SwiGLU: null or fp32 [rows, 2I]
+    float* gate_up;             // 16-bit SwiGLU: null or fp32 [rows, 2I]; kNarrowDact: read
     // fp4
     const uint8_t *a_scales, *b_scales;
     int scale_pitch, scale_vec;
@@ -97,8 +99,9 @@ int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, const CUten
                            const CUtensorMap* tmap_b, cudaStream_t stream);
 // kind: kFp4Nv, kFp4Mx or kNarrow16.  The maps, innermost first; with `chunked` a row is (K-block, 128 bytes), otherwise all of
 // its bytes and one K-block: tmap_a {bytes, rows, K-blocks} in boxes {128, slot_rows (32 without chunks), chunks}; tmap_b {bytes,
-// rows, halves, K-blocks, experts} in boxes {128, 128 / halves, halves, chunks, 1} with SwiGLU's gate and up rows as two halves.
-int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int swiglu, int64_t tiles, const CUtensorMap* tmap_a,
+// rows, halves, K-blocks, experts} in boxes {128, 128 / halves, halves, chunks, 1} with SwiGLU's gate and up rows as two halves, or, for
+// weights contracted over their rows, {bytes, rows, experts} in boxes {128, 64, 1}.
+int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int form, int64_t tiles, const CUtensorMap* tmap_a,
                                   const CUtensorMap* tmap_b, cudaStream_t stream);
 int cam_expert_narrow_max_stages(void);
 int cam_expert_narrow_fixed_smem(int fp4, int slot_rows);  // shared memory beside the stages

@@ -72,20 +72,6 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* tma
         : "memory");
 }
 
-// MN-major tile with 128-byte swizzle: chunks of 64 values along M (or N), each [64 of the contraction][128 bytes]; chunks are
-// 8192 bytes apart (leading byte offset), groups of 8 of the contraction 1024 bytes (stride byte offset).
-__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr) {
-    return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(8192 >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
-           (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
-}
-
-// 32 bytes that are read once: a whole sector per thread
-__device__ __forceinline__ void ld_nc_f8(const float* p, float* v) {
-    asm volatile("ld.global.nc.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-                 : "l"(p));
-}
-
 // Tiles of the weight gradients: 256 x 256 of every expert's [m_dim, n_dim]; `rows` are the rows summed over.
 struct GradTileWalker {
     const int* off;
@@ -360,10 +346,7 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
                             float a[4], d[4];
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
-                                const float da = __uint_as_float(v[part * 16 + 4 * i + k]);
-                                const float gg = g[4 * i + k], s = sigmoid_fast(gg);
-                                a[k] = da * u[4 * i + k] * (s * (1.f + gg * (1.f - s)));
-                                d[k] = da * (gg * s);
+                                gated_gradients(__uint_as_float(v[part * 16 + 4 * i + k]), g[4 * i + k], u[4 * i + k], a[k], d[k]);
                             }
                             v[part * 8 + 2 * i] = pack16(a[0], a[1], fp16);  // words 0..15: dg; their da has been used
                             v[part * 8 + 2 * i + 1] = pack16(a[2], a[3], fp16);

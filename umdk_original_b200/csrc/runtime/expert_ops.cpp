@@ -54,7 +54,7 @@ int env_switch(const char* name) {
 struct FewRows {
     int slot_rows, kblocks, chunked, chunks, stages, split;
     int64_t upper;   // row blocks there can be
-    int64_t cycles;  // estimate
+    int64_t turns, turn_kblocks, turn_fixed;  // turns of the SMs; K-blocks of a tile and cycles beside them in a turn
 };
 
 FewRows plan_few_rows(int rows, int num_experts, int64_t n_tiles, int row_bytes, bool fp4) {
@@ -83,7 +83,9 @@ FewRows plan_few_rows(int rows, int num_experts, int64_t n_tiles, int row_bytes,
         if (forced > 0 ? split <= forced : best < 0 || cost < best) {
             best = cost;
             f.split = split;
-            f.cycles = turns * (blocks_k * (770 + f.slot_rows) + fixed);  // tall tiles also take their rows from L2
+            f.turns = turns;
+            f.turn_kblocks = blocks_k;
+            f.turn_fixed = fixed;
         }
     }
     return f;
@@ -102,28 +104,42 @@ bool few_rows_pay_fp4(int rows, int num_experts, int n_dim, bool swiglu) {
     return mean <= 128 || (mean + 255) / 256 * num_experts * ((n_dim + (swiglu ? 127 : 255)) / (swiglu ? 128 : 256)) < 32;
 }
 
-// 16 bits above that: the pairs' tiles are larger still, 512 weight rows x 256, and the smaller of two estimates decides.  Pairs: turns
-// of the SMs x (K-blocks of 700 + 3 per row cycles, or the memory's time for their weights, and 18000 for a tile's start and end).
-// One expert of 7168 x 2048, 512 rows 112 (pairs) / 77 us; 8 of 2048 x 1024, 256 rows 66 / 56, 384 rows 65 / 71; 4 of 7168 x 2048, 160
-// rows 110 / 196.  Over 66 sizes (these, 16 of 4096 x 1024, 64 of 2048 x 768; 16 - 768 rows) the choice is at most 2 % behind the better
-// form, over 24 others 4 %.
-bool few_rows_pay_16(int rows, int num_experts, int n_dim, bool swiglu, int k) {
+// 16 bits, above 128 rows in the forward pass and always in the backward pass: the smaller of two estimates in cycles decides, with
+// constants fitted to kernel times (L2 cold) of 66 forward and 44 backward sizes: 1 to 64 experts of 2048 x 768 to 7168 x 2048, 16 to
+// 2048 rows each.  A turn of the pairs takes, per K-block, a start and the MMAs of its rows, or the memory's time for the weights if
+// many pairs are busy; its tiles are 512 weight rows x 256 rows, with gate and up 256 of each, dact's 256 x 256.
+//   forward, pairs / few rows: one expert of 7168 x 2048, 512 rows 112 / 77 us; 8 of 2048 x 1024, 256 rows 66 / 56, 384 rows 65 / 71;
+//     4 of 7168 x 2048, 160 rows 110 / 196
+//   dact and dx: one of 7168 x 2048, 256 rows 99 / 56, 768 rows 104 / 136; 8 of 2048 x 1024, 256 rows 69 / 62, 384 rows 69 / 89;
+//     16 of 4096 x 2048, 375 rows 290 / 431
+bool few_rows_pay_16(int rows, int num_experts, int n_dim, int form, int k) {
     const int sw = env_switch("UMDK_CAM_EXPERT_NARROW");
     if (sw >= 0) return sw != 0;
+    const bool swiglu = form == cam::kMlpUp, dact = form == cam::kMlpDact, backward = dact || form == cam::kMlpDx;
     const int64_t mean = (static_cast<int64_t>(rows) + num_experts - 1) / num_experts;
-    if (mean <= 128) return true;
-    const int step = swiglu ? 64 : 128, wide = swiglu ? 256 : 512;
+    if (!backward && mean <= 128) return true;
+    const int step = swiglu ? 64 : 128, wide = swiglu || dact ? 256 : 512;
     const int64_t parts = (mean + 255) / 256, cols = ((mean + parts - 1) / parts + 31) / 32 * 32;
-    const int64_t most = cam::sm_count_of_current_device() / 2;
-    const int64_t tiles = num_experts * parts * ((n_dim + wide - 1) / wide), busy = tiles < most ? tiles : most;
-    const int64_t turns = (tiles + most - 1) / most, work = 700 + 3 * cols, memory = 1420 * busy / most;
+    const int64_t most = cam::sm_count_of_current_device() / 2, live = rows < num_experts ? rows : num_experts;
+    const int64_t tiles = live * parts * ((n_dim + wide - 1) / wide), busy = tiles < most ? tiles : most;
+    const int64_t turns = (tiles + most - 1) / most, memory = 1420 * busy / most;
     const FewRows f = plan_few_rows(rows, num_experts, (n_dim + step - 1) / step, k * 2, false);
-    return f.cycles < turns * (f.kblocks * (work > memory ? work : memory) + 18000);
+    // tall tiles also take their rows from L2
+    const int64_t few = f.turns * (f.turn_kblocks * (dact ? 807 : backward ? 760 : 770 + f.slot_rows) + f.turn_fixed);
+    int64_t pairs;
+    if (dact) {
+        pairs = 8000 + turns * (f.kblocks * (550 + 400 * busy / most) + 1000);
+    } else {
+        const int64_t work = backward ? 560 + cols * 5 / 2 : 700 + 3 * cols;
+        pairs = turns * f.kblocks * (work > memory ? work : memory) + (backward ? 9500 : 18000 * turns);
+    }
+    return few < pairs;
 }
 
-// The form for few rows: maps and launch.  `row_bytes` of the row operand and of the weights' rows; n_dim, the operands' scales and
-// outputs are set.
-int launch_narrow(cam::NarrowParams* p, int kind, bool swiglu, const void* a, const void* w, int row_bytes, const char* what, cudaStream_t stream) {
+// The form for few rows: maps and launch.  `row_bytes` of the row operand (and of the weights' rows, unless they are contracted
+// over their rows); n_dim, the operands' scales and outputs are set.
+int launch_narrow(cam::NarrowParams* p, int kind, int form, const void* a, const void* w, int row_bytes, const char* what, cudaStream_t stream) {
+    const bool swiglu = form == cam::kNarrowSwiglu;
     const int step = swiglu ? 64 : 128;
     const int64_t n_tiles = (p->n_dim + step - 1) / step;
     const FewRows f = plan_few_rows(p->rows, p->num_experts, n_tiles, row_bytes, kind != cam::kNarrow16);
@@ -140,10 +156,14 @@ int launch_narrow(cam::NarrowParams* p, int kind, bool swiglu, const void* a, co
     const uint64_t da[3] = {bytes, static_cast<uint64_t>(p->rows), blocks_k}, sa[2] = {pitch, 128};
     const uint32_t ba[3] = {128, p->chunks > 1 ? static_cast<uint32_t>(p->slot_rows) : 32u, static_cast<uint32_t>(p->chunks)};
     if (cam_encode_tmap(&ta, a, 3, da, sa, ba) != 0) return -1;
+    if (form == cam::kNarrowDact || form == cam::kNarrowByRows) {
+        if (map_3d(&tb, w, n * 2, static_cast<uint64_t>(row_bytes / 2), static_cast<uint64_t>(p->num_experts), 64) != 0) return -1;
+        return launched(cam_launch_expert_gemm_narrow(p, kind, form, f.upper * n_tiles, &ta, &tb, stream), what);
+    }
     const uint64_t db[5] = {bytes, n, halves, blocks_k, static_cast<uint64_t>(p->num_experts)}, sb[4] = {pitch, pitch * n, 128, pitch * n * halves};
     const uint32_t bb[5] = {128, static_cast<uint32_t>(step), static_cast<uint32_t>(halves), static_cast<uint32_t>(p->chunks), 1};
     if (cam_encode_tmap(&tb, w, 5, db, sb, bb) != 0) return -1;
-    return launched(cam_launch_expert_gemm_narrow(p, kind, swiglu, f.upper * n_tiles, &ta, &tb, stream), what);
+    return launched(cam_launch_expert_gemm_narrow(p, kind, form, f.upper * n_tiles, &ta, &tb, stream), what);
 }
 
 }  // namespace
@@ -194,7 +214,7 @@ extern "C" int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, 
         p.b_gscale = w_gscale;
         p.out_gscale = out_gscale;
         p.out_scales = static_cast<uint8_t*>(out_s);
-        return launch_narrow(&p, fmt, swiglu != 0, a_q, w_q, k_dim / 2, "grouped_gemm_fp4", stream);
+        return launch_narrow(&p, fmt, swiglu ? cam::kNarrowSwiglu : cam::kNarrowPlain, a_q, w_q, k_dim / 2, "grouped_gemm_fp4", stream);
     }
     cam::GroupedGemmFp4Params p{};
     p.expert_offsets = offsets;
@@ -226,8 +246,7 @@ int row_product(int form, const char* what, const void* a, int k, const void* w,
     EXP_CHECK(a && w && offsets && out, "%s: null operand", what);
     EXP_CHECK(rows >= 1 && num_experts >= 1, "%s: empty problem", what);
     EXP_CHECK(k >= 8 && n >= 8 && k % 8 == 0 && n % 8 == 0, "%s: sizes %d and %d must be multiples of 8", what, k, n);
-    if (!by_rows && few_rows_pay_16(rows, num_experts, n, form == cam::kMlpUp, k)) {
-        const bool swiglu = form == cam::kMlpUp;
+    if (few_rows_pay_16(rows, num_experts, n, form, k)) {
         cam::NarrowParams p{};
         p.expert_offsets = offsets;
         p.num_experts = num_experts;
@@ -236,7 +255,8 @@ int row_product(int form, const char* what, const void* a, int k, const void* w,
         p.fp16 = dtype == 1;
         p.out = out;
         p.gate_up = gate_up;
-        return launch_narrow(&p, cam::kNarrow16, swiglu, a, w, k * 2, what, stream);
+        const int narrow = form == cam::kMlpUp ? cam::kNarrowSwiglu : form == cam::kMlpDact ? cam::kNarrowDact : by_rows ? cam::kNarrowByRows : cam::kNarrowPlain;
+        return launch_narrow(&p, cam::kNarrow16, narrow, a, w, k * 2, what, stream);
     }
     cam::GroupedMlpParams p{};
     p.expert_offsets = offsets;
