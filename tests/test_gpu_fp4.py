@@ -242,6 +242,15 @@ def test_few_rows(ops, fmt, m, e, k, n, swiglu):
     assert ((val - act).abs() <= torch.maximum(0.25 * d, act.abs() / 6) + cut + slack).all()
 
 
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("split", ["1", "2", "4"])
+@pytest.mark.parametrize("m,e,k,n,swiglu", [(40, 4, 1024, 512, True), (700, 3, 2176, 1024, False), (900, 2, 4352, 512, True)])
+def test_tiles_shared_by_a_cluster(ops, fmt, split, m, e, k, n, swiglu, monkeypatch):
+    monkeypatch.setenv("UMDK_CAM_EXPERT_NARROW", "1")
+    monkeypatch.setenv("UMDK_CAM_EXPERT_SPLIT", split)
+    test_few_rows(ops, fmt, m, e, k, n, swiglu)
+
+
 def test_status_is_clean(ops):
     from umdk_original_b200.ops import cam_ops
     assert cam_ops.native_module().expert_ops_status()[0] == 0

@@ -148,6 +148,15 @@ def test_few_rows(ops, dtype, m, e, h, inter):
     check({"y": y.detach(), "dx": dx, "dw1": dw1, "dw2": dw2}, want, tol, tiny * (m + 2 * inter + h))
 
 
+@pytest.mark.parametrize("split", ["1", "2", "4"])
+@pytest.mark.parametrize("m,e,h,inter", [(33, 2, 1032, 520), (700, 3, 640, 328), (1300, 1, 2048, 512)])
+def test_tiles_shared_by_a_cluster(ops, split, m, e, h, inter, monkeypatch):
+    """The form for few rows at any number of rows, with 1, 2 and 4 CTAs per tile and several tiles per cluster."""
+    monkeypatch.setenv("UMDK_CAM_EXPERT_NARROW", "1")
+    monkeypatch.setenv("UMDK_CAM_EXPERT_SPLIT", split)
+    test_few_rows(ops, torch.bfloat16, m, e, h, inter)
+
+
 def test_two_runs_give_the_same_bits(ops):
     x, w1, w2, dy, off = make(torch.bfloat16, 1000, 344, "block borders")
     runs = []

@@ -1,5 +1,7 @@
-// Row products of the expert-MLP operators for experts with few rows (decode): 4-bit or 16-bit operands, plain or with the
-// SwiGLU epilogue.  One CTA computes 128 weight rows x the rows of an expert (at most 32, 64 or 128 of them).
+// Row products of the expert-MLP operators for experts with few rows (decode, small training batches): 4-bit or 16-bit operands,
+// plain or with the SwiGLU epilogue; in 16 bits also the backward products dact and dx (formulas in grouped_mlp.cu), whose weights are
+// contracted over their rows and read in the tensor core's MN-major form.  One CTA computes 128 weight rows x the rows of an expert (at
+// most 32, 64 or 128 of them).
 //
 // What bounds these calls is the stream of weights, so the form differs from the CTA pairs (grouped_gemm_fp4.cu,
 // grouped_mlp.cu) in what it spends per weight byte:

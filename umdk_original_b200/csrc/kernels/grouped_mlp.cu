@@ -22,6 +22,8 @@
 // for every value of da, and its epilogue is what takes long: with an accumulator to spare it runs beside the MMAs of the next tile
 // (16 x 1024 rows, 4096 x 2048: 225 us, with 512 x 256 tiles 288).
 //
+// With few rows per expert, or few tiles in all, up, down, dact and dx are computed by expert_gemm_narrow.cu instead.
+//
 // K-blocks of 64 values (128 bytes) come by TMA.  An operand whose contraction index is not its contiguous one (w2 of dact, w1 of dx,
 // both operands of dw) is loaded as [64 of the contraction][64 values] boxes and read by the tensor core in its MN-major form;
 // nothing is transposed in memory.

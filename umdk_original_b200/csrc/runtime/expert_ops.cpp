@@ -72,13 +72,15 @@ FewRows plan_few_rows(int rows, int num_experts, int64_t n_tiles, int row_bytes,
     const int fit = room / (f.chunks * per_chunk), most = cam_expert_narrow_max_stages();
     f.stages = fit < most ? fit : most;
     // CTAs per tile: turns of the SMs x cycles of a turn (a K-block at an SM's share of the memory bandwidth, a fixed part, the
-    // exchange inside the cluster)
+    // exchange inside the cluster, which the next tile waits for).  Forward pass of one expert of 7168 x 2048 in 16 bits, with 1, 2, 4:
+    // 128 rows 62, 52, 52 us (mixed as chosen here 46), 384 rows 77, 81, 118 us.
     const int unit = fp4 ? 4 : f.chunks, units = (f.kblocks + unit - 1) / unit;
     const int forced = env_switch("UMDK_CAM_EXPERT_SPLIT");
     int64_t best = -1;
     for (int split = 1; split <= 4 && split <= units; split *= 2) {  // clusters of 8 find too few places at once
         const int64_t turns = (blocks * n_tiles + sms / split - 1) / (sms / split);
-        const int64_t blocks_k = static_cast<int64_t>((units + split - 1) / split) * unit, fixed = 1500 + (split > 1 ? 2000 : 0);
+        const int64_t blocks_k = static_cast<int64_t>((units + split - 1) / split) * unit;
+        const int64_t fixed = 1500 + (split == 1 ? 0 : turns > 1 ? 2000 * split : fp4 ? 4000 : 2000);
         const int64_t cost = turns * (blocks_k * 770 + fixed);
         if (forced > 0 ? split <= forced : best < 0 || cost < best) {
             best = cost;
