@@ -157,6 +157,33 @@ def test_tiles_shared_by_a_cluster(ops, split, m, e, h, inter, monkeypatch):
     test_few_rows(ops, torch.bfloat16, m, e, h, inter)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("h,inter", [(8, 8), (264, 136), (4104, 520)])
+@pytest.mark.parametrize("cnt,head,tail", [([1], 0, 0), ([2], 0, 0), ([0, 1, 0, 1], 0, 0), ([3], 0, 0), ([0, 1, 0], 1, 1), ([5, 0, 2], 2, 3), ([16], 0, 0),
+                                           ([0, 0], 0, 2)])
+def test_a_handful_of_rows(ops, dtype, h, inter, cnt, head, tail):
+    """The form on the ordinary cores: one, two and more rows, several blocks of rows, rows of no expert, a NaN in an idle expert."""
+    gen = torch.Generator(device=DEV).manual_seed(h + sum(cnt))
+    e, m = len(cnt), head + sum(cnt) + tail
+    x = torch.randn(m, h, device=DEV, generator=gen).to(dtype)
+    w1 = (torch.randn(e, 2 * inter, h, device=DEV, generator=gen) * h ** -0.5).to(dtype)
+    w2 = (torch.randn(e, h, inter, device=DEV, generator=gen) * inter ** -0.5).to(dtype)
+    dy = torch.randn(m, h, device=DEV, generator=gen).to(dtype)
+    off = offsets_of(cnt, head, DEV)
+    half, tiny = bounds(dtype)
+    want, tol = formula64(x, w1, w2, dy, off, half, acc)
+    for j in range(e):
+        if cnt[j] == 0:
+            w1[j], w2[j] = float("nan"), float("nan")
+    x[:head], x[m - tail:] = float("nan"), float("nan")
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+    y = ops.grouped_mlp(*leaves, off)
+    with torch.no_grad():
+        assert torch.equal(ops.grouped_mlp(x, w1, w2, off), y)
+    dx, dw1, dw2 = torch.autograd.grad(y, leaves, dy)
+    check({"y": y.detach(), "dx": dx, "dw1": dw1, "dw2": dw2}, want, tol, tiny * (m + 2 * inter + h))
+
+
 def test_two_runs_give_the_same_bits(ops):
     x, w1, w2, dy, off = make(torch.bfloat16, 1000, 344, "block borders")
     runs = []

@@ -50,6 +50,7 @@ KERNEL_SOURCES = [
     "kernels/grouped_gemm_fp4.cu",
     "kernels/grouped_mlp.cu",
     "kernels/expert_gemm_narrow.cu",
+    "kernels/expert_gemv.cu",
     "runtime/cam_runtime.cpp",
     "runtime/expert_ops.cpp",
 ]

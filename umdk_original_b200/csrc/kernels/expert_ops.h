@@ -54,6 +54,8 @@ struct GroupedMlpParams {
     float* gate_up;             // [rows, 2I] fp32: written by kMlpUp (or null), read by kMlpDact
 };
 
+constexpr int kGvMaxSmem = 96 * 1024;  // shared memory of the form on the ordinary cores (expert_gemv.cu): up to four rows
+
 // Form of the row products for experts with few rows (expert_gemm_narrow.cu): tiles of 128 weight rows x slot_rows rows.
 constexpr int kNarrow16 = 2;  // beside the formats of fp4.cuh: 16-bit operands
 // Weights contracted over their columns, plain or with SwiGLU; over their rows (16 bits): the gradient of the activation, or plain
@@ -103,6 +105,8 @@ int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, const CUten
 // weights contracted over their rows, {bytes, rows, experts} in boxes {128, 64, 1}.
 int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int form, int64_t tiles, const CUtensorMap* tmap_a,
                                   const CUtensorMap* tmap_b, cudaStream_t stream);
+// up and down (kMlpUp, kMlpDown) of a handful of rows; x and w 16-byte aligned
+int cam_launch_expert_gemv(const cam::GroupedMlpParams* p, int swiglu, const void* x, const void* w, cudaStream_t stream);
 int cam_expert_narrow_max_stages(void);
 int cam_expert_narrow_fixed_smem(int fp4, int slot_rows);  // shared memory beside the stages
 int cam_narrow_status(CamStatus* out);

@@ -138,6 +138,15 @@ bool few_rows_pay_16(int rows, int num_experts, int n_dim, int form, int k) {
     return few < pairs;
 }
 
+// Up and down of a handful of rows on the ordinary cores (expert_gemv.cu)?  Forward pass, few-row form / this one, steady loop: one
+// expert of 7168 x 2048 with 1, 2, 3, 4 rows 26.7 / 19.9, 27.1 / 21.5, 27.3 / 24.4, 26.9 / 27.9 us; 8 of them 28.6 / 21.5, 40 / 36, 58 / 53,
+// 64 / 67; 16 of 4096 x 1024 21 / 10, 23 / 16, 26 / 26, 29 / 30.  Small experts gain longer: one of 2048 x 1024, 4 rows 15 / 11, 12 rows
+// 16 / 18; 6 of 1000 x 344, 4 - 16 rows 16 - 24 / 10 - 12.
+bool gemv_pays(int rows, int n_dim, int k, int form) {
+    if (env_switch("UMDK_CAM_EXPERT_NARROW") >= 0 || (form != cam::kMlpUp && form != cam::kMlpDown) || k > cam::kGvMaxSmem / 8) return false;
+    return rows <= 3 || (rows <= 16 && static_cast<int64_t>(rows) * n_dim * (form == cam::kMlpUp ? 2 : 1) * k < 1 << 24);
+}
+
 // The form for few rows: maps and launch.  `row_bytes` of the row operand (and of the weights' rows, unless they are contracted
 // over their rows); n_dim, the operands' scales and outputs are set.
 int launch_narrow(cam::NarrowParams* p, int kind, int form, const void* a, const void* w, int row_bytes, const char* what, cudaStream_t stream) {
@@ -248,6 +257,19 @@ int row_product(int form, const char* what, const void* a, int k, const void* w,
     EXP_CHECK(a && w && offsets && out, "%s: null operand", what);
     EXP_CHECK(rows >= 1 && num_experts >= 1, "%s: empty problem", what);
     EXP_CHECK(k >= 8 && n >= 8 && k % 8 == 0 && n % 8 == 0, "%s: sizes %d and %d must be multiples of 8", what, k, n);
+    if (gemv_pays(rows, n, k, form)) {
+        EXP_CHECK(aligned(a, 16) && aligned(w, 16), "%s: rows and weights must be 16-byte aligned", what);
+        cam::GroupedMlpParams p{};
+        p.expert_offsets = offsets;
+        p.num_experts = num_experts;
+        p.rows = rows;
+        p.n_dim = n;
+        p.k_dim = k;
+        p.fp16 = dtype == 1;
+        p.out = out;
+        p.gate_up = gate_up;
+        return launched(cam_launch_expert_gemv(&p, form == cam::kMlpUp, a, w, stream), what);
+    }
     if (few_rows_pay_16(rows, num_experts, n, form, k)) {
         cam::NarrowParams p{};
         p.expert_offsets = offsets;
