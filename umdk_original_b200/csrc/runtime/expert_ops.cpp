@@ -336,10 +336,11 @@ extern "C" int cam_grouped_mlp_dw(const void* a, const void* b, const int* offse
     p.n_dim = n_dim;
     p.fp16 = dtype == 1;
     p.out = dw;
-    CUtensorMap ta, tb;
+    CUtensorMap ta, tb, tout;
+    if (map_3d(&tout, dw, static_cast<uint64_t>(n_dim) * 2, static_cast<uint64_t>(m_dim), static_cast<uint64_t>(num_experts), 128) != 0) return -1;
     if (map_2d(&ta, a, static_cast<uint64_t>(m_dim) * 2, static_cast<uint64_t>(rows), 64) != 0) return -1;
     if (map_2d(&tb, b, static_cast<uint64_t>(n_dim) * 2, static_cast<uint64_t>(rows), 64) != 0) return -1;
-    return launched(cam_launch_grouped_mlp(&p, cam::kMlpDw, &ta, &ta, &tb, stream), "grouped_mlp (dw)");
+    return launched(cam_launch_grouped_mlp(&p, cam::kMlpDw, &ta, &tout, &tb, stream), "grouped_mlp (dw)");
 }
 
 extern "C" int cam_expert_ops_status(CamStatus* out) {
