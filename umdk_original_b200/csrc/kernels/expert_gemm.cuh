@@ -228,6 +228,18 @@ __device__ __forceinline__ void ld_nc_f8(const float* p, float* v) {
                  : "l"(p));
 }
 
+// A box in shared memory (128-byte swizzle) to a matrix; what lies outside of it is not written
+__device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t smem_src, int32_t c0, int32_t c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(tmap)),
+                 "r"(smem_src), "r"(c0), "r"(c1)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const void* tmap, uint32_t smem_src, int32_t c0, int32_t c1, int32_t c2) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(tmap)),
+                 "r"(smem_src), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
+
 // silu(gate) * up of 32 columns, then scales (two blocks of 16 or one of 32) and codes; `gate` and `up` are raw accumulators.
 template <int FMT>
 __device__ __forceinline__ void fp4_swiglu32(const uint32_t* gate, const uint32_t* up, float alpha, float out_g, uint4& codes, uint32_t& scales) {

@@ -91,9 +91,10 @@ int cam_launch_quantize_fp4(const void* x, int dtype, int fmt, void* q, void* s,
                             int64_t groups_per_scale, cudaStream_t stream);
 int cam_launch_dequantize_fp4(const void* q, const void* s, int dtype, int fmt, void* out, int64_t groups,
                               const float* gscale, int64_t groups_per_scale, cudaStream_t stream);
-// tmap_a: boxes of 128 rows, tmap_a32: of 32 rows, both on A [rows, K / 2 bytes]; tmap_b: boxes of 128 rows on W [E N, K / 2]
+// tmap_a: boxes of 128 rows, tmap_a32: of 32 rows, both on A [rows, K / 2 bytes]; tmap_b: boxes of 128 rows on W [E N, K / 2];
+// tmap_out (not with SwiGLU, where any map does): boxes of 32 rows on the result [rows, 2 N bytes]
 int cam_launch_grouped_gemm_fp4(const cam::GroupedGemmFp4Params* p, int fmt, int swiglu, const CUtensorMap* tmap_a,
-                                const CUtensorMap* tmap_a32, const CUtensorMap* tmap_b, cudaStream_t stream);
+                                const CUtensorMap* tmap_a32, const CUtensorMap* tmap_b, const CUtensorMap* tmap_out, cudaStream_t stream);
 // tmap_a: the row operand in boxes of 128 rows (kMlpDw: 64 rows), tmap_a32: in boxes of 32 rows; tmap_b: the weights
 // [E, rows, columns] in boxes of 128 rows, or of 64 where their row is the contraction index (kMlpDact, kMlpDx), or for kMlpDw
 // the second row operand in boxes of 64 rows, and tmap_a32 the result [E, m_dim, n_dim] in boxes of 128 rows.  All boxes are 128

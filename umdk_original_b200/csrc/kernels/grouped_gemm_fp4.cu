@@ -40,8 +40,8 @@ constexpr int kF4SfBlock = 4 * 512;            // scales of 128 rows (mxfp4 uses
 constexpr int kF4SfStage = 3 * kF4SfBlock;
 constexpr int kF4SfGroup = 4;                  // K-blocks whose scales travel together
 constexpr int kF4SfSlots = 2 * kF4SfGroup;     // two groups
-constexpr int kF4StgPitch = 272;               // bf16 rows of 128 columns, 16 bytes apart from a multiple of 128
-constexpr int kF4StgBytes = 128 * kF4StgPitch;
+constexpr int kF4StgBox = 32 * 128;             // 32 bf16 rows of 64 columns
+constexpr int kF4StgBytes = 8 * kF4StgBox;
 // the plain form gives up a stage for the staging of its rows
 __host__ __device__ constexpr int fp4_stages(bool swiglu) { return swiglu ? 5 : 4; }
 __host__ __device__ constexpr int fp4_smem(bool swiglu) {
@@ -94,7 +94,7 @@ __device__ __forceinline__ void tc_copy_scales_pair(uint32_t taddr, uint64_t des
 template <int FMT, bool SWIGLU>
 __global__ void __launch_bounds__(kF4Threads, 1)
 grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
-                        const __grid_constant__ CUtensorMap tmap_b, const GroupedGemmFp4Params p) {
+                        const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_out, const GroupedGemmFp4Params p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {  // swizzled TMA tiles need it; the same in both CTAs of a pair
         if (threadIdx.x == 0) gemm_record_status(&g_fp4_status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
@@ -337,24 +337,33 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                     else p.out_scales[at] = static_cast<uint8_t>(scales);
                 }
             } else {
-                // 128 columns at a time go through shared memory as bf16 and leave as one 256-byte bulk copy per row.  (Stores of
-                // 64 bytes per thread straight from registers: 16 x 1024 rows, K 2048, N 7168 167 -> 231 us.)
-                __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) + grow * p.n_dim;
+                // Two warps share 32 rows x 64 columns, which go through shared memory as bf16 and leave as one tensor copy; rows of a
+                // block of 32 that ends inside it are stored from registers.
+                const int box = q * 2 + (cq >> 1);
+                uint8_t* at = stg + box * kF4StgBox + lane * 128;
+                const bool whole = rows >= q * 32 + 32, issues = (cq & 1) == 0 && lane == 0;
                 auto push_half = [&](const uint32_t (&v)[32], int c0) {
-                    uint8_t* srow = stg + r * kF4StgPitch;
-                    if (cq == 0) bulk_wait_group_read<0>();  // the copies that read this buffer are done with it
-                    named_bar_sync(1, kF4EpiThreads);
+                    uint4 o[4];
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-                        *reinterpret_cast<uint4*>(srow + cq * 64 + j * 2) =
-                            pack_bf16x8(__uint_as_float(v[j]) * alpha, __uint_as_float(v[j + 1]) * alpha, __uint_as_float(v[j + 2]) * alpha,
-                                        __uint_as_float(v[j + 3]) * alpha, __uint_as_float(v[j + 4]) * alpha, __uint_as_float(v[j + 5]) * alpha,
-                                        __uint_as_float(v[j + 6]) * alpha, __uint_as_float(v[j + 7]) * alpha);
-                    fence_proxy_async_smem();
-                    named_bar_sync(1, kF4EpiThreads);
-                    if (cq == 0) {
-                        if (valid) bulk_store_s2g(orow + c0, srow, 256);
-                        bulk_commit_group();
+                    for (int j = 0; j < 4; ++j)
+                        o[j] = pack_bf16x8(__uint_as_float(v[8 * j]) * alpha, __uint_as_float(v[8 * j + 1]) * alpha, __uint_as_float(v[8 * j + 2]) * alpha,
+                                           __uint_as_float(v[8 * j + 3]) * alpha, __uint_as_float(v[8 * j + 4]) * alpha, __uint_as_float(v[8 * j + 5]) * alpha,
+                                           __uint_as_float(v[8 * j + 6]) * alpha, __uint_as_float(v[8 * j + 7]) * alpha);
+                    if (whole) {  // the same in both warps
+                        if (issues) bulk_wait_group_read<0>();  // the copy that reads this buffer is done with it
+                        named_bar_sync(1 + box, 64);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(at + ((((cq & 1) * 4 + j) ^ (static_cast<int>(lane) & 7)) << 4)) = o[j];
+                        fence_proxy_async_smem();
+                        named_bar_sync(1 + box, 64);
+                        if (issues) {
+                            tma_store_2d(&tmap_out, smem_u32(stg + box * kF4StgBox), (c0 + (cq >> 1) * 64) * 2, row0 + q * 32);
+                            bulk_commit_group();
+                        }
+                    } else if (valid) {
+                        uint4* to = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + grow * p.n_dim + c0 + cq * 32);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) to[j] = o[j];
                     }
                 };
                 const int c_lo = nt * 256;
@@ -362,7 +371,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                 if (c_lo + 128 < p.n_dim) push_half(v1, c_lo + 128);  // same answer in every thread of the CTA
             }
         }
-        if (!SWIGLU && cq == 0) bulk_wait_group<0>();  // every row this thread sent has been written
+        if (!SWIGLU && (cq & 1) == 0) bulk_wait_group<0>();  // everything this thread sent has been written
         if (!ok) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
         // rows of no expert
         const int et = static_cast<int>(threadIdx.x) - kF4EpiWarp0 * 32;
@@ -390,21 +399,21 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
 namespace {
 
 template <int FMT, bool SWIGLU>
-int launch_fp4(const cam::GroupedGemmFp4Params* p, const CUtensorMap* ta, const CUtensorMap* ta32, const CUtensorMap* tb, cudaStream_t stream) {
+int launch_fp4(const cam::GroupedGemmFp4Params* p, const CUtensorMap* ta, const CUtensorMap* ta32, const CUtensorMap* tb, const CUtensorMap* tout, cudaStream_t stream) {
     static cam::PairLimit limit;
     // at most one row block per expert beyond the full ones
     const int64_t n_tiles = SWIGLU ? p->n_dim / 256 : (p->n_dim + 255) / 256;
     const int64_t blocks = p->rows / 256 + (p->rows < p->num_experts ? p->rows : p->num_experts);
-    return cam::launch_pairs(limit, cam::grouped_gemm_fp4_kernel<FMT, SWIGLU>, cam::kF4Threads, cam::fp4_smem(SWIGLU), blocks * n_tiles, stream, *ta, *ta32, *tb, *p);
+    return cam::launch_pairs(limit, cam::grouped_gemm_fp4_kernel<FMT, SWIGLU>, cam::kF4Threads, cam::fp4_smem(SWIGLU), blocks * n_tiles, stream, *ta, *ta32, *tb, *tout, *p);
 }
 
 }  // namespace
 
 extern "C" int cam_launch_grouped_gemm_fp4(const cam::GroupedGemmFp4Params* p, int fmt, int swiglu, const CUtensorMap* tmap_a,
-                                           const CUtensorMap* tmap_a32, const CUtensorMap* tmap_b, cudaStream_t stream) {
+                                           const CUtensorMap* tmap_a32, const CUtensorMap* tmap_b, const CUtensorMap* tmap_out, cudaStream_t stream) {
     if (fmt == cam::kFp4Nv)
-        return swiglu ? launch_fp4<cam::kFp4Nv, true>(p, tmap_a, tmap_a32, tmap_b, stream) : launch_fp4<cam::kFp4Nv, false>(p, tmap_a, tmap_a32, tmap_b, stream);
-    return swiglu ? launch_fp4<cam::kFp4Mx, true>(p, tmap_a, tmap_a32, tmap_b, stream) : launch_fp4<cam::kFp4Mx, false>(p, tmap_a, tmap_a32, tmap_b, stream);
+        return swiglu ? launch_fp4<cam::kFp4Nv, true>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream) : launch_fp4<cam::kFp4Nv, false>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
+    return swiglu ? launch_fp4<cam::kFp4Mx, true>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream) : launch_fp4<cam::kFp4Mx, false>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
 }
 
 extern "C" int cam_fp4_status(CamStatus* out) { return static_cast<int>(cudaMemcpyFromSymbol(out, cam::g_fp4_status, sizeof(CamStatus))); }

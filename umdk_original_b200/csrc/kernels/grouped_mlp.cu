@@ -77,13 +77,6 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* tma
         : "memory");
 }
 
-// 64 columns x 128 rows in shared memory (128-byte swizzle) to a matrix; what lies outside of it is not written
-__device__ __forceinline__ void tma_store_3d(const void* tmap, uint32_t smem_src, int32_t c0, int32_t c1, int32_t c2) {
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(tmap)),
-                 "r"(smem_src), "r"(c0), "r"(c1), "r"(c2)
-                 : "memory");
-}
-
 // Tiles of the weight gradients: 256 x 256 of every expert's [m_dim, n_dim]; `rows` are the rows summed over.
 struct GradTileWalker {
     const int* off;

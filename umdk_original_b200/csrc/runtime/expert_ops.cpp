@@ -241,12 +241,13 @@ extern "C" int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, 
     p.out_gscale = out_gscale;
     p.out = out;
     p.out_scales = static_cast<uint8_t*>(out_s);
-    CUtensorMap ta, ta32, tb;
+    CUtensorMap ta, ta32, tb, tout;
     const uint64_t bytes = static_cast<uint64_t>(k_dim) / 2;
     if (map_2d(&ta, a_q, bytes, static_cast<uint64_t>(rows), 128) != 0) return -1;
     if (map_2d(&ta32, a_q, bytes, static_cast<uint64_t>(rows), 32) != 0) return -1;
     if (map_2d(&tb, w_q, bytes, static_cast<uint64_t>(num_experts) * n_dim, 128) != 0) return -1;
-    return launched(cam_launch_grouped_gemm_fp4(&p, fmt, swiglu, &ta, &ta32, &tb, stream), "grouped_gemm_fp4");
+    if (!swiglu && map_2d(&tout, out, static_cast<uint64_t>(n_dim) * 2, static_cast<uint64_t>(rows), 32) != 0) return -1;
+    return launched(cam_launch_grouped_gemm_fp4(&p, fmt, swiglu, &ta, &ta32, &tb, swiglu ? &tb : &tout, stream), "grouped_gemm_fp4");
 }
 
 namespace {
