@@ -97,10 +97,10 @@ int cam_launch_grouped_gemm_fp4(const cam::GroupedGemmFp4Params* p, int fmt, int
                                 const CUtensorMap* tmap_a32, const CUtensorMap* tmap_b, const CUtensorMap* tmap_out, cudaStream_t stream);
 // tmap_a: the row operand in boxes of 128 rows (kMlpDw: 64 rows), tmap_a32: in boxes of 32 rows; tmap_b: the weights
 // [E, rows, columns] in boxes of 128 rows, or of 64 where their row is the contraction index (kMlpDact, kMlpDx), or for kMlpDw
-// the second row operand in boxes of 64 rows, and tmap_a32 the result [E, m_dim, n_dim] in boxes of 128 rows.  All boxes are 128
-// bytes wide.
+// the second row operand in boxes of 64 rows.  tmap_out: the result in boxes of 32 rows (kMlpUp, kMlpDown, kMlpDx), or [E, m_dim, n_dim]
+// in boxes of 128 rows (kMlpDw).  All boxes are 128 bytes wide.  Not used, any map does: tmap_a32 of kMlpDw, tmap_out of kMlpDact.
 int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, const CUtensorMap* tmap_a, const CUtensorMap* tmap_a32,
-                           const CUtensorMap* tmap_b, cudaStream_t stream);
+                           const CUtensorMap* tmap_b, const CUtensorMap* tmap_out, cudaStream_t stream);
 // kind: kFp4Nv, kFp4Mx or kNarrow16.  The maps, innermost first; with `chunked` a row is (K-block, 128 bytes), otherwise all of
 // its bytes and one K-block: tmap_a {bytes, rows, K-blocks} in boxes {128, slot_rows (32 without chunks), chunks}; tmap_b {bytes,
 // rows, halves, K-blocks, experts} in boxes {128, 128 / halves, halves, chunks, 1} with SwiGLU's gate and up rows as two halves, or, for

@@ -451,7 +451,7 @@ struct PartWalker {
 template <bool W_MN, bool SWIGLU>
 __global__ void __launch_bounds__(kEmThreads, 1)
 grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
-                            const __grid_constant__ CUtensorMap tmap_b, const GroupedMlpParams p) {
+                            const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_out, const GroupedMlpParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {  // swizzled TMA tiles need it; the same in both CTAs of a pair
         if (threadIdx.x == 0) gemm_record_status(&g_mlp_status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
@@ -591,27 +591,32 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
         const int cq = ew >> 2;   // which 32 rows of each 128
         const int f = q * 32 + static_cast<int>(lane);  // column inside a block of 128
         const bool fp16 = p.fp16 != 0;
-        uint8_t* out = static_cast<uint8_t*>(p.out);
-        // 128 rows x 128 columns go through shared memory and leave as one bulk copy per row: w16 holds rows (2 i, 2 i + 1) of this
-        // thread's 32; the rows start at row r0 of the tile, the columns at column c of a matrix `width` wide with rows `pitch` apart
-        auto push = [&](const uint32_t* w16, int r0, uint8_t* base, size_t pitch, int c, int width) {
-            if (cq == 0) bulk_wait_group_read<0>();  // the copies that read this buffer are done with it
-            named_bar_sync(1, kEmEpiThreads);
-            if (r0 + cq * 32 < rows) {
-                uint8_t* at = stg + (cq * 32) * kEmStgPitch + f * 2;
+        // Two warps share 32 rows x 64 columns, which go through shared memory and leave as one tensor copy; rows of a block of 32 that
+        // ends inside it are stored from registers.  w16 holds rows (2 i, 2 i + 1) of this thread's 32, which start at row r0 + 32 cq
+        // of the tile; column c of the result is the block's first.
+        const int box = cq * 2 + (q >> 1), x = f & 63;
+        uint8_t* stage = stg + box * 4096;
+        const bool issues = (q & 1) == 0 && lane == 0;
+        auto push = [&](const uint32_t* w16, int r0, int c) {
+            const int first = r0 + cq * 32;
+            if (first >= rows || c + (q >> 1) * 64 >= p.n_dim) return;  // the same in both warps
+            if (first + 32 <= rows) {
+                if (issues) bulk_wait_group_read<0>();  // the copy that reads this buffer is done with it
+                named_bar_sync(1 + box, 64);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    *reinterpret_cast<uint16_t*>(at + (2 * j) * kEmStgPitch) = static_cast<uint16_t>(w16[j]);
-                    *reinterpret_cast<uint16_t*>(at + (2 * j + 1) * kEmStgPitch) = static_cast<uint16_t>(w16[j] >> 16);
+                for (int j = 0; j < 32; ++j)
+                    *reinterpret_cast<uint16_t*>(stage + j * 128 + (((x >> 3) ^ (j & 7)) << 4) + (x & 7) * 2) = static_cast<uint16_t>(w16[j >> 1] >> (16 * (j & 1)));
+                fence_proxy_async_smem();
+                named_bar_sync(1 + box, 64);
+                if (issues) {
+                    tma_store_2d(&tmap_out, smem_u32(stage), (c + (q >> 1) * 64) * 2, row0 + first);
+                    bulk_commit_group();
                 }
-            }
-            fence_proxy_async_smem();
-            named_bar_sync(1, kEmEpiThreads);
-            if (cq == 0) {
-                if (r0 + f < rows)
-                    bulk_store_s2g(base + static_cast<size_t>(row0 + r0 + f) * pitch + static_cast<size_t>(c) * 2, stg + f * kEmStgPitch,
-                                   static_cast<uint32_t>(min(128, width - c)) * 2u);
-                bulk_commit_group();
+            } else if (c + f < p.n_dim) {
+                uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + static_cast<size_t>(row0 + first) * p.n_dim + c + f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (first + j < rows) to[static_cast<size_t>(j) * p.n_dim] = static_cast<uint16_t>(w16[j >> 1] >> (16 * (j & 1)));
             }
         };
         uint32_t tcount = 0;
@@ -661,8 +666,8 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
                 }
                 hand_back();
                 if (c_lo < p.n_dim) {  // the same in every thread of the CTA
-                    push(act[0], 0, out, static_cast<size_t>(p.n_dim) * 2, c_lo, p.n_dim);
-                    if (two) push(act[1], 128, out, static_cast<size_t>(p.n_dim) * 2, c_lo, p.n_dim);
+                    push(act[0], 0, c_lo);
+                    if (two) push(act[1], 128, c_lo);
                 }
             } else {
                 uint32_t res[4][16];  // [128 rows][block]
@@ -680,11 +685,11 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int c = c_lo + (i & 1) * 128;
-                    if (c < p.n_dim && (i < 2 || two)) push(res[i], (i >> 1) * 128, out, static_cast<size_t>(p.n_dim) * 2, c, p.n_dim);
+                    if (c < p.n_dim && (i < 2 || two)) push(res[i], (i >> 1) * 128, c);
                 }
             }
         }
-        if (cq == 0) bulk_wait_group<0>();  // every row this thread sent has been written
+        if ((q & 1) == 0) bulk_wait_group<0>();  // everything this thread sent has been written
         if (!ok) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
         if (!SWIGLU)  // rows of no expert; act and dgu of such rows are read by nothing
             zero_loose_rows(p.out, p.n_dim / 8, p.expert_offsets, p.num_experts, p.rows, static_cast<int>(threadIdx.x) - kEmEpiWarp0 * 32, kEmEpiThreads);
@@ -706,12 +711,12 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
 namespace {
 
 template <bool W_MN, bool SWIGLU>
-int launch_rows(const cam::GroupedMlpParams* p, const CUtensorMap* ta, const CUtensorMap* ta32, const CUtensorMap* tb, cudaStream_t stream) {
+int launch_rows(const cam::GroupedMlpParams* p, const CUtensorMap* ta, const CUtensorMap* ta32, const CUtensorMap* tb, const CUtensorMap* tout, cudaStream_t stream) {
     static cam::PairLimit limit;
     const int64_t nblk = (p->n_dim + 127) / 128, n_tiles = SWIGLU ? (nblk + 1) / 2 : (nblk + 3) / 4;
     // parts of an expert's rows: at most one beyond the full ones
     const int64_t parts = p->rows / 256 + (p->rows < p->num_experts ? p->rows : p->num_experts);
-    return cam::launch_pairs(limit, cam::grouped_gemm_16_rows_kernel<W_MN, SWIGLU>, cam::kEmThreads, cam::kErSmem, parts * n_tiles, stream, *ta, *ta32, *tb, *p);
+    return cam::launch_pairs(limit, cam::grouped_gemm_16_rows_kernel<W_MN, SWIGLU>, cam::kEmThreads, cam::kErSmem, parts * n_tiles, stream, *ta, *ta32, *tb, *tout, *p);
 }
 
 template <bool DW>
@@ -725,13 +730,13 @@ int launch_square(const cam::GroupedMlpParams* p, const CUtensorMap* ta, const C
 }  // namespace
 
 extern "C" int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, const CUtensorMap* tmap_a, const CUtensorMap* tmap_a32,
-                                      const CUtensorMap* tmap_b, cudaStream_t stream) {
+                                      const CUtensorMap* tmap_b, const CUtensorMap* tmap_out, cudaStream_t stream) {
     switch (form) {
-        case cam::kMlpUp: return launch_rows<false, true>(p, tmap_a, tmap_a32, tmap_b, stream);
-        case cam::kMlpDown: return launch_rows<false, false>(p, tmap_a, tmap_a32, tmap_b, stream);
+        case cam::kMlpUp: return launch_rows<false, true>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
+        case cam::kMlpDown: return launch_rows<false, false>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
         case cam::kMlpDact: return launch_square<false>(p, tmap_a, tmap_a32, tmap_b, stream);
-        case cam::kMlpDx: return launch_rows<true, false>(p, tmap_a, tmap_a32, tmap_b, stream);
-        case cam::kMlpDw: return launch_square<true>(p, tmap_a, tmap_a32, tmap_b, stream);
+        case cam::kMlpDx: return launch_rows<true, false>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
+        case cam::kMlpDw: return launch_square<true>(p, tmap_a, tmap_out, tmap_b, stream);  // tmap_a32 is not used
     }
     return static_cast<int>(cudaErrorInvalidValue);
 }

@@ -110,8 +110,8 @@ bool few_rows_pay_fp4(int rows, int num_experts, int n_dim, bool swiglu) {
 // constants fitted to kernel times (L2 cold) of 66 forward and 44 backward sizes: 1 to 64 experts of 2048 x 768 to 7168 x 2048, 16 to
 // 2048 rows each.  A turn of the pairs takes, per K-block, a start and the MMAs of its rows, or the memory's time for the weights if
 // many pairs are busy; its tiles are 512 weight rows x 256 rows, with gate and up 256 of each, dact's 256 x 256.
-//   forward, pairs / few rows: one expert of 7168 x 2048, 512 rows 112 / 77 us; 8 of 2048 x 1024, 256 rows 66 / 56, 384 rows 65 / 71;
-//     4 of 7168 x 2048, 160 rows 110 / 196
+//   forward, pairs / few rows: one expert of 7168 x 2048, 512 rows 105 / 77 us; 8 of 2048 x 1024, 256 rows 60 / 56, 384 rows 56 / 71;
+//     4 of 7168 x 2048, 160 rows 103 / 138
 //   dact and dx: one of 7168 x 2048, 256 rows 99 / 56, 768 rows 104 / 136; 8 of 2048 x 1024, 256 rows 69 / 62, 384 rows 69 / 89;
 //     16 of 4096 x 2048, 375 rows 290 / 431
 bool few_rows_pay_16(int rows, int num_experts, int n_dim, int form, int k) {
@@ -296,7 +296,10 @@ int row_product(int form, const char* what, const void* a, int k, const void* w,
     if (map_2d(&ta, a, static_cast<uint64_t>(k) * 2, static_cast<uint64_t>(rows), 128) != 0) return -1;
     if (map_2d(&ta32, a, static_cast<uint64_t>(k) * 2, static_cast<uint64_t>(rows), 32) != 0) return -1;
     if (map_3d(&tb, w, static_cast<uint64_t>(w_cols) * 2, static_cast<uint64_t>(w_rows), static_cast<uint64_t>(num_experts), by_rows ? 64 : 128) != 0) return -1;
-    return launched(cam_launch_grouped_mlp(&p, form, &ta, &ta32, &tb, stream), what);
+    if (form == cam::kMlpDact) return launched(cam_launch_grouped_mlp(&p, form, &ta, &ta32, &tb, &ta, stream), what);
+    CUtensorMap tout;
+    if (map_2d(&tout, out, static_cast<uint64_t>(n) * 2, static_cast<uint64_t>(rows), 32) != 0) return -1;
+    return launched(cam_launch_grouped_mlp(&p, form, &ta, &ta32, &tb, &tout, stream), what);
 }
 
 }  // namespace
@@ -341,7 +344,7 @@ extern "C" int cam_grouped_mlp_dw(const void* a, const void* b, const int* offse
     if (map_3d(&tout, dw, static_cast<uint64_t>(n_dim) * 2, static_cast<uint64_t>(m_dim), static_cast<uint64_t>(num_experts), 128) != 0) return -1;
     if (map_2d(&ta, a, static_cast<uint64_t>(m_dim) * 2, static_cast<uint64_t>(rows), 64) != 0) return -1;
     if (map_2d(&tb, b, static_cast<uint64_t>(n_dim) * 2, static_cast<uint64_t>(rows), 64) != 0) return -1;
-    return launched(cam_launch_grouped_mlp(&p, cam::kMlpDw, &ta, &tout, &tb, stream), "grouped_mlp (dw)");
+    return launched(cam_launch_grouped_mlp(&p, cam::kMlpDw, &ta, &ta, &tb, &tout, stream), "grouped_mlp (dw)");
 }
 
 extern "C" int cam_expert_ops_status(CamStatus* out) {
