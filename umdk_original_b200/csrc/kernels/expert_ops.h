@@ -97,8 +97,8 @@ int cam_launch_grouped_gemm_fp4(const cam::GroupedGemmFp4Params* p, int fmt, int
                                 const CUtensorMap* tmap_a32, const CUtensorMap* tmap_b, const CUtensorMap* tmap_out, cudaStream_t stream);
 // tmap_a: the row operand in boxes of 128 rows (kMlpDw: 64 rows), tmap_a32: in boxes of 32 rows; tmap_b: the weights
 // [E, rows, columns] in boxes of 128 rows, or of 64 where their row is the contraction index (kMlpDact, kMlpDx), or for kMlpDw
-// the second row operand in boxes of 64 rows.  tmap_out: the result in boxes of 32 rows (kMlpUp, kMlpDown, kMlpDx), or [E, m_dim, n_dim]
-// in boxes of 128 rows (kMlpDw).  All boxes are 128 bytes wide.  Not used, any map does: tmap_a32 of kMlpDw, tmap_out of kMlpDact.
+// the second row operand in boxes of 64 rows.  tmap_out: the result in boxes of 32 rows, as [rows, 2, I] for kMlpDact, or [E, m_dim,
+// n_dim] in boxes of 128 rows (kMlpDw).  All boxes are 128 bytes wide.  Not used, any map does: tmap_a32 of kMlpDw.
 int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, const CUtensorMap* tmap_a, const CUtensorMap* tmap_a32,
                            const CUtensorMap* tmap_b, const CUtensorMap* tmap_out, cudaStream_t stream);
 // kind: kFp4Nv, kFp4Mx or kNarrow16.  The maps, innermost first; with `chunked` a row is (K-block, 128 bytes), otherwise all of

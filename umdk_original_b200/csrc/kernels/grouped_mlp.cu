@@ -25,6 +25,9 @@
 // epilogue fills on its own: 16 gradients of 4096 x 2048 from 16 rows each (268 MB) 104 -> 52 us against one copy per row, 0.8 of a
 // plain copy's rate, and 512 rows 125 -> 102.
 //
+// The other products write boxes of 32 rows x 64 columns, each filled by two warps; the last, ragged rows of a block are stored from
+// registers.  Against one copy per row: up and down of 4 experts of 7168 x 2048, 256 rows 123 -> 116 us, dact and dx 115 -> 109.
+//
 // With few rows per expert, or few tiles in all, up, down, dact and dx are computed by expert_gemm_narrow.cu instead.
 //
 // K-blocks of 64 values (128 bytes) come by TMA.  An operand whose contraction index is not its contiguous one (w2 of dact, w1 of dx,
@@ -44,8 +47,7 @@ constexpr int kEmEpiWarp0 = 4;
 constexpr int kEmStages = 6;
 constexpr int kEmTile = 128 * 128;  // 128 rows x 64 values of A, or as many of B
 constexpr int kEmStageBytes = 2 * kEmTile;
-constexpr int kEmStgPitch = 272;
-constexpr int kEmStgBytes = 128 * kEmStgPitch;
+constexpr int kEmStgBytes = 32768;  // results on their way out: 128 rows x 128 columns of 16 bits, in boxes 128 bytes wide
 constexpr int kEmSmem = kEmStages * kEmStageBytes + kEmStgBytes + 1024;
 static_assert(kEmSmem <= 232448, "exceeds the shared memory of one CTA");
 constexpr uint32_t kEmTmemCols = 512;
@@ -102,7 +104,7 @@ struct GradTileWalker {
 template <bool DW>
 __global__ void __launch_bounds__(kEmThreads, 1)
 grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
-                       const __grid_constant__ CUtensorMap tmap_b, const GroupedMlpParams p) {
+                       const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_out, const GroupedMlpParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {  // swizzled TMA tiles need it; the same in both CTAs of a pair
         if (threadIdx.x == 0) gemm_record_status(&g_mlp_status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
@@ -282,23 +284,7 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
         const int cq = ew >> 2;   // which 32-column quarter of each 128-column half
         const int r = q * 32 + static_cast<int>(lane);
         const bool fp16 = p.fp16 != 0;
-        uint8_t* srow = stg + r * kEmStgPitch;
         uint32_t tcount = 0;
-        // 128 columns of packed values (16 words per thread) go through shared memory and leave as one bulk copy per row, to
-        // column c0 of `orow` (null: the row is not stored) of a matrix `width` wide
-        auto push = [&](const uint32_t* w16, uint8_t* orow, int c0, int width) {
-            if (cq == 0) bulk_wait_group_read<0>();  // the copies that read this buffer are done with it
-            named_bar_sync(1, kEmEpiThreads);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<uint4*>(srow + cq * 64 + j * 16) = make_uint4(w16[4 * j], w16[4 * j + 1], w16[4 * j + 2], w16[4 * j + 3]);
-            fence_proxy_async_smem();
-            named_bar_sync(1, kEmEpiThreads);
-            if (cq == 0) {
-                if (orow != nullptr) bulk_store_s2g(orow + static_cast<size_t>(c0) * 2, srow, static_cast<uint32_t>(min(128, width - c0)) * 2u);
-                bulk_commit_group();
-            }
-        };
         for (int tile = pair_id; ok && locate(tile); tile += num_pairs, ++tcount) {
             const uint32_t b = tcount & 1u;
             const int first = (DW ? mt * 256 : 0) + static_cast<int>(cta) * BM;  // of this CTA's rows of the tile
@@ -335,7 +321,33 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
                 load(0);
                 if (!mbar_wait_bounded(&bar_tfull[b], (tcount >> 1) & 1u, abort_flag, 2000000000ull, 64u)) { ok = false; break; }
                 tc_fence_after_sync();
-                uint8_t* orow = valid ? static_cast<uint8_t*>(p.out) + orow_i * (4 * static_cast<size_t>(p.n_dim)) : nullptr;
+                // Two warps share 32 rows x 64 columns, which go through shared memory and leave as one tensor copy; rows of a block of
+                // 32 that ends inside it are stored from registers.  `part`: 0 dg, 1 du.
+                const int box = q * 2 + (cq >> 1);
+                uint8_t* at = stg + box * 4096 + lane * 128;
+                const bool whole = first + q * 32 + 32 <= rows, issues = (cq & 1) == 0 && lane == 0;
+                auto push = [&](const uint32_t* w16, int c0, int part) {
+                    if (c0 + (cq >> 1) * 64 >= p.n_dim) return;  // the same in both warps
+                    if (whole) {
+                        if (issues) bulk_wait_group_read<0>();  // the copy that reads this buffer is done with it
+                        named_bar_sync(1 + box, 64);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            *reinterpret_cast<uint4*>(at + ((((cq & 1) * 4 + j) ^ (r & 7)) << 4)) = make_uint4(w16[4 * j], w16[4 * j + 1], w16[4 * j + 2], w16[4 * j + 3]);
+                        fence_proxy_async_smem();
+                        named_bar_sync(1 + box, 64);
+                        if (issues) {
+                            tma_store_3d(&tmap_out, smem_u32(stg + box * 4096), (c0 + (cq >> 1) * 64) * 2, part, row0 + first + q * 32);
+                            bulk_commit_group();
+                        }
+                    } else if (valid) {
+                        const int c = c0 + cq * 32;
+                        uint16_t* to = static_cast<uint16_t*>(p.out) + (2 * orow_i + part) * p.n_dim + c;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (c + 8 * j < p.n_dim) *reinterpret_cast<uint4*>(to + 8 * j) = make_uint4(w16[4 * j], w16[4 * j + 1], w16[4 * j + 2], w16[4 * j + 3]);
+                    }
+                };
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t v[32];
@@ -360,10 +372,8 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
                         }
                         if (2 * h + part < 3) load(2 * h + part + 1);
                     }
-                    if (c0 < p.n_dim) {  // the same in every thread of the CTA
-                        push(v, orow, c0, p.n_dim);
-                        push(du, orow != nullptr ? orow + static_cast<size_t>(p.n_dim) * 2 : nullptr, c0, p.n_dim);
-                    }
+                    push(v, c0, 0);
+                    push(du, c0, 1);
                 }
                 continue;
             }
@@ -392,14 +402,14 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
                 fence_proxy_async_smem();
                 named_bar_sync(1 + pair, kEmEpiThreads / 2);
                 if (issues) {
-                    if (first < p.m_dim) tma_store_3d(&tmap_a32, smem_u32(stg + pair * 16384), c0 * 2, first, e);
+                    if (first < p.m_dim) tma_store_3d(&tmap_out, smem_u32(stg + pair * 16384), c0 * 2, first, e);
                     bulk_commit_group();
                 }
             };
             store_half(v0, 0);
             store_half(v1, 1);
         }
-        if (DW ? (ew & 7) == 0 : cq == 0) bulk_wait_group<0>();  // everything this thread sent has been written
+        if (DW ? (ew & 7) == 0 : (cq & 1) == 0) bulk_wait_group<0>();  // everything this thread sent has been written
         if (!ok) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
     }
 
@@ -720,11 +730,11 @@ int launch_rows(const cam::GroupedMlpParams* p, const CUtensorMap* ta, const CUt
 }
 
 template <bool DW>
-int launch_square(const cam::GroupedMlpParams* p, const CUtensorMap* ta, const CUtensorMap* ta32, const CUtensorMap* tb, cudaStream_t stream) {
+int launch_square(const cam::GroupedMlpParams* p, const CUtensorMap* ta, const CUtensorMap* ta32, const CUtensorMap* tb, const CUtensorMap* tout, cudaStream_t stream) {
     static cam::PairLimit limit;
     const int64_t blocks = DW ? static_cast<int64_t>(p->num_experts) * ((p->m_dim + 255) / 256)
                               : p->rows / 256 + (p->rows < p->num_experts ? p->rows : p->num_experts);
-    return cam::launch_pairs(limit, cam::grouped_gemm_16_square_kernel<DW>, cam::kEmThreads, cam::kEmSmem, blocks * ((p->n_dim + 255) / 256), stream, *ta, *ta32, *tb, *p);
+    return cam::launch_pairs(limit, cam::grouped_gemm_16_square_kernel<DW>, cam::kEmThreads, cam::kEmSmem, blocks * ((p->n_dim + 255) / 256), stream, *ta, *ta32, *tb, *tout, *p);
 }
 
 }  // namespace
@@ -734,9 +744,9 @@ extern "C" int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, 
     switch (form) {
         case cam::kMlpUp: return launch_rows<false, true>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
         case cam::kMlpDown: return launch_rows<false, false>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
-        case cam::kMlpDact: return launch_square<false>(p, tmap_a, tmap_a32, tmap_b, stream);
+        case cam::kMlpDact: return launch_square<false>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
         case cam::kMlpDx: return launch_rows<true, false>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
-        case cam::kMlpDw: return launch_square<true>(p, tmap_a, tmap_out, tmap_b, stream);  // tmap_a32 is not used
+        case cam::kMlpDw: return launch_square<true>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
     }
     return static_cast<int>(cudaErrorInvalidValue);
 }

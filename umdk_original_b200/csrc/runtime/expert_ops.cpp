@@ -112,8 +112,8 @@ bool few_rows_pay_fp4(int rows, int num_experts, int n_dim, bool swiglu) {
 // many pairs are busy; its tiles are 512 weight rows x 256 rows, with gate and up 256 of each, dact's 256 x 256.
 //   forward, pairs / few rows: one expert of 7168 x 2048, 512 rows 105 / 77 us; 8 of 2048 x 1024, 256 rows 60 / 56, 384 rows 56 / 71;
 //     4 of 7168 x 2048, 160 rows 103 / 138
-//   dact and dx: one of 7168 x 2048, 256 rows 99 / 56, 768 rows 104 / 136; 8 of 2048 x 1024, 256 rows 69 / 62, 384 rows 69 / 89;
-//     16 of 4096 x 2048, 375 rows 290 / 431
+//   dact and dx: one of 7168 x 2048, 256 rows 93 / 56, 768 rows 97 / 128; 8 of 2048 x 1024, 128 rows 56 / 50, 384 rows 63 / 87; 16 of
+//     4096 x 2048, 375 rows 281 / 425
 bool few_rows_pay_16(int rows, int num_experts, int n_dim, int form, int k) {
     const int sw = env_switch("UMDK_CAM_EXPERT_NARROW");
     if (sw >= 0) return sw != 0;
@@ -130,10 +130,10 @@ bool few_rows_pay_16(int rows, int num_experts, int n_dim, int form, int k) {
     const int64_t few = f.turns * (f.turn_kblocks * (dact ? 807 : backward ? 760 : 770 + f.slot_rows) + f.turn_fixed);
     int64_t pairs;
     if (dact) {
-        pairs = 8000 + turns * (f.kblocks * (550 + 400 * busy / most) + 1000);
+        pairs = 4000 + turns * (f.kblocks * (550 + 400 * busy / most) + 1000);
     } else {
         const int64_t work = backward ? 560 + cols * 5 / 2 : 700 + 3 * cols;
-        pairs = turns * f.kblocks * (work > memory ? work : memory) + (backward ? 9500 : 18000 * turns);
+        pairs = turns * f.kblocks * (work > memory ? work : memory) + (backward ? 7000 : 18000 * turns);
     }
     return few < pairs;
 }
@@ -296,9 +296,15 @@ int row_product(int form, const char* what, const void* a, int k, const void* w,
     if (map_2d(&ta, a, static_cast<uint64_t>(k) * 2, static_cast<uint64_t>(rows), 128) != 0) return -1;
     if (map_2d(&ta32, a, static_cast<uint64_t>(k) * 2, static_cast<uint64_t>(rows), 32) != 0) return -1;
     if (map_3d(&tb, w, static_cast<uint64_t>(w_cols) * 2, static_cast<uint64_t>(w_rows), static_cast<uint64_t>(num_experts), by_rows ? 64 : 128) != 0) return -1;
-    if (form == cam::kMlpDact) return launched(cam_launch_grouped_mlp(&p, form, &ta, &ta32, &tb, &ta, stream), what);
     CUtensorMap tout;
-    if (map_2d(&tout, out, static_cast<uint64_t>(n) * 2, static_cast<uint64_t>(rows), 32) != 0) return -1;
+    const uint64_t width = static_cast<uint64_t>(n) * 2;
+    if (form == cam::kMlpDact) {
+        const uint64_t dims[3] = {width, 2, static_cast<uint64_t>(rows)}, strides[2] = {width, 2 * width};
+        const uint32_t box[3] = {128, 1, 32};
+        if (cam_encode_tmap(&tout, out, 3, dims, strides, box) != 0) return -1;
+    } else if (map_2d(&tout, out, width, static_cast<uint64_t>(rows), 32) != 0) {
+        return -1;
+    }
     return launched(cam_launch_grouped_mlp(&p, form, &ta, &ta32, &tb, &tout, stream), what);
 }
 
