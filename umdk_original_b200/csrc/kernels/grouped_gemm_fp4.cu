@@ -15,7 +15,7 @@
 // they touch: one K-block at a time (16 bytes of every row) took them 1070 cycles where the MMAs take 512.
 //
 // Measured (one call, L2 cold): 16 experts of 1024 rows, 7168 -> 2 x 2048 with SwiGLU: nvfp4 240 us (4.0 PFLOP/s), mxfp4 184 us (5.2);
-// 32 of 1024 rows, 2048 -> 7168: 287 us (3.4) and 240 us (4.0).  Under back-to-back calls the power limit takes a third of that.
+// 32 of 1024 rows, 2048 -> 7168: 285 us (3.4) and 215 us (4.5; 238 with one copy per row instead of boxes of 32 x 64).  Under back-to-back calls the power limit takes a third of that.
 // What bounds it is the work in shared memory: a K-block brings 32 KiB per CTA by TMA, the MMAs read as much, and the nvfp4 scales
 // are written, transposed and copied on, 24 KiB more; half of that for mxfp4, which is what it is faster by.
 // Tried in place of this arrangement (nvfp4 / mxfp4 us for the first of these sizes, 240 / 184 as it is):
