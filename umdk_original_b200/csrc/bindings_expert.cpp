@@ -1,6 +1,7 @@
 // PyTorch bindings of the expert-MLP operators that need no Buffer: 4-bit quantisation, grouped products of 4-bit operands, the
 // gated feed-forward block of 16-bit experts with its backward pass.
 // Schemas are added to the library that bindings.cpp defines.
+#include <ATen/TensorSubclassLikeUtils.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -305,10 +306,19 @@ Mlp3 call_mlp_train(const at::Tensor& x, const at::Tensor& w1, const at::Tensor&
 
 // What the backward pass will read of an input.  The rows of a dispatch are views of memory that the next dispatch on that Buffer
 // overwrites, behind the back of autograd's version counters, and a program of several layers dispatches again before it runs
-// backward: such memory (any that PyTorch's allocators do not own) is copied.
+// backward: such memory (any that PyTorch's allocators do not own) is copied.  A tracer's stand-ins (torch.compile) do not know whose
+// memory the traced program will see, so a traced program always copies, by an operator of this library: a plain clone may be
+// removed by the compiler's passes, or moved into the backward pass, where it would come too late.
 at::Tensor kept_for_backward(const at::Tensor& t) {
+    if (at::isTensorSubclassLike(t)) {
+        static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("umdk_cam_op_lib::grouped_mlp_keep", "")
+                             .typed<at::Tensor(const at::Tensor&)>();
+        return op.call(t);
+    }
     return t.storage().unsafeGetStorageImpl()->resizable() ? t : t.clone();
 }
+
+at::Tensor grouped_mlp_keep(const at::Tensor& t) { return t.clone(); }
 
 struct GroupedMlpFunction : public torch::autograd::Function<GroupedMlpFunction> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2,
@@ -373,7 +383,10 @@ TORCH_LIBRARY_FRAGMENT(umdk_cam_op_lib, m) {
     m.def("grouped_mlp_train(Tensor x, Tensor w1, Tensor w2, Tensor expert_offsets) -> (Tensor, Tensor, Tensor)");
     m.def("grouped_mlp_backward(Tensor dy, Tensor x, Tensor w1, Tensor w2, Tensor expert_offsets, Tensor act, Tensor gate_up, "
           "bool need_dx=True, bool need_dw1=True, bool need_dw2=True) -> (Tensor, Tensor, Tensor)");
+    m.def("grouped_mlp_keep(Tensor t) -> Tensor");
 }
+
+TORCH_LIBRARY_IMPL(umdk_cam_op_lib, CompositeExplicitAutograd, m) { m.impl("grouped_mlp_keep", &grouped_mlp_keep); }
 
 TORCH_LIBRARY_IMPL(umdk_cam_op_lib, CUDA, m) {
     m.impl("quantize_fp4", &quantize_fp4_cuda);
@@ -403,4 +416,5 @@ TORCH_LIBRARY_IMPL(umdk_cam_op_lib, Autograd, m) {
     m.impl("grouped_mlp", &grouped_mlp_autograd);
     m.impl("grouped_mlp_train", torch::autograd::autogradNotImplementedFallback());
     m.impl("grouped_mlp_backward", torch::autograd::autogradNotImplementedFallback());
+    m.impl("grouped_mlp_keep", torch::autograd::autogradNotImplementedFallback());
 }
