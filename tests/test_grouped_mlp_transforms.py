@@ -55,6 +55,36 @@ def test_compiled_is_eager(backend):
     assert all(torch.equal(a, b) for a, b in zip(*runs))
 
 
+@pytest.mark.parametrize("which", range(3))
+@pytest.mark.parametrize("no_grad", [False, True])
+def test_forward_mode_is_refused(which, no_grad):
+    """A tangent is not dropped: neither by dual tensors nor by torch.func.jvp, whichever operand carries it."""
+    import torch.autograd.forward_ad as fwad
+    args = tensors()[:3]
+    off = offsets_of([4, 3, 6])
+
+    def f(t):
+        return ops.grouped_mlp(*[t if i == which else a for i, a in enumerate(args)], off)
+    with torch.set_grad_enabled(not no_grad):
+        with fwad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            f(fwad.make_dual(args[which], torch.ones_like(args[which])))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.func.jvp(f, (args[which],), (torch.ones_like(args[which]),))
+        with fwad.dual_level():
+            assert torch.equal(f(args[which]), f(args[which].clone()))  # nothing here carries a tangent
+
+
+def test_functorch():
+    """Batches of calls are computed one by one; gradients inside torch.func are refused, not left out."""
+    x, w1, w2, dy = tensors()
+    off = offsets_of([4, 3, 6])
+    xs = torch.stack([x, x.flip(0)])
+    got = torch.func.vmap(lambda t: ops.grouped_mlp(t, w1, w2, off))(xs)
+    assert torch.equal(got, torch.stack([ops.grouped_mlp(t, w1, w2, off) for t in xs]))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda w: ops.grouped_mlp(x, w, w2, off).float().sum())(w1)
+
+
 @pytest.mark.gpu
 def test_compiled_layers_after_the_next_dispatch():
     """Two compiled layers share a Buffer: the second dispatch overwrites the rows that the first layer's experts saw."""

@@ -353,6 +353,9 @@ void check_capture(const at::Tensor& t, const char* what) {
 }
 
 at::Tensor grouped_mlp_autograd(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, const at::Tensor& expert_offsets) {
+    // a dual tensor need not require a gradient: without this its tangent would be dropped
+    for (const at::Tensor* t : {&x, &w1, &w2})
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), "umdk_cam_op_lib: grouped_mlp has no forward-mode derivative");
     if (at::GradMode::is_enabled() && (x.requires_grad() || w1.requires_grad() || w2.requires_grad())) {
         if (x.is_cuda()) {
             c10::cuda::CUDAGuard guard(x.device());
