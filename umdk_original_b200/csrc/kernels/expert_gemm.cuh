@@ -257,9 +257,9 @@ __device__ __forceinline__ void fp4_swiglu32(const uint32_t* gate, const uint32_
     uint32_t sc[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        float d, inv;
-        sc[h] = fp4_scale<FMT>(amax[h], out_g, __fmul_rn(6.f, out_g), d, inv);
-        c[h] = fp4_codes16<FMT>(act + 16 * h, d, inv, amax[h] < 0x7F800000u);
+        Fp4Divisor div;
+        sc[h] = fp4_scale<FMT>(amax[h], out_g, __fmul_rn(6.f, out_g), div);
+        c[h] = fp4_codes16<FMT>(act + 16 * h, div);
     }
     codes = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
     scales = sc[0] | (sc[1] << 8);

@@ -446,9 +446,9 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                         amax = max(amax, __float_as_uint(g[j]) & 0x7FFFFFFFu);
                     }
                     if (KIND == kFp4Mx) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-                    float d, inv;
-                    const uint32_t code = fp4_scale<KIND>(amax, out_g, __fmul_rn(6.f, out_g), d, inv);
-                    const uint2 codes = fp4_codes16<KIND>(g, d, inv, amax < 0x7F800000u);
+                    Fp4Divisor div;
+                    const uint32_t code = fp4_scale<KIND>(amax, out_g, __fmul_rn(6.f, out_g), div);
+                    const uint2 codes = fp4_codes16<KIND>(g, div);
                     if (live) {
                         const size_t at = static_cast<size_t>(row0 + t) * (p.n_dim / 16) + nt * 4 + ch;  // in units of 16 columns
                         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + at * 8) = codes;

@@ -100,9 +100,9 @@ quantize_fp4_kernel(const uint4* __restrict__ x, uint2* __restrict__ q, uint8_t*
         if (i >= groups) continue;
         float g = 1.f;
         if (FMT == kFp4Nv && gscale != nullptr) g = __ldg(gscale + (groups_per_scale > 0 ? i / groups_per_scale : 0));
-        float d, inv;
-        const uint32_t code = fp4_scale<FMT>(amax, g, __fmul_rn(6.f, g), d, inv);
-        q[i] = fp4_codes16<FMT>(f, d, inv, amax < 0x7F800000u);
+        Fp4Divisor div;
+        const uint32_t code = fp4_scale<FMT>(amax, g, __fmul_rn(6.f, g), div);
+        q[i] = fp4_codes16<FMT>(f, div);
         if (FMT == kFp4Nv) s[i] = static_cast<uint8_t>(code);
         else if ((i & 1) == 0) s[i >> 1] = static_cast<uint8_t>(code);
     }
