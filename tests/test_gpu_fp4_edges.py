@@ -93,3 +93,24 @@ def test_infinite_divisor(ops):
     cq, cs = ops.quantize_fp4(x, 16, g)
     assert torch.equal(s.cpu().view(torch.uint8), cs.view(torch.uint8))
     assert (codes(q)[0, :15] == 0).all() and (codes(cq)[0, :15] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("block,g", [(16, None), (16, 0.0123), (16, 1e-20), (32, None)])
+def test_bytes_and_the_sign_of_zero(ops, dtype, block, g):
+    """Packed bytes are the CPU key's, zeros of both signs and negative values that round to zero among them."""
+    gen = torch.Generator().manual_seed(22)
+    x = torch.randn(16, 8 * block, generator=gen)
+    x[:, ::5] = -0.0
+    x[:, 1::5] = 0.0
+    x[:, 2::7] *= -1e-4
+    x[3], x[4] = 0.0, -0.0
+    x[5, :block] = -1e-7  # with some scales these blocks get the scale zero
+    x = x.to(dtype)
+    gs = None if g is None else torch.tensor([g])
+    q, s = ops.quantize_fp4(x.to(DEV), block, None if gs is None else gs.to(DEV))
+    cq, cs = ops.quantize_fp4(x, block, gs)
+    assert torch.equal(s.cpu().view(torch.uint8), cs.view(torch.uint8))
+    assert torch.equal(q.cpu(), cq)
+    nibbles = torch.stack([cq & 15, cq >> 4], -1).flatten(-2)
+    assert torch.equal(nibbles >> 3, torch.signbit(x).to(torch.uint8))

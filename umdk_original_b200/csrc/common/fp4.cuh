@@ -2,7 +2,7 @@
 //   e2m1     values 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives; two to a byte, the even element in the low nibble
 //   nvfp4    blocks of 16: s = e4m3(amax / (6 g)), q = e2m1(x / (s g)), x ~ q s g with one fp32 scale g per tensor or expert
 //   mxfp4    blocks of 32: s = 2^k, the smallest with 2^k >= amax / 6 (k >= -126; an all-zero block has 2^-127), x ~ q s
-// All roundings are to nearest, ties to even.  A NaN anywhere in an nvfp4 block makes its scale NaN (and with it the whole
+// All roundings are to nearest, ties to even; what rounds to zero keeps its sign.  A NaN anywhere in an nvfp4 block makes its scale NaN (and with it the whole
 // block); an infinity takes the largest scale and saturates to 6.  In mxfp4 NaN gives the scale code 255 (NaN), an
 // infinity the scale 2^127.
 #pragma once
@@ -108,29 +108,30 @@ __device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
     return r;
 }
 
-// x / d rounded to nearest, for nvfp4: with t = x inv and inv = 1 / d rounded to nearest, one remainder step t + (x - t d) inv gives
+// -x / d rounded to nearest, for nvfp4: with t = x inv and inv = 1 / d rounded to nearest, one remainder step t + (x - t d) inv gives
 // the correctly rounded quotient (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990),
-// so that a quotient half-way between two e2m1 values is seen as one.  In pairs the arithmetic of 32768 x 7168 bf16 values stays hidden
-// behind memory: 95 us, one at a time 99.
-__device__ __forceinline__ void fp4_divide_plain(const float* v, const Fp4Divisor& q, float (&y)[16]) {
-    const uint64_t inv = pair_of(q.inv, q.inv), minus_d = pair_of(-q.d, -q.d);
+// so that a quotient half-way between two e2m1 values is seen as one.  All of it is negated, because a remainder of zero is +0: added
+// to t it would lose the sign of x = -0, subtracted from -t it does not.  In pairs the arithmetic of 32768 x 7168 bf16 values stays
+// hidden behind memory (94 us; one at a time 99).
+__device__ __forceinline__ void fp4_minus_quotients(const float* v, const Fp4Divisor& q, float (&y)[16]) {
+    const uint64_t minus_inv = pair_of(-q.inv, -q.inv), d = pair_of(q.d, q.d);
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
-        const uint64_t x = pair_of(v[i], v[i + 1]), t = mul_pair(x, inv), z = fma_pair(fma_pair(t, minus_d, x), inv, t);
+        const uint64_t x = pair_of(v[i], v[i + 1]), t = mul_pair(x, minus_inv), z = fma_pair(fma_pair(t, d, x), minus_inv, t);
         asm("mov.b64 {%0, %1}, %2;" : "=f"(y[i]), "=f"(y[i + 1]) : "l"(z));
     }
 }
 // The same for blocks that are not plain.  Below 2^-60 values and divisor are taken times 2^64: 1 / d overflows below 2^-128, and the
 // remainder, 2^-48 of the value, is cut below 2^-101.  t is cut to 16, so that no remainder is infinity minus infinity; what is cut
 // saturates whatever the step adds.  Beside an infinite d all values are nothing.
-__device__ __forceinline__ void fp4_divide_any(const float* v, float d, float (&y)[16]) {
+__device__ __forceinline__ void fp4_minus_quotients_any(const float* v, float d, float (&y)[16]) {
     const float lift = d > 0.f && d < 0x1p-60f ? 0x1p64f : 1.f;
     d = __float_as_uint(d) == 0x7F800000u ? 0.f : d * lift;
     const float inv = d > 0.f ? __fdiv_rn(1.f, d) : 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const float x = v[i] * lift, t = fminf(fmaxf(x * inv, -16.f), 16.f);
-        y[i] = __fmaf_rn(__fmaf_rn(-t, d, x), inv, t);
+        y[i] = copysignf(__fmaf_rn(__fmaf_rn(-t, d, x), inv, t), -x);
     }
 }
 
@@ -142,12 +143,13 @@ __device__ __forceinline__ uint2 fp4_codes16(const float* v, const Fp4Divisor& q
 #pragma unroll
         for (int i = 0; i < 16; ++i) y[i] = v[i] * q.inv;
     } else if (q.plain) {
-        fp4_divide_plain(v, q, y);
+        fp4_minus_quotients(v, q, y);
     } else {
-        fp4_divide_any(v, q.d, y);
+        fp4_minus_quotients_any(v, q.d, y);
     }
-    return make_uint2(pack_e2m1x8(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]),
-                      pack_e2m1x8(y[8], y[9], y[10], y[11], y[12], y[13], y[14], y[15]));
+    const uint32_t flip = FMT == kFp4Mx ? 0u : 0x88888888u;  // the signs
+    return make_uint2(pack_e2m1x8(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]) ^ flip,
+                      pack_e2m1x8(y[8], y[9], y[10], y[11], y[12], y[13], y[14], y[15]) ^ flip);
 }
 
 }  // namespace cam

@@ -70,8 +70,9 @@ int launch_flat(Kernel kernel, int64_t groups, cudaStream_t stream, Args... args
     return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
+// 16-bit rows: six blocks per SM (40 registers), 32768 x 7168 bf16 to nvfp4 94 us; with the four that 52 registers leave 101.
 template <int FMT, int DT>
-__global__ void __launch_bounds__(kQThreads)
+__global__ void __launch_bounds__(kQThreads, DT == kDtFp32 ? 4 : 6)
 quantize_fp4_kernel(const uint4* __restrict__ x, uint2* __restrict__ q, uint8_t* __restrict__ s, int64_t groups,
                     const float* __restrict__ gscale, int64_t groups_per_scale) {
     constexpr int V = DT == kDtFp32 ? 4 : 2;  // 16-byte loads of a group
