@@ -69,6 +69,14 @@ __device__ __forceinline__ void abort_drain(const volatile uint32_t* abort_flag)
     const uint64_t t0 = globaltimer_ns();
     for (int i = 0; i < 4000 && globaltimer_ns() - t0 < 2000000ull; ++i) __nanosleep(1000);
 }
+// The epilogue's wait for a tile.  The warps of an epilogue meet at named barriers, and a wait that runs out is not seen by all of them
+// in the same tile: whoever left the tile loop alone would leave the others at a barrier for good.  So nobody leaves it.  After a wait
+// that ran out a warp goes through the tiles that are left without waiting; what it writes means nothing (the status says so), every
+// barrier has its threads and the loop ends.
+__device__ __forceinline__ void epilogue_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t sleep_ns) {
+    if (!aborted(abort_flag)) mbar_wait_bounded(bar, parity, abort_flag, 2000000000ull, sleep_ns);
+    __syncwarp();
+}
 // Position in a ring of stages: stage and the parity of its current turn
 struct Ring {
     uint32_t s = 0, ph = 0;

@@ -305,13 +305,13 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         const float a_g = p.a_gscale != nullptr ? __ldg(p.a_gscale) : 1.f;
         const float out_g = p.out_gscale != nullptr ? __ldg(p.out_gscale) : 1.f;
         uint32_t tcount = 0;
-        for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
+        for (int tile = pair_id; w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
             row0 += static_cast<int>(cta) * BM;
             rows = max(0, min(BM, rows - static_cast<int>(cta) * BM));
             const bool valid = r < rows;
             const size_t grow = static_cast<size_t>(row0 + (valid ? r : 0));
             const float alpha = p.b_gscale != nullptr ? a_g * __ldg(p.b_gscale + e) : a_g;
-            if (!mbar_wait_bounded(bar_tfull, tcount & 1u, abort_flag, 2000000000ull, 64u)) { ok = false; break; }
+            epilogue_wait(bar_tfull, tcount & 1u, abort_flag, 64u);
             tc_fence_after_sync();
             const uint32_t t0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + cq * 32;
             uint32_t v0[32], v1[32];  // columns cq*32.. of the first 128-column half, same of the second
@@ -372,7 +372,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             }
         }
         if (!SWIGLU && (cq & 1) == 0) bulk_wait_group<0>();  // everything this thread sent has been written
-        if (!ok) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
+        if (*abort_flag) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
         // rows of no expert
         const int et = static_cast<int>(threadIdx.x) - kF4EpiWarp0 * 32;
         if constexpr (SWIGLU) {

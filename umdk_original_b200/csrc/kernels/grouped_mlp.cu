@@ -285,7 +285,7 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
         const int r = q * 32 + static_cast<int>(lane);
         const bool fp16 = p.fp16 != 0;
         uint32_t tcount = 0;
-        for (int tile = pair_id; ok && locate(tile); tile += num_pairs, ++tcount) {
+        for (int tile = pair_id; locate(tile); tile += num_pairs, ++tcount) {
             const uint32_t b = tcount & 1u;
             const int first = (DW ? mt * 256 : 0) + static_cast<int>(cta) * BM;  // of this CTA's rows of the tile
             const bool valid = first + r < (DW ? p.m_dim : rows);
@@ -319,7 +319,7 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
                     }
                 };
                 load(0);
-                if (!mbar_wait_bounded(&bar_tfull[b], (tcount >> 1) & 1u, abort_flag, 2000000000ull, 64u)) { ok = false; break; }
+                epilogue_wait(&bar_tfull[b], (tcount >> 1) & 1u, abort_flag, 64u);
                 tc_fence_after_sync();
                 // Two warps share 32 rows x 64 columns, which go through shared memory and leave as one tensor copy; rows of a block of
                 // 32 that ends inside it are stored from registers.  `part`: 0 dg, 1 du.
@@ -377,7 +377,7 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
                 }
                 continue;
             }
-            if (!mbar_wait_bounded(&bar_tfull[b], (tcount >> 1) & 1u, abort_flag, 2000000000ull, 64u)) { ok = false; break; }
+            epilogue_wait(&bar_tfull[b], (tcount >> 1) & 1u, abort_flag, 64u);
             tc_fence_after_sync();
             uint32_t v0[32], v1[32];  // columns cq*32.. of the first 128-column half, same of the second
             tmem_ld_32x32b_x32(t0, v0);
@@ -410,7 +410,7 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
             store_half(v1, 1);
         }
         if (DW ? (ew & 7) == 0 : (cq & 1) == 0) bulk_wait_group<0>();  // everything this thread sent has been written
-        if (!ok) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
+        if (*abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
     }
 
     // ------------------------------------------------------------------ teardown
@@ -509,7 +509,6 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
     pdl_release();
     PartWalker w(p.expert_offsets, p.num_experts, n_tiles, p.rows);
     int e, nt, row0, rows;
-    bool ok = true;
     // result columns of this CTA's two blocks; past the last block nothing is loaded that exists (zeros) and nothing is stored
     auto col_lo = [&]() { return SWIGLU ? (2 * nt + static_cast<int>(cta)) * 128 : (4 * nt + 2 * static_cast<int>(cta)) * 128; };
 
@@ -630,7 +629,7 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
             }
         };
         uint32_t tcount = 0;
-        for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
+        for (int tile = pair_id; w.locate(tile, e, nt, row0, rows); tile += num_pairs, ++tcount) {
             const uint32_t t0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(cq * 32);
             const int c_lo = col_lo();
             const bool two = rows > 128;  // a second 128 rows: the same in every thread of the CTA
@@ -643,7 +642,7 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
                     else mbar_arrive_cluster(map_to_cta(bar_tempty, 0));
                 }
             };
-            if (!mbar_wait_bounded(bar_tfull, tcount & 1u, abort_flag, 2000000000ull, 64u)) { ok = false; break; }
+            epilogue_wait(bar_tfull, tcount & 1u, abort_flag, 64u);
             tc_fence_after_sync();
             if constexpr (SWIGLU) {
                 uint32_t act[2][16];
@@ -700,7 +699,7 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
             }
         }
         if ((q & 1) == 0) bulk_wait_group<0>();  // everything this thread sent has been written
-        if (!ok) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
+        if (*abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
         if (!SWIGLU)  // rows of no expert; act and dgu of such rows are read by nothing
             zero_loose_rows(p.out, p.n_dim / 8, p.expert_offsets, p.num_experts, p.rows, static_cast<int>(threadIdx.x) - kEmEpiWarp0 * 32, kEmEpiThreads);
     }
