@@ -74,7 +74,7 @@ __device__ __forceinline__ void abort_drain(const volatile uint32_t* abort_flag)
 // that ran out a warp goes through the tiles that are left without waiting; what it writes means nothing (the status says so), every
 // barrier has its threads and the loop ends.
 __device__ __forceinline__ void epilogue_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t sleep_ns) {
-    if (!aborted(abort_flag)) mbar_wait_bounded(bar, parity, abort_flag, 2000000000ull, sleep_ns);
+    if (!mbar_try_wait(bar, parity) && *abort_flag == 0u) mbar_wait_bounded(bar, parity, abort_flag, 2000000000ull, sleep_ns);
     __syncwarp();
 }
 // Position in a ring of stages: stage and the parity of its current turn
