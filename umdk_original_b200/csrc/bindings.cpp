@@ -1024,11 +1024,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         .def("act_s", &Buffer::act_s);
     m.def("set_phase_mask", [](int mask) { g_phase_mask = mask; });
     m.def("get_phase_mask", []() { return g_phase_mask; });
-    // (code, who, block, detail) of the first wait that ran out in a kernel of the operators without a Buffer, on the current device
-    m.def("expert_ops_status", []() {
+    // (code, who, block, detail) of a wait that ran out in a product of the operators without a Buffer, on the current device
+    m.def("expert_ops_status", [](bool clear) {
         CamStatus st{};
-        CAM_RT(cam_expert_ops_status(&st));
+        CAM_RT(cam_expert_ops_status(&st, clear));
         return std::make_tuple(st.code, st.who, st.block, st.detail);
+    }, py::arg("clear") = false);
+    m.def("expert_ops_set_status", [](int code, int who, int detail, int block) {
+        const CamStatus st{code, who, detail, block};
+        CAM_RT(cam_expert_ops_set_status(&st));
     });
     m.def("status_string", [](int code) { return std::string(cam_status_string(code)); });
 }

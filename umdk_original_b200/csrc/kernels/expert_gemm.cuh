@@ -26,6 +26,13 @@ __device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok;
 }
+// A wait that ran out.  `st` lies in host memory that the device can write, where the next call, and the host at any time, sees it
+// without a copy: one 16-byte store, unless an earlier one is there already.
+__device__ __forceinline__ void record_status(CamStatus* st, int code, int who, int detail) {
+    if (*reinterpret_cast<volatile int32_t*>(&st->code) != 0) return;
+    asm volatile("st.volatile.global.v4.s32 [%0], {%1, %2, %3, %4};" ::"l"(st), "r"(code), "r"(who), "r"(detail), "r"(static_cast<int>(blockIdx.x)) : "memory");
+    __threadfence_system();
+}
 // Bounded: after kWaitPolls polls (each of which the hardware may itself hold for a while), or once another role has given up,
 // it returns with *abort set; the pipeline then runs to the end of its tile without waiting, its results mean nothing, and the CTA
 // lets the copies in flight land (abort_drain) before it leaves.

@@ -36,8 +36,6 @@ static_assert(kNwSfCol0 + kNwScaleSlots * kNwSfCols <= kNwTmemCols, "tensor memo
 constexpr int kNwCtrlBytes = 1024;
 static_assert((2 * kNwMaxStages + 10) * 8 + 16 <= kNwCtrlBytes, "barriers");
 
-static __device__ CamStatus g_narrow_status;
-
 namespace {
 
 template <int KIND>
@@ -145,7 +143,7 @@ __global__ void __launch_bounds__(narrow_threads(KIND), 1)
 expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const NarrowParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {  // swizzled TMA tiles need it; the same in all CTAs of a cluster
-        if (threadIdx.x == 0) gemm_record_status(&g_narrow_status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
+        if (threadIdx.x == 0) record_status(p.status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
         return;
     }
     constexpr bool FP4 = KIND != kNarrow16, SWIGLU = FORM == kNarrowSwiglu, DACT = FORM == kNarrowDact;
@@ -251,7 +249,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                 __syncwarp();
             }
         }
-        if (leader && *abort_flag) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 0, 0);
+        if (leader && *abort_flag) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 0, 0);
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer
         const bool leader = elect_one();
@@ -309,7 +307,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             if (leader) tc_commit(&bar_tfull[b]);
             __syncwarp();
         }
-        if (leader && *abort_flag) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
+        if (leader && *abort_flag) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
     } else if (warp < EPI0) {
         if constexpr (FP4) {
         if (warp >= 4) {
@@ -361,7 +359,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                     if (lane == 0) mbar_arrive(&bar_sf[mine]);
                 }
             }
-            if (!ok && lane == 0) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 3, static_cast<int>(count));
+            if (!ok && lane == 0) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 3, static_cast<int>(count));
         }
         }
     } else {
@@ -502,7 +500,7 @@ expert_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                 if (te < split) arrive_release_cluster(map_to_cta(bar_free, static_cast<uint32_t>(te)));
             }
         }
-        if (!ok && te == 0) gemm_record_status(&g_narrow_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
+        if (!ok && te == 0) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
         if constexpr (!DACT)  // dgu of rows of no expert is read by nothing
             zero_loose_rows(p.out, (FP4 && SWIGLU) ? p.n_dim / 32 : p.n_dim / 8, p.expert_offsets, p.num_experts, p.rows, te, kNwEpiThreads);
         if constexpr (FP4 && SWIGLU)
@@ -577,5 +575,3 @@ extern "C" int cam_expert_narrow_max_stages(void) { return cam::kNwMaxStages; }
 extern "C" int cam_expert_narrow_fixed_smem(int fp4, int slot_rows) {
     return cam::kNwCtrlBytes + (fp4 ? cam::kNwScaleSlots * cam::kNwSfSlot : 0) + slot_rows * cam::kNwPitch * 4;
 }
-
-extern "C" int cam_narrow_status(CamStatus* out) { return static_cast<int>(cudaMemcpyFromSymbol(out, cam::g_narrow_status, sizeof(CamStatus))); }

@@ -27,6 +27,7 @@ inline cudaLaunchAttribute pdl_attribute() {
 constexpr int kDtBf16 = 0, kDtFp16 = 1, kDtFp32 = 2;
 
 struct GroupedGemmFp4Params {
+    CamStatus* status;          // where a wait that ran out is recorded (host memory)
     const int* expert_offsets;  // [E+1] first row of every expert
     int num_experts, rows;      // rows of A and of the outputs
     int n_dim, k_dim;           // N (2I for the SwiGLU form), K
@@ -44,6 +45,7 @@ struct GroupedGemmFp4Params {
 constexpr int kMlpUp = 0, kMlpDown = 1, kMlpDact = 2, kMlpDx = 3, kMlpDw = 4;
 
 struct GroupedMlpParams {
+    CamStatus* status;          // where a wait that ran out is recorded (host memory)
     const int* expert_offsets;  // [E+1]
     int num_experts, rows;      // rows of the row operands
     int m_dim;                  // kMlpDw: rows of an expert's gradient
@@ -61,6 +63,7 @@ constexpr int kNarrow16 = 2;  // beside the formats of fp4.cuh: 16-bit operands
 // Weights contracted over their columns, plain or with SwiGLU; over their rows (16 bits): the gradient of the activation, or plain
 constexpr int kNarrowPlain = 0, kNarrowSwiglu = 1, kNarrowDact = 2, kNarrowByRows = 3;
 struct NarrowParams {
+    CamStatus* status;          // where a wait that ran out is recorded (host memory)
     const int* expert_offsets;
     int num_experts, rows;
     int n_dim;                  // columns of the result; with SwiGLU: I, the weights have 2I rows
@@ -111,7 +114,4 @@ int cam_launch_expert_gemm_narrow(const cam::NarrowParams* p, int kind, int form
 int cam_launch_expert_gemv(const cam::GroupedMlpParams* p, int swiglu, const void* x, const void* w, cudaStream_t stream);
 int cam_expert_narrow_max_stages(void);
 int cam_expert_narrow_fixed_smem(int fp4, int slot_rows);  // shared memory beside the stages
-int cam_narrow_status(CamStatus* out);
-int cam_mlp_status(CamStatus* out);
-int cam_fp4_status(CamStatus* out);  // of the current device: the first wait that ran out in a kernel of that file
 }

@@ -55,8 +55,6 @@ constexpr uint32_t kF4LaunchRegs = 80, kF4CtrlRegs = 32, kF4SfRegs = 56, kF4EpiR
 static_assert(128 * kF4CtrlRegs + 128 * kF4SfRegs + kF4EpiThreads * kF4EpiRegs <= kF4LaunchRegs * kF4Threads,
               "setmaxnreg budget exceeds the registers the CTA owns: the kernel would hang");
 
-static __device__ CamStatus g_fp4_status;
-
 namespace {
 
 // D (+)= (A sfa) (B sfb), e2m1 x e2m1, on the pair; the formats differ in the scales' type and block
@@ -97,7 +95,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                         const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_out, const GroupedGemmFp4Params p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {  // swizzled TMA tiles need it; the same in both CTAs of a pair
-        if (threadIdx.x == 0) gemm_record_status(&g_fp4_status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
+        if (threadIdx.x == 0) record_status(p.status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
         return;
     }
     constexpr int NS = fp4_stages(SWIGLU);
@@ -194,7 +192,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                     __syncwarp();
                 }
             }
-            if (leader && *abort_flag) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 0, 0);
+            if (leader && *abort_flag) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 0, 0);
         } else if (warp == 1 && cta == 0) {
             // ------------------------------------------------------------ MMA issuer (first CTA only)
             const bool leader = elect_one();
@@ -238,7 +236,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                 if (leader) tc_commit_both(smem_u32(bar_tfull));
                 __syncwarp();
             }
-            if (leader && *abort_flag) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
+            if (leader && *abort_flag) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
         }
     } else if (warp < kF4EpiWarp0) {
         reg_dealloc<kF4SfRegs>();
@@ -293,7 +291,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                     }
                 }
             }
-            if (!ok && lane == 0) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 3, static_cast<int>(groups.s));
+            if (!ok && lane == 0) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 3, static_cast<int>(groups.s));
         }
     } else {
         reg_alloc<kF4EpiRegs>();
@@ -372,7 +370,7 @@ grouped_gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             }
         }
         if (!SWIGLU && (cq & 1) == 0) bulk_wait_group<0>();  // everything this thread sent has been written
-        if (*abort_flag) gemm_record_status(&g_fp4_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
+        if (*abort_flag) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
         // rows of no expert
         const int et = static_cast<int>(threadIdx.x) - kF4EpiWarp0 * 32;
         if constexpr (SWIGLU) {
@@ -415,5 +413,3 @@ extern "C" int cam_launch_grouped_gemm_fp4(const cam::GroupedGemmFp4Params* p, i
         return swiglu ? launch_fp4<cam::kFp4Nv, true>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream) : launch_fp4<cam::kFp4Nv, false>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
     return swiglu ? launch_fp4<cam::kFp4Mx, true>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream) : launch_fp4<cam::kFp4Mx, false>(p, tmap_a, tmap_a32, tmap_b, tmap_out, stream);
 }
-
-extern "C" int cam_fp4_status(CamStatus* out) { return static_cast<int>(cudaMemcpyFromSymbol(out, cam::g_fp4_status, sizeof(CamStatus))); }

@@ -56,8 +56,6 @@ constexpr uint32_t kEmLaunchRegs = 96, kEmCtrlRegs = 40, kEmEpiRegs = 104;
 static_assert(128 * kEmCtrlRegs + kEmEpiThreads * kEmEpiRegs <= kEmLaunchRegs * kEmThreads,
               "setmaxnreg budget exceeds the registers the CTA owns: the kernel would hang");
 
-static __device__ CamStatus g_mlp_status;
-
 namespace {
 
 __device__ __forceinline__ void tc_mma_16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -107,7 +105,7 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
                        const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_out, const GroupedMlpParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {  // swizzled TMA tiles need it; the same in both CTAs of a pair
-        if (threadIdx.x == 0) gemm_record_status(&g_mlp_status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
+        if (threadIdx.x == 0) record_status(p.status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
         return;
     }
     constexpr int NS = kEmStages;
@@ -217,7 +215,7 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
                     __syncwarp();
                 }
             }
-            if (leader && *abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 0, 0);
+            if (leader && *abort_flag) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 0, 0);
         } else if (warp == 1 && cta == 0) {
             // ------------------------------------------------------------ MMA issuer (first CTA only)
             const bool leader = elect_one();
@@ -251,7 +249,7 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
                 if (leader) tc_commit_both(smem_u32(&bar_tfull[b]));
                 __syncwarp();
             }
-            if (leader && *abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
+            if (leader && *abort_flag) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
         } else if (DW && warp == 2) {
             // ------------------------------------------------------------ zeros behind the last row (both CTAs)
             uint32_t it = 0, phases = 0;  // bit s: parity of stage s's next ragged block
@@ -274,7 +272,7 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
                     else mbar_arrive_cluster(map_to_cta(&bar_full[s], 0));
                 }
             }
-            if (!ok && lane == 0) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 5, static_cast<int>(it));
+            if (!ok && lane == 0) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 5, static_cast<int>(it));
         }
     } else {
         reg_alloc<kEmEpiRegs>();
@@ -410,7 +408,7 @@ grouped_gemm_16_square_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
             store_half(v1, 1);
         }
         if (DW ? (ew & 7) == 0 : (cq & 1) == 0) bulk_wait_group<0>();  // everything this thread sent has been written
-        if (*abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
+        if (*abort_flag) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
     }
 
     // ------------------------------------------------------------------ teardown
@@ -464,7 +462,7 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
                             const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_out, const GroupedMlpParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {  // swizzled TMA tiles need it; the same in both CTAs of a pair
-        if (threadIdx.x == 0) gemm_record_status(&g_mlp_status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
+        if (threadIdx.x == 0) record_status(p.status, CAM_ERR_BAD_INDEX, 4, static_cast<int>(smem_u32(smem) & 1023u));
         return;
     }
     constexpr int NS = kErStages;
@@ -555,7 +553,7 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
                     __syncwarp();
                 }
             }
-            if (leader && *abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 0, 1);
+            if (leader && *abort_flag) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 0, 1);
         } else if (warp == 1 && cta == 0) {
             // ------------------------------------------------------------ MMA issuer (first CTA only)
             const bool leader = elect_one();
@@ -590,7 +588,7 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
                 if (leader) tc_commit_both(smem_u32(bar_tfull));
                 __syncwarp();
             }
-            if (leader && *abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
+            if (leader && *abort_flag) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 1, static_cast<int>(tcount));
         }
     } else {
         reg_alloc<kEmEpiRegs>();
@@ -699,7 +697,7 @@ grouped_gemm_16_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
             }
         }
         if ((q & 1) == 0) bulk_wait_group<0>();  // everything this thread sent has been written
-        if (*abort_flag) gemm_record_status(&g_mlp_status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
+        if (*abort_flag) record_status(p.status, CAM_ERR_TIMEOUT_PIPELINE, 2, static_cast<int>(tcount));
         if (!SWIGLU)  // rows of no expert; act and dgu of such rows are read by nothing
             zero_loose_rows(p.out, p.n_dim / 8, p.expert_offsets, p.num_experts, p.rows, static_cast<int>(threadIdx.x) - kEmEpiWarp0 * 32, kEmEpiThreads);
     }
@@ -749,5 +747,3 @@ extern "C" int cam_launch_grouped_mlp(const cam::GroupedMlpParams* p, int form, 
     }
     return static_cast<int>(cudaErrorInvalidValue);
 }
-
-extern "C" int cam_mlp_status(CamStatus* out) { return static_cast<int>(cudaMemcpyFromSymbol(out, cam::g_mlp_status, sizeof(CamStatus))); }

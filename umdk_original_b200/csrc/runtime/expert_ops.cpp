@@ -1,12 +1,16 @@
 // Host side of the expert-MLP operators that need no Buffer: checks, tensor maps, launches.
 #include "expert_ops.h"
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
+#include <cstring>
+#include <mutex>
 
 #include "../kernels/expert_ops.h"
 #include "../kernels/launch.h"
+#include "cam_runtime.h"
 
 namespace {
 
@@ -42,6 +46,52 @@ int map_3d(CUtensorMap* out, const void* base, uint64_t bytes, uint64_t rows, ui
 
 int launched(int rc, const char* what) {
     return rc == 0 ? 0 : refuse("%s: launch failed: %s", what, cudaGetErrorString(static_cast<cudaError_t>(rc)));
+}
+
+// A status word per device, in host memory that every device can write: it is there when the call that went wrong has ended, and
+// reading it costs the host nothing.  Stays for the life of the process.
+constexpr int kMaxDevices = 64;
+struct alignas(64) StatusWord {
+    CamStatus st;
+};
+std::atomic<StatusWord*> g_words{nullptr};
+
+StatusWord* status_words() {
+    StatusWord* w = g_words.load(std::memory_order_acquire);
+    if (w != nullptr) return w;
+    static std::mutex lock;
+    std::lock_guard<std::mutex> guard(lock);
+    w = g_words.load(std::memory_order_relaxed);
+    if (w != nullptr) return w;
+    void* p = nullptr;
+    // the first call may be one that is captured
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    const cudaError_t err = cudaHostAlloc(&p, kMaxDevices * sizeof(StatusWord), cudaHostAllocPortable | cudaHostAllocMapped);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (err != cudaSuccess) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    std::memset(p, 0, kMaxDevices * sizeof(StatusWord));
+    g_words.store(static_cast<StatusWord*>(p), std::memory_order_release);
+    return static_cast<StatusWord*>(p);
+}
+
+// The current device's status word for a product that is about to be launched; refused while an earlier failure stands there.
+int status_for_launch(const char* what, CamStatus** out) {
+    int dev = 0;
+    const cudaError_t err = cudaGetDevice(&dev);
+    EXP_CHECK(err == cudaSuccess, "%s: %s", what, cudaGetErrorString(err));
+    EXP_CHECK(dev >= 0 && dev < kMaxDevices, "%s: device index %d not supported", what, dev);
+    StatusWord* w = status_words();
+    EXP_CHECK(w != nullptr, "%s: no host memory for the status word", what);
+    CamStatus* st = &w[dev].st;
+    const int code = __atomic_load_n(&st->code, __ATOMIC_ACQUIRE);
+    EXP_CHECK(code == 0, "%s: an earlier expert product on device %d gave up (%s; who=%d, detail=%d, block=%d) and its results mean nothing; "
+              "ops.check_expert_ops() reports and clears this", what, dev, cam_status_string(code), st->who, st->detail, st->block);
+    *out = st;
+    return 0;
 }
 
 // Environment switch: -1 unset, otherwise its number.
@@ -210,8 +260,11 @@ extern "C" int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, 
     EXP_CHECK(n_dim >= 128 && n_dim % (swiglu ? 256 : 128) == 0, "grouped_gemm_fp4: N %d must be a multiple of %d", n_dim, swiglu ? 256 : 128);
     EXP_CHECK(static_cast<int64_t>(num_experts) * n_dim < (1ll << 31), "grouped_gemm_fp4: weight rows overflow");
     EXP_CHECK(aligned(a_s, 4) && aligned(w_s, 4), "grouped_gemm_fp4: scales must be 4-byte aligned");
+    CamStatus* status = nullptr;
+    if (status_for_launch("grouped_gemm_fp4", &status) != 0) return -1;
     if (few_rows_pay_fp4(rows, num_experts, swiglu ? n_dim / 2 : n_dim, swiglu != 0)) {
         cam::NarrowParams p{};
+        p.status = status;
         p.expert_offsets = offsets;
         p.num_experts = num_experts;
         p.rows = rows;
@@ -228,6 +281,7 @@ extern "C" int cam_grouped_gemm_fp4(const void* a_q, const void* a_s, int rows, 
         return launch_narrow(&p, fmt, swiglu ? cam::kNarrowSwiglu : cam::kNarrowPlain, a_q, w_q, k_dim / 2, "grouped_gemm_fp4", stream);
     }
     cam::GroupedGemmFp4Params p{};
+    p.status = status;
     p.expert_offsets = offsets;
     p.num_experts = num_experts;
     p.rows = rows;
@@ -258,6 +312,8 @@ int row_product(int form, const char* what, const void* a, int k, const void* w,
     EXP_CHECK(a && w && offsets && out, "%s: null operand", what);
     EXP_CHECK(rows >= 1 && num_experts >= 1, "%s: empty problem", what);
     EXP_CHECK(k >= 8 && n >= 8 && k % 8 == 0 && n % 8 == 0, "%s: sizes %d and %d must be multiples of 8", what, k, n);
+    CamStatus* status = nullptr;
+    if (status_for_launch(what, &status) != 0) return -1;
     if (gemv_pays(rows, n, k, form)) {
         EXP_CHECK(aligned(a, 16) && aligned(w, 16), "%s: rows and weights must be 16-byte aligned", what);
         cam::GroupedMlpParams p{};
@@ -273,6 +329,7 @@ int row_product(int form, const char* what, const void* a, int k, const void* w,
     }
     if (few_rows_pay_16(rows, num_experts, n, form, k)) {
         cam::NarrowParams p{};
+        p.status = status;
         p.expert_offsets = offsets;
         p.num_experts = num_experts;
         p.rows = rows;
@@ -284,6 +341,7 @@ int row_product(int form, const char* what, const void* a, int k, const void* w,
         return launch_narrow(&p, cam::kNarrow16, narrow, a, w, k * 2, what, stream);
     }
     cam::GroupedMlpParams p{};
+    p.status = status;
     p.expert_offsets = offsets;
     p.num_experts = num_experts;
     p.rows = rows;
@@ -338,7 +396,10 @@ extern "C" int cam_grouped_mlp_dw(const void* a, const void* b, const int* offse
     EXP_CHECK(a && b && offsets && dw, "grouped_mlp (dw): null operand");
     EXP_CHECK(rows >= 1 && num_experts >= 1, "grouped_mlp (dw): empty problem");
     EXP_CHECK(m_dim >= 8 && n_dim >= 8 && m_dim % 8 == 0 && n_dim % 8 == 0, "grouped_mlp (dw): sizes %d and %d must be multiples of 8", m_dim, n_dim);
+    CamStatus* status = nullptr;
+    if (status_for_launch("grouped_mlp (dw)", &status) != 0) return -1;
     cam::GroupedMlpParams p{};
+    p.status = status;
     p.expert_offsets = offsets;
     p.num_experts = num_experts;
     p.rows = rows;
@@ -353,9 +414,24 @@ extern "C" int cam_grouped_mlp_dw(const void* a, const void* b, const int* offse
     return launched(cam_launch_grouped_mlp(&p, cam::kMlpDw, &ta, &ta, &tb, &tout, stream), "grouped_mlp (dw)");
 }
 
-extern "C" int cam_expert_ops_status(CamStatus* out) {
-    int rc = cam_fp4_status(out);
-    if (rc == 0 && out->code == 0) rc = cam_mlp_status(out);
-    if (rc == 0 && out->code == 0) rc = cam_narrow_status(out);
-    return rc == 0 ? 0 : refuse("expert_ops_status: %s", cudaGetErrorString(static_cast<cudaError_t>(rc)));
+extern "C" int cam_expert_ops_status(CamStatus* out, int clear) {
+    *out = CamStatus{};
+    StatusWord* w = g_words.load(std::memory_order_acquire);
+    if (w == nullptr) return 0;  // no product has been launched
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err == cudaSuccess) err = cudaDeviceSynchronize();
+    EXP_CHECK(err == cudaSuccess, "expert_ops_status: %s", cudaGetErrorString(err));
+    EXP_CHECK(dev >= 0 && dev < kMaxDevices, "expert_ops_status: device index %d not supported", dev);
+    if (__atomic_load_n(&w[dev].st.code, __ATOMIC_ACQUIRE) == 0) return 0;
+    *out = w[dev].st;
+    if (clear) w[dev].st = CamStatus{};
+    return 0;
+}
+
+extern "C" int cam_expert_ops_set_status(const CamStatus* st) {
+    CamStatus* at = nullptr;
+    if (status_for_launch("expert_ops_set_status", &at) != 0) return -1;
+    *at = *st;
+    return 0;
 }

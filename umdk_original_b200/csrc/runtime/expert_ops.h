@@ -1,5 +1,6 @@
 // C interface of the expert-MLP operators that need no Buffer.  Like cam_runtime.h: no PyTorch, raw device pointers, 0 on
-// success and cam_last_error() otherwise; nothing here allocates or waits.
+// success and cam_last_error() otherwise.  The products write to one page of host memory, allocated by the first of them; nothing else
+// allocates, and only cam_expert_ops_status waits.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -39,8 +40,10 @@ int cam_grouped_mlp_dx(const void* dgu, const void* w1, const int* offsets, int 
 int cam_grouped_mlp_dw(const void* a, const void* b, const int* offsets, int rows, int num_experts, int m_dim, int n_dim, int dtype,
                        void* dw, cudaStream_t stream);
 
-// First wait that ran out in a kernel of these operators on the current device (code 0: none); waits for the device.
-int cam_expert_ops_status(CamStatus* out);
+// A wait inside a product that ran out on the current device (code 0: none); waits for the device, and clears it where asked to.
+// Until it is cleared every further product on that device is refused.  cam_expert_ops_set_status is for tests of the host's side.
+int cam_expert_ops_status(CamStatus* out, int clear);
+int cam_expert_ops_set_status(const CamStatus* st);
 
 #ifdef __cplusplus
 }

@@ -19,6 +19,20 @@ _EXPERT_OPS = ("quantize_fp4", "dequantize_fp4", "grouped_gemm_fp4", "grouped_ge
                "grouped_mlp_train", "grouped_mlp_backward")
 
 
+def check_expert_ops(device=None) -> None:
+    """Waits for the device (default: the current one) and raises ``CamError`` if a wait inside a product of the operators above ran
+    out there since the last check (results since then mean nothing), the counterpart of ``Buffer.check``.  Without a check the next
+    product on that device is refused, and all further ones, until this has reported and cleared it."""
+    import torch
+
+    from ..utils.errors import raise_for_status
+    if not torch.cuda.is_available():
+        return
+    with torch.cuda.device(device):
+        code, who, block, detail = native_module().expert_ops_status(True)
+    raise_for_status(code, who, detail, block)
+
+
 def __getattr__(name):
     if name not in _EXPERT_OPS:
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
