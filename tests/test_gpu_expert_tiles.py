@@ -168,3 +168,17 @@ def test_clusters(ops, fmt, split, cnt, k, swiglu, monkeypatch):
 def test_chosen_form_swiglu(ops, fmt, cnt, k, inter):
     """The form and the split that the rule takes for few rows."""
     check_swiglu(ops, fmt, cnt, 0, 5, k, inter)
+
+
+def test_gradient_at_an_odd_offset(ops):
+    """The gradient that autograd hands over is a slice of another one's memory, two bytes past a 16-byte boundary."""
+    m, h, inter = 40, 64, 32
+    gen = torch.Generator(device=DEV).manual_seed(41)
+    x = torch.randn(m, h, device=DEV, generator=gen).to(torch.bfloat16)
+    leaves = [x.requires_grad_(), *[(torch.randn(*s, device=DEV, generator=gen) / 8).to(torch.bfloat16).requires_grad_() for s in ((2, 2 * inter, h), (2, h, inter))]]
+    off = offsets_of([17, 23], device=DEV)
+    dy = torch.randn(m * h + 1, device=DEV, generator=gen).to(torch.bfloat16)
+    y = ops.grouped_mlp(*leaves, off)
+    got = torch.autograd.grad(torch.cat([y.new_zeros(1), y.flatten()]), leaves, dy, retain_graph=True)
+    want = torch.autograd.grad(y, leaves, dy[1:].view(m, h).clone())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

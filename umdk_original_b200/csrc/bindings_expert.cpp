@@ -251,19 +251,21 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mlp_grads_empty(const at::Tensor&
     return {like(x, need_dx), like(w1, need_dw1), like(w2, need_dw2)};
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> grouped_mlp_backward_cuda(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w1,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> grouped_mlp_backward_cuda(const at::Tensor& dy_in, const at::Tensor& x, const at::Tensor& w1,
                                                                          const at::Tensor& w2, const at::Tensor& expert_offsets,
                                                                          const at::Tensor& act, const at::Tensor& gate_up, bool need_dx,
                                                                          bool need_dw1, bool need_dw2) {
     const MlpProblem p = check_mlp(x, w1, w2, expert_offsets);
-    check_operand(dy, x, "dy");
+    check_operand(dy_in, x, "dy");
+    c10::cuda::CUDAGuard guard(x.device());
+    // autograd hands out slices of larger gradients, at any offset: the caller has no say in it
+    const at::Tensor dy = reinterpret_cast<uintptr_t>(dy_in.data_ptr()) % 16 == 0 ? dy_in : dy_in.clone();
     check_operand(act, x, "act");
     check_operand(gate_up, x, "gate_up");
     CAM_ASSERT(dy.scalar_type() == x.scalar_type() && dy.sizes() == x.sizes(), "grouped_mlp: dy must be like x");
     CAM_ASSERT(act.scalar_type() == x.scalar_type() && act.dim() == 2 && act.size(0) == p.rows && act.size(1) == p.inter, "grouped_mlp: act must be [M, I]");
     CAM_ASSERT(gate_up.scalar_type() == at::kFloat && gate_up.dim() == 2 && gate_up.size(0) == p.rows && gate_up.size(1) == 2 * p.inter,
                "grouped_mlp: gate_up must be float32 [M, 2I]");
-    c10::cuda::CUDAGuard guard(x.device());
     auto out = mlp_grads_empty(x, w1, w2, need_dx, need_dw1, need_dw2);
     auto& [dx, dw1, dw2] = out;
     if (p.rows == 0) {
