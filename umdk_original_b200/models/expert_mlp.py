@@ -43,7 +43,11 @@ class ExpertMLP(torch.nn.Module):
 @dataclass
 class Fp4ExpertMLP:
     """The same experts in 4 bits: ``nvfp4`` (e4m3 scale per 16 values and one fp32 scale per expert) or ``mxfp4`` (power-of-two
-    scale per 32).  Rows are quantised on the way in, the activation between the two products is quantised by the first one."""
+    scale per 32).  Rows are quantised on the way in, the activation between the two products is quantised by the first one.
+
+    nvfp4 block scales reach from 2^-9 to 448.  With ``x_gs`` and ``act_gs`` at None (1) rows and activations have to fit them: blocks
+    whose largest magnitude is below 6 x 2^-10 become zeros, what is above 2688 is cut; ``calibrate`` sets both from sample rows.
+    mxfp4 scales reach over the whole range of fp32.  Plain tensors, no module: move or store the fields."""
     w1_q: torch.Tensor   # [E_l, 2I, h / 2] e2m1 pairs
     w1_s: torch.Tensor   # [E_l, 2I, h / block]
     w2_q: torch.Tensor   # [E_l, h, I / 2]
@@ -72,6 +76,26 @@ class Fp4ExpertMLP:
         q1, s1, g1 = one(w1)
         q2, s2, g2 = one(w2)
         return Fp4ExpertMLP(q1, s1, q2, s2, g1, g2)
+
+    @torch.no_grad()
+    def calibrate(self, rows: torch.Tensor, expert_offsets: torch.Tensor, margin: float = 4.0) -> "Fp4ExpertMLP":
+        """nvfp4: sets ``x_gs`` and ``act_gs`` so that the largest row value and the largest activation that these rows give have block
+        scales of 448 / ``margin``: later ones may be ``margin`` times as large, and 1000 times smaller without losing bits of
+        their scales.  Rows of no expert do not count.  Waits for the device; nothing to do for mxfp4."""
+        if self.block == 32:
+            return self
+
+        def scale(values: torch.Tensor, what: str) -> torch.Tensor:
+            top = float(values.abs().amax()) if values.numel() else 0.0
+            if not top < float("inf"):
+                raise ValueError(f"calibrate: {what} hold NaN or infinity")
+            return torch.full((1,), top * margin / (6.0 * 448.0) if top > 0 else 1.0, dtype=torch.float32, device=rows.device)
+        first, last = (min(max(int(expert_offsets[i]), 0), rows.shape[0]) for i in (0, -1))
+        self.x_gs = scale(rows[first:last].float(), "rows")
+        q, s = ops.quantize_fp4(rows, 16, self.x_gs)
+        gate, up = ops.grouped_gemm_fp4(q, s, self.w1_q, self.w1_s, expert_offsets, self.x_gs, self.w1_gs)[first:last].float().chunk(2, -1)
+        self.act_gs = scale(torch.nn.functional.silu(gate) * up, "activations")
+        return self
 
     def __call__(self, rows: torch.Tensor, expert_offsets: torch.Tensor) -> torch.Tensor:
         """rows [M, h] bf16 / fp16 / fp32 -> [M, h] bf16; rows of no expert give zeros."""
