@@ -5,9 +5,11 @@
 //   dact    da = dy W2, s = 1 / (1 + e^-g):  dg = da u s (1 + g (1 - s)),  du = da g s    one kernel, da never leaves it
 //   dx      dx = dg Wg + du Wu = dgu W1
 //   dw      dW2 = dy^T act,  dW1 = dgu^T x, the sums over the rows of the expert
-// What is rounded to 16 bits: act and dgu, because they are operands of the next product, and the results.  Gate and up are
-// kept in fp32 for the backward pass and da stays in the accumulator, so that no result is more than one rounding of an
-// operand and its own away from the formula.
+// What is rounded to 16 bits: act and dgu, because they are operands of the next product and the tensor core takes no wider ones at
+// this rate, and the results.  Gate and up are kept in fp32 for the backward pass and da stays in the accumulator, so that no result is
+// more than one rounding of an operand and its own away from the formula: the relative error of y, dx and both weight gradients is
+// 1.41 times what it would be with act and dgu in fp32 (256 rows, 1024 x 512: 2.34e-3 against 1.66e-3 in bf16, 2.93e-4 against
+// 2.07e-4 in fp16).  In fp16 it is also a limit of range: act and dgu past 65504 become infinite where the formula's result might not.
 //
 // up, down and dx (grouped_gemm_16_rows_kernel): the weights are the M operand of the tensor core, the rows of the expert its N
 // operand in steps of 32, so that the tensor time, and at the power limit the energy, follow the rows present: an expert of 375
