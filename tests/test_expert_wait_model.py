@@ -1,4 +1,4 @@
-"""Model of what the epilogue warps of the expert products do when a wait runs out, on the CPU.
+"""Model of what the epilogue warps of the grouped products do when a wait runs out, on the CPU.
 
 Warps of an epilogue share staging buffers, two or more to a buffer, and meet at a named barrier for each tile.  The wait for a tile
 is bounded; after one that ran out, whether a warp still sees the tile complete or sees the abort flag first is a matter of timing.
@@ -60,3 +60,17 @@ def test_no_warp_decides_alone(name, count):
             if re.search(r"\bbreak\b", line):
                 assert "named_bar_and(1, kNwEpiThreads, got)" in line
         assert "named_bar_and" in code or re.search(r"for \(int tile = pair_id; (w\.)?locate\(", code)
+
+
+@pytest.mark.parametrize("name", ["grouped_gemm.cu", "grouped_gemm_mx.cu", "grouped_gemm_mx2.cu", "grouped_gemm_i8.cu",
+                                  "grouped_gemm_rows_n.cuh", "fused_moe_mx.cu"])
+def test_warps_of_the_8_bit_products_leave_together(name):
+    """All epilogue warps of a CTA agree on the answer of a wait before the first barrier that would need them all; inside a sum over
+    K-blocks, which has no barrier, the lanes of a warp agree."""
+    for text in epilogues(name):
+        code = re.sub(r"//[^\n]*", "", text)
+        first = code.index("named_bar_and(1, k")
+        assert first < code.index("named_bar_sync(")
+        for line in code.splitlines():
+            if re.search(r"\bbreak\b", line):
+                assert "named_bar_and(1, k" in line or ("__all_sync(" in line and code.index(line) < first)

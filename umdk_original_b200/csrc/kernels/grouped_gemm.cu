@@ -210,7 +210,7 @@ grouped_gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                     wh1 = __ldg(bs_hi + kb + 2);
                 }
                 const uint32_t a = it & 1u, aph = (it >> 1) & 1u;
-                if (!mbar_wait_bounded(&bar_tfull[a], aph, abort_flag)) { ok = false; break; }
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(&bar_tfull[a], aph, abort_flag))) { ok = false; break; }
                 tc_fence_after_sync();
                 const uint32_t t0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + a * BN + cq * 32;
                 uint32_t v[32];
@@ -227,7 +227,8 @@ grouped_gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) fma_pair(acc[32 + j], acc[33 + j], s_hi, v[j], v[j + 1]);
             }
-            if (!ok) break;
+            // one decision for all epilogue threads: one that gave up must not leave the others at a named barrier
+            if (!named_bar_and(1, kEpiThreads, ok)) { ok = false; break; }
 
             if (p.mode == 1) {
                 // SwiGLU on matching gate/up columns, then 1x128 fp8 requantisation of the row block.

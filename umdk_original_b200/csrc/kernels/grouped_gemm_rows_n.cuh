@@ -342,7 +342,8 @@ grouped_gemm_rows_n_kernel(const __grid_constant__ CUtensorMap tmap_a, const __g
         const int te = ew * 32 + static_cast<int>(lane);          // 0..511
         uint32_t tcount = 0;
         for (int tile = pair_id; ok && w.locate(tile, e, nt, row0, rows, rot_num, rot_den); tile += num_pairs, ++tcount) {
-            if (!mbar_wait_bounded(bar_tfull, tcount & 1u, abort_flag, 2000000000ull, 256u)) { ok = false; break; }
+            // one decision for all epilogue threads: one that gave up must not leave the others at a named barrier
+            if (!named_bar_and(1, kMTEpiThreads, mbar_wait_bounded(bar_tfull, tcount & 1u, abort_flag, 2000000000ull, 256u))) { ok = false; break; }
             tc_fence_after_sync();
 #pragma unroll 1
             for (int r0 = 0; r0 < rows; r0 += 128) {  // rows [r0, r0 + 128) of the tile; the same trips in all threads
