@@ -2,8 +2,9 @@
 //
 // A thread owns 16 consecutive values: one nvfp4 block, or half of an mxfp4 block whose maximum it exchanges with its
 // neighbour.  Rows are whole blocks, so the tensor is one flat array of them and the scales come out in row order.
-// Bound by memory: 2 bytes (bf16) in, 0.56 out per value.  32768 x 7168 bf16 to nvfp4 and back, 1.2 GB: 193 us, 6.2 TB/s, 0.97 of a
-// plain copy's rate.  Accesses of 32 bytes per thread fill whole sectors; with 16 bytes the same took 242 us.
+// Bound by memory: 2 bytes (bf16) in, 0.56 out per value.  32768 x 7168 bf16 to nvfp4 and back in a steady loop, 1.2 GB: 195 us
+// (191 to 198 on several boards), 6.2 TB/s, 0.96 of a plain copy's rate.  Accesses of 32 bytes per thread fill whole sectors; with 16
+// bytes the same took 242 us.
 #include "../common/fp4.cuh"
 #include "expert_ops.h"
 
