@@ -111,14 +111,16 @@ def check_swiglu(ops, fmt, cnt, head, tail, k, inter):
 
 # ---------------------------------------------------------------------------- several tiles per pair
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
-@pytest.mark.parametrize("k", [640, 2176])  # 3 and 9 K-blocks: a group of four scales is never whole at the end
-def test_pairs_product(ops, fmt, k, monkeypatch):
+@pytest.mark.parametrize("k,n", [(640, 5120), (2176, 5120), (1280, 4992)])
+def test_pairs_product(ops, fmt, k, n, monkeypatch):
+    """15 x 20 tiles; 3, 9 and 5 K-blocks, so that a group of four scales is never whole at the end; scales of 1280 values are read in
+    wide pieces; 4992 columns end in half a tile."""
     monkeypatch.setenv("UMDK_CAM_EXPERT_NARROW", "0")
-    check_plain(ops, fmt, ROWS, 3, 70, k, 5120)  # 15 x 20 tiles
+    check_plain(ops, fmt, ROWS, 3, 70, k, n)
 
 
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
-@pytest.mark.parametrize("k", [640, 2176])
+@pytest.mark.parametrize("k", [640, 2176, 1280])
 def test_pairs_swiglu(ops, fmt, k, monkeypatch):
     monkeypatch.setenv("UMDK_CAM_EXPERT_NARROW", "0")
     check_swiglu(ops, fmt, ROWS, 3, 70, k, 2560)  # 15 x 20 tiles
