@@ -1,0 +1,294 @@
+"""Norm, routing and rows grouped by expert on the GPU: sizes past 32 bits, graphs, streams, threads, memory of a dispatch."""
+import threading
+
+import pytest
+import torch
+
+from layer_cases import group64
+from umdk_original_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+BF = torch.bfloat16
+
+
+def make(t=50, h=264, e=8, k=3, dtype=BF, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    r = lambda *s, d=dtype: torch.randn(*s, device=DEV, generator=g).to(d)  # noqa: E731
+    return dict(x=r(t, h), residual=r(t, h), weight=r(h), gate=r(e, h) * h ** -0.5, bias=0.1 * r(e, d=torch.float32), dout=r(t, h), ds=r(t, h),
+                e=e, k=k)
+
+
+def chain(c, x, residual, weight, gate):
+    """One pass through all of them, as a block uses them (the experts double their rows)."""
+    y, s = ops.add_rms_norm(x, residual, weight)
+    idx, w = ops.moe_route(y @ gate.t(), c["k"], c["bias"], "sigmoid", 4, 2, 2)
+    rows, _, off, slots = ops.moe_group_rows(y, idx, c["e"])
+    out = ops.moe_ungroup_rows(rows * 2, slots, w, s)
+    return out, s, idx, w, rows, off, slots
+
+
+def step(c, leaves):
+    res = chain(c, *leaves)
+    return [t.detach() for t in res] + list(torch.autograd.grad(res[:2], leaves, (c["dout"], c["ds"])))
+
+
+def leaves_of(c):
+    return [c[n].clone().requires_grad_() for n in ("x", "residual", "weight", "gate")]
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b)) and len(a) == len(b)
+
+
+def test_capture_and_replay():
+    """Forward and backward in one CUDA graph, replayed with other data; two graphs that are replayed in turn; a side stream."""
+    c = make()
+    leaves = leaves_of(c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = step(c, leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    want = step(c, leaves)
+    assert same(first, want)
+    del first
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    others = [leaves, leaves_of(make(seed=4))]
+    for g, l in zip(graphs, others):
+        with torch.cuda.graph(g):
+            outs.append(step(c, l))
+    c2 = make(seed=9)
+    with torch.no_grad():
+        for a, n in zip(leaves, ("x", "residual", "weight", "gate")):
+            a.copy_(c2[n])
+    for n in ("bias", "dout", "ds"):
+        c[n].copy_(c2[n])
+    for order in ((0, 1), (1, 0)):
+        for i in order:
+            graphs[i].replay()
+        for i in (0, 1):
+            assert same([t.clone() for t in outs[i]], step(c, others[i]))
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    c = make()
+    cases = {
+        "rms_norm": lambda t: ops.rms_norm(t, c["weight"]),
+        "add_rms_norm": lambda t: ops.add_rms_norm(c["x"], t, c["weight"])[1],
+        "moe_route": lambda t: ops.moe_route(t, 2)[1],
+        "moe_group_rows": lambda t: ops.moe_group_rows(t, torch.zeros(50, 1, dtype=torch.int64, device=DEV), 2)[0],
+        "moe_ungroup_rows": lambda t: ops.moe_ungroup_rows(t, torch.arange(50, device=DEV, dtype=torch.int32)[:, None].contiguous()),
+    }
+    for name, fn in cases.items():
+        fn(c["x"])  # whatever has to be loaded is
+        leaf = c["x"].clone().requires_grad_()
+        eager = fn(leaf)  # holds the leaf's accumulation node
+        g = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match=f"{name} is captured.*let go of its outputs"):
+            with torch.cuda.graph(g):
+                fn(leaf)
+        del eager
+        g = torch.cuda.CUDAGraph()
+        idx = torch.zeros(50, 1, dtype=torch.int64, device=DEV)
+        slots = torch.arange(50, device=DEV, dtype=torch.int32)[:, None].contiguous()
+        fn = {"moe_group_rows": lambda t: ops.moe_group_rows(t, idx, 2)[0], "moe_ungroup_rows": lambda t: ops.moe_ungroup_rows(t, slots)}.get(name, fn)
+        ones = torch.ones_like(fn(c["x"]))
+        with torch.cuda.graph(g):
+            out = fn(leaf)
+            grad, = torch.autograd.grad(out, leaf, ones)
+        g.replay()
+        again = fn(leaf)
+        assert torch.equal(out, again) and torch.equal(grad, torch.autograd.grad(again, leaf, ones)[0])
+
+
+def test_waits_for_another_stream():
+    """The kernels may start before the one ahead of them on their stream has finished, but not before an event they wait for."""
+    c = make()
+    leaves = leaves_of(c)
+    want = step(c, leaves)
+    late = [torch.zeros_like(t).requires_grad_() for t in leaves]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = step(c, leaves)  # kernels ahead on this stream
+    with torch.cuda.stream(side), torch.no_grad():
+        torch.cuda._sleep(2_000_000)  # about a millisecond
+        for a, b in zip(late, leaves):
+            a.copy_(b)
+    torch.cuda.current_stream().wait_stream(side)
+    assert same(got, want) and same(step(c, late), want)
+
+
+def test_calls_from_two_host_threads():
+    c = make(seed=3)
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            leaves = leaves_of(c)
+            for _ in range(20):
+                got[i] = step(c, leaves)
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    want = step(c, leaves_of(c))
+    assert same(got[0], want) and same(got[1], want)
+
+
+def test_norm_past_32_bits():
+    """2^31 values and more: the last rows are what they are on their own."""
+    h, rows = 8192, 2 ** 18 + 700
+    x = torch.randn(4096, h, device=DEV).to(BF).repeat(65, 1)[:rows]
+    w = torch.randn(h, device=DEV).to(BF).requires_grad_()
+    x.requires_grad_()
+    y = ops.rms_norm(x, w)
+    part = x.detach()[-300:].clone().requires_grad_()
+    y2 = ops.rms_norm(part, w)
+    assert torch.equal(y[-300:], y2)
+    dy = torch.randn(300, h, device=DEV).to(BF)
+    full = torch.zeros_like(y)
+    full[-300:] = dy
+    dx, dw = torch.autograd.grad(y, (x, w), full)
+    dx2, dw2 = torch.autograd.grad(y2, (part, w), dy)
+    assert torch.equal(dx[-300:], dx2) and not dx[:1000].any()
+    # the same rows in other blocks: half a step of bf16 each, and the order of 300 sums in fp32
+    assert ((dw - dw2).abs().double() <= dw2.abs().double() * 2.0 ** -7 + 300 * 2.0 ** -20).all()
+    del y, y2, full, dx
+    q, s, _, _ = ops.rms_norm_quant(x.detach(), w.detach(), 3)
+    q2, s2, _, _ = ops.rms_norm_quant(part.detach(), w.detach(), 3)
+    assert torch.equal(q[-300:].view(torch.int8), q2.view(torch.int8)) and torch.equal(s[-300:], s2)
+
+
+def test_rows_past_32_bits():
+    t, k, h, e = 40000, 8, 8192, 16
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(t, h, device=DEV, generator=g).to(BF)
+    idx = torch.rand(t, e, device=DEV, generator=g).topk(k, -1).indices
+    w = torch.rand(t, k, device=DEV, generator=g).requires_grad_()
+    x.requires_grad_()
+    rows, _, off, slots = ops.moe_group_rows(x, idx, e)
+    assert int(off[-1]) == t * k and torch.equal(slots.flatten().sort().values, torch.arange(t * k, device=DEV, dtype=torch.int32))
+    for j in (0, k - 1):
+        at = slots[:, j].long()
+        for i in (0, t - 5):
+            assert torch.equal(rows[at[i: i + 5]], x[i: i + 5])
+    out = ops.moe_ungroup_rows(rows, slots, w)
+    dout = torch.randn(t, h, device=DEV, generator=g).to(BF)
+    dx, dw = torch.autograd.grad(out, (x, w), dout)
+    i = slice(t - 40, t)
+    share = w.detach()[i].double().sum(-1, keepdim=True)
+    assert ((out[i].double() - x[i].double() * share).abs() <= (x[i].double() * share).abs() * (2.0 ** -8 + 2.0 ** -20)).all()
+    # every row's gradient is rounded, and their sum is
+    assert ((dx[i].double() - dout[i].double() * share).abs() <= (dout[i].double() * share).abs() * 2 * (2.0 ** -8 + 2.0 ** -16)).all()
+    dots = (x[i].double() * dout[i].double())
+    assert ((dw[i].double() - dots.sum(-1, keepdim=True)).abs() <= dots.abs().sum(-1, keepdim=True) * (h / 16 + 64) * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("t,k,e", [(1023, 8, 256), (1024, 8, 256), (1025, 8, 256), (5000, 2, 3), (40000, 8, 1024), (70001, 3, 61), (300000, 1, 2), (9, 32, 1024)])
+@pytest.mark.parametrize("drop", [0.0, 0.3])
+def test_sort_of_many_pairs(t, k, e, drop):
+    """Against a stable sort: one block, a cluster, uneven experts, pairs of no expert."""
+    g = torch.Generator(device=DEV).manual_seed(t)
+    idx = (torch.rand(t, k, device=DEV, generator=g) ** 3 * e).long()
+    if drop:
+        idx = torch.where(torch.rand(t, k, device=DEV, generator=g) < drop, torch.full_like(idx, -1), idx)
+    x = torch.arange(t, device=DEV, dtype=torch.float32)[:, None].contiguous()
+    rows, _, off, slots = ops.moe_group_rows(x, idx, e)
+    key = torch.where(idx < 0, torch.full_like(idx, e), idx).flatten()
+    order = key.argsort(stable=True)
+    count = torch.bincount(key, minlength=e + 1)[:e]
+    n = int(count.sum())
+    assert torch.equal(off[1:].long(), count.cumsum(0)) and int(off[0]) == 0
+    want = torch.full((t * k,), -1, dtype=torch.int32, device=DEV)
+    want[order[:n]] = torch.arange(n, device=DEV, dtype=torch.int32)
+    assert torch.equal(slots.flatten(), want)
+    assert torch.equal(rows[:n, 0].long(), order[:n] // k) and not rows[n:].any()
+
+
+def test_group_rows_is_the_order_of_a_dispatch():
+    """One rank: the rows that a dispatch hands out, in the same order."""
+    from umdk_original_b200 import Buffer, CamConfig
+    dev = torch.device("cuda", 0)
+    t, h, e, k = 40, 256, 8, 3
+    g = torch.Generator().manual_seed(2)
+    idx = torch.stack([torch.randperm(e, generator=g)[:k] for _ in range(t)]).to(dev)
+    x, w = torch.randn(t, h, generator=g).to(dev, BF), torch.rand(t, k, generator=g).to(dev)
+    buf = Buffer(None, CamConfig(num_experts=e, max_tokens=t, hidden=h, topk=k, timeout_ms=2000.0), name="order", device=dev, rank=0, num_ranks=1)
+    rx, _, _, per_e, _ = ops.moe_dispatch_prefill_quant(x, idx, w, buf.capacity, buf.name, 0, 1, 0)
+    rows, _, off, _ = ops.moe_group_rows(x, idx, e)
+    assert torch.equal(rows, rx[: t * k]) and torch.equal(off[1:].long(), per_e.cumsum(0).long())
+    buf.check()
+    buf.destroy()
+
+
+def test_rows_of_a_dispatch_keep_their_gradients():
+    """The rows of a dispatch are overwritten by the next one; what a backward pass reads of them was kept."""
+    from umdk_original_b200 import Buffer, CamConfig
+    dev = torch.device("cuda", 0)
+    t, h = 16, 128
+    g = torch.Generator().manual_seed(3)
+    idx, one = torch.randint(0, 2, (t, 1), generator=g).to(dev), torch.ones(t, 1, device=dev)
+    x = torch.randn(t, h, generator=g).to(dev, BF)
+    buf = Buffer(None, CamConfig(num_experts=2, max_tokens=t, hidden=h, topk=1, timeout_ms=2000.0), name="kept", device=dev, rank=0, num_ranks=1)
+    rx = ops.moe_dispatch_prefill_quant(x, idx, one, buf.capacity, buf.name, 0, 1, 0)[0][:t]
+    rx0, weight = rx.clone(), torch.ones(h, device=dev, dtype=BF, requires_grad=True)
+    slots, w = torch.arange(t, device=dev, dtype=torch.int32)[:, None].contiguous(), one.clone().requires_grad_()
+    y, out = ops.rms_norm(rx, weight), ops.moe_ungroup_rows(rx, slots, w)
+    ops.moe_dispatch_prefill_quant(-2 * x, idx, one, buf.capacity, buf.name, 0, 1, 0)
+    assert not torch.equal(rx, rx0)
+    ones = torch.ones_like(y)
+    got = torch.autograd.grad(y, weight, ones) + torch.autograd.grad(out, w, ones)
+    want = torch.autograd.grad(ops.rms_norm(rx0, weight), weight, ones) + torch.autograd.grad(ops.moe_ungroup_rows(rx0, slots, w), w, ones)
+    assert same(got, want)
+    buf.check()
+    buf.destroy()
+
+
+def test_operands_of_another_device_are_refused():
+    c = make()
+    for call in (lambda: ops.rms_norm(c["x"], c["weight"].cpu()), lambda: ops.add_rms_norm(c["x"], c["residual"].cpu(), c["weight"]),
+                 lambda: ops.moe_route(c["x"], 2, torch.zeros(264)), lambda: ops.moe_group_rows(c["x"], torch.zeros(50, 1, dtype=torch.int64), 2),
+                 lambda: ops.moe_ungroup_rows(c["x"], torch.zeros(5, 1, dtype=torch.int32))):
+        with pytest.raises(RuntimeError, match="device"):
+            call()
+
+
+def test_odd_alignment():
+    """Operands that start at any element."""
+    c = make(h=264)
+    idx = torch.randint(0, 8, (50, 3), device=DEV)
+
+    def shifted(t, n):
+        buf = torch.empty(t.numel() + n, device=DEV, dtype=t.dtype)
+        return buf[n:].view(t.shape).copy_(t)
+    rows, _, off, slots = ops.moe_group_rows(c["x"], idx, 8)
+    for n in (1, 2, 4):
+        r2, _, off2, slots2 = ops.moe_group_rows(shifted(c["x"], n), idx, 8)
+        assert torch.equal(rows, r2) and torch.equal(off, off2) and torch.equal(slots, slots2)
+        w = torch.rand(50, 3, device=DEV)
+        assert torch.equal(ops.moe_ungroup_rows(rows, slots, w, c["residual"]), ops.moe_ungroup_rows(shifted(rows, n), slots, w, shifted(c["residual"], n)))
+        assert torch.equal(ops.moe_route(c["x"], 3)[0], ops.moe_route(shifted(c["x"], n), 3)[0])
+    with pytest.raises(RuntimeError, match="aligned"):
+        ops.rms_norm_quant(shifted(torch.zeros(4, 128, device=DEV, dtype=BF), 1), torch.ones(128, device=DEV, dtype=BF), 3)
+    q8 = torch.randint(-100, 100, (50, 264), device=DEV, dtype=torch.int8)
+    assert torch.equal(ops.moe_group_rows(shifted(q8, 3), idx, 8)[0], ops.moe_group_rows(q8, idx, 8)[0])
+    want = group64(q8, idx, 8)
+    assert torch.equal(ops.moe_group_rows(q8, idx, 8)[0].float(), want[0])
+
+
+def test_slots_out_of_range_are_left_out():
+    rows = torch.randn(6, 40, device=DEV).to(BF).requires_grad_()
+    slots = torch.tensor([[0, 6], [2 ** 31 - 1, 3], [-2 ** 31, -1]], device=DEV, dtype=torch.int32)
+    w = torch.rand(3, 2, device=DEV).requires_grad_()
+    out = ops.moe_ungroup_rows(rows, slots, w)
+    inside = ops.moe_ungroup_rows(rows, torch.tensor([[0, -1], [-1, 3], [-1, -1]], device=DEV, dtype=torch.int32), w)
+    assert torch.equal(out, inside) and not out[2].any()
+    a, b = (torch.autograd.grad(o, (rows, w), torch.ones_like(o)) for o in (out, inside))
+    assert same(a, b) and not a[0][[1, 2, 4, 5]].any() and not a[1][2].any()
+    none = ops.moe_ungroup_rows(rows[:0].detach(), slots, w)
+    assert not none.any()

@@ -51,11 +51,15 @@ KERNEL_SOURCES = [
     "kernels/grouped_mlp.cu",
     "kernels/expert_gemm_narrow.cu",
     "kernels/expert_gemv.cu",
+    "kernels/rms_norm.cu",
+    "kernels/moe_route.cu",
+    "kernels/group_rows.cu",
     "runtime/cam_runtime.cpp",
     "runtime/expert_ops.cpp",
+    "runtime/layer_ops.cpp",
 ]
 
-BINDING_SOURCES = ["bindings.cpp", "bindings_expert.cpp"]
+BINDING_SOURCES = ["bindings.cpp", "bindings_expert.cpp", "bindings_layer.cpp"]
 
 
 def _nvcc() -> str:

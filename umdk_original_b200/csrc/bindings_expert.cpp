@@ -1,46 +1,12 @@
 // PyTorch bindings of the expert-MLP operators that need no Buffer: 4-bit quantisation, grouped products of 4-bit operands, the
 // gated feed-forward block of 16-bit experts with its backward pass.
 // Schemas are added to the library that bindings.cpp defines.
-#include <ATen/TensorSubclassLikeUtils.h>
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGraphsC10Utils.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/extension.h>
-#include <torch/library.h>
-
-#include <string>
-#include <tuple>
-
-#include "runtime/cam_runtime.h"
+#include "bindings_common.h"
 #include "runtime/expert_ops.h"
 
 namespace {
 
-#define CAM_ASSERT(cond, ...) TORCH_CHECK(cond, "umdk_cam_op_lib: ", __VA_ARGS__)
-#define CAM_RT(call) TORCH_CHECK((call) == 0, "umdk_cam_op_lib: ", cam_last_error())
-
-using OptTensor = c10::optional<at::Tensor>;
-
-// Numbers enter messages as text: formatting them through the string streams of TORCH_CHECK crashes in a process whose C++
-// runtime libraries disagree about the locale.
-std::string num(int64_t v) { return std::to_string(v); }
-std::string shape(at::IntArrayRef v) {
-    std::string s = "[";
-    for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + num(v[i]);
-    return s + "]";
-}
-
-bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-void check_operand(const at::Tensor& t, const at::Tensor& with, const char* what) {
-    CAM_ASSERT(t.device() == with.device(), what, " must be on ", with.device().str(), ", the device of the rows");
-    CAM_ASSERT(t.is_contiguous(), what, " must be contiguous");
-}
-
-int dtype_of(at::ScalarType t, const char* what) {
-    CAM_ASSERT(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat, what, " must be bfloat16, float16 or float32");
-    return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : 2;
-}
+using namespace umdk;
 
 at::ScalarType scale_type(int64_t block) {
     CAM_ASSERT(block == 16 || block == 32, "block must be 16 (nvfp4) or 32 (mxfp4), got ", num(block));
@@ -306,20 +272,6 @@ Mlp3 call_mlp_train(const at::Tensor& x, const at::Tensor& w1, const at::Tensor&
     return op.call(x, w1, w2, off);
 }
 
-// What the backward pass will read of an input.  The rows of a dispatch are views of memory that the next dispatch on that Buffer
-// overwrites, behind the back of autograd's version counters, and a program of several layers dispatches again before it runs
-// backward: such memory (any that PyTorch's allocators do not own) is copied.  A tracer's stand-ins (torch.compile) do not know whose
-// memory the traced program will see, so a traced program always copies, by an operator of this library: a plain clone may be
-// removed by the compiler's passes, or moved into the backward pass, where it would come too late.
-at::Tensor kept_for_backward(const at::Tensor& t) {
-    if (at::isTensorSubclassLike(t)) {
-        static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("umdk_cam_op_lib::grouped_mlp_keep", "")
-                             .typed<at::Tensor(const at::Tensor&)>();
-        return op.call(t);
-    }
-    return t.storage().unsafeGetStorageImpl()->resizable() ? t : t.clone();
-}
-
 at::Tensor grouped_mlp_keep(const at::Tensor& t) { return t.clone(); }
 
 struct GroupedMlpFunction : public torch::autograd::Function<GroupedMlpFunction> {
@@ -343,32 +295,8 @@ struct GroupedMlpFunction : public torch::autograd::Function<GroupedMlpFunction>
     }
 };
 
-// A captured backward pass that accumulates into a leaf whose accumulation node belongs to an eager graph (another stream) makes
-// the autograd engine synchronise a stream that is not captured, which ends the process.  Refused while it can still be.
-void check_capture(const at::Tensor& t, const char* what) {
-    if (!t.requires_grad() || !t.is_leaf() || !t.is_cuda()) return;
-    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (accumulator == nullptr) return;
-    const auto stream = accumulator->stream();
-    CAM_ASSERT(!stream.has_value() || *stream == at::cuda::getCurrentCUDAStream(t.device().index()).unwrap(), "grouped_mlp is captured into a CUDA graph while a graph of derivatives that was recorded outside the capture still holds ",
-               what, "; let go of its outputs before the capture");
-}
-
 at::Tensor grouped_mlp_autograd(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, const at::Tensor& expert_offsets) {
-    // a dual tensor need not require a gradient: without this its tangent would be dropped
-    for (const at::Tensor* t : {&x, &w1, &w2})
-        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), "umdk_cam_op_lib: grouped_mlp has no forward-mode derivative");
-    if (at::GradMode::is_enabled() && (x.requires_grad() || w1.requires_grad() || w2.requires_grad())) {
-        if (x.is_cuda()) {
-            c10::cuda::CUDAGuard guard(x.device());
-            if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
-                check_capture(x, "x");
-                check_capture(w1, "w1");
-                check_capture(w2, "w2");
-            }
-        }
-        return GroupedMlpFunction::apply(x, w1, w2, expert_offsets);
-    }
+    if (records_graph("grouped_mlp", {{&x, "x"}, {&w1, "w1"}, {&w2, "w2"}})) return GroupedMlpFunction::apply(x, w1, w2, expert_offsets);
     at::AutoDispatchBelowADInplaceOrView guard;
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("umdk_cam_op_lib::grouped_mlp", "")
                          .typed<at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&)>();

@@ -1,0 +1,135 @@
+// Loads, stores and sums shared by the operators round the experts.  Rows are bf16, fp16 or fp32; arithmetic is fp32.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "../common/ptx.cuh"
+#include "expert_ops.h"
+
+namespace cam {
+
+template <int DT>
+constexpr int kBytes = DT == kDtFp32 ? 4 : 2;
+
+// eight consecutive values as they lie in memory
+template <int DT>
+struct Raw8 {
+    uint4 v[DT == kDtFp32 ? 2 : 1];
+};
+
+__device__ __forceinline__ uint4 load16_stream(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// 32-byte pieces for fp32: p is 32-byte aligned wherever rows of eight values are, which the launchers check
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load8(const void* base, int64_t i) {
+    Raw8<DT> r;
+    const char* p = static_cast<const char*>(base) + i * kBytes<DT>;
+    r.v[0] = load16_stream(p);
+    if constexpr (DT == kDtFp32) r.v[1] = load16_stream(p + 16);
+    return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void widen8(const Raw8<DT>& r, float* f) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.v);
+    if constexpr (DT == kDtFp32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == kDtBf16) {
+                f[2 * i] = __uint_as_float(w[i] << 16);
+                f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            } else {
+                const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                f[2 * i] = t.x;
+                f[2 * i + 1] = t.y;
+            }
+        }
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ Raw8<DT> narrow8(const float* f) {
+    Raw8<DT> r;
+    uint32_t* w = reinterpret_cast<uint32_t*>(r.v);
+    if constexpr (DT == kDtFp32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == kDtBf16) {
+                const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&p);
+            } else {
+                const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&p);
+            }
+        }
+    }
+    return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(void* base, int64_t i, const Raw8<DT>& r) {
+    uint4* p = reinterpret_cast<uint4*>(static_cast<char*>(base) + i * kBytes<DT>);
+    p[0] = r.v[0];
+    if constexpr (DT == kDtFp32) p[1] = r.v[1];
+}
+
+template <int DT>
+__device__ __forceinline__ float load1(const void* base, int64_t i) {
+    if constexpr (DT == kDtFp32) return __ldg(static_cast<const float*>(base) + i);
+    const unsigned short b = __ldg(static_cast<const unsigned short*>(base) + i);
+    if constexpr (DT == kDtBf16) return __uint_as_float(static_cast<uint32_t>(b) << 16);
+    return __half2float(__ushort_as_half(b));
+}
+
+template <int DT>
+__device__ __forceinline__ void store1(void* base, int64_t i, float v) {
+    if constexpr (DT == kDtFp32) static_cast<float*>(base)[i] = v;
+    else if constexpr (DT == kDtBf16) static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(base)[i] = __float2half_rn(v);
+}
+
+// A value rounded to a type and widened again
+template <int DT>
+__device__ __forceinline__ float rounded(float v) {
+    if constexpr (DT == kDtBf16) return __bfloat162float(__float2bfloat16_rn(v));
+    if constexpr (DT == kDtFp16) return __half2float(__float2half_rn(v));
+    return v;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
+}
+
+// A kernel launch that may start while its predecessor ends (programmatic dependent launch)
+template <class Kernel, class... Args>
+int launch_pdl(Kernel kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1] = {pdl_attribute()};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace cam

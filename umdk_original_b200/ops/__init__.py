@@ -16,7 +16,8 @@ grouped_gemm_fp8_swiglu = ops.grouped_gemm_fp8_swiglu
 # imported beside an extension that was built before they existed.  They have one overload each, which is called directly: the
 # choice among overloads costs 0.6 us of the 7 that such a call takes on the host.
 _EXPERT_OPS = ("quantize_fp4", "dequantize_fp4", "grouped_gemm_fp4", "grouped_gemm_fp4_swiglu", "grouped_mlp",
-               "grouped_mlp_train", "grouped_mlp_backward")
+               "grouped_mlp_train", "grouped_mlp_backward", "rms_norm", "add_rms_norm", "rms_norm_train", "rms_norm_backward",
+               "rms_norm_quant", "moe_route", "moe_route_backward", "moe_group_rows", "moe_ungroup_rows", "moe_ungroup_rows_backward")
 
 
 def check_expert_ops(device=None) -> None:
