@@ -49,7 +49,7 @@ struct RouteParams {
     int64_t rows;
     int experts, k, groups, topk_groups, group_top, sigmoid, renormalize;
     float scale;
-    int vec;                // a lane's logits can be read in one piece
+    int vec, vec_bias;      // a lane's logits and biases can be read in pieces of 16 bytes (set by the launcher)
     int64_t* idx;           // [rows, k]
     float* weights;         // [rows, k]
     const float* dweights;  // backward
@@ -93,7 +93,6 @@ int cam_launch_rms_norm(const cam::RmsNormParams* p, int dtype, cudaStream_t str
 int cam_rms_norm_backward_blocks(int64_t rows, int h);
 int cam_launch_rms_norm_backward(const cam::RmsNormBackwardParams* p, int dtype, cudaStream_t stream);
 int cam_launch_moe_route(const cam::RouteParams* p, int dtype, cudaStream_t stream);
-int cam_launch_moe_route_backward(const cam::RouteParams* p, int dtype, cudaStream_t stream);
 int cam_launch_group_rows(const cam::GroupRowsParams* p, cudaStream_t stream);
 int cam_launch_ungroup_rows(const cam::UngroupRowsParams* p, int dtype, cudaStream_t stream);
 int cam_launch_ungroup_rows_backward(const cam::UngroupRowsParams* p, int dtype, cudaStream_t stream);

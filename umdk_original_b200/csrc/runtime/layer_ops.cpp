@@ -147,7 +147,7 @@ extern "C" int cam_moe_route_backward(const float* dweights, const void* logits,
     p.idx = const_cast<int64_t*>(idx);
     p.dweights = dweights;
     p.dlogits = dlogits;
-    return launched(cam_launch_moe_route_backward(&p, dtype, stream), "moe_route_backward");
+    return launched(cam_launch_moe_route(&p, dtype, stream), "moe_route_backward");
 }
 
 namespace {
