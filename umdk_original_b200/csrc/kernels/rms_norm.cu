@@ -3,13 +3,14 @@
 //   s = x + residual (rounded to the residual's type),  r = 1 / sqrt(mean(s^2) + eps),  y = s r w
 //   dx = dresidual = ds + r (w dy - s r mean(w dy s r)),   dw = sum over the rows of dy s r
 //
-// Bound by memory in both directions.  A row stays in the registers of the threads that share it: read once, summed, scaled and
-// written.  Rows of up to 1024 values belong to one warp, longer ones to a block.  The norm is that of the rounded sum, so a
-// backward pass (or a later layer) that reads the stored sum sees the numbers that were normalised.
+// Bound by memory in both directions, with the issue slots close behind: arithmetic runs on pairs (16-bit sums in one instruction,
+// products and sums of two fp32 values in one).  A row stays in the registers of the threads that share it: read once, summed, scaled and
+// written.  A thread owns 16 consecutive values at a time, so blocks of 128 for e4m3 are eight lanes.  The norm is that of the
+// rounded sum, so a backward pass (or a later layer) that reads the stored sum sees the numbers that were normalised.
 #include "../common/quant.cuh"
+#include "launch.h"
 #include "layer_ops.h"
 #include "layer_values.cuh"
-#include "launch.h"
 
 namespace cam {
 
@@ -18,372 +19,737 @@ namespace {
 constexpr int kRowsOnly = 0, kInt8 = 2, kE4m3 = 3;
 constexpr int kWarpRows = 8;  // rows of a block where a row belongs to a warp
 
-// Places of a thread's values: with VEC pieces of eight consecutive ones, otherwise (odd widths, any alignment) single ones.
-template <bool VEC>
-__device__ __forceinline__ int place(int v, int j, int t, int threads) {
-    return VEC ? (v * threads + t) * 8 + j : (v * 8 + j) * threads + t;
+// ------------------------------------------------------------------------------------------------
+// Pairs of fp32 values, sixteen values as they lie in memory
+// ------------------------------------------------------------------------------------------------
+using Pair = unsigned long long;
+
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 split(Pair v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
 
-template <int DT, bool VEC>
-__device__ __forceinline__ void load_piece(const void* base, int64_t row0, int v, int t, int threads, int h, float* f) {
-    if constexpr (VEC) {
-        const int c = place<true>(v, 0, t, threads);
-        if (c < h) widen8<DT>(load8<DT>(base, row0 + c), f);
-        else {
+template <int DT>
+constexpr int kWords = DT == kDtFp32 ? 16 : 8;  // 32-bit words of sixteen values
+
+template <int DT>
+struct Raw16 {
+    uint32_t w[kWords<DT>];
+};
+
+template <int DT>
+__device__ __forceinline__ Pair widen2(const Raw16<DT>& r, int i) {
+    if constexpr (DT == kDtFp32) return pair(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+    else if constexpr (DT == kDtBf16) return pair(__uint_as_float(r.w[i] << 16), __uint_as_float(r.w[i] & 0xFFFF0000u));
+    else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+        return pair(f.x, f.y);
+    }
+}
+template <int DT>
+__device__ __forceinline__ void narrow2(Raw16<DT>& r, int i, Pair v) {
+    const float2 f = split(v);
+    if constexpr (DT == kDtFp32) {
+        r.w[2 * i] = __float_as_uint(f.x);
+        r.w[2 * i + 1] = __float_as_uint(f.y);
+    } else if constexpr (DT == kDtBf16) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
+        r.w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+        const __half2 b = __floats2half2_rn(f.x, f.y);
+        r.w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+}
+// x + r of one type, rounded once
+template <int DT>
+__device__ __forceinline__ Raw16<DT> add16(const Raw16<DT>& x, const Raw16<DT>& r) {
+    Raw16<DT> s;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = 0.f;
+    for (int i = 0; i < kWords<DT>; ++i) {
+        if constexpr (DT == kDtFp32) s.w[i] = __float_as_uint(__uint_as_float(x.w[i]) + __uint_as_float(r.w[i]));
+        else if constexpr (DT == kDtBf16) {
+            const __nv_bfloat162 v = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&x.w[i]), *reinterpret_cast<const __nv_bfloat162*>(&r.w[i]));
+            s.w[i] = *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+            const __half2 v = __hadd2(*reinterpret_cast<const __half2*>(&x.w[i]), *reinterpret_cast<const __half2*>(&r.w[i]));
+            s.w[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
+    return s;
+}
+
+__device__ __forceinline__ void load32(uint32_t* v, const void* p) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
+// How rows can be read: 32 bytes at a time, 16 (rows of a multiple of 8 values), or one value (odd widths, any alignment)
+constexpr int kBy32 = 16, kBy16 = 8, kByOne = 1;
+
+// Column of the first of a thread's sixteen values (kByOne: of value j)
+template <int VEC>
+__device__ __forceinline__ int column(int v, int j, int t, int threads) {
+    return VEC == kByOne ? (v * 16 + j) * threads + t : (v * threads + t) * 16 + j;
+}
+
+// Zeros past the row.  `cached`: what every row reads, through L1.
+template <int DT, int VEC>
+__device__ __forceinline__ Raw16<DT> load16(const void* base, int64_t row0, int v, int t, int threads, int h, bool cached = false) {
+    Raw16<DT> r;
+    if constexpr (VEC == kByOne) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int c = column<VEC>(v, j, t, threads);
+            if constexpr (DT == kDtFp32) r.w[j] = c < h ? __float_as_uint(load1<DT>(base, row0 + c)) : 0u;
+            else {
+                const uint32_t b = c < h ? __ldg(static_cast<const unsigned short*>(base) + row0 + c) : 0u;
+                r.w[j / 2] = j % 2 ? r.w[j / 2] | b << 16 : b;
+            }
         }
     } else {
+        const int c = column<VEC>(v, 0, t, threads);
+        const char* p = static_cast<const char*>(base) + (row0 + c) * kBytes<DT>;
+        if (VEC == kBy32 && !cached) {
+            if (c < h) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int c = place<false>(v, j, t, threads);
-            f[j] = c < h ? load1<DT>(base, row0 + c) : 0.f;
+                for (int i = 0; i < kWords<DT>; i += 8) load32(r.w + i, p + i * 4);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kWords<DT>; ++i) r.w[i] = 0u;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords<DT>; i += 4) {
+                uint4 q = make_uint4(0u, 0u, 0u, 0u);
+                if (c + i * 4 / kBytes<DT> < h) q = cached ? __ldg(reinterpret_cast<const uint4*>(p + i * 4)) : load16_stream(p + i * 4);
+                r.w[i] = q.x, r.w[i + 1] = q.y, r.w[i + 2] = q.z, r.w[i + 3] = q.w;
+            }
+        }
+    }
+    return r;
+}
+
+template <int DT, int VEC>
+__device__ __forceinline__ void store16(void* base, int64_t row0, int v, int t, int threads, int h, const Raw16<DT>& r) {
+    if constexpr (VEC == kByOne) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int c = column<VEC>(v, j, t, threads);
+            if (c >= h) continue;
+            if constexpr (DT == kDtFp32) static_cast<uint32_t*>(base)[row0 + c] = r.w[j];
+            else static_cast<unsigned short*>(base)[row0 + c] = static_cast<unsigned short>(r.w[j / 2] >> (j % 2 * 16));
+        }
+    } else {
+        const int c = column<VEC>(v, 0, t, threads);
+        char* p = static_cast<char*>(base) + (row0 + c) * kBytes<DT>;
+        if constexpr (VEC == kBy32) {
+            if (c < h) {
+#pragma unroll
+                for (int i = 0; i < kWords<DT>; i += 8) store32(p + i * 4, r.w + i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords<DT>; i += 4) {
+                if (c + i * 4 / kBytes<DT> < h) *reinterpret_cast<uint4*>(p + i * 4) = make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
+            }
         }
     }
 }
 
-template <int DT, bool VEC>
-__device__ __forceinline__ void store_piece(void* base, int64_t row0, int v, int t, int threads, int h, const float* f) {
-    if constexpr (VEC) {
-        const int c = place<true>(v, 0, t, threads);
-        if (c < h) store8<DT>(base, row0 + c, narrow8<DT>(f));
-    } else {
+// Weights of a thread's sixteen columns
+template <int DT, int VEC>
+__device__ __forceinline__ void load_weight(const void* w, bool fp32, int v, int t, int threads, int h, Pair* out) {
+    if (DT == kDtFp32 || fp32) {
+        const Raw16<kDtFp32> r = load16<kDtFp32, VEC>(w, 0, v, t, threads, h, true);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int c = place<false>(v, j, t, threads);
-            if (c < h) store1<DT>(base, row0 + c, f[j]);
-        }
+        for (int i = 0; i < 8; ++i) out[i] = widen2<kDtFp32>(r, i);
+    } else {
+        const Raw16<DT> r = load16<DT, VEC>(w, 0, v, t, threads, h, true);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[i] = widen2<DT>(r, i);
     }
 }
 
-// Weights are read by every row: through L1.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load_weight(const void* w, bool fp32, int v, int t, int threads, int h, float* f) {
-    if constexpr (VEC) {
-        const int c = place<true>(v, 0, t, threads);
-        if (c >= h) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = 0.f;
-        } else if (fp32 || DT == kDtFp32) {
-            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w) + c);
-            const float4 a = __ldg(p), b = __ldg(p + 1);
-            f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-        } else if constexpr (DT != kDtFp32) {
-            Raw8<DT> r;
-            r.v[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(w) + c * 2));
-            widen8<DT>(r, f);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int c = place<false>(v, j, t, threads);
-            f[j] = c >= h ? 0.f : fp32 ? load1<kDtFp32>(w, c) : load1<DT>(w, c);
-        }
-    }
+// Sum (and maximum) over the threads that share a row, with one barrier: `red`, 64 floats of the block, is one of two that take turns
+// where there are several rows.  The warps' sums are added in their order.
+template <bool WARP, int N>
+__device__ __forceinline__ void clear_sums(float (&red)[N]) {
+    // places of warps that the block does not have; the first barrier comes before they are read
+    if (!WARP && threadIdx.x < N && (threadIdx.x & 31) >= blockDim.x >> 5) red[threadIdx.x] = 0.f;
+    if (!WARP && blockDim.x < N && threadIdx.x + blockDim.x < N && ((threadIdx.x + blockDim.x) & 31) >= blockDim.x >> 5) red[threadIdx.x + blockDim.x] = 0.f;
 }
-
-// Sum (and maximum) over the threads that share a row; `red`: 64 floats of the block.
 template <bool WARP, bool MAX>
 __device__ __forceinline__ void over_row(float& sum, float& top, float* red) {
     sum = warp_sum(sum);
     if (MAX) top = warp_max(top);
-    if constexpr (!WARP) {
-        const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-        __syncthreads();  // the row before has been read from `red`
-        if (lane == 0) {
+    if constexpr (WARP) {
+        __syncwarp();
+    } else {
+        const int warps = blockDim.x >> 5;
+        if ((threadIdx.x & 31) == 0) {
             red[threadIdx.x >> 5] = sum;
             if (MAX) red[32 + (threadIdx.x >> 5)] = top;
         }
         __syncthreads();
-        sum = warp_sum(lane < warps ? red[lane] : 0.f);
-        if (MAX) top = warp_max(lane < warps ? red[32 + lane] : 0.f);
+        sum = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < warps; i += 4) {  // what is behind the last warp is zero
+            const float4 v = *reinterpret_cast<const float4*>(red + i);
+            sum += v.x + v.y + (v.z + v.w);
+            if (MAX) {
+                const float4 m = *reinterpret_cast<const float4*>(red + 32 + i);
+                top = fmaxf(fmaxf(top, fmaxf(m.x, m.y)), fmaxf(m.z, m.w));
+            }
+        }
     }
 }
 
-// Threads of a block at most: four pieces per thread up to 8192 values, two beyond
-constexpr int norm_threads(int pieces, bool warp) { return warp || pieces == 4 ? 256 : 1024; }
-static_assert(kWarpRows * 32 == 256 && 256 * 4 * 8 >= 8192 && 1024 * 2 * 8 >= kNormMaxHidden, "every row has its threads");
+// ------------------------------------------------------------------------------------------------
+// Forward
+// ------------------------------------------------------------------------------------------------
+// Sixteen values of a row in 8 bits
+template <int VEC>
+__device__ __forceinline__ void store_int8(void* q, int64_t row0, int v, int t, int threads, int h, const Pair* y, float inv) {
+    uint32_t o[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const float2 f = split(y[j / 2]);
+        const int a = max(-127, min(127, __float2int_rn((j % 2 ? f.y : f.x) * inv)));  // NaN becomes 0; the row's scale is NaN then
+        if constexpr (VEC == kByOne) {
+            const int c = column<VEC>(v, j, t, threads);
+            if (c < h) static_cast<int8_t*>(q)[row0 + c] = static_cast<int8_t>(a);
+        } else {
+            o[j / 4] |= (static_cast<uint32_t>(a) & 0xFFu) << (j % 4 * 8);
+        }
+    }
+    if constexpr (VEC != kByOne) {
+        const int c = column<VEC>(v, 0, t, threads);
+        uint2* p = reinterpret_cast<uint2*>(static_cast<int8_t*>(q) + row0 + c);
+        if (c < h) p[0] = make_uint2(o[0], o[1]);
+        if (c + 8 < h) p[1] = make_uint2(o[2], o[3]);
+    }
+}
 
-template <int DT, int MODE, int NV, bool VEC, bool WARP>
-__global__ void __launch_bounds__(norm_threads(NV, WARP))
+// Power-of-two scale: the least 2^k >= max(amax, 1e-4) / 448.  448 = 1.75 x 2^8, so k is the exponent of amax less 8, one more where the
+// significand is above 1.75: exact, without a division.
+__device__ __forceinline__ void block_scale(float amax, bool power_of_two, float& scale, float& inv) {
+    const float a = fmaxf(amax, 1e-4f);
+    if (power_of_two) {
+        const uint32_t b = __float_as_uint(a), e = (b >> 23) - 8u + ((b & 0x7FFFFFu) > 0x600000u ? 1u : 0u);
+        scale = __uint_as_float(e << 23);
+        inv = __uint_as_float((254u - e) << 23);
+    } else {
+        scale = a * (1.f / 448.f);
+        inv = __fdividef(448.f, a);
+    }
+}
+
+template <int DT, int MODE, int NP, int VEC, bool WARP>
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : NP == 2 ? 512 : 256)
 rms_norm_kernel(const RmsNormParams p) {
-    __shared__ float red[64];
-    const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
-    const int h = p.h;
-    const int64_t row0 = row * h;
+    __shared__ __align__(16) float red[64];
+    clear_sums<WARP>(red);
+    const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x, h = p.h;
+    const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * kWarpRows + (threadIdx.x >> 5) : blockIdx.x, row0 = row * h;
     pdl_wait();
     pdl_release();
     if (WARP && row >= p.rows) return;
-    float s[NV * 8], w[NV * 8];
+    Pair s[NP][8];
+    {
+        Raw16<DT> x[NP];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) load_piece<DT, VEC>(p.x, row0, v, t, threads, h, s + 8 * v);
-    if (p.residual != nullptr) {
-        if (DT == kDtFp32 || p.res_type == kDtFp32) {
+        for (int v = 0; v < NP; ++v) x[v] = load16<DT, VEC>(p.x, row0, v, t, threads, h);
+        if (p.residual == nullptr) {
 #pragma unroll
-            for (int v = 0; v < NV; ++v) load_piece<kDtFp32, VEC>(p.residual, row0, v, t, threads, h, w + 8 * v);
+            for (int v = 0; v < NP; ++v) {
 #pragma unroll
-            for (int i = 0; i < NV * 8; ++i) s[i] += w[i];
+                for (int i = 0; i < 8; ++i) s[v][i] = widen2<DT>(x[v], i);
+            }
+        } else if (DT != kDtFp32 && p.res_type == kDtFp32) {
+            Raw16<kDtFp32> r[NP];
 #pragma unroll
-            for (int v = 0; v < NV; ++v) store_piece<kDtFp32, VEC>(p.sum, row0, v, t, threads, h, s + 8 * v);
+            for (int v = 0; v < NP; ++v) r[v] = load16<kDtFp32, VEC>(p.residual, row0, v, t, threads, h);
+#pragma unroll
+            for (int v = 0; v < NP; ++v) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    s[v][i] = add2(widen2<DT>(x[v], i), widen2<kDtFp32>(r[v], i));
+                    narrow2<kDtFp32>(r[v], i, s[v][i]);
+                }
+                store16<kDtFp32, VEC>(p.sum, row0, v, t, threads, h, r[v]);
+            }
         } else {
+            Raw16<DT> r[NP];
 #pragma unroll
-            for (int v = 0; v < NV; ++v) load_piece<DT, VEC>(p.residual, row0, v, t, threads, h, w + 8 * v);
+            for (int v = 0; v < NP; ++v) r[v] = load16<DT, VEC>(p.residual, row0, v, t, threads, h);
 #pragma unroll
-            for (int i = 0; i < NV * 8; ++i) s[i] = rounded<DT>(s[i] + w[i]);
+            for (int v = 0; v < NP; ++v) {
+                r[v] = add16<DT>(x[v], r[v]);
 #pragma unroll
-            for (int v = 0; v < NV; ++v) store_piece<DT, VEC>(p.sum, row0, v, t, threads, h, s + 8 * v);
+                for (int i = 0; i < 8; ++i) s[v][i] = widen2<DT>(r[v], i);
+                store16<DT, VEC>(p.sum, row0, v, t, threads, h, r[v]);
+            }
         }
     }
+    Pair squares = 0ull;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) load_weight<DT, VEC>(p.weight, p.weight_type == kDtFp32, v, t, threads, h, w + 8 * v);
-    float sum = 0.f, top = 0.f;
+    for (int v = 0; v < NP; ++v) {
 #pragma unroll
-    for (int i = 0; i < NV * 8; ++i) {
-        sum = fmaf(s[i], s[i], sum);
-        if (MODE == kInt8) top = fmaxf(top, fabsf(s[i] * w[i]));
+        for (int i = 0; i < 8; ++i) squares = fma2(s[v][i], s[v][i], squares);
+    }
+    const float2 halves = split(squares);
+    float sum = halves.x + halves.y, top = 0.f;
+    // times the weight already: int8 needs the largest product along with the sum
+#pragma unroll
+    for (int v = 0; v < NP; ++v) {
+        Pair w[8];
+        load_weight<DT, VEC>(p.weight, p.weight_type == kDtFp32, v, t, threads, h, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            s[v][i] = mul2(s[v][i], w[i]);
+            if (MODE == kInt8) {
+                const float2 f = split(s[v][i]);
+                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+        }
     }
     over_row<WARP, MODE == kInt8>(sum, top, red);
     const float rstd = 1.f / sqrtf(sum / static_cast<float>(h) + p.eps);
     if (p.rstd != nullptr && t == 0) p.rstd[row] = rstd;
+    const Pair rstd2 = pair(rstd, rstd);
+    const float inv8 = 127.f / (top * rstd + 1e-12f);
+    if (MODE == kInt8 && t == 0) p.scales[row] = 1.f / inv8;
 #pragma unroll
-    for (int i = 0; i < NV * 8; ++i) s[i] = s[i] * rstd * w[i];
-    if (MODE == kRowsOnly || p.y != nullptr) {
+    for (int v = 0; v < NP; ++v) {
 #pragma unroll
-        for (int v = 0; v < NV; ++v) store_piece<DT, VEC>(p.y, row0, v, t, threads, h, s + 8 * v);
-    }
-    if constexpr (MODE == kInt8) {
-        // a row with NaN has a NaN scale
-        const float inv = 127.f / (top * rstd + 1e-12f);
+        for (int i = 0; i < 8; ++i) s[v][i] = mul2(s[v][i], rstd2);
+        if (MODE == kRowsOnly || p.y != nullptr) {
+            Raw16<DT> y;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            int q[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = max(-127, min(127, __float2int_rn(s[8 * v + j] * inv)));
-            if constexpr (VEC) {
-                const int c = place<true>(v, 0, t, threads);
-                uint2 o = make_uint2(0u, 0u);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    o.x |= (static_cast<uint32_t>(q[j]) & 0xFFu) << (8 * j);
-                    o.y |= (static_cast<uint32_t>(q[4 + j]) & 0xFFu) << (8 * j);
-                }
-                if (c < h) *reinterpret_cast<uint2*>(static_cast<int8_t*>(p.q) + row0 + c) = o;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int c = place<false>(v, j, t, threads);
-                    if (c < h) static_cast<int8_t*>(p.q)[row0 + c] = static_cast<int8_t>(q[j]);
-                }
-            }
+            for (int i = 0; i < 8; ++i) narrow2<DT>(y, i, s[v][i]);
+            store16<DT, VEC>(p.y, row0, v, t, threads, h, y);
         }
-        if (t == 0) p.scales[row] = 1.f / inv;
-    }
-    if constexpr (MODE == kE4m3) {
-        // a block of 128 values: sixteen consecutive lanes
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            float* f = s + 8 * v;
+        if constexpr (MODE == kInt8) store_int8<VEC>(p.q, row0, v, t, threads, h, s[v], inv8);
+        if constexpr (MODE == kE4m3) {
+            // a block of 128 values: eight consecutive lanes
             float amax = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(f[j]));
-#pragma unroll
-            for (int o = 8; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-            float scale, inv;
-            if (p.quant_mode == 4) ue8m0_scale(amax, scale, inv);
-            else {
-                const float a = fmaxf(amax, 1e-4f);
-                inv = 448.f / a;
-                scale = a / 448.f;
+            for (int i = 0; i < 8; ++i) {
+                const float2 f = split(s[v][i]);
+                amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
             }
-            const int c = place<true>(v, 0, t, threads);
+#pragma unroll
+            for (int o = 4; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+            float scale, inv;
+            block_scale(amax, p.quant_mode == 4, scale, inv);
+            const Pair inv2 = pair(inv, inv);
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 a = split(mul2(s[v][2 * i], inv2)), b = split(mul2(s[v][2 * i + 1], inv2));
+                o[i] = pack_e4m3x4(a.x, a.y, b.x, b.y);
+            }
+            const int c = column<VEC>(v, 0, t, threads);
             if (c < h) {
-                *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.q) + row0 + c) =
-                    make_uint2(pack_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv), pack_e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
-                if ((t & 15) == 0) p.scales[row * (h / 128) + (c >> 7)] = scale;
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.q) + row0 + c) = make_uint4(o[0], o[1], o[2], o[3]);
+                if ((t & 7) == 0) p.scales[row * (h / 128) + (c >> 7)] = scale;
             }
         }
     }
 }
 
+// ------------------------------------------------------------------------------------------------
+// Backward
+// ------------------------------------------------------------------------------------------------
 // Rows are shared out to the blocks in turn; a thread keeps the sums of its columns' weight gradients over all of its rows, and the
 // block's go to `partial`, which a second kernel adds up in a fixed order.
-template <int DT, int NV, bool VEC, bool WARP, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-rms_norm_backward_kernel(const RmsNormBackwardParams p) {
-    __shared__ float red[64];
-    __shared__ float cols[WARP ? kWarpRows * NV * 256 : 1];
-    const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x, warp = threadIdx.x >> 5;
-    const int h = p.h;
+//
+// With STAGES > 0 every thread has a ring of its own pieces of the rows ahead in shared memory: it reads only what it (fp32: its warp)
+// copied, so a wait for its own copies is all that the data needs, and the copies of a later row go out when it has read the place that
+// they go to.
+
+// Everything goes in halves of eight values, and the ring is read again after the exchange rather than kept, so that 64 registers do and
+// two blocks of 7168 columns share an SM.
+
+// Column of value j of half `i`.  The halves are eight consecutive values each, and so are a warp's: 16 bytes per thread that were a
+// half of 32 consecutive ones would fetch every sector twice (8192 x 7168 bf16: 138 us).
+template <int VEC>
+__device__ __forceinline__ int half_column(int i, int j, int t, int threads) {
+    return VEC == kByOne ? (i * 8 + j) * threads + t : (i * threads + t) * 8 + j;
+}
+
+// Eight values of a row as pairs
+template <int DT, int VEC>
+__device__ __forceinline__ void load_half(const void* base, int64_t row0, int i, int t, int threads, int h, Pair* out) {
+    if constexpr (VEC == kByOne) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = half_column<VEC>(i, 2 * j, t, threads), d = half_column<VEC>(i, 2 * j + 1, t, threads);
+            out[j] = pair(c < h ? load1<DT>(base, row0 + c) : 0.f, d < h ? load1<DT>(base, row0 + d) : 0.f);
+        }
+    } else {
+        const int c = half_column<VEC>(i, 0, t, threads);
+        Raw8<DT> r = {};
+        if (c < h) {
+            if constexpr (DT == kDtFp32) load32(reinterpret_cast<uint32_t*>(r.v), static_cast<const float*>(base) + row0 + c);
+            else r = load8<DT>(base, row0 + c);
+        }
+        float f[8];
+        widen8<DT>(r, f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[j] = pair(f[2 * j], f[2 * j + 1]);
+    }
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void store_half(void* base, int64_t row0, int i, int t, int threads, int h, const Pair* v) {
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 e = split(v[j]);
+        f[2 * j] = e.x;
+        f[2 * j + 1] = e.y;
+    }
+    if constexpr (VEC == kByOne) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = half_column<VEC>(i, j, t, threads);
+            if (c < h) store1<DT>(base, row0 + c, f[j]);
+        }
+    } else {
+        const int c = half_column<VEC>(i, 0, t, threads);
+        const Raw8<DT> r = narrow8<DT>(f);
+        if (c < h) {
+            if constexpr (DT == kDtFp32) store32(static_cast<float*>(base) + row0 + c, reinterpret_cast<const uint32_t*>(r.v));
+            else store8<DT>(base, row0 + c, r);
+        }
+    }
+}
+
+template <int DT>
+constexpr int kCopies = kBytes<DT> / 2;  // 16-byte copies of eight values
+
+// A thread's sixteen values of an operand to the ring; returns where the next operand's begin (`ring`, for the whole block or warp).  Eight
+// fp32 values are 32 bytes: there a warp's copies take turns by 16 bytes, so that each fetches whole sectors, and a thread reads
+// what others of its warp copied.
+template <int DT>
+__device__ __forceinline__ uint32_t ring_copy(uint32_t ring, int threads, int t, int h, const void* base, int64_t row0) {
+    const int lane = t & 31;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < kCopies<DT>; ++j) {
+            const int unit = DT == kDtFp32 ? (t - lane) * 2 + j * 32 + lane : t, c = i * threads * 8 + unit * (8 / kCopies<DT>);
+            if (c < h)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + (i * kCopies<DT> * threads + unit) * 16), "l"(static_cast<const char*>(base) + (row0 + c) * kBytes<DT>) : "memory");
+        }
+    }
+    return ring + 2 * kCopies<DT> * threads * 16;
+}
+template <int DT>
+__device__ __forceinline__ void ring_half(uint32_t ring, int i, int threads, int t, int h, Pair* out) {
+    Raw8<DT> r = {};
+    if (half_column<kBy16>(i, 0, t, threads) < h) {
+#pragma unroll
+        for (int j = 0; j < kCopies<DT>; ++j)
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.v[j].x), "=r"(r.v[j].y), "=r"(r.v[j].z), "=r"(r.v[j].w) : "r"(ring + ((i * threads + t) * kCopies<DT> + j) * 16) : "memory");
+    }
+    float f[8];
+    widen8<DT>(r, f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = pair(f[2 * j], f[2 * j + 1]);
+}
+
+// Registers of a thread at most; the launcher counts with them
+template <int ST, int STAGES>
+constexpr int kBackwardRegisters = STAGES == 0 ? 128 : ST == kDtFp32 ? 96 : 64;
+
+template <int DT, int ST, int WT, int VEC, bool WARP, int THREADS, int STAGES>
+__global__ void __launch_bounds__(THREADS, THREADS > 512 ? 1 : 65536 / (THREADS * kBackwardRegisters<ST, STAGES>))
+rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
+    extern __shared__ __align__(16) uint8_t dynamic[];  // WARP: per warp; the stages, and at the end the warps' sums
+    __shared__ __align__(16) float red[128];
+    clear_sums<WARP>(red);
+    const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x, warp = threadIdx.x >> 5, h = p.h;
     const int64_t first = WARP ? static_cast<int64_t>(blockIdx.x) * kWarpRows + warp : blockIdx.x;
     const int64_t step = WARP ? static_cast<int64_t>(gridDim.x) * kWarpRows : gridDim.x;
-    const bool sum32 = DT == kDtFp32 || p.sum_type == kDtFp32;
+    const uint32_t slots = smem_u32(dynamic) + (WARP ? warp * STAGES * stage_bytes : 0u);
     pdl_wait();
     pdl_release();
-    float w[NV * 8], acc[NV * 8];
+    auto copy = [&](int64_t row, int stage) {
+        if (row < p.rows) {
+            uint32_t next = ring_copy<DT>(slots + stage * stage_bytes, threads, t, h, p.dy, row * h);
+            next = ring_copy<ST>(next, threads, t, h, p.sum, row * h);
+            if (p.dsum != nullptr) ring_copy<ST>(next, threads, t, h, p.dsum, row * h);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if constexpr (STAGES > 0) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) load_weight<DT, VEC>(p.weight, p.weight_type == kDtFp32, v, t, threads, h, w + 8 * v);
+        for (int i = 0; i < STAGES; ++i) copy(first + i * step, i);
+    }
+    Raw16<WT> w;  // as it lies in memory: sixteen values in two halves
 #pragma unroll
-    for (int i = 0; i < NV * 8; ++i) acc[i] = 0.f;
+    for (int i = 0; i < 2; ++i) {
+        Pair f[4];
+        load_half<WT, VEC>(p.weight, 0, i, t, threads, h, f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) narrow2<WT>(w, 4 * i + j, f[j]);
+    }
+    Pair acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = 0ull;
+    int stage = 0, turn = 0;
     for (int64_t row = first; row < p.rows; row += step) {
         const int64_t row0 = row * h;
-        float dy[NV * 8], hat[NV * 8], ds[NV * 8];
-#pragma unroll
-        for (int v = 0; v < NV; ++v) load_piece<DT, VEC>(p.dy, row0, v, t, threads, h, dy + 8 * v);
-        if (sum32) {
-#pragma unroll
-            for (int v = 0; v < NV; ++v) load_piece<kDtFp32, VEC>(p.sum, row0, v, t, threads, h, hat + 8 * v);
-        } else {
-#pragma unroll
-            for (int v = 0; v < NV; ++v) load_piece<DT, VEC>(p.sum, row0, v, t, threads, h, hat + 8 * v);
-        }
-        if (p.dsum == nullptr) {
-#pragma unroll
-            for (int i = 0; i < NV * 8; ++i) ds[i] = 0.f;
-        } else if (sum32) {
-#pragma unroll
-            for (int v = 0; v < NV; ++v) load_piece<kDtFp32, VEC>(p.dsum, row0, v, t, threads, h, ds + 8 * v);
-        } else {
-#pragma unroll
-            for (int v = 0; v < NV; ++v) load_piece<DT, VEC>(p.dsum, row0, v, t, threads, h, ds + 8 * v);
-        }
         const float rstd = __ldg(p.rstd + row);
-        float along = 0.f, none = 0.f;
+        const Pair rstd2 = pair(rstd, rstd);
+        const uint32_t at_dy = slots + stage * stage_bytes, at_s = at_dy + 2 * kCopies<DT> * threads * 16, at_ds = at_s + 2 * kCopies<ST> * threads * 16;
+        Pair dy[8], s[8];
+        if constexpr (STAGES > 0) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES > 0 ? STAGES - 1 : 0) : "memory");
+            if (DT == kDtFp32 || ST == kDtFp32) __syncwarp();
+        } else {
 #pragma unroll
-        for (int i = 0; i < NV * 8; ++i) {
-            hat[i] *= rstd;
-            acc[i] = fmaf(dy[i], hat[i], acc[i]);
-            dy[i] *= w[i];
-            along = fmaf(dy[i], hat[i], along);
-        }
-        over_row<WARP, false>(along, none, red);
-        along /= static_cast<float>(h);
-#pragma unroll
-        for (int i = 0; i < NV * 8; ++i) ds[i] = fmaf(rstd, fmaf(-along, hat[i], dy[i]), ds[i]);
-        if (p.dx != nullptr) {
-#pragma unroll
-            for (int v = 0; v < NV; ++v) store_piece<DT, VEC>(p.dx, row0, v, t, threads, h, ds + 8 * v);
-        }
-        if (p.dres != nullptr) {
-            if (sum32) {
-#pragma unroll
-                for (int v = 0; v < NV; ++v) store_piece<kDtFp32, VEC>(p.dres, row0, v, t, threads, h, ds + 8 * v);
-            } else {
-#pragma unroll
-                for (int v = 0; v < NV; ++v) store_piece<DT, VEC>(p.dres, row0, v, t, threads, h, ds + 8 * v);
+            for (int i = 0; i < 2; ++i) {
+                load_half<DT, VEC>(p.dy, row0, i, t, threads, h, dy + 4 * i);
+                load_half<ST, VEC>(p.sum, row0, i, t, threads, h, s + 4 * i);
             }
+        }
+        Pair products = 0ull;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            Pair* g = dy + 4 * i;
+            Pair* hat = s + 4 * i;
+            if constexpr (STAGES > 0) {
+                ring_half<DT>(at_dy, i, threads, t, h, g);
+                ring_half<ST>(at_s, i, threads, t, h, hat);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                hat[j] = mul2(hat[j], rstd2);
+                acc[4 * i + j] = fma2(g[j], hat[j], acc[4 * i + j]);
+                g[j] = mul2(g[j], widen2<WT>(w, 4 * i + j));
+                products = fma2(g[j], hat[j], products);
+            }
+        }
+        const float2 sides = split(products);
+        float along = sides.x + sides.y, none = 0.f;
+        over_row<WARP, false>(along, none, red + turn * 64);
+        turn ^= 1;
+        const float share = -along / static_cast<float>(h);
+        const Pair share2 = pair(share, share);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            Pair* g = dy + 4 * i;
+            Pair* hat = s + 4 * i;
+            Pair d[4] = {0ull, 0ull, 0ull, 0ull};
+            if constexpr (STAGES > 0) {
+                ring_half<DT>(at_dy, i, threads, t, h, g);
+                ring_half<ST>(at_s, i, threads, t, h, hat);
+                if (p.dsum != nullptr) ring_half<ST>(at_ds, i, threads, t, h, d);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    hat[j] = mul2(hat[j], rstd2);
+                    g[j] = mul2(g[j], widen2<WT>(w, 4 * i + j));
+                }
+            } else {
+                if (p.dsum != nullptr) load_half<ST, VEC>(p.dsum, row0, i, t, threads, h, d);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[j] = fma2(rstd2, fma2(share2, hat[j], g[j]), d[j]);
+            if (p.dx != nullptr) store_half<DT, VEC>(p.dx, row0, i, t, threads, h, d);
+            if (p.dres != nullptr) store_half<ST, VEC>(p.dres, row0, i, t, threads, h, d);
+        }
+        if constexpr (STAGES > 0) {
+            if (DT == kDtFp32 || ST == kDtFp32) __syncwarp();
+            copy(row + STAGES * step, stage);
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
     }
     if (p.partial == nullptr) return;
     float* mine = p.partial + static_cast<int64_t>(blockIdx.x) * h;
     if constexpr (WARP) {
+        // all rings have been read: the memory takes the warps' sums
+        float* cols = reinterpret_cast<float*>(dynamic);
+        if (STAGES > 0) asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int c = place<VEC>(v, j, t, threads);
-                if (c < h) cols[warp * NV * 256 + c] = acc[8 * v + j];
-            }
+        for (int j = 0; j < 16; ++j) {
+            const int c = half_column<VEC>(j / 8, j % 8, t, threads);
+            const float2 f = split(acc[j / 2]);
+            if (c < h) cols[warp * h + c] = j % 2 ? f.y : f.x;
         }
         __syncthreads();
         for (int c = threadIdx.x; c < h; c += blockDim.x) {
             float a = 0.f;
 #pragma unroll
-            for (int r = 0; r < kWarpRows; ++r) a += cols[r * NV * 256 + c];
+            for (int r = 0; r < kWarpRows; ++r) a += cols[r * h + c];
             mine[c] = a;
         }
     } else {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) store_piece<kDtFp32, VEC>(mine, 0, v, t, threads, h, acc + 8 * v);
+        store_half<kDtFp32, VEC>(mine, 0, 0, t, threads, h, acc);
+        store_half<kDtFp32, VEC>(mine, 0, 1, t, threads, h, acc + 4);
     }
 }
 
-// dw[c] = sum over the parts: 32 columns and 8 shares of the parts per block
+// dw[c] = sum over the parts: 32 columns and 32 shares of the parts per block
 template <int DT>
-__global__ void __launch_bounds__(256) add_parts_kernel(const float* __restrict__ partial, int parts, int h, void* dw) {
-    __shared__ float red[8][33];
+__global__ void __launch_bounds__(1024) add_parts_kernel(const float* __restrict__ partial, int parts, int h, void* dw) {
+    __shared__ float red[32][33];
     const int lane = threadIdx.x & 31, share = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     pdl_wait();
     pdl_release();
     float a = 0.f;
     if (c < h) {
 #pragma unroll 8
-        for (int i = share; i < parts; i += 8) a += __ldg(partial + static_cast<int64_t>(i) * h + c);
+        for (int i = share; i < parts; i += 32) a += __ldg(partial + static_cast<int64_t>(i) * h + c);
     }
     red[share][lane] = a;
     __syncthreads();
-    if (share == 0 && c < h) {
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += red[i][lane];
-        store1<DT>(dw, c, sum);
-    }
+    // a warp per column: the shares in a tree
+    const float sum = warp_sum(red[lane][share]);
+    const int col = blockIdx.x * 32 + share;
+    if (lane == 0 && col < h) store1<DT>(dw, col, sum);
 }
 
-// Threads that share a row and pieces of eight values per thread
+// ------------------------------------------------------------------------------------------------
+// Launches
+// ------------------------------------------------------------------------------------------------
+// Threads that share a row and sixteens of values per thread.  They follow from the width alone: a row's sums are added in the same
+// order however many rows there are.
 struct Shape {
     bool warp;
-    int threads, pieces;
+    int threads, sixteens;
 };
 
-Shape shape_of(int h, int warp_pieces, int block_pieces) {
-    const int pieces = (h + 7) / 8;
-    if (pieces <= 32 * warp_pieces) {
-        const int per = (pieces + 31) / 32;
-        return {true, kWarpRows * 32, per <= 1 ? 1 : per <= 2 ? 2 : 4};
-    }
-    const int threads = ((pieces + block_pieces - 1) / block_pieces + 31) / 32 * 32;
-    return {false, threads, block_pieces};
+Shape shape_of(int h, int most) {
+    const int pieces = (h + 15) / 16;
+    if (pieces <= 32 * most) return {true, kWarpRows * 32, pieces <= 32 ? 1 : 2};
+    return {false, ((pieces + most - 1) / most + 31) / 32 * 32, most};
+}
+static_assert(kWarpRows * 32 == 256 && 512 * 2 * 16 >= kNormMaxHidden, "every row has its threads");
+
+int64_t turns_of(const Shape& s, int64_t rows) { return s.warp ? (rows + kWarpRows - 1) / kWarpRows : rows; }
+
+bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
+
+template <int DT, int MODE, int VEC>
+int launch_norm(const RmsNormParams& p, cudaStream_t stream) {
+    const Shape s = shape_of(p.h, 2);
+    const dim3 grid(static_cast<unsigned>(turns_of(s, p.rows)));
+    if (!s.warp) return launch_pdl(rms_norm_kernel<DT, MODE, 2, VEC, false>, grid, s.threads, 0, stream, p);
+    return s.sixteens == 1 ? launch_pdl(rms_norm_kernel<DT, MODE, 1, VEC, true>, grid, s.threads, 0, stream, p) : launch_pdl(rms_norm_kernel<DT, MODE, 2, VEC, true>, grid, s.threads, 0, stream, p);
 }
 
-template <int DT, int MODE, int NV, bool VEC>
-int launch_norm(const RmsNormParams& p, const Shape& s, cudaStream_t stream) {
-    if (s.warp)
-        return launch_pdl(rms_norm_kernel<DT, MODE, NV, VEC, true>, dim3(static_cast<unsigned>((p.rows + kWarpRows - 1) / kWarpRows)), s.threads, 0, stream, p);
-    if constexpr (NV >= 2) return launch_pdl(rms_norm_kernel<DT, MODE, NV, VEC, false>, dim3(static_cast<unsigned>(p.rows)), s.threads, 0, stream, p);
-    return static_cast<int>(cudaErrorInvalidValue);
-}
-
-template <int DT, int MODE, bool VEC>
-int launch_norm_pieces(const RmsNormParams& p, cudaStream_t stream) {
-    const Shape s = shape_of(p.h, 4, p.h > 8192 ? 2 : 4);
-    if (s.pieces == 1) return launch_norm<DT, MODE, 1, VEC>(p, s, stream);
-    if (s.pieces == 2) return launch_norm<DT, MODE, 2, VEC>(p, s, stream);
-    return launch_norm<DT, MODE, 4, VEC>(p, s, stream);
+// How all operands of a launch can be read
+template <class... Pointers>
+int access_of(int h, Pointers... ps) {
+    if (h % 16 == 0 && (aligned32(ps) && ...)) return kBy32;
+    return h % 8 == 0 && (aligned16(ps) && ...) ? kBy16 : kByOne;
 }
 
 template <int DT>
 int launch_norm_type(const RmsNormParams& p, cudaStream_t stream) {
-    const bool vec = p.h % 8 == 0 && aligned16(p.x) && aligned16(p.residual) && aligned16(p.weight) && aligned16(p.y) && aligned16(p.sum) && aligned16(p.q);
-    if (p.quant_mode == 0) return vec ? launch_norm_pieces<DT, kRowsOnly, true>(p, stream) : launch_norm_pieces<DT, kRowsOnly, false>(p, stream);
-    if (p.quant_mode == 2) return vec ? launch_norm_pieces<DT, kInt8, true>(p, stream) : launch_norm_pieces<DT, kInt8, false>(p, stream);
-    return vec && p.h % 128 == 0 ? launch_norm_pieces<DT, kE4m3, true>(p, stream) : static_cast<int>(cudaErrorInvalidValue);
+    const int access = access_of(p.h, p.x, p.residual, p.weight, p.y, p.sum, p.q);
+    if (p.quant_mode == 0)
+        return access == kBy32 ? launch_norm<DT, kRowsOnly, kBy32>(p, stream) : access == kBy16 ? launch_norm<DT, kRowsOnly, kBy16>(p, stream) : launch_norm<DT, kRowsOnly, kByOne>(p, stream);
+    if (p.quant_mode == 2)
+        return access == kBy32 ? launch_norm<DT, kInt8, kBy32>(p, stream) : access == kBy16 ? launch_norm<DT, kInt8, kBy16>(p, stream) : launch_norm<DT, kInt8, kByOne>(p, stream);
+    if (access == kByOne || p.h % 128 != 0) return static_cast<int>(cudaErrorInvalidValue);
+    return access == kBy32 ? launch_norm<DT, kE4m3, kBy32>(p, stream) : launch_norm<DT, kE4m3, kBy16>(p, stream);
 }
 
-Shape backward_shape(int h) { return shape_of(h, 2, 2); }
+// A launch of the backward pass
+struct Backward {
+    Shape shape;
+    int blocks;                     // of an SM
+    int stages, stage_bytes, smem;  // stages: 0 without a ring
+};
 
-template <int DT, int NV, bool VEC>
-int launch_backward(const RmsNormBackwardParams& p, const Shape& s, cudaStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(p.parts));
-    if (s.warp) return launch_pdl(rms_norm_backward_kernel<DT, NV, VEC, true, kWarpRows * 32>, grid, s.threads, 0, stream, p);
-    if constexpr (NV == 2) {
-        if (s.threads <= 512) return launch_pdl(rms_norm_backward_kernel<DT, 2, VEC, false, 512>, grid, s.threads, 0, stream, p);
-        return launch_pdl(rms_norm_backward_kernel<DT, 2, VEC, false, 1024>, grid, s.threads, 0, stream, p);
-    }
-    return static_cast<int>(cudaErrorInvalidValue);
+int blocks_by_registers(const Shape& s, int registers) { return s.threads > 512 ? 1 : 65536 / (registers * s.threads); }
+
+Backward backward_of(const RmsNormBackwardParams& p, int dtype, bool ring) {
+    Backward r{shape_of(p.h, 1), 0, 0, 0, 0};
+    const int group = r.shape.warp ? 32 : r.shape.threads, groups = r.shape.threads / group;
+    const int size = dtype == kDtFp32 ? 4 : 2, sum = p.sum_type == kDtFp32 ? 4 : size, copies = size + sum + (p.dsum != nullptr ? sum : 0);
+    const int sums = r.shape.warp ? kWarpRows * p.h * 4 : 0, room = 220 * 1024;
+    const Backward plain{r.shape, blocks_by_registers(r.shape, 128), 0, 0, sums};
+    r.blocks = blocks_by_registers(r.shape, sum == 2 ? 64 : 96);
+    // below two turns of all blocks there is nothing to load ahead
+    if (!ring || turns_of(r.shape, p.rows) <= 2 * static_cast<int64_t>(r.blocks) * sm_count_of_current_device()) return plain;
+    r.stage_bytes = group * 16 * copies;
+    const int per_stage = r.stage_bytes * groups;
+    // all blocks with four stages, or as many as fit with two
+    r.stages = r.blocks * (4 * per_stage + 1024) <= room ? 4 : 2;
+    r.smem = r.stages * per_stage > sums ? r.stages * per_stage : sums;
+    const int fit = room / (r.smem + 1024);
+    if (fit < 1) return plain;
+    r.blocks = r.blocks < fit ? r.blocks : fit;
+    return r;
+}
+
+template <int DT, int ST, int WT, int VEC, bool WARP, int THREADS, int STAGES>
+int launch_backward_kernel(const RmsNormBackwardParams& p, const Backward& r, cudaStream_t stream) {
+    static SmemLimitCache limit;
+    auto kernel = rms_norm_backward_kernel<DT, ST, WT, VEC, WARP, THREADS, STAGES>;
+    const cudaError_t err = limit.ensure(kernel, r.smem);
+    if (err != cudaSuccess) return static_cast<int>(err);
+    return launch_pdl(kernel, dim3(static_cast<unsigned>(p.parts)), r.shape.threads, static_cast<size_t>(r.smem), stream, p, static_cast<uint32_t>(r.stage_bytes));
+}
+
+template <int DT, int ST, int WT, int VEC, int STAGES>
+int launch_backward(const RmsNormBackwardParams& p, const Backward& r, cudaStream_t stream) {
+    if (r.shape.warp) return launch_backward_kernel<DT, ST, WT, VEC, true, 256, STAGES>(p, r, stream);
+    return r.shape.threads <= 512 ? launch_backward_kernel<DT, ST, WT, VEC, false, 512, STAGES>(p, r, stream) : launch_backward_kernel<DT, ST, WT, VEC, false, 1024, STAGES>(p, r, stream);
+}
+
+template <int DT, int ST, int WT>
+int launch_backward_types(RmsNormBackwardParams p, cudaStream_t stream) {
+    int access = access_of(p.h, p.dy, p.dsum, p.sum, p.weight, p.dx, p.dres, p.partial);
+    // fp32 goes by 32 bytes
+    const bool all32 = aligned32(p.dy) && aligned32(p.dsum) && aligned32(p.sum) && aligned32(p.weight) && aligned32(p.dx) && aligned32(p.dres) && aligned32(p.partial);
+    if (!all32 && (DT == kDtFp32 || ST == kDtFp32 || WT == kDtFp32 || !aligned32(p.partial))) access = kByOne;
+    const Backward r = backward_of(p, DT, access != kByOne);
+    const int64_t blocks = static_cast<int64_t>(r.blocks) * sm_count_of_current_device();
+    p.parts = static_cast<int>(p.parts < blocks ? p.parts : blocks);
+    const int rc = access == kByOne  ? launch_backward<DT, ST, WT, kByOne, 0>(p, r, stream)
+                   : r.stages == 4   ? launch_backward<DT, ST, WT, kBy16, 4>(p, r, stream)
+                   : r.stages == 2   ? launch_backward<DT, ST, WT, kBy16, 2>(p, r, stream)
+                                     : launch_backward<DT, ST, WT, kBy16, 0>(p, r, stream);
+    if (rc != 0 || p.dweight == nullptr) return rc;
+    return launch_pdl(add_parts_kernel<WT>, dim3(static_cast<unsigned>((p.h + 31) / 32)), 1024, 0, stream, static_cast<const float*>(p.partial), p.parts, p.h, p.dweight);
 }
 
 template <int DT>
 int launch_backward_type(const RmsNormBackwardParams& p, cudaStream_t stream) {
-    const bool vec = p.h % 8 == 0 && aligned16(p.dy) && aligned16(p.dsum) && aligned16(p.sum) && aligned16(p.weight) && aligned16(p.dx) &&
-                     aligned16(p.dres) && aligned16(p.partial);
-    const Shape s = backward_shape(p.h);
-    int rc;
-    if (s.pieces == 1) rc = vec ? launch_backward<DT, 1, true>(p, s, stream) : launch_backward<DT, 1, false>(p, s, stream);
-    else rc = vec ? launch_backward<DT, 2, true>(p, s, stream) : launch_backward<DT, 2, false>(p, s, stream);
-    if (rc != 0 || p.dweight == nullptr) return rc;
-    auto add = p.weight_type == kDtFp32 ? add_parts_kernel<kDtFp32> : p.weight_type == kDtFp16 ? add_parts_kernel<kDtFp16> : add_parts_kernel<kDtBf16>;
-    return launch_pdl(add, dim3(static_cast<unsigned>((p.h + 31) / 32)), 256, 0, stream, static_cast<const float*>(p.partial), p.parts, p.h, p.dweight);
+    if (DT == kDtFp32) return launch_backward_types<kDtFp32, kDtFp32, kDtFp32>(p, stream);
+    if (p.sum_type == kDtFp32)
+        return p.weight_type == kDtFp32 ? launch_backward_types<DT, kDtFp32, kDtFp32>(p, stream) : launch_backward_types<DT, kDtFp32, DT>(p, stream);
+    return p.weight_type == kDtFp32 ? launch_backward_types<DT, DT, kDtFp32>(p, stream) : launch_backward_types<DT, DT, DT>(p, stream);
 }
 
 }  // namespace
@@ -395,11 +761,11 @@ extern "C" int cam_launch_rms_norm(const cam::RmsNormParams* p, int dtype, cudaS
     return dtype == kDtBf16 ? launch_norm_type<kDtBf16>(*p, stream) : dtype == kDtFp16 ? launch_norm_type<kDtFp16>(*p, stream) : launch_norm_type<kDtFp32>(*p, stream);
 }
 
+// Most blocks that a launch for these rows has
 extern "C" int cam_rms_norm_backward_blocks(int64_t rows, int h) {
     using namespace cam;
-    const Shape s = backward_shape(h);
-    const int64_t turns = s.warp ? (rows + kWarpRows - 1) / kWarpRows : rows;
-    const int64_t most = static_cast<int64_t>(sm_count_of_current_device()) * (s.threads <= 512 ? 2 : 1);
+    const Shape s = shape_of(h, 1);
+    const int64_t turns = turns_of(s, rows), most = static_cast<int64_t>(sm_count_of_current_device()) * blocks_by_registers(s, 64);
     return static_cast<int>(turns < most ? turns : most);
 }
 
