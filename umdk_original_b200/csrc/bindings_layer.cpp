@@ -270,10 +270,9 @@ Two moe_ungroup_rows_backward_cuda(const at::Tensor& dout, const at::Tensor& row
     const auto floats = rows.options().dtype(at::kFloat);
     at::Tensor drows = need_drows ? at::empty_like(rows) : none_of(rows);
     at::Tensor dw = need_dweights ? at::empty({p.tokens, p.k}, floats) : at::empty({0}, floats);
-    at::Tensor used = drows.numel() > 0 ? at::zeros({p.num_rows}, rows.options().dtype(at::kByte)) : at::Tensor();
     CAM_RT(cam_moe_ungroup_rows_backward(data_or_null(dout), data_or_null(rows), p.dtype, p.num_rows, p.h, static_cast<const int*>(data_or_null(slots)),
                                          p.tokens, p.k, given(weights) ? floats_or_null(*weights) : nullptr, data_or_null(drows), floats_or_null(dw),
-                                         static_cast<unsigned char*>(data_or_null(used)), stream_now()));
+                                         stream_now()));
     return {drows, dw};
 }
 

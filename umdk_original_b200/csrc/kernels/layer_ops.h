@@ -81,7 +81,6 @@ struct UngroupRowsParams {
     const void* residual;   // [tokens, h] or null
     void* out;              // [tokens, h]
     const void* dout;       // backward
-    uint8_t* used;          // [num_rows], zeroed by the caller
     void* drows;            // [num_rows, h] or null
     float* dweights;        // [tokens, k] or null
 };

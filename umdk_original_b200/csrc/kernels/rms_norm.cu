@@ -20,36 +20,8 @@ constexpr int kRowsOnly = 0, kInt8 = 2, kE4m3 = 3;
 constexpr int kWarpRows = 8;  // rows of a block where a row belongs to a warp
 
 // ------------------------------------------------------------------------------------------------
-// Pairs of fp32 values, sixteen values as they lie in memory
+// Sixteen values as they lie in memory
 // ------------------------------------------------------------------------------------------------
-using Pair = unsigned long long;
-
-__device__ __forceinline__ Pair pair(float a, float b) {
-    Pair r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 split(Pair v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-    Pair r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-    Pair r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
 template <int DT>
 constexpr int kWords = DT == kDtFp32 ? 16 : 8;  // 32-bit words of sixteen values
 
@@ -97,14 +69,6 @@ __device__ __forceinline__ Raw16<DT> add16(const Raw16<DT>& x, const Raw16<DT>& 
         }
     }
     return s;
-}
-
-__device__ __forceinline__ void load32(uint32_t* v, const void* p) {
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "l"(p));
-}
-__device__ __forceinline__ void store32(void* p, const uint32_t* v) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
 // How rows can be read: 32 bytes at a time, 16 (rows of a multiple of 8 values), or one value (odd widths, any alignment)
@@ -654,8 +618,6 @@ Shape shape_of(int h, int most) {
 static_assert(kWarpRows * 32 == 256 && 512 * 2 * 16 >= kNormMaxHidden, "every row has its threads");
 
 int64_t turns_of(const Shape& s, int64_t rows) { return s.warp ? (rows + kWarpRows - 1) / kWarpRows : rows; }
-
-bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 
 template <int DT, int MODE, int VEC>
 int launch_norm(const RmsNormParams& p, cudaStream_t stream) {

@@ -216,10 +216,9 @@ extern "C" int cam_moe_ungroup_rows(const void* rows, int dtype, int64_t num_row
 
 extern "C" int cam_moe_ungroup_rows_backward(const void* dout, const void* rows, int dtype, int64_t num_rows, int h, const int* slots,
                                              int64_t tokens, int k, const float* weights, void* drows, float* dweights,
-                                             unsigned char* used, cudaStream_t stream) {
+                                             cudaStream_t stream) {
     if (check_ungroup("moe_ungroup_rows_backward", dtype, num_rows, h, tokens, k) != 0) return -1;
     LAYER_CHECK(tokens == 0 || (dout && slots), "moe_ungroup_rows_backward: null operand");
-    LAYER_CHECK(drows == nullptr || used != nullptr, "moe_ungroup_rows_backward: no workspace");
     LAYER_CHECK(dweights == nullptr || rows != nullptr || num_rows == 0, "moe_ungroup_rows_backward: null rows");
     if (drows == nullptr && dweights == nullptr) return 0;
     cam::UngroupRowsParams p{};
@@ -231,7 +230,6 @@ extern "C" int cam_moe_ungroup_rows_backward(const void* dout, const void* rows,
     p.k = k;
     p.weights = weights;
     p.dout = dout;
-    p.used = used;
     p.drows = drows;
     p.dweights = dweights;
     return launched(cam_launch_ungroup_rows_backward(&p, dtype, stream), "moe_ungroup_rows_backward");
