@@ -24,7 +24,8 @@ def randn(g, *shape, dtype=torch.float32, scale=1.0):
 # ------------------------------------------------------------------------------------------------
 # Norm
 # ------------------------------------------------------------------------------------------------
-# widths on both sides of the kernel's borders: 256, 512, 1024 (warps with 1, 2, 4 pieces), 8192 (four or two pieces per thread), 16384
+# widths on both sides of the kernels' borders: 512 and 1024 (a warp with one or two sixteens, a block), 8192 (blocks of 512 threads
+# backward), and of multiples of 8 and 16
 WIDTHS = [1, 7, 8, 64, 255, 256, 264, 512, 520, 1000, 1024, 1032, 1023, 2056, 4096, 7168, 8192, 8200, 16383, 16384]
 
 

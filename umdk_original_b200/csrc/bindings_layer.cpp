@@ -50,12 +50,13 @@ NormProblem check_norm(const char* op, const at::Tensor& x, const OptTensor& res
     return p;
 }
 
-// y, sum (empty without a residual), rstd (empty unless kept)
+// y, sum (undefined without a residual), rstd (undefined unless kept)
 Three norm_forward(const char* op, const at::Tensor& x, const OptTensor& residual, const at::Tensor& weight, double eps, bool keep) {
     const NormProblem p = check_norm(op, x, residual, weight, eps);
     c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor y = at::empty_like(x), sum = given(residual) ? at::empty_like(*residual) : none_of(x);
-    at::Tensor rstd = at::empty({keep ? p.rows : 0}, x.options().dtype(at::kFloat));
+    at::Tensor y = at::empty_like(x), sum, rstd;
+    if (given(residual)) sum = at::empty_like(*residual);
+    if (keep) rstd = at::empty({p.rows}, x.options().dtype(at::kFloat));
     if (p.rows == 0) return {y, sum, rstd};
     CAM_RT(cam_rms_norm(x.data_ptr(), p.dtype, given(residual) ? residual->data_ptr() : nullptr, p.res_type, weight.data_ptr(), p.weight_type, p.rows,
                         p.h, static_cast<float>(eps), y.data_ptr(), data_or_null(sum), floats_or_null(rstd), 0, nullptr, nullptr, stream_now()));
@@ -70,7 +71,9 @@ Two add_rms_norm_cuda(const at::Tensor& x, const at::Tensor& residual, const at:
     return {y, sum};
 }
 Three rms_norm_train_cuda(const at::Tensor& x, const OptTensor& residual, const at::Tensor& weight, double eps) {
-    return norm_forward("rms_norm_train", x, residual, weight, eps, true);
+    auto out = norm_forward("rms_norm_train", x, residual, weight, eps, true);
+    if (!std::get<1>(out).defined()) std::get<1>(out) = none_of(x);
+    return out;
 }
 
 // dx (of dy's type), dresidual (of the sum's type, empty where that is dx's: then they are the same numbers), dweight
@@ -214,7 +217,7 @@ Four moe_group_rows_cuda(const at::Tensor& x, const at::Tensor& topk_idx, int64_
     at::Tensor rows = at::empty({t * k, x.size(1)}, x.options());
     const auto ints = x.options().dtype(at::kInt);
     at::Tensor offsets = at::empty({num_experts + 1}, ints), slots = at::empty({t, k}, ints);
-    CAM_RT(cam_moe_group_rows(data_or_null(x), x.size(1) * x.element_size(), given(scales) ? floats_or_null(*scales) : nullptr, static_cast<int>(cols),
+    CAM_RT(cam_moe_group_rows(data_or_null(x), x.size(1) * x.element_size(), static_cast<int>(x.element_size()), given(scales) ? floats_or_null(*scales) : nullptr, static_cast<int>(cols),
                               data_or_null(topk_idx), topk_idx.scalar_type() == at::kLong, t, static_cast<int>(k), static_cast<int>(num_experts),
                               data_or_null(rows), floats_or_null(row_scales), offsets.data_ptr<int>(), static_cast<int*>(data_or_null(slots)), stream_now()));
     return {rows, row_scales, offsets, slots};

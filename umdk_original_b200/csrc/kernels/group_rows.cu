@@ -145,53 +145,80 @@ __global__ void __launch_bounds__(kSortThreads) sort_pairs_kernel(const GroupRow
     if (blocks > 1) cluster.sync();  // nobody leaves while its totals are read
 }
 
+// How rows are copied: in pieces of 16 bytes, or (ES: bytes of an element) where they start anywhere, in the pieces of each destination row
+constexpr int kPieces16 = 0;
+
+template <int ES>
+__device__ __host__ __forceinline__ int64_t pieces_of(int64_t row_bytes) { return ES == kPieces16 ? row_bytes / 16 : (row_bytes + 15 + 15) / 16; }
+
 // Items of a token: the pieces of its row, then its scales
-template <class Unit>
-__device__ __forceinline__ void copy_item(const GroupRowsParams& p, int64_t token, int64_t c, int64_t units, const int* slot) {
-    if (c < units) {
-        const Unit v = __ldg(static_cast<const Unit*>(p.x) + token * units + c);
-        Unit* rows = static_cast<Unit*>(p.rows);
+template <int ES>
+__device__ __forceinline__ void copy_item(const GroupRowsParams& p, int64_t token, int64_t c, int64_t pieces, const int* slot) {
+    if (c < pieces) {
+        const char* x = static_cast<const char*>(p.x);
+        char* rows = static_cast<char*>(p.rows);
+        if constexpr (ES == kPieces16) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(x) + token * pieces + c);
 #pragma unroll 8
-        for (int j = 0; j < p.k; ++j) {
-            const int s = slot[j];
-            if (s >= 0) rows[s * units + c] = v;
+            for (int j = 0; j < p.k; ++j) {
+                const int s = slot[j];
+                if (s >= 0) reinterpret_cast<uint4*>(rows)[s * pieces + c] = v;
+            }
+        } else {
+            const char* hi = x + p.tokens * p.row_bytes;
+#pragma unroll 4
+            for (int j = 0; j < p.k; ++j) {
+                const int s = slot[j];
+                if (s < 0) continue;
+                char* row = rows + s * p.row_bytes;
+                const int64_t at = c * 16 - static_cast<int64_t>(reinterpret_cast<uintptr_t>(row) & 15u);  // in the row
+                if (at >= p.row_bytes || at <= -16) continue;
+                const uint4 v = load_window(x + token * p.row_bytes + at, x, hi);
+                if (at >= 0 && at + 16 <= p.row_bytes) *reinterpret_cast<uint4*>(row + at) = v;
+                else store_some<ES>(row + at, v, at < 0 ? static_cast<int>(-at) / ES : 0, p.row_bytes - at < 16 ? static_cast<int>(p.row_bytes - at) / ES : 16 / ES);
+            }
         }
     } else {
-        const float v = __ldg(p.scales + token * p.scale_cols + (c - units));
+        const float v = __ldg(p.scales + token * p.scale_cols + (c - pieces));
         for (int j = 0; j < p.k; ++j) {
             const int s = slot[j];
-            if (s >= 0) p.row_scales[static_cast<int64_t>(s) * p.scale_cols + (c - units)] = v;
+            if (s >= 0) p.row_scales[static_cast<int64_t>(s) * p.scale_cols + (c - pieces)] = v;
         }
     }
 }
 
 // Zeros to the rows (and scales) of no expert
-template <class Unit>
-__device__ __forceinline__ void clear_tail(const GroupRowsParams& p, int64_t from, int64_t units, int64_t first, int64_t step) {
-    const int64_t pairs = p.tokens * p.k;
-    for (int64_t i = from * units + first; i < pairs * units; i += step) static_cast<Unit*>(p.rows)[i] = Unit{};
+template <int ES>
+__device__ __forceinline__ void clear_tail(const GroupRowsParams& p, int64_t from, int64_t first, int64_t step) {
+    const int64_t pairs = p.tokens * p.k, begin = from * p.row_bytes, end = pairs * p.row_bytes;
+    char* rows = static_cast<char*>(p.rows);  // 16-byte aligned
+    for (int64_t i = begin / 16 + first; i * 16 < end; i += step) {
+        if (i * 16 >= begin && i * 16 + 16 <= end) *reinterpret_cast<uint4*>(rows + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        else if constexpr (ES != kPieces16)
+            store_some<ES>(rows + i * 16, make_uint4(0u, 0u, 0u, 0u), begin > i * 16 ? static_cast<int>(begin - i * 16) / ES : 0, end - i * 16 < 16 ? static_cast<int>(end - i * 16) / ES : 16 / ES);
+    }
     for (int64_t i = from * p.scale_cols + first; i < pairs * p.scale_cols; i += step) p.row_scales[i] = 0.f;
 }
 
 // The sorted pairs' rows.  The first blocks write zeros to the rows of no expert.
-template <class Unit, class Index>
+template <int ES, class Index>
 __global__ void __launch_bounds__(256) group_rows_kernel(const GroupRowsParams p, unsigned zero_blocks) {
-    const Index units = static_cast<Index>(p.row_bytes / sizeof(Unit)), items = units + static_cast<Index>(p.scale_cols);
+    const Index pieces = static_cast<Index>(pieces_of<ES>(p.row_bytes)), items = pieces + static_cast<Index>(p.scale_cols);
     pdl_wait();
     pdl_release();
     if (blockIdx.x < zero_blocks) {
-        clear_tail<Unit>(p, __ldg(p.offsets + p.experts), static_cast<int64_t>(units), static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, static_cast<int64_t>(zero_blocks) * 256);
+        clear_tail<ES>(p, __ldg(p.offsets + p.experts), static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, static_cast<int64_t>(zero_blocks) * 256);
         return;
     }
     const Index i = static_cast<Index>(blockIdx.x - zero_blocks) * 256 + threadIdx.x;
     if (i >= static_cast<Index>(p.tokens) * items) return;
     const Index token = i / items;
-    copy_item<Unit>(p, static_cast<int64_t>(token), static_cast<int64_t>(i - token * items), static_cast<int64_t>(units), p.slots + static_cast<int64_t>(token) * p.k);
+    copy_item<ES>(p, static_cast<int64_t>(token), static_cast<int64_t>(i - token * items), static_cast<int64_t>(pieces), p.slots + static_cast<int64_t>(token) * p.k);
 }
 
 // Few pairs, one launch: every block finds the places of its own token's pairs by comparing them with all ids, and `parts` blocks share the
 // token's row.  The place of a pair is the number of ids below its own, or equal to it and earlier.
-template <class Unit>
+template <int ES>
 __global__ void __launch_bounds__(256) group_few_rows_kernel(const GroupRowsParams p, unsigned parts) {
     __shared__ int counts[kLayerMaxTopk + 1];
     __shared__ uint16_t ids[kFewPairs];
@@ -241,28 +268,28 @@ __global__ void __launch_bounds__(256) group_few_rows_kernel(const GroupRowsPara
     }
     __syncthreads();
     if (part == 0 && static_cast<int>(threadIdx.x) < p.k) p.slots[token * p.k + threadIdx.x] = counts[threadIdx.x];
-    const int64_t units = p.row_bytes / static_cast<int64_t>(sizeof(Unit)), items = units + p.scale_cols;
-    for (int64_t c = part * 256 + threadIdx.x; c < items; c += parts * 256) copy_item<Unit>(p, token, c, units, counts);
+    const int64_t pieces = pieces_of<ES>(p.row_bytes), items = pieces + p.scale_cols;
+    for (int64_t c = part * 256 + threadIdx.x; c < items; c += parts * 256) copy_item<ES>(p, token, c, pieces, counts);
     if (counts[kLayerMaxTopk] < pairs)
-        clear_tail<Unit>(p, counts[kLayerMaxTopk], units, static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, static_cast<int64_t>(gridDim.x) * 256);
+        clear_tail<ES>(p, counts[kLayerMaxTopk], static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, static_cast<int64_t>(gridDim.x) * 256);
 }
 
-template <class Unit>
+template <int ES>
 int launch_copy(const GroupRowsParams& p, cudaStream_t stream) {
-    const int64_t items = p.row_bytes / static_cast<int64_t>(sizeof(Unit)) + p.scale_cols, blocks = (p.tokens * items + 255) / 256;
+    const int64_t items = pieces_of<ES>(p.row_bytes) + p.scale_cols, blocks = (p.tokens * items + 255) / 256;
     const int64_t zero = sm_count_of_current_device();
     if (blocks + zero > 0x7FFFFFFF) return static_cast<int>(cudaErrorInvalidValue);
     const dim3 grid(static_cast<unsigned>(blocks + zero));
-    if (blocks * 256 < 0x7FFFFFFF) return launch_pdl(group_rows_kernel<Unit, uint32_t>, grid, 256, 0, stream, p, static_cast<unsigned>(zero));
-    return launch_pdl(group_rows_kernel<Unit, uint64_t>, grid, 256, 0, stream, p, static_cast<unsigned>(zero));
+    if (blocks * 256 < 0x7FFFFFFF) return launch_pdl(group_rows_kernel<ES, uint32_t>, grid, 256, 0, stream, p, static_cast<unsigned>(zero));
+    return launch_pdl(group_rows_kernel<ES, uint64_t>, grid, 256, 0, stream, p, static_cast<unsigned>(zero));
 }
 
-template <class Unit>
+template <int ES>
 int launch_few(const GroupRowsParams& p, cudaStream_t stream) {
     // as many blocks per token as fill the SMs twice, of 256 items at least
-    const int64_t items = p.row_bytes / static_cast<int64_t>(sizeof(Unit)) + p.scale_cols, most = (items + 255) / 256;
+    const int64_t items = pieces_of<ES>(p.row_bytes) + p.scale_cols, most = (items + 255) / 256;
     const int64_t want = (2 * sm_count_of_current_device() + p.tokens - 1) / p.tokens, parts = want < most ? want : most;
-    return launch_pdl(group_few_rows_kernel<Unit>, dim3(static_cast<unsigned>(p.tokens * parts)), 256, 0, stream, p, static_cast<unsigned>(parts));
+    return launch_pdl(group_few_rows_kernel<ES>, dim3(static_cast<unsigned>(p.tokens * parts)), 256, 0, stream, p, static_cast<unsigned>(parts));
 }
 
 int launch_sort(const GroupRowsParams& p, cudaStream_t stream) {
@@ -286,36 +313,31 @@ int launch_sort(const GroupRowsParams& p, cudaStream_t stream) {
     return static_cast<int>(cudaLaunchKernelEx(&cfg, sort_pairs_kernel, p));
 }
 
-// Values of a row in pieces of B bytes: 32 (whole sectors per thread), 16, or one value
+// Values of a row in pieces of B bytes: 32 (whole sectors per thread) or 16
 template <int DT, int B>
 struct Piece {
     static constexpr int N = B / kBytes<DT>;
-    static constexpr int kWords = B >= 4 ? B / 4 : 1;
+    static constexpr int kWords = B / 4;
     uint32_t w[kWords];
     __device__ __forceinline__ void load(const void* base, int64_t i) {
         const char* p = static_cast<const char*>(base) + i * kBytes<DT>;
         if constexpr (B == 32) load32(w, p);
-        else if constexpr (B == 16) {
+        else {
             const uint4 v = load16_stream(p);
             w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-        } else {
-            w[0] = __float_as_uint(load1<DT>(base, i));
         }
     }
     __device__ __forceinline__ void store(void* base, int64_t i) const {
         char* p = static_cast<char*>(base) + i * kBytes<DT>;
         if constexpr (B == 32) store32(p, w);
-        else if constexpr (B == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-        else store1<DT>(base, i, __uint_as_float(w[0]));
+        else *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) w[i] = 0u;
     }
-    // one value: in the lower half, beside a zero
     __device__ __forceinline__ Pair get(int i) const {
-        if constexpr (N == 1) return pair(__uint_as_float(w[0]), 0.f);
-        else if constexpr (DT == kDtFp32) return pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        if constexpr (DT == kDtFp32) return pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
         else if constexpr (DT == kDtBf16) return pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
         else {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
@@ -324,8 +346,7 @@ struct Piece {
     }
     __device__ __forceinline__ void set(int i, Pair v) {
         const float2 f = split(v);
-        if constexpr (N == 1) w[0] = __float_as_uint(f.x);
-        else if constexpr (DT == kDtFp32) {
+        if constexpr (DT == kDtFp32) {
             w[2 * i] = __float_as_uint(f.x);
             w[2 * i + 1] = __float_as_uint(f.y);
         } else if constexpr (DT == kDtBf16) {
@@ -342,7 +363,7 @@ struct Piece {
 template <int DT, int B, int U, class Index>
 __global__ void __launch_bounds__(256) ungroup_rows_kernel(const UngroupRowsParams p) {
     using P = Piece<DT, B>;
-    constexpr int N = P::N, H = N > 1 ? N / 2 : 1;
+    constexpr int N = P::N, H = N / 2;
     const Index pieces = static_cast<Index>(p.h / N);
     pdl_wait();
     pdl_release();
@@ -382,6 +403,71 @@ __global__ void __launch_bounds__(256) ungroup_rows_kernel(const UngroupRowsPara
     out.store(p.out, to);
 }
 
+// A piece of sixteen bytes of a row that starts anywhere, as fp32 values
+template <int DT>
+__device__ __forceinline__ void widen_piece(const uint4& v, Pair* f) {
+    Piece<DT, 16> q;
+    q.w[0] = v.x, q.w[1] = v.y, q.w[2] = v.z, q.w[3] = v.w;
+#pragma unroll
+    for (int i = 0; i < Piece<DT, 16>::N / 2; ++i) f[i] = q.get(i);
+}
+template <int DT>
+__device__ __forceinline__ uint4 narrow_piece(const Pair* f) {
+    Piece<DT, 16> q;
+#pragma unroll
+    for (int i = 0; i < Piece<DT, 16>::N / 2; ++i) q.set(i, f[i]);
+    return make_uint4(q.w[0], q.w[1], q.w[2], q.w[3]);
+}
+
+// The same for rows of odd widths: pieces of the result's rows, the others' at whatever address those columns have
+template <int DT, class Index>
+__global__ void __launch_bounds__(256) ungroup_odd_rows_kernel(const UngroupRowsParams p) {
+    constexpr int N = 16 / kBytes<DT>, U = 4;
+    const Index pieces = static_cast<Index>((p.h + 2 * N - 2) / N);
+    pdl_wait();
+    pdl_release();
+    const Index i = static_cast<Index>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= static_cast<Index>(p.tokens) * pieces) return;
+    const Index token = i / pieces;
+    const int64_t bytes = static_cast<int64_t>(p.h) * kBytes<DT>, pair0 = static_cast<int64_t>(token) * p.k;
+    char* out = static_cast<char*>(p.out) + static_cast<int64_t>(token) * bytes;
+    const int64_t at = static_cast<int64_t>(i - token * pieces) * 16 - static_cast<int64_t>(reinterpret_cast<uintptr_t>(out) & 15u);  // in the row
+    if (at >= bytes || at <= -16) return;
+    const char* rows = static_cast<const char*>(p.rows);
+    Pair acc[N / 2];
+#pragma unroll
+    for (int v = 0; v < N / 2; ++v) acc[v] = 0ull;
+    for (int j0 = 0; j0 < p.k; j0 += U) {
+        uint4 row[U];
+        float w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = j0 + u < p.k ? __ldg(p.slots + pair0 + j0 + u) : -1;
+            const bool in = s >= 0 && s < p.num_rows;
+            w[u] = !in ? 0.f : p.weights != nullptr ? __ldg(p.weights + pair0 + j0 + u) : 1.f;
+            row[u] = in ? load_window(rows + s * bytes + at, rows, rows + p.num_rows * bytes) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const Pair w2 = pair(w[u], w[u]);
+            Pair f[N / 2];
+            widen_piece<DT>(row[u], f);
+#pragma unroll
+            for (int v = 0; v < N / 2; ++v) acc[v] = fma2(w2, f[v], acc[v]);
+        }
+    }
+    if (p.residual != nullptr) {
+        const char* r = static_cast<const char*>(p.residual);
+        Pair f[N / 2];
+        widen_piece<DT>(load_window(r + static_cast<int64_t>(token) * bytes + at, r, r + p.tokens * bytes), f);
+#pragma unroll
+        for (int v = 0; v < N / 2; ++v) acc[v] = add2(acc[v], f[v]);
+    }
+    const uint4 v = narrow_piece<DT>(acc);
+    if (at >= 0 && at + 16 <= bytes) *reinterpret_cast<uint4*>(out + at) = v;
+    else store_some<kBytes<DT>>(out + at, v, at < 0 ? static_cast<int>(-at) / kBytes<DT> : 0, bytes - at < 16 ? static_cast<int>(bytes - at) / kBytes<DT> : N);
+}
+
 // Sums of eight values over the lanes of a warp: lane 4 j has the sum of value j.  Values are halved between the lanes as they are added:
 // 9 exchanges instead of 40.
 __device__ __forceinline__ float warp_sums8(const float (&v)[8]) {
@@ -400,14 +486,17 @@ constexpr int kZeroRange = 4096;  // rows that a block looks after at a time: a 
 
 // Gradients of rows (weight x gradient of the token) and of weights (row . gradient of the token), a token per warp or block.  The first
 // `zero_blocks` write zeros to rows that no token uses: each marks its share of the rows by looking at all slots.
+constexpr int kOddRows = 0;  // B: rows that start anywhere, in pieces of sixteen bytes of each row
+
 template <int DT, int B, int U, bool WARP>
 __global__ void __launch_bounds__(256) ungroup_rows_backward_kernel(const UngroupRowsParams p, unsigned zero_blocks, int range) {
-    using P = Piece<DT, B>;
-    constexpr int N = P::N, H = N > 1 ? N / 2 : 1;
+    using P = Piece<DT, B == kOddRows ? 16 : B>;
+    constexpr int N = P::N, H = N / 2;
+    const int64_t bytes = static_cast<int64_t>(p.h) * kBytes<DT>;
     __shared__ float red[8][8];
     __shared__ uint32_t used[kZeroRange / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int t = WARP ? lane : threadIdx.x, threads = WARP ? 32 : blockDim.x, pieces = p.h / N;
+    const int t = WARP ? lane : threadIdx.x, threads = WARP ? 32 : blockDim.x, pieces = B == kOddRows ? (p.h + 2 * N - 2) / N : p.h / N;
     pdl_wait();
     pdl_release();
     if (blockIdx.x < zero_blocks) {
@@ -435,7 +524,11 @@ __global__ void __launch_bounds__(256) ungroup_rows_backward_kernel(const Ungrou
                 while (left != 0u) {
                     const int64_t row = from + i * 32 + __ffs(left) - 1;
                     left &= left - 1u;
-                    for (int c = lane; c < pieces; c += 32) none.store(p.drows, row * p.h + c * N);
+                    if constexpr (B == kOddRows) {
+                        for (int c = lane; c < p.h; c += 32) store1<DT>(p.drows, row * p.h + c, 0.f);
+                    } else {
+                        for (int c = lane; c < pieces; c += 32) none.store(p.drows, row * p.h + c * N);
+                    }
                 }
             }
             __syncthreads();
@@ -454,7 +547,51 @@ __global__ void __launch_bounds__(256) ungroup_rows_backward_kernel(const Ungrou
             slot[u] = s < p.num_rows ? s : -1;
             w[u] = slot[u] < 0 ? 0.f : p.weights != nullptr ? __ldg(p.weights + pair0 + j0 + u) : 1.f;
         }
-        for (int c = t; c < pieces; c += threads) {
+        if constexpr (B == kOddRows) {
+            const char* rows = static_cast<const char*>(p.rows);
+            const char* dout = static_cast<const char*>(p.dout);
+            // the pieces are those of the rows written, or of those read where none are written
+            const uintptr_t base = reinterpret_cast<uintptr_t>(p.drows != nullptr ? static_cast<const char*>(p.drows) : rows);
+            for (int c = t; c < pieces; c += threads) {
+                uint4 row[U];
+                int at[U];  // in the row; past it: nothing
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int64_t row0 = slot[u] * bytes;
+                    const int64_t place = static_cast<int64_t>(c) * 16 - static_cast<int64_t>((base + row0) & 15u);
+                    at[u] = slot[u] >= 0 && place < bytes && place > -16 ? static_cast<int>(place) : static_cast<int>(bytes);
+                    if (p.dweights != nullptr && at[u] < bytes) row[u] = load_window(rows + row0 + at[u], rows, rows + p.num_rows * bytes);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (at[u] >= bytes) continue;
+                    const int from = at[u] < 0 ? -at[u] / kBytes<DT> : 0, left = (static_cast<int>(bytes) - at[u]) / kBytes<DT>, to = left < N ? left : N;
+                    Pair d[H], f[H];
+                    uint4 v = load_window(dout + token * bytes + at[u], dout, dout + p.tokens * bytes);
+                    if (from > 0 || to < N) v = keep_some<kBytes<DT>>(v, from, to);
+                    widen_piece<DT>(v, d);
+                    if (p.dweights != nullptr) {
+                        if (from > 0 || to < N) row[u] = keep_some<kBytes<DT>>(row[u], from, to);
+                        widen_piece<DT>(row[u], f);
+                        Pair sum = 0ull;
+#pragma unroll
+                        for (int i = 0; i < H; ++i) sum = fma2(d[i], f[i], sum);
+                        const float2 e = split(sum);
+                        dot[u] += e.x + e.y;
+                    }
+                    if (p.drows != nullptr) {
+                        const Pair w2 = pair(w[u], w[u]);
+#pragma unroll
+                        for (int i = 0; i < H; ++i) d[i] = mul2(w2, d[i]);
+                        const uint4 o = narrow_piece<DT>(d);
+                        char* to_row = static_cast<char*>(p.drows) + slot[u] * bytes + at[u];
+                        if (from == 0 && to == N) *reinterpret_cast<uint4*>(to_row) = o;
+                        else store_some<kBytes<DT>>(to_row, o, from, to);
+                    }
+                }
+            }
+        }
+        for (int c = B == kOddRows ? pieces : t; c < pieces; c += threads) {
             P d, row[U];
             d.load(p.dout, token0 + c * N);
             if (p.dweights != nullptr) {
@@ -503,7 +640,7 @@ __global__ void __launch_bounds__(256) ungroup_rows_backward_kernel(const Ungrou
     }
 }
 
-// Bytes of the pieces that all operands can be read in: 32, 16, or 0 for single values
+// Bytes of the pieces that all operands can be read in: 32, 16, or 0 for rows that start anywhere
 int piece_of(const UngroupRowsParams& p, int bytes) {
     const int64_t row = static_cast<int64_t>(p.h) * bytes;
     if (row % 32 == 0 && aligned32(p.rows) && aligned32(p.residual) && aligned32(p.out) && aligned32(p.dout) && aligned32(p.drows)) return 32;
@@ -524,9 +661,18 @@ int launch_ungroup_piece(const UngroupRowsParams& p, cudaStream_t stream) {
 }
 
 template <int DT>
+int launch_ungroup_odd(const UngroupRowsParams& p, cudaStream_t stream) {
+    constexpr int N = 16 / kBytes<DT>;
+    const int64_t n = p.tokens * ((p.h + 2 * N - 2) / N), blocks = (n + 255) / 256;
+    if (blocks > 0x7FFFFFFF) return static_cast<int>(cudaErrorInvalidValue);
+    const dim3 grid(static_cast<unsigned>(blocks));
+    return blocks * 256 < 0x7FFFFFFF ? launch_pdl(ungroup_odd_rows_kernel<DT, uint32_t>, grid, 256, 0, stream, p) : launch_pdl(ungroup_odd_rows_kernel<DT, uint64_t>, grid, 256, 0, stream, p);
+}
+
+template <int DT>
 int launch_ungroup_type(const UngroupRowsParams& p, cudaStream_t stream) {
     const int piece = piece_of(p, kBytes<DT>);
-    return piece == 32 ? launch_ungroup_piece<DT, 32>(p, stream) : piece == 16 ? launch_ungroup_piece<DT, 16>(p, stream) : launch_ungroup_piece<DT, kBytes<DT>>(p, stream);
+    return piece == 32 ? launch_ungroup_piece<DT, 32>(p, stream) : piece == 16 ? launch_ungroup_piece<DT, 16>(p, stream) : launch_ungroup_odd<DT>(p, stream);
 }
 
 template <int DT, int B, int U>
@@ -559,7 +705,7 @@ int launch_ungroup_backward_piece(const UngroupRowsParams& p, cudaStream_t strea
 template <int DT>
 int launch_ungroup_backward_type(const UngroupRowsParams& p, cudaStream_t stream) {
     const int piece = piece_of(p, kBytes<DT>);
-    return piece == 32 ? launch_ungroup_backward_piece<DT, 32>(p, stream) : piece == 16 ? launch_ungroup_backward_piece<DT, 16>(p, stream) : launch_ungroup_backward_piece<DT, kBytes<DT>>(p, stream);
+    return piece == 32 ? launch_ungroup_backward_piece<DT, 32>(p, stream) : piece == 16 ? launch_ungroup_backward_piece<DT, 16>(p, stream) : launch_ungroup_backward_piece<DT, kOddRows>(p, stream);
 }
 
 }  // namespace
@@ -568,21 +714,18 @@ int launch_ungroup_backward_type(const UngroupRowsParams& p, cudaStream_t stream
 
 extern "C" int cam_launch_group_rows(const cam::GroupRowsParams* p, cudaStream_t stream) {
     using namespace cam;
-    const uintptr_t bits = reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(p->rows) | static_cast<uintptr_t>(p->row_bytes);
+    const bool whole = p->row_bytes % 16 == 0 && aligned16(p->x) && aligned16(p->rows);
     // Comparing the pairs of every token with all others costs instructions, the sort costs a launch.  One launch / sort and copy: 128 tokens
     // x 8 of 7168 bf16 6.4 / 9.2 us, 777 x 2 of 1000 7.7 / 7.0 us.
     const int64_t pairs = p->tokens * p->k;
     if (pairs > 0 && pairs <= kFewPairs && p->tokens * pairs <= kFewCompares) {
-        if (bits % 16 == 0) return launch_few<uint4>(*p, stream);
-        if (bits % 4 == 0) return launch_few<uint32_t>(*p, stream);
-        return bits % 2 == 0 ? launch_few<uint16_t>(*p, stream) : launch_few<uint8_t>(*p, stream);
+        if (whole) return launch_few<kPieces16>(*p, stream);
+        return p->elem_bytes == 4 ? launch_few<4>(*p, stream) : p->elem_bytes == 2 ? launch_few<2>(*p, stream) : launch_few<1>(*p, stream);
     }
     const int rc = launch_sort(*p, stream);
     if (rc != 0 || p->tokens == 0) return rc;
-    if (bits % 16 == 0) return launch_copy<uint4>(*p, stream);
-    if (bits % 4 == 0) return launch_copy<uint32_t>(*p, stream);
-    if (bits % 2 == 0) return launch_copy<uint16_t>(*p, stream);
-    return launch_copy<uint8_t>(*p, stream);
+    if (whole) return launch_copy<kPieces16>(*p, stream);
+    return p->elem_bytes == 4 ? launch_copy<4>(*p, stream) : p->elem_bytes == 2 ? launch_copy<2>(*p, stream) : launch_copy<1>(*p, stream);
 }
 
 extern "C" int cam_launch_ungroup_rows(const cam::UngroupRowsParams* p, int dtype, cudaStream_t stream) {

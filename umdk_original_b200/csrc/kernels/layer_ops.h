@@ -64,6 +64,7 @@ struct GroupRowsParams {
     int64_t tokens;
     int k, experts, scale_cols;
     int64_t row_bytes;
+    int elem_bytes;         // 1, 2 or 4
     void* rows;             // [tokens * k, row_bytes]
     float* row_scales;      // [tokens * k, scale_cols]
     int* offsets;           // [experts + 1]

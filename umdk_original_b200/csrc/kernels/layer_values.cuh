@@ -143,6 +143,67 @@ __device__ __forceinline__ float rounded(float v) {
     return v;
 }
 
+// ------------------------------------------------------------------------------------------------
+// Rows of odd widths: 16 bytes from and to any address
+// ------------------------------------------------------------------------------------------------
+// Byte by byte: at the ends of the memory alone
+static __device__ __noinline__ uint4 load_window_at_end(const char* at, const char* lo, const char* hi) {
+    uint32_t r[4] = {0u, 0u, 0u, 0u};
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t b = at + i >= lo && at + i < hi ? __ldg(reinterpret_cast<const unsigned char*>(at) + i) : 0u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] |= i / 4 == k ? b << (i % 4 * 8) : 0u;
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Sixteen bytes from any address, of memory that reaches from lo to hi; what is outside comes as zeros.  Two aligned pieces, of which the
+// second is the first one of a neighbouring thread and lies in L1, shifted together.
+__device__ __forceinline__ uint4 load_window(const char* at, const char* lo, const char* hi) {
+    const uint32_t d = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at) & 15u);
+    const char* a = at - d;
+    if (a < lo || a + (d != 0u ? 32 : 16) > hi) return load_window_at_end(at, lo, hi);
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(a));
+    if (d == 0u) return u;
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(a) + 1);
+    uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    if (d & 8u) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (d & 4u) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    const uint32_t bits = (d & 3u) * 8u;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+// Elements of ES bytes at places from..to - 1 of a piece, which starts at an aligned address
+template <int ES>
+__device__ __forceinline__ void store_some(char* at, const uint4& v, int from, int to) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 16 / ES; ++i) {
+        if (i < from || i >= to) continue;
+        if constexpr (ES == 4) *reinterpret_cast<uint32_t*>(at + 4 * i) = w[i];
+        else if constexpr (ES == 2) *reinterpret_cast<uint16_t*>(at + 2 * i) = static_cast<uint16_t>(w[i / 2] >> (i % 2 * 16));
+        else *reinterpret_cast<uint8_t*>(at + i) = static_cast<uint8_t>(w[i / 4] >> (i % 4 * 8));
+    }
+}
+// Zeros at the other places
+template <int ES>
+__device__ __forceinline__ uint4 keep_some(const uint4& v, int from, int to) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 16 / ES; ++i) {
+        if (i >= from && i < to) continue;
+        if constexpr (ES == 4) w[i] = 0u;
+        else w[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);

@@ -340,6 +340,7 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p, int
 #pragma unroll
         for (int i = 1; i < VPL; ++i) top = fmaxf(top, x[i]);
         top = seg_max<L>(top);
+        nan = nan || top == CUDART_INF_F;  // a softmax of infinity has no value
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) sum += quick_exp(x[i] - top);

@@ -71,91 +71,110 @@ __device__ __forceinline__ Raw16<DT> add16(const Raw16<DT>& x, const Raw16<DT>& 
     return s;
 }
 
-// How rows can be read: 32 bytes at a time, 16 (rows of a multiple of 8 values), or one value (odd widths, any alignment)
+// How rows can be read: 32 bytes at a time, 16 (rows of a multiple of 8 values), or one value (other widths, operands that are not
+// aligned)
 constexpr int kBy32 = 16, kBy16 = 8, kByOne = 1;
+
+// Where a thread's values of a row lie
+struct Place {
+    int64_t row0;  // first value of the row
+    int t, threads, h;
+};
 
 // Column of the first of a thread's sixteen values (kByOne: of value j)
 template <int VEC>
-__device__ __forceinline__ int column(int v, int j, int t, int threads) {
-    return VEC == kByOne ? (v * 16 + j) * threads + t : (v * threads + t) * 16 + j;
+__device__ __forceinline__ int column(const Place& at, int v, int j) {
+    return VEC == kByOne ? (v * 16 + j) * at.threads + at.t : (v * at.threads + at.t) * 16 + j;
 }
 
-// Zeros past the row.  `cached`: what every row reads, through L1.
+// Zeros past the row
 template <int DT, int VEC>
-__device__ __forceinline__ Raw16<DT> load16(const void* base, int64_t row0, int v, int t, int threads, int h, bool cached = false) {
+__device__ __forceinline__ Raw16<DT> load16(const void* base, const Place& at, int v) {
     Raw16<DT> r;
+    const int c = column<VEC>(at, v, 0);
+    const char* p = static_cast<const char*>(base) + (at.row0 + c) * kBytes<DT>;
     if constexpr (VEC == kByOne) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const int c = column<VEC>(v, j, t, threads);
-            if constexpr (DT == kDtFp32) r.w[j] = c < h ? __float_as_uint(load1<DT>(base, row0 + c)) : 0u;
+            const int d = column<VEC>(at, v, j);
+            if constexpr (DT == kDtFp32) r.w[j] = d < at.h ? __float_as_uint(load1<DT>(base, at.row0 + d)) : 0u;
             else {
-                const uint32_t b = c < h ? __ldg(static_cast<const unsigned short*>(base) + row0 + c) : 0u;
+                const uint32_t b = d < at.h ? __ldg(static_cast<const unsigned short*>(base) + at.row0 + d) : 0u;
                 r.w[j / 2] = j % 2 ? r.w[j / 2] | b << 16 : b;
             }
         }
-    } else {
-        const int c = column<VEC>(v, 0, t, threads);
-        const char* p = static_cast<const char*>(base) + (row0 + c) * kBytes<DT>;
-        if (VEC == kBy32 && !cached) {
-            if (c < h) {
+    } else if constexpr (VEC == kBy32) {
+        if (c < at.h) {
 #pragma unroll
-                for (int i = 0; i < kWords<DT>; i += 8) load32(r.w + i, p + i * 4);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kWords<DT>; ++i) r.w[i] = 0u;
-            }
+            for (int i = 0; i < kWords<DT>; i += 8) load32(r.w + i, p + i * 4);
         } else {
 #pragma unroll
-            for (int i = 0; i < kWords<DT>; i += 4) {
-                uint4 q = make_uint4(0u, 0u, 0u, 0u);
-                if (c + i * 4 / kBytes<DT> < h) q = cached ? __ldg(reinterpret_cast<const uint4*>(p + i * 4)) : load16_stream(p + i * 4);
-                r.w[i] = q.x, r.w[i + 1] = q.y, r.w[i + 2] = q.z, r.w[i + 3] = q.w;
-            }
+            for (int i = 0; i < kWords<DT>; ++i) r.w[i] = 0u;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kWords<DT>; i += 4) {
+            const int d = c + i * 4 / kBytes<DT>;
+            uint4 q = make_uint4(0u, 0u, 0u, 0u);
+            if (d < at.h) q = load16_stream(p + i * 4);
+            r.w[i] = q.x, r.w[i + 1] = q.y, r.w[i + 2] = q.z, r.w[i + 3] = q.w;
         }
     }
     return r;
 }
 
 template <int DT, int VEC>
-__device__ __forceinline__ void store16(void* base, int64_t row0, int v, int t, int threads, int h, const Raw16<DT>& r) {
+__device__ __forceinline__ void store16(void* base, const Place& at, int v, const Raw16<DT>& r) {
+    const int c = column<VEC>(at, v, 0);
+    char* p = static_cast<char*>(base) + (at.row0 + c) * kBytes<DT>;
     if constexpr (VEC == kByOne) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const int c = column<VEC>(v, j, t, threads);
-            if (c >= h) continue;
-            if constexpr (DT == kDtFp32) static_cast<uint32_t*>(base)[row0 + c] = r.w[j];
-            else static_cast<unsigned short*>(base)[row0 + c] = static_cast<unsigned short>(r.w[j / 2] >> (j % 2 * 16));
+            const int d = column<VEC>(at, v, j);
+            if (d >= at.h) continue;
+            if constexpr (DT == kDtFp32) static_cast<uint32_t*>(base)[at.row0 + d] = r.w[j];
+            else static_cast<unsigned short*>(base)[at.row0 + d] = static_cast<unsigned short>(r.w[j / 2] >> (j % 2 * 16));
+        }
+    } else if constexpr (VEC == kBy32) {
+        if (c < at.h) {
+#pragma unroll
+            for (int i = 0; i < kWords<DT>; i += 8) store32(p + i * 4, r.w + i);
         }
     } else {
-        const int c = column<VEC>(v, 0, t, threads);
-        char* p = static_cast<char*>(base) + (row0 + c) * kBytes<DT>;
-        if constexpr (VEC == kBy32) {
-            if (c < h) {
 #pragma unroll
-                for (int i = 0; i < kWords<DT>; i += 8) store32(p + i * 4, r.w + i);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kWords<DT>; i += 4) {
-                if (c + i * 4 / kBytes<DT> < h) *reinterpret_cast<uint4*>(p + i * 4) = make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
-            }
+        for (int i = 0; i < kWords<DT>; i += 4) {
+            const int d = c + i * 4 / kBytes<DT>;
+            if (d < at.h) *reinterpret_cast<uint4*>(p + i * 4) = make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
         }
     }
 }
 
-// Weights of a thread's sixteen columns
+// Weights of a thread's sixteen columns, which every row reads: through L1
 template <int DT, int VEC>
-__device__ __forceinline__ void load_weight(const void* w, bool fp32, int v, int t, int threads, int h, Pair* out) {
-    if (DT == kDtFp32 || fp32) {
-        const Raw16<kDtFp32> r = load16<kDtFp32, VEC>(w, 0, v, t, threads, h, true);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = widen2<kDtFp32>(r, i);
+__device__ __forceinline__ void load_weight_as(const void* w, const Place& at, int v, Pair* out) {
+    Raw16<DT> r;
+    if constexpr (VEC == kByOne) {
+        Place first = at;
+        first.row0 = 0;
+        r = load16<DT, VEC>(w, first, v);
     } else {
-        const Raw16<DT> r = load16<DT, VEC>(w, 0, v, t, threads, h, true);
+        const int c = column<VEC>(at, v, 0);
+        const char* p = static_cast<const char*>(w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = widen2<DT>(r, i);
+        for (int i = 0; i < kWords<DT>; i += 4) {
+            const int d = c + i * 4 / kBytes<DT>;
+            uint4 q = make_uint4(0u, 0u, 0u, 0u);
+            if (d < at.h) q = __ldg(reinterpret_cast<const uint4*>(p + static_cast<int64_t>(d) * kBytes<DT>));
+            r.w[i] = q.x, r.w[i + 1] = q.y, r.w[i + 2] = q.z, r.w[i + 3] = q.w;
+        }
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = widen2<DT>(r, i);
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void load_weight(const void* w, bool fp32, const Place& at, int v, Pair* out) {
+    if (DT == kDtFp32 || fp32) load_weight_as<kDtFp32, VEC>(w, at, v, out);
+    else load_weight_as<DT, VEC>(w, at, v, out);
 }
 
 // Sum (and maximum) over the threads that share a row, with one barrier: `red`, 64 floats of the block, is one of two that take turns
@@ -197,24 +216,27 @@ __device__ __forceinline__ void over_row(float& sum, float& top, float* red) {
 // ------------------------------------------------------------------------------------------------
 // Sixteen values of a row in 8 bits
 template <int VEC>
-__device__ __forceinline__ void store_int8(void* q, int64_t row0, int v, int t, int threads, int h, const Pair* y, float inv) {
+__device__ __forceinline__ void store_int8(void* q, const Place& at, int v, const Pair* y, float inv) {
     uint32_t o[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         const float2 f = split(y[j / 2]);
         const int a = max(-127, min(127, __float2int_rn((j % 2 ? f.y : f.x) * inv)));  // NaN becomes 0; the row's scale is NaN then
-        if constexpr (VEC == kByOne) {
-            const int c = column<VEC>(v, j, t, threads);
-            if (c < h) static_cast<int8_t*>(q)[row0 + c] = static_cast<int8_t>(a);
-        } else {
-            o[j / 4] |= (static_cast<uint32_t>(a) & 0xFFu) << (j % 4 * 8);
-        }
+        o[j / 4] |= (static_cast<uint32_t>(a) & 0xFFu) << (j % 4 * 8);
     }
-    if constexpr (VEC != kByOne) {
-        const int c = column<VEC>(v, 0, t, threads);
-        uint2* p = reinterpret_cast<uint2*>(static_cast<int8_t*>(q) + row0 + c);
-        if (c < h) p[0] = make_uint2(o[0], o[1]);
-        if (c + 8 < h) p[1] = make_uint2(o[2], o[3]);
+    int8_t* row = static_cast<int8_t*>(q) + at.row0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = column<VEC>(at, v, VEC == kByOne ? 0 : 8 * i);
+        if constexpr (VEC != kByOne) {
+            if (c < at.h) *reinterpret_cast<uint2*>(row + c) = make_uint2(o[2 * i], o[2 * i + 1]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int d = column<VEC>(at, v, 8 * i + j);
+                if (d < at.h) row[d] = static_cast<int8_t>(o[2 * i + j / 4] >> (j % 4 * 8));
+            }
+        }
     }
 }
 
@@ -233,12 +255,13 @@ __device__ __forceinline__ void block_scale(float amax, bool power_of_two, float
 }
 
 template <int DT, int MODE, int NP, int VEC, bool WARP>
-__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : NP == 2 ? 512 : 256)
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : NP == 2 ? 512 : 1024)
 rms_norm_kernel(const RmsNormParams p) {
     __shared__ __align__(16) float red[64];
     clear_sums<WARP>(red);
     const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x, h = p.h;
     const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * kWarpRows + (threadIdx.x >> 5) : blockIdx.x, row0 = row * h;
+    const Place at{row0, t, threads, h};
     pdl_wait();
     pdl_release();
     if (WARP && row >= p.rows) return;
@@ -246,7 +269,7 @@ rms_norm_kernel(const RmsNormParams p) {
     {
         Raw16<DT> x[NP];
 #pragma unroll
-        for (int v = 0; v < NP; ++v) x[v] = load16<DT, VEC>(p.x, row0, v, t, threads, h);
+        for (int v = 0; v < NP; ++v) x[v] = load16<DT, VEC>(p.x, at, v);
         if (p.residual == nullptr) {
 #pragma unroll
             for (int v = 0; v < NP; ++v) {
@@ -256,7 +279,7 @@ rms_norm_kernel(const RmsNormParams p) {
         } else if (DT != kDtFp32 && p.res_type == kDtFp32) {
             Raw16<kDtFp32> r[NP];
 #pragma unroll
-            for (int v = 0; v < NP; ++v) r[v] = load16<kDtFp32, VEC>(p.residual, row0, v, t, threads, h);
+            for (int v = 0; v < NP; ++v) r[v] = load16<kDtFp32, VEC>(p.residual, at, v);
 #pragma unroll
             for (int v = 0; v < NP; ++v) {
 #pragma unroll
@@ -264,18 +287,18 @@ rms_norm_kernel(const RmsNormParams p) {
                     s[v][i] = add2(widen2<DT>(x[v], i), widen2<kDtFp32>(r[v], i));
                     narrow2<kDtFp32>(r[v], i, s[v][i]);
                 }
-                store16<kDtFp32, VEC>(p.sum, row0, v, t, threads, h, r[v]);
+                store16<kDtFp32, VEC>(p.sum, at, v, r[v]);
             }
         } else {
             Raw16<DT> r[NP];
 #pragma unroll
-            for (int v = 0; v < NP; ++v) r[v] = load16<DT, VEC>(p.residual, row0, v, t, threads, h);
+            for (int v = 0; v < NP; ++v) r[v] = load16<DT, VEC>(p.residual, at, v);
 #pragma unroll
             for (int v = 0; v < NP; ++v) {
                 r[v] = add16<DT>(x[v], r[v]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) s[v][i] = widen2<DT>(r[v], i);
-                store16<DT, VEC>(p.sum, row0, v, t, threads, h, r[v]);
+                store16<DT, VEC>(p.sum, at, v, r[v]);
             }
         }
     }
@@ -291,7 +314,7 @@ rms_norm_kernel(const RmsNormParams p) {
 #pragma unroll
     for (int v = 0; v < NP; ++v) {
         Pair w[8];
-        load_weight<DT, VEC>(p.weight, p.weight_type == kDtFp32, v, t, threads, h, w);
+        load_weight<DT, VEC>(p.weight, p.weight_type == kDtFp32, at, v, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             s[v][i] = mul2(s[v][i], w[i]);
@@ -315,9 +338,9 @@ rms_norm_kernel(const RmsNormParams p) {
             Raw16<DT> y;
 #pragma unroll
             for (int i = 0; i < 8; ++i) narrow2<DT>(y, i, s[v][i]);
-            store16<DT, VEC>(p.y, row0, v, t, threads, h, y);
+            store16<DT, VEC>(p.y, at, v, y);
         }
-        if constexpr (MODE == kInt8) store_int8<VEC>(p.q, row0, v, t, threads, h, s[v], inv8);
+        if constexpr (MODE == kInt8) store_int8<VEC>(p.q, at, v, s[v], inv8);
         if constexpr (MODE == kE4m3) {
             // a block of 128 values: eight consecutive lanes
             float amax = 0.f;
@@ -337,7 +360,7 @@ rms_norm_kernel(const RmsNormParams p) {
                 const float2 a = split(mul2(s[v][2 * i], inv2)), b = split(mul2(s[v][2 * i + 1], inv2));
                 o[i] = pack_e4m3x4(a.x, a.y, b.x, b.y);
             }
-            const int c = column<VEC>(v, 0, t, threads);
+            const int c = column<VEC>(at, v, 0);
             if (c < h) {
                 *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.q) + row0 + c) = make_uint4(o[0], o[1], o[2], o[3]);
                 if ((t & 7) == 0) p.scales[row * (h / 128) + (c >> 7)] = scale;
@@ -362,25 +385,25 @@ rms_norm_kernel(const RmsNormParams p) {
 // Column of value j of half `i`.  The halves are eight consecutive values each, and so are a warp's: 16 bytes per thread that were a
 // half of 32 consecutive ones would fetch every sector twice (8192 x 7168 bf16: 138 us).
 template <int VEC>
-__device__ __forceinline__ int half_column(int i, int j, int t, int threads) {
-    return VEC == kByOne ? (i * 8 + j) * threads + t : (i * threads + t) * 8 + j;
+__device__ __forceinline__ int half_column(const Place& at, int i, int j) {
+    return VEC == kByOne ? (i * 8 + j) * at.threads + at.t : (i * at.threads + at.t) * 8 + j;
 }
 
 // Eight values of a row as pairs
 template <int DT, int VEC>
-__device__ __forceinline__ void load_half(const void* base, int64_t row0, int i, int t, int threads, int h, Pair* out) {
+__device__ __forceinline__ void load_half(const void* base, const Place& at, int i, Pair* out) {
     if constexpr (VEC == kByOne) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int c = half_column<VEC>(i, 2 * j, t, threads), d = half_column<VEC>(i, 2 * j + 1, t, threads);
-            out[j] = pair(c < h ? load1<DT>(base, row0 + c) : 0.f, d < h ? load1<DT>(base, row0 + d) : 0.f);
+            const int d = half_column<VEC>(at, i, 2 * j), e = half_column<VEC>(at, i, 2 * j + 1);
+            out[j] = pair(d < at.h ? load1<DT>(base, at.row0 + d) : 0.f, e < at.h ? load1<DT>(base, at.row0 + e) : 0.f);
         }
     } else {
-        const int c = half_column<VEC>(i, 0, t, threads);
+        const int c = half_column<VEC>(at, i, 0);
         Raw8<DT> r = {};
-        if (c < h) {
-            if constexpr (DT == kDtFp32) load32(reinterpret_cast<uint32_t*>(r.v), static_cast<const float*>(base) + row0 + c);
-            else r = load8<DT>(base, row0 + c);
+        if (c < at.h) {
+            if constexpr (DT == kDtFp32) load32(reinterpret_cast<uint32_t*>(r.v), static_cast<const float*>(base) + at.row0 + c);
+            else r = load8<DT>(base, at.row0 + c);
         }
         float f[8];
         widen8<DT>(r, f);
@@ -389,7 +412,7 @@ __device__ __forceinline__ void load_half(const void* base, int64_t row0, int i,
     }
 }
 template <int DT, int VEC>
-__device__ __forceinline__ void store_half(void* base, int64_t row0, int i, int t, int threads, int h, const Pair* v) {
+__device__ __forceinline__ void store_half(void* base, const Place& at, int i, const Pair* v) {
     float f[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -400,15 +423,15 @@ __device__ __forceinline__ void store_half(void* base, int64_t row0, int i, int 
     if constexpr (VEC == kByOne) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int c = half_column<VEC>(i, j, t, threads);
-            if (c < h) store1<DT>(base, row0 + c, f[j]);
+            const int d = half_column<VEC>(at, i, j);
+            if (d < at.h) store1<DT>(base, at.row0 + d, f[j]);
         }
     } else {
-        const int c = half_column<VEC>(i, 0, t, threads);
+        const int c = half_column<VEC>(at, i, 0);
         const Raw8<DT> r = narrow8<DT>(f);
-        if (c < h) {
-            if constexpr (DT == kDtFp32) store32(static_cast<float*>(base) + row0 + c, reinterpret_cast<const uint32_t*>(r.v));
-            else store8<DT>(base, row0 + c, r);
+        if (c < at.h) {
+            if constexpr (DT == kDtFp32) store32(static_cast<float*>(base) + at.row0 + c, reinterpret_cast<const uint32_t*>(r.v));
+            else store8<DT>(base, at.row0 + c, r);
         }
     }
 }
@@ -436,7 +459,7 @@ __device__ __forceinline__ uint32_t ring_copy(uint32_t ring, int threads, int t,
 template <int DT>
 __device__ __forceinline__ void ring_half(uint32_t ring, int i, int threads, int t, int h, Pair* out) {
     Raw8<DT> r = {};
-    if (half_column<kBy16>(i, 0, t, threads) < h) {
+    if ((i * threads + t) * 8 < h) {
 #pragma unroll
         for (int j = 0; j < kCopies<DT>; ++j)
             asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.v[j].x), "=r"(r.v[j].y), "=r"(r.v[j].z), "=r"(r.v[j].w) : "r"(ring + ((i * threads + t) * kCopies<DT> + j) * 16) : "memory");
@@ -479,7 +502,7 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         Pair f[4];
-        load_half<WT, VEC>(p.weight, 0, i, t, threads, h, f);
+        load_half<WT, VEC>(p.weight, Place{0, t, threads, h}, i, f);
 #pragma unroll
         for (int j = 0; j < 4; ++j) narrow2<WT>(w, 4 * i + j, f[j]);
     }
@@ -488,7 +511,7 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
     for (int i = 0; i < 8; ++i) acc[i] = 0ull;
     int stage = 0, turn = 0;
     for (int64_t row = first; row < p.rows; row += step) {
-        const int64_t row0 = row * h;
+        const Place at{row * h, t, threads, h};
         const float rstd = __ldg(p.rstd + row);
         const Pair rstd2 = pair(rstd, rstd);
         const uint32_t at_dy = slots + stage * stage_bytes, at_s = at_dy + 2 * kCopies<DT> * threads * 16, at_ds = at_s + 2 * kCopies<ST> * threads * 16;
@@ -499,8 +522,8 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                load_half<DT, VEC>(p.dy, row0, i, t, threads, h, dy + 4 * i);
-                load_half<ST, VEC>(p.sum, row0, i, t, threads, h, s + 4 * i);
+                load_half<DT, VEC>(p.dy, at, i, dy + 4 * i);
+                load_half<ST, VEC>(p.sum, at, i, s + 4 * i);
             }
         }
         Pair products = 0ull;
@@ -541,12 +564,12 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
                     g[j] = mul2(g[j], widen2<WT>(w, 4 * i + j));
                 }
             } else {
-                if (p.dsum != nullptr) load_half<ST, VEC>(p.dsum, row0, i, t, threads, h, d);
+                if (p.dsum != nullptr) load_half<ST, VEC>(p.dsum, at, i, d);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) d[j] = fma2(rstd2, fma2(share2, hat[j], g[j]), d[j]);
-            if (p.dx != nullptr) store_half<DT, VEC>(p.dx, row0, i, t, threads, h, d);
-            if (p.dres != nullptr) store_half<ST, VEC>(p.dres, row0, i, t, threads, h, d);
+            if (p.dx != nullptr) store_half<DT, VEC>(p.dx, at, i, d);
+            if (p.dres != nullptr) store_half<ST, VEC>(p.dres, at, i, d);
         }
         if constexpr (STAGES > 0) {
             if (DT == kDtFp32 || ST == kDtFp32) __syncwarp();
@@ -556,6 +579,7 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
     }
     if (p.partial == nullptr) return;
     float* mine = p.partial + static_cast<int64_t>(blockIdx.x) * h;
+    const Place cols_at{0, t, threads, h};
     if constexpr (WARP) {
         // all rings have been read: the memory takes the warps' sums
         float* cols = reinterpret_cast<float*>(dynamic);
@@ -563,7 +587,7 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const int c = half_column<VEC>(j / 8, j % 8, t, threads);
+            const int c = half_column<VEC>(cols_at, j / 8, j % 8);
             const float2 f = split(acc[j / 2]);
             if (c < h) cols[warp * h + c] = j % 2 ? f.y : f.x;
         }
@@ -575,8 +599,8 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
             mine[c] = a;
         }
     } else {
-        store_half<kDtFp32, VEC>(mine, 0, 0, t, threads, h, acc);
-        store_half<kDtFp32, VEC>(mine, 0, 1, t, threads, h, acc + 4);
+        store_half<kDtFp32, VEC>(mine, cols_at, 0, acc);
+        store_half<kDtFp32, VEC>(mine, cols_at, 1, acc + 4);
     }
 }
 
@@ -621,10 +645,11 @@ int64_t turns_of(const Shape& s, int64_t rows) { return s.warp ? (rows + kWarpRo
 
 template <int DT, int MODE, int VEC>
 int launch_norm(const RmsNormParams& p, cudaStream_t stream) {
-    const Shape s = shape_of(p.h, 2);
+    constexpr int most = VEC == kByOne ? 1 : 2;  // with two, single values leave too few threads: 8192 x 4095 bf16 178 us instead of 103
+    const Shape s = shape_of(p.h, most);
     const dim3 grid(static_cast<unsigned>(turns_of(s, p.rows)));
-    if (!s.warp) return launch_pdl(rms_norm_kernel<DT, MODE, 2, VEC, false>, grid, s.threads, 0, stream, p);
-    return s.sixteens == 1 ? launch_pdl(rms_norm_kernel<DT, MODE, 1, VEC, true>, grid, s.threads, 0, stream, p) : launch_pdl(rms_norm_kernel<DT, MODE, 2, VEC, true>, grid, s.threads, 0, stream, p);
+    if (!s.warp) return launch_pdl(rms_norm_kernel<DT, MODE, most, VEC, false>, grid, s.threads, 0, stream, p);
+    return s.sixteens == 1 ? launch_pdl(rms_norm_kernel<DT, MODE, 1, VEC, true>, grid, s.threads, 0, stream, p) : launch_pdl(rms_norm_kernel<DT, MODE, most, VEC, true>, grid, s.threads, 0, stream, p);
 }
 
 // How all operands of a launch can be read

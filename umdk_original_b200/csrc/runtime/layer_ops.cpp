@@ -160,13 +160,15 @@ int check_pairs(const char* what, int64_t tokens, int k) {
 
 }  // namespace
 
-extern "C" int cam_moe_group_rows(const void* x, int64_t row_bytes, const float* scales, int scale_cols, const void* idx, int idx_i64,
+extern "C" int cam_moe_group_rows(const void* x, int64_t row_bytes, int elem_bytes, const float* scales, int scale_cols, const void* idx, int idx_i64,
                                   int64_t tokens, int k, int experts, void* rows, float* row_scales, int* offsets, int* slots,
                                   cudaStream_t stream) {
     if (check_pairs("moe_group_rows", tokens, k) != 0) return -1;
     LAYER_CHECK(offsets != nullptr && (tokens == 0 || (x && idx && rows && slots)), "moe_group_rows: null operand");
     LAYER_CHECK(experts >= 1 && experts <= cam::kRouteMaxExperts, "moe_group_rows: %d experts; 1 to %d", experts, cam::kRouteMaxExperts);
     LAYER_CHECK(row_bytes >= 1 && row_bytes < (1ll << 28) && scale_cols >= 0 && scale_cols < (1 << 28), "moe_group_rows: rows of %lld bytes", static_cast<long long>(row_bytes));
+    LAYER_CHECK(elem_bytes == 1 || elem_bytes == 2 || elem_bytes == 4, "moe_group_rows: elements of %d bytes", elem_bytes);
+    LAYER_CHECK(row_bytes % elem_bytes == 0 && reinterpret_cast<uintptr_t>(x) % elem_bytes == 0 && (reinterpret_cast<uintptr_t>(rows) & 15u) == 0, "moe_group_rows: rows must be 16-byte aligned");
     LAYER_CHECK(scale_cols == 0 || tokens == 0 || (scales && row_scales), "moe_group_rows: null scales");
     cam::GroupRowsParams p{};
     p.x = x;
@@ -178,6 +180,7 @@ extern "C" int cam_moe_group_rows(const void* x, int64_t row_bytes, const float*
     p.experts = experts;
     p.scale_cols = scale_cols;
     p.row_bytes = row_bytes;
+    p.elem_bytes = elem_bytes;
     p.rows = rows;
     p.row_scales = row_scales;
     p.offsets = offsets;

@@ -26,9 +26,9 @@ int cam_moe_route(const void* logits, int dtype, int64_t rows, int experts, int 
 int cam_moe_route_backward(const float* dweights, const void* logits, int dtype, const int64_t* idx, int64_t rows, int experts, int k,
                            int sigmoid, int renormalize, float scale, void* dlogits, cudaStream_t stream);
 
-// x [tokens, row_bytes], scales [tokens, scale_cols] or null, idx [tokens, k] int32 / int64 -> rows [tokens * k, row_bytes], row_scales,
+// x [tokens, row_bytes] of elements of 1, 2 or 4 bytes, scales [tokens, scale_cols] or null, idx [tokens, k] int32 / int64 -> rows [tokens * k, row_bytes], row_scales,
 // offsets int32 [experts + 1], slots int32 [tokens, k] (-1: the id is outside [0, experts)); rows past offsets[experts] are zeros
-int cam_moe_group_rows(const void* x, int64_t row_bytes, const float* scales, int scale_cols, const void* idx, int idx_i64, int64_t tokens,
+int cam_moe_group_rows(const void* x, int64_t row_bytes, int elem_bytes, const float* scales, int scale_cols, const void* idx, int idx_i64, int64_t tokens,
                        int k, int experts, void* rows, float* row_scales, int* offsets, int* slots, cudaStream_t stream);
 // out[t] = residual[t] + sum_j weights[t, j] rows[slots[t, j]]; slots outside [0, num_rows) add nothing
 int cam_moe_ungroup_rows(const void* rows, int dtype, int64_t num_rows, int h, const int* slots, int64_t tokens, int k, const float* weights,

@@ -183,7 +183,8 @@ def moe_route_cpu(logits, k, bias=None, score="softmax", num_groups=1, topk_grou
         w = torch.where(empty, torch.zeros_like(w), w / w.sum(-1, keepdim=True))
     else:
         w = torch.where(empty, torch.zeros_like(l), s.gather(1, idx.clamp(min=0)))
-    w = torch.where(logits.isnan().any(-1, keepdim=True), torch.full_like(w, float("nan")), w * scale)
+    bad = logits.isnan() if score == "sigmoid" else logits.isnan() | (x == float("inf"))
+    w = torch.where(bad.any(-1, keepdim=True), torch.full_like(w, float("nan")), w * scale)
     return idx, w.float()
 
 
@@ -288,6 +289,8 @@ def moe_ungroup_rows_backward_cpu(dout, rows, slots, topk_weights=None, need_dro
     d = dout.float()
     drows, dw = rows.new_empty(0), torch.empty(0)
     if need_drows:
+        named = slots[valid]
+        _check(named.unique().numel() == named.numel(), f"{op}: a row belongs to one slot at most")
         drows = torch.zeros(rows.shape, dtype=torch.float32)
         drows[slots[valid].long()] = (d[:, None] * w[..., None])[valid]
         drows = drows.to(rows.dtype)
