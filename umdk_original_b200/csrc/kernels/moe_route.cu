@@ -313,8 +313,9 @@ __device__ __forceinline__ uint32_t open_groups(const RouteParams& p, int64_t ro
 template <int L>
 constexpr int kRouteRows = 128 / L;  // tokens of a block of four warps
 
-template <int DT, int L, int VPL>
-__global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p, int scratch_bytes) {
+// SCORES: ranks or groups go by scores; otherwise everything goes by logits
+template <int DT, int L, int VPL, bool SCORES>
+__global__ void __launch_bounds__(128, VPL <= 16 ? 6 : 4) moe_route_kernel(const RouteParams p, int scratch_bytes) {
     extern __shared__ double scratch[];  // scratch_bytes per warp
     constexpr uint32_t kIndex = DT != kDtFp32 ? 0xFFFFu : L * VPL <= 256 ? 0xFFu : 0x3FFu;  // bits of a key that hold the index
     constexpr uint32_t kIndexScore = L * VPL <= 256 ? 0xFFu : 0x3FFu;
@@ -328,12 +329,18 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p, int
     double* warp_scratch = reinterpret_cast<double*>(reinterpret_cast<char*>(scratch) + warp * scratch_bytes);
     float x[VPL];
     load_logits<DT, VPL>(p, row, sub, x);
-    bool nan = false;
+    // a NaN or infinity among the logits, or what a lane lacks of the row: values are looked at one by one then
+    float finite = 0.f;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) nan |= x[i] != x[i];
-    if (__any_sync(0xFFFFFFFFu, nan)) nan = seg_max<L>(nan ? 1.f : 0.f) != 0.f;
-    const bool grouped = p.topk_groups < p.groups, by_score = p.bias != nullptr;
-    const bool need_scores = by_score || (grouped && p.group_top == 2);
+    for (int i = 0; i < VPL; ++i) finite = fmaf(x[i], 0.f, finite);
+    bool odd = __any_sync(0xFFFFFFFFu, finite != 0.f), nan = false;
+    if (odd) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) nan |= x[i] != x[i];
+        nan = seg_max<L>(nan ? 1.f : 0.f) != 0.f;
+    }
+    const bool grouped = p.topk_groups < p.groups, by_score = SCORES && p.bias != nullptr;
+    constexpr bool need_scores = SCORES;
     float top = 0.f, inv_sum = 0.f;
     if (!p.sigmoid && (need_scores || !p.renormalize)) {
         top = x[0];
@@ -361,31 +368,38 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p, int
 #pragma unroll
             for (int i = 0; i < VPL; ++i) b[i] = first + i < p.experts ? __ldg(p.bias + first + i) : 0.f;
         }
+        finite = 0.f;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const float v = (p.sigmoid ? quick_sigmoid(x[i]) : quick_exp(x[i] - top) * inv_sum) + b[i];
-            value[i] = x[i] > -CUDART_INF_F && v > -CUDART_INF_F ? v : -CUDART_INF_F;
+            value[i] = (p.sigmoid ? quick_sigmoid(x[i]) : quick_exp(x[i] - top) * inv_sum) + b[i];
+            finite = fmaf(value[i], 0.f, finite);
+        }
+        odd = odd || __any_sync(0xFFFFFFFFu, finite != 0.f);
+        if (odd) {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) value[i] = x[i] > -CUDART_INF_F && value[i] > -CUDART_INF_F ? value[i] : -CUDART_INF_F;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) value[i] = x[i] > -CUDART_INF_F ? x[i] : -CUDART_INF_F;
+        for (int i = 0; i < VPL; ++i) value[i] = x[i];
+        if (odd) {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) value[i] = x[i] > -CUDART_INF_F ? x[i] : -CUDART_INF_F;
+        }
     }
-    bool unclear = false, unclear_groups = false;
+    bool unclear = false, unclear_groups = false, closed = false;  // closed: all of this lane's experts are
     uint32_t open = 0xFFFFFFFFu;
     if (grouped) {
         open = open_groups<DT, L, VPL>(p, row, value, reinterpret_cast<float*>(warp_scratch) + seg * p.experts, need_scores, unclear_groups);
         const int size = p.experts / p.groups;
-        const bool whole = size % VPL == 0;
-        if (whole) {
-            if (first < p.experts && !(open >> (first / size) & 1u)) {
-#pragma unroll
-                for (int i = 0; i < VPL; ++i) value[i] = x[i] = -CUDART_INF_F;
-            }
+        if (size % VPL == 0) {
+            closed = first < p.experts && !(open >> (first / size) & 1u);
         } else {
 #pragma unroll
             for (int i = 0; i < VPL; ++i) {
                 if (first + i < p.experts && !(open >> ((first + i) / size) & 1u)) value[i] = x[i] = -CUDART_INF_F;
             }
+            odd = true;
         }
     }
     uint32_t key[VPL];
@@ -400,20 +414,33 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p, int
         } else {
             o = ordered(r) & ~index;
         }
-        key[i] = r > -CUDART_INF_F ? o | (index - static_cast<uint32_t>(first + i)) : 0u;
+        key[i] = o | (index - static_cast<uint32_t>(first + i));
+    }
+    if (odd) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            if (!((by_score ? value[i] : x[i]) > -CUDART_INF_F)) key[i] = 0u;
+        }
     }
     sort_down<VPL>(key);
+    // the largest key stays in a register, the others wait in shared memory, with a zero behind them
+    uint32_t* list = reinterpret_cast<uint32_t*>(warp_scratch) + lane;
+#pragma unroll
+    for (int i = 1; i < VPL; ++i) list[32 * i] = key[i];
+    list[32 * VPL] = 0u;
+    uint32_t head = closed ? 0u : key[0];
+    const uint32_t* rest = list + 32;
     const bool exact_keys = DT != kDtFp32 && !by_score;
     const int candidates = exact_keys ? p.k : min(p.k + 1, L), turns = exact_keys ? p.k : candidates + 1;
     uint32_t taken = 0u, next = 0u;
     for (int j = 0; j < turns; ++j) {
-        uint32_t m = key[0];
+        uint32_t m = head;
 #pragma unroll
         for (int o = L / 2; o >= 1; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        const bool mine = key[0] == m;
-#pragma unroll
-        for (int i = 0; i + 1 < VPL; ++i) key[i] = mine ? key[i + 1] : key[i];
-        if (mine) key[VPL - 1] = 0u;
+        if (head == m && m != 0u) {
+            head = *rest;
+            rest += 32;
+        }
         if (sub == j) taken = m;
         next = m;
     }
@@ -578,10 +605,13 @@ template <int DT, int L, int VPL>
 int launch_route(RouteParams p, cudaStream_t stream) {
     p.vec = whole_pieces<DT>(p, VPL);
     p.vec_bias = p.experts % VPL == 0 && aligned16(p.bias);
-    // a row of doubles for the whole warp, or a row of floats for each of its tokens
-    const int floats = 32 / L * p.experts * 4, doubles = p.experts * 8, scratch = ((floats > doubles ? floats : doubles) + 15) / 16 * 16;
+    // of a warp: a row of doubles, a row of floats for each token, the lanes' lists; one after the other
+    const int floats = 32 / L * p.experts * 4, doubles = p.experts * 8, lists = (VPL + 1) * 128;
+    int scratch = floats > doubles ? floats : doubles;
+    scratch = ((scratch > lists ? scratch : lists) + 15) / 16 * 16;
     const dim3 grid(static_cast<unsigned>((p.rows + kRouteRows<L> - 1) / kRouteRows<L>));
-    return launch_pdl(moe_route_kernel<DT, L, VPL>, grid, 128, static_cast<size_t>(4) * scratch, stream, p, scratch);
+    const bool scores = p.bias != nullptr || (p.topk_groups < p.groups && p.group_top == 2);
+    return launch_pdl(scores ? moe_route_kernel<DT, L, VPL, true> : moe_route_kernel<DT, L, VPL, false>, grid, 128, static_cast<size_t>(4) * scratch, stream, p, scratch);
 }
 
 template <int DT>
