@@ -3,6 +3,7 @@
 #pragma once
 #include <ATen/TensorSubclassLikeUtils.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -78,12 +79,28 @@ inline bool records_graph(const char* op, std::initializer_list<std::pair<const 
         wanted = wanted || t->requires_grad();
     }
     if (!at::GradMode::is_enabled() || !wanted) return false;
-    for (const auto& [t, what] : operands) {
-        if (t == nullptr || !t->defined() || !t->is_cuda()) continue;
-        c10::cuda::CUDAGuard guard(t->device());
-        if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) check_capture(*t, op, what);
+    const at::Tensor& first = *operands.begin()->first;  // the operands of a call share a device
+    if (first.is_cuda()) {
+        c10::cuda::CUDAGuard guard(first.device());
+        if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+            for (const auto& [t, what] : operands) {
+                if (t != nullptr && t->defined()) check_capture(*t, op, what);
+            }
+        }
     }
     return true;
 }
+
+// Inside a backward pass: its own operators are called below autograd, whose fallback for operators without a derivative costs more than
+// they do.  With create_graph the fallback stays in the way, and whoever differentiates again is told that there is no derivative.
+struct BackwardGuard {
+    c10::optional<at::AutoDispatchBelowADInplaceOrView> below;
+    BackwardGuard() {
+        if (!at::GradMode::is_enabled()) below.emplace();
+    }
+};
+
+// Results of the CUDA implementations, which know where and what they are
+inline at::Tensor cuda_empty(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& on) { return at::detail::empty_cuda(sizes, type, on.device(), c10::nullopt); }
 
 }  // namespace umdk

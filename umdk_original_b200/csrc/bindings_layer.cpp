@@ -16,6 +16,8 @@ cudaStream_t stream_now() { return at::cuda::getCurrentCUDAStream().stream(); }
 void* data_or_null(const at::Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
 float* floats_or_null(const at::Tensor& t) { return static_cast<float*>(data_or_null(t)); }
 at::Tensor none_of(const at::Tensor& like) { return at::empty({0}, like.options()); }
+at::Tensor cuda_like(const at::Tensor& t) { return cuda_empty(t.sizes(), t.scalar_type(), t); }
+at::Tensor cuda_none(const at::Tensor& like) { return cuda_empty({0}, like.scalar_type(), like); }
 
 // ------------------------------------------------------------------------------------------------
 // Norm
@@ -54,9 +56,9 @@ NormProblem check_norm(const char* op, const at::Tensor& x, const OptTensor& res
 Three norm_forward(const char* op, const at::Tensor& x, const OptTensor& residual, const at::Tensor& weight, double eps, bool keep) {
     const NormProblem p = check_norm(op, x, residual, weight, eps);
     c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor y = at::empty_like(x), sum, rstd;
-    if (given(residual)) sum = at::empty_like(*residual);
-    if (keep) rstd = at::empty({p.rows}, x.options().dtype(at::kFloat));
+    at::Tensor y = cuda_like(x), sum, rstd;
+    if (given(residual)) sum = cuda_like(*residual);
+    if (keep) rstd = cuda_empty({p.rows}, at::kFloat, x);
     if (p.rows == 0) return {y, sum, rstd};
     CAM_RT(cam_rms_norm(x.data_ptr(), p.dtype, given(residual) ? residual->data_ptr() : nullptr, p.res_type, weight.data_ptr(), p.weight_type, p.rows,
                         p.h, static_cast<float>(eps), y.data_ptr(), data_or_null(sum), floats_or_null(rstd), 0, nullptr, nullptr, stream_now()));
@@ -72,15 +74,15 @@ Two add_rms_norm_cuda(const at::Tensor& x, const at::Tensor& residual, const at:
 }
 Three rms_norm_train_cuda(const at::Tensor& x, const OptTensor& residual, const at::Tensor& weight, double eps) {
     auto out = norm_forward("rms_norm_train", x, residual, weight, eps, true);
-    if (!std::get<1>(out).defined()) std::get<1>(out) = none_of(x);
+    if (!std::get<1>(out).defined()) std::get<1>(out) = cuda_none(x);
     return out;
 }
 
 // dx (of dy's type), dresidual (of the sum's type, empty where that is dx's: then they are the same numbers), dweight
-Three norm_grads_empty(const at::Tensor& dy, const at::Tensor& sum, const at::Tensor& weight, bool need_dx, bool need_dres, bool need_dw) {
+template <class Like, class None>
+Three norm_grads_empty(Like like, None none, const at::Tensor& dy, const at::Tensor& sum, const at::Tensor& weight, bool need_dx, bool need_dres, bool need_dw) {
     const bool one = dy.scalar_type() == sum.scalar_type();
-    return {need_dx || (one && need_dres) ? at::empty_like(dy) : none_of(dy), !one && need_dres ? at::empty_like(sum) : none_of(sum),
-            need_dw ? at::empty_like(weight) : none_of(weight)};
+    return {need_dx || (one && need_dres) ? like(dy) : none(dy), !one && need_dres ? like(sum) : none(sum), need_dw ? like(weight) : none(weight)};
 }
 
 Three rms_norm_backward_cuda(const at::Tensor& dy, const OptTensor& dsum, const at::Tensor& sum, const at::Tensor& weight, const at::Tensor& rstd,
@@ -93,14 +95,14 @@ Three rms_norm_backward_cuda(const at::Tensor& dy, const OptTensor& dsum, const 
         CAM_ASSERT(dsum->sizes() == sum.sizes() && dsum->scalar_type() == sum.scalar_type(), "rms_norm_backward: dsum must be like sum");
     }
     c10::cuda::CUDAGuard guard(dy.device());
-    auto out = norm_grads_empty(dy, sum, weight, need_dx, need_dres, need_dw);
+    auto out = norm_grads_empty(cuda_like, cuda_none, dy, sum, weight, need_dx, need_dres, need_dw);
     auto& [dx, dres, dw] = out;
     if (p.rows == 0) {
         dw.zero_();
         return out;
     }
     const int parts = cam_rms_norm_backward_parts(p.rows, p.h);
-    at::Tensor partial = need_dw ? at::empty({parts, p.h}, rstd.options()) : at::Tensor();
+    at::Tensor partial = need_dw ? cuda_empty({parts, p.h}, at::kFloat, dy) : at::Tensor();
     CAM_RT(cam_rms_norm_backward(dy.data_ptr(), p.dtype, given(dsum) ? dsum->data_ptr() : nullptr, sum.data_ptr(), p.res_type, weight.data_ptr(),
                                  p.weight_type, rstd.data_ptr<float>(), p.rows, p.h, data_or_null(dx), data_or_null(dres), data_or_null(dw),
                                  floats_or_null(partial), parts, stream_now()));
@@ -120,8 +122,8 @@ Four rms_norm_quant_cuda(const at::Tensor& x, const at::Tensor& weight, int64_t 
     auto scales_of = x.sizes().vec();
     if (quant_mode == 2) scales_of.pop_back();
     else scales_of.back() = p.h / 128;
-    at::Tensor q = at::empty(x.sizes(), x.options().dtype(qt)), s = at::empty(scales_of, x.options().dtype(at::kFloat));
-    at::Tensor sum = given(residual) ? at::empty_like(*residual) : none_of(x), y = with_rows ? at::empty_like(x) : none_of(x);
+    at::Tensor q = cuda_empty(x.sizes(), qt, x), s = cuda_empty(scales_of, at::kFloat, x);
+    at::Tensor sum = given(residual) ? cuda_like(*residual) : cuda_none(x), y = with_rows ? cuda_like(x) : cuda_none(x);
     if (p.rows == 0) return {q, s, sum, y};
     CAM_RT(cam_rms_norm(x.data_ptr(), p.dtype, given(residual) ? residual->data_ptr() : nullptr, p.res_type, weight.data_ptr(), p.weight_type, p.rows,
                         p.h, static_cast<float>(eps), data_or_null(y), data_or_null(sum), nullptr, static_cast<int>(quant_mode), q.data_ptr(),
@@ -159,7 +161,7 @@ Two moe_route_cuda(const at::Tensor& logits, int64_t k, const OptTensor& bias, c
     CAM_ASSERT(k <= e / num_groups * topk_groups, "moe_route: k ", num(k), " of the ", num(e / num_groups * topk_groups), " experts in ", num(topk_groups), " groups");
     CAM_ASSERT(group_top == 1 || group_top == 2, "moe_route: group_top must be 1 or 2, got ", num(group_top));
     c10::cuda::CUDAGuard guard(logits.device());
-    at::Tensor idx = at::empty({t, k}, logits.options().dtype(at::kLong)), w = at::empty({t, k}, logits.options().dtype(at::kFloat));
+    at::Tensor idx = cuda_empty({t, k}, at::kLong, logits), w = cuda_empty({t, k}, at::kFloat, logits);
     if (t == 0) return {idx, w};
     CAM_RT(cam_moe_route(logits.data_ptr(), dt, t, static_cast<int>(e), static_cast<int>(k), given(bias) ? bias->data_ptr<float>() : nullptr, sigmoid,
                          static_cast<int>(num_groups), static_cast<int>(topk_groups), static_cast<int>(group_top), renormalize,
@@ -179,7 +181,7 @@ at::Tensor moe_route_backward_cuda(const at::Tensor& dweights, const at::Tensor&
     const int dt = dtype_of(logits.scalar_type(), "logits");
     const bool sigmoid = sigmoid_of(score);
     c10::cuda::CUDAGuard guard(logits.device());
-    at::Tensor dlogits = at::empty_like(logits);
+    at::Tensor dlogits = cuda_like(logits);
     if (logits.size(0) == 0) return dlogits;
     CAM_RT(cam_moe_route_backward(dweights.data_ptr<float>(), logits.data_ptr(), dt, topk_idx.data_ptr<int64_t>(), logits.size(0),
                                   static_cast<int>(logits.size(1)), static_cast<int>(k), sigmoid, renormalize, static_cast<float>(scale),
@@ -203,8 +205,8 @@ Four moe_group_rows_cuda(const at::Tensor& x, const at::Tensor& topk_idx, int64_
     CAM_ASSERT(num_experts >= 1 && num_experts <= 1024, "moe_group_rows: ", num(num_experts), " experts; 1 to 1024");
     CAM_ASSERT(t * k < (1ll << 31) - 512 && x.size(1) < (1 << 26), "moe_group_rows: ", num(t), " tokens with ", num(k), " choices, rows of ", num(x.size(1)));
     int64_t cols = 0;
-    at::Tensor row_scales = at::empty({0}, x.options().dtype(at::kFloat));
     c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor row_scales;
     if (given(scales)) {
         check_operand(*scales, x, "scales");
         CAM_ASSERT(scales->scalar_type() == at::kFloat && (scales->dim() == 1 || scales->dim() == 2) && scales->size(0) == t, "moe_group_rows: scales must be float32 [T] or [T, s]");
@@ -212,11 +214,12 @@ Four moe_group_rows_cuda(const at::Tensor& x, const at::Tensor& topk_idx, int64_
         CAM_ASSERT(cols >= 1 && cols < (1 << 26), "moe_group_rows: scales must be float32 [T] or [T, s]");
         auto of = scales->sizes().vec();
         of[0] = t * k;
-        row_scales = at::empty(of, scales->options());
+        row_scales = cuda_empty(of, at::kFloat, x);
+    } else {
+        row_scales = cuda_empty({0}, at::kFloat, x);
     }
-    at::Tensor rows = at::empty({t * k, x.size(1)}, x.options());
-    const auto ints = x.options().dtype(at::kInt);
-    at::Tensor offsets = at::empty({num_experts + 1}, ints), slots = at::empty({t, k}, ints);
+    at::Tensor rows = cuda_empty({t * k, x.size(1)}, x.scalar_type(), x);
+    at::Tensor offsets = cuda_empty({num_experts + 1}, at::kInt, x), slots = cuda_empty({t, k}, at::kInt, x);
     CAM_RT(cam_moe_group_rows(data_or_null(x), x.size(1) * x.element_size(), static_cast<int>(x.element_size()), given(scales) ? floats_or_null(*scales) : nullptr, static_cast<int>(cols),
                               data_or_null(topk_idx), topk_idx.scalar_type() == at::kLong, t, static_cast<int>(k), static_cast<int>(num_experts),
                               data_or_null(rows), floats_or_null(row_scales), offsets.data_ptr<int>(), static_cast<int*>(data_or_null(slots)), stream_now()));
@@ -255,7 +258,7 @@ at::Tensor moe_ungroup_rows_cuda(const at::Tensor& rows, const at::Tensor& slots
                    "moe_ungroup_rows: residual must be [T, h] of the rows' type");
     }
     c10::cuda::CUDAGuard guard(rows.device());
-    at::Tensor out = at::empty({p.tokens, p.h}, rows.options());
+    at::Tensor out = cuda_empty({p.tokens, p.h}, rows.scalar_type(), rows);
     if (p.tokens == 0) return out;
     CAM_RT(cam_moe_ungroup_rows(data_or_null(rows), p.dtype, p.num_rows, p.h, slots.data_ptr<int>(), p.tokens, p.k,
                                 given(weights) ? weights->data_ptr<float>() : nullptr, given(residual) ? residual->data_ptr() : nullptr,
@@ -270,9 +273,8 @@ Two moe_ungroup_rows_backward_cuda(const at::Tensor& dout, const at::Tensor& row
     CAM_ASSERT(dout.scalar_type() == rows.scalar_type() && dout.dim() == 2 && dout.size(0) == p.tokens && dout.size(1) == p.h,
                "moe_ungroup_rows_backward: dout must be [T, h] of the rows' type");
     c10::cuda::CUDAGuard guard(rows.device());
-    const auto floats = rows.options().dtype(at::kFloat);
-    at::Tensor drows = need_drows ? at::empty_like(rows) : none_of(rows);
-    at::Tensor dw = need_dweights ? at::empty({p.tokens, p.k}, floats) : at::empty({0}, floats);
+    at::Tensor drows = need_drows ? cuda_like(rows) : cuda_none(rows);
+    at::Tensor dw = need_dweights ? cuda_empty({p.tokens, p.k}, at::kFloat, rows) : cuda_empty({0}, at::kFloat, rows);
     CAM_RT(cam_moe_ungroup_rows_backward(data_or_null(dout), data_or_null(rows), p.dtype, p.num_rows, p.h, static_cast<const int*>(data_or_null(slots)),
                                          p.tokens, p.k, given(weights) ? floats_or_null(*weights) : nullptr, data_or_null(drows), floats_or_null(dw),
                                          stream_now()));
@@ -292,7 +294,7 @@ Three rms_norm_train_meta(const at::Tensor& x, const OptTensor& residual, const 
 }
 Three rms_norm_backward_meta(const at::Tensor& dy, const OptTensor&, const at::Tensor& sum, const at::Tensor& weight, const at::Tensor&, bool need_dx,
                              bool need_dres, bool need_dw) {
-    return norm_grads_empty(dy, sum, weight, need_dx, need_dres, need_dw);
+    return norm_grads_empty([](const at::Tensor& t) { return at::empty_like(t); }, none_of, dy, sum, weight, need_dx, need_dres, need_dw);
 }
 Four rms_norm_quant_meta(const at::Tensor& x, const at::Tensor&, int64_t quant_mode, const OptTensor& residual, double, bool with_rows) {
     const at::ScalarType qt = norm_quant_type(quant_mode);
@@ -345,8 +347,6 @@ struct RmsNormFunction : public torch::autograd::Function<RmsNormFunction> {
         auto [y, sum, rstd] = op.call(x, residual, weight, eps);
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({given(residual) ? sum : kept_for_backward(x), weight, rstd});
-        ctx->saved_data["dtype"] = static_cast<int64_t>(x.scalar_type());
-        ctx->saved_data["residual"] = given(residual);
         if (given(residual)) return {y, sum};
         return {y};
     }
@@ -354,12 +354,14 @@ struct RmsNormFunction : public torch::autograd::Function<RmsNormFunction> {
         static auto op = find_op<Three(const at::Tensor&, const OptTensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, bool, bool, bool)>(
             "umdk_cam_op_lib::rms_norm_backward");
         // needs_input_grad counts the tensors that were given
-        const bool with = ctx->saved_data["residual"].toBool();
+        const bool with = grads.size() > 1;
         const bool need_dx = ctx->needs_input_grad(0), need_dres = with && ctx->needs_input_grad(1), need_dw = ctx->needs_input_grad(with ? 2 : 1);
-        at::Tensor dy = grads[0], ds = grads.size() > 1 ? grads[1] : at::Tensor();
+        const at::Tensor dy = grads[0], ds = with ? grads[1] : at::Tensor();
         if (!dy.defined() && !ds.defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
         const auto s = ctx->get_saved_variables();
-        if (!dy.defined()) dy = at::zeros_like(s[0], s[0].options().dtype(static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt())));
+        // the sum alone is used; autograd brings its gradient to x's type
+        if (!dy.defined()) return {need_dx ? ds : at::Tensor(), need_dres ? ds : at::Tensor(), need_dw ? at::zeros_like(s[1]) : at::Tensor(), at::Tensor()};
+        BackwardGuard guard;
         auto [dx, dres, dw] = op.call(dy.contiguous(), ds.defined() ? OptTensor(ds.contiguous()) : OptTensor(), s[0], s[1], s[2], need_dx, need_dres, need_dw);
         const bool one = dy.scalar_type() == s[0].scalar_type();
         return {need_dx ? dx : at::Tensor(), need_dres ? (one ? dx : dres) : at::Tensor(), need_dw ? dw : at::Tensor(), at::Tensor()};
@@ -399,9 +401,7 @@ struct RouteFunction : public torch::autograd::Function<RouteFunction> {
         ctx->set_materialize_grads(false);
         ctx->mark_non_differentiable({idx});
         ctx->save_for_backward({kept_for_backward(logits), idx});
-        ctx->saved_data["score"] = score;
-        ctx->saved_data["renormalize"] = renormalize;
-        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["plan"] = std::vector<double>{score == "sigmoid" ? 1.0 : 0.0, renormalize ? 1.0 : 0.0, scale};
         return {idx, w};
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -409,7 +409,9 @@ struct RouteFunction : public torch::autograd::Function<RouteFunction> {
         variable_list out(9);
         if (!grads[1].defined()) return out;
         const auto s = ctx->get_saved_variables();
-        out[0] = op.call(grads[1].contiguous(), s[0], s[1], ctx->saved_data["score"].toStringRef(), ctx->saved_data["renormalize"].toBool(), ctx->saved_data["scale"].toDouble());
+        const auto plan = ctx->saved_data["plan"].toDoubleVector();
+        BackwardGuard guard;
+        out[0] = op.call(grads[1].contiguous(), s[0], s[1], plan[0] != 0.0 ? "sigmoid" : "softmax", plan[1] != 0.0, plan[2]);
         return out;
     }
 };
@@ -448,6 +450,7 @@ struct GroupRowsFunction : public torch::autograd::Function<GroupRowsFunction> {
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         variable_list out(4);
+        BackwardGuard guard;
         if (grads[0].defined()) out[0] = call_ungroup(grads[0].contiguous(), ctx->get_saved_variables()[0], OptTensor(), OptTensor());
         return out;
     }
@@ -471,8 +474,9 @@ struct UngroupRowsFunction : public torch::autograd::Function<UngroupRowsFunctio
         at::Tensor out = call_ungroup(rows, slots, weights, residual);
         // the rows themselves enter the gradient of the weights only
         const bool rows_read = given(weights) && weights->requires_grad();
-        ctx->save_for_backward({rows_read ? kept_for_backward(rows) : rows, kept_for_backward(slots), given(weights) ? kept_for_backward(*weights) : at::Tensor()});
-        ctx->saved_data["residual"] = given(residual);
+        variable_list kept = {rows_read ? kept_for_backward(rows) : rows, kept_for_backward(slots), given(weights) ? kept_for_backward(*weights) : at::Tensor()};
+        if (given(residual)) kept.emplace_back();  // its place says that there was one
+        ctx->save_for_backward(kept);
         return out;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -481,9 +485,10 @@ struct UngroupRowsFunction : public torch::autograd::Function<UngroupRowsFunctio
         if (!grads[0].defined()) return out;
         const auto s = ctx->get_saved_variables();
         // needs_input_grad counts the tensors that were given
-        const bool weighted = s[2].defined(), residual = ctx->saved_data["residual"].toBool();
+        const bool weighted = s[2].defined(), residual = s.size() > 3;
         const bool need_rows = ctx->needs_input_grad(0), need_weights = weighted && ctx->needs_input_grad(2);
         if (need_rows || need_weights) {
+            BackwardGuard guard;
             auto [drows, dw] = op.call(grads[0].contiguous(), s[0], s[1], s[2].defined() ? OptTensor(s[2]) : OptTensor(), need_rows, need_weights);
             if (need_rows) out[0] = drows;
             if (need_weights) out[2] = dw;
