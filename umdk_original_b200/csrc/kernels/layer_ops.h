@@ -49,7 +49,7 @@ struct RouteParams {
     int64_t rows;
     int experts, k, groups, topk_groups, group_top, sigmoid, renormalize;
     float scale;
-    int vec, vec_bias;      // a lane's logits and biases can be read in pieces of 16 bytes (set by the launcher)
+    int vec, vec_bias;      // a lane's logits and biases can be read in whole pieces (set by the launcher)
     int64_t* idx;           // [rows, k]
     float* weights;         // [rows, k]
     const float* dweights;  // backward

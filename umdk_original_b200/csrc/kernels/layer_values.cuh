@@ -60,7 +60,6 @@ __device__ __forceinline__ uint4 load16_stream(const void* p) {
     return v;
 }
 
-// 32-byte pieces for fp32: p is 32-byte aligned wherever rows of eight values are, which the launchers check
 template <int DT>
 __device__ __forceinline__ Raw8<DT> load8(const void* base, int64_t i) {
     Raw8<DT> r;
@@ -133,14 +132,6 @@ __device__ __forceinline__ void store1(void* base, int64_t i, float v) {
     if constexpr (DT == kDtFp32) static_cast<float*>(base)[i] = v;
     else if constexpr (DT == kDtBf16) static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(v);
     else static_cast<__half*>(base)[i] = __float2half_rn(v);
-}
-
-// A value rounded to a type and widened again
-template <int DT>
-__device__ __forceinline__ float rounded(float v) {
-    if constexpr (DT == kDtBf16) return __bfloat162float(__float2bfloat16_rn(v));
-    if constexpr (DT == kDtFp16) return __half2float(__float2half_rn(v));
-    return v;
 }
 
 // ------------------------------------------------------------------------------------------------

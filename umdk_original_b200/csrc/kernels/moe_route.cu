@@ -30,29 +30,33 @@ __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(
 // Consecutive logits of a lane; what is past the row is -inf
 template <int DT, int VPL>
 __device__ __forceinline__ void load_logits(const RouteParams& p, int64_t row, int lane, float* x) {
+    constexpr int kShare = VPL * kBytes<DT>, kWords = kShare / 4;  // of a lane
     const int64_t at = row * p.experts + lane * VPL;
-    if (VPL * kBytes<DT> >= 16 && p.vec) {
+    if (kShare >= 16 && p.vec) {
 #pragma unroll
-        for (int v = 0; v < VPL * kBytes<DT> / 16; ++v) {
-            constexpr int N = 16 / kBytes<DT>;
-            if (lane * VPL < p.experts) {
-                const uint4 r = load16_stream(static_cast<const char*>(p.logits) + at * kBytes<DT> + v * 16);
-                const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+        for (int i = 0; i < VPL; ++i) x[i] = -CUDART_INF_F;
+        if (lane * VPL < p.experts) {
+            const char* from = static_cast<const char*>(p.logits) + at * kBytes<DT>;
+            uint32_t w[kWords > 0 ? kWords : 1];
+            if constexpr (kShare >= 32) {
+                // whole sectors: two pieces of 16 bytes would fetch them twice
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (DT == kDtFp32) x[v * N + i] = __uint_as_float(w[i]);
-                    else if constexpr (DT == kDtBf16) {
-                        x[v * N + 2 * i] = __uint_as_float(w[i] << 16);
-                        x[v * N + 2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-                    } else {
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                        x[v * N + 2 * i] = f.x;
-                        x[v * N + 2 * i + 1] = f.y;
-                    }
+                for (int i = 0; i < kWords; i += 8) load32(w + i, from + i * 4);
+            } else if constexpr (kShare == 16) {
+                const uint4 v = load16_stream(from);
+                w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+            }
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                if constexpr (DT == kDtFp32) x[i] = __uint_as_float(w[i]);
+                else if constexpr (DT == kDtBf16) {
+                    x[2 * i] = __uint_as_float(w[i] << 16);
+                    x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+                } else {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                    x[2 * i] = f.x;
+                    x[2 * i + 1] = f.y;
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; ++i) x[v * N + i] = -CUDART_INF_F;
             }
         }
     } else {
@@ -514,16 +518,25 @@ __global__ void __launch_bounds__(128, VPL <= 16 ? 6 : 4) moe_route_kernel(const
 
 template <int DT, int VPL>
 __device__ __forceinline__ void store_logits(const RouteParams& p, int64_t row, int lane, const float* x) {
+    constexpr int kShare = VPL * kBytes<DT>;
     const int64_t at = row * p.experts + lane * VPL;
-    if (VPL * kBytes<DT> >= 16 && p.vec) {
-        if (lane * VPL < p.experts) {
+    if (kShare >= 16 && p.vec) {
+        if (lane * VPL >= p.experts) return;
+        char* to = static_cast<char*>(p.dlogits) + at * kBytes<DT>;
+        if constexpr (DT == kDtFp32 && kShare >= 32) {
 #pragma unroll
-            for (int v = 0; v < VPL; v += 16 / kBytes<DT>) {
-                uint4 r;
-                if constexpr (DT == kDtFp32) r = *reinterpret_cast<const uint4*>(x + v);
-                else r = narrow8<DT>(x + v).v[0];
-                *reinterpret_cast<uint4*>(static_cast<char*>(p.dlogits) + (at + v) * kBytes<DT>) = r;
+            for (int i = 0; i < VPL; i += 8) store32(to + i * 4, reinterpret_cast<const uint32_t*>(x + i));
+        } else if constexpr (DT == kDtFp32 && kShare == 16) {
+            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(x);
+        } else if constexpr (kShare >= 32) {
+#pragma unroll
+            for (int i = 0; i < VPL; i += 16) {
+                const uint4 a = narrow8<DT>(x + i).v[0], b = narrow8<DT>(x + i + 8).v[0];
+                const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                store32(to + i * 2, w);
             }
+        } else if constexpr (kShare == 16) {
+            *reinterpret_cast<uint4*>(to) = narrow8<DT>(x).v[0];
         }
     } else {
 #pragma unroll
@@ -595,10 +608,13 @@ __global__ void __launch_bounds__(256) moe_route_backward_kernel(const RoutePara
     if (lead) store1<DT>(p.dlogits, row0 + id, d + rest);
 }
 
-// Whether a lane's share can be read in pieces of 16 bytes: it is whole ones and so is the row
+// Whether a lane's share can be read in pieces of 32 bytes, or one of 16: it is whole ones and so is the row
 template <int DT>
 bool whole_pieces(const RouteParams& p, int vpl) {
-    return p.experts % vpl == 0 && vpl * kBytes<DT> % 16 == 0 && p.experts * kBytes<DT> % 16 == 0 && aligned16(p.logits) && aligned16(p.dlogits);
+    const int share = vpl * kBytes<DT>;
+    if (p.experts % vpl != 0 || share < 16) return false;
+    return share >= 32 ? aligned32(p.logits) && aligned32(p.dlogits) && p.experts * kBytes<DT> % 32 == 0
+                       : aligned16(p.logits) && aligned16(p.dlogits) && p.experts * kBytes<DT> % 16 == 0;
 }
 
 template <int DT, int L, int VPL>
