@@ -457,13 +457,11 @@ __device__ __forceinline__ uint32_t ring_copy(uint32_t ring, int threads, int t,
     return ring + 2 * kCopies<DT> * threads * 16;
 }
 template <int DT>
-__device__ __forceinline__ void ring_half(uint32_t ring, int i, int threads, int t, int h, Pair* out) {
-    Raw8<DT> r = {};
-    if ((i * threads + t) * 8 < h) {
+__device__ __forceinline__ void ring_half(uint32_t ring, int i, int threads, int t, Pair* out) {
+    Raw8<DT> r;
 #pragma unroll
-        for (int j = 0; j < kCopies<DT>; ++j)
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.v[j].x), "=r"(r.v[j].y), "=r"(r.v[j].z), "=r"(r.v[j].w) : "r"(ring + ((i * threads + t) * kCopies<DT> + j) * 16) : "memory");
-    }
+    for (int j = 0; j < kCopies<DT>; ++j)
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.v[j].x), "=r"(r.v[j].y), "=r"(r.v[j].z), "=r"(r.v[j].w) : "r"(ring + ((i * threads + t) * kCopies<DT> + j) * 16) : "memory");
     float f[8];
     widen8<DT>(r, f);
 #pragma unroll
@@ -495,6 +493,20 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     if constexpr (STAGES > 0) {
+        // places past the row, which no copy ever reaches, are read with the others
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if ((i * threads + t) * 8 < h) continue;
+            for (int stage = 0; stage < STAGES; ++stage) {
+                uint32_t at = slots + stage * stage_bytes;
+                for (int operand = 0; operand < (p.dsum != nullptr ? 3 : 2); ++operand) {
+                    const int copies = operand == 0 ? kCopies<DT> : kCopies<ST>;
+                    for (int j = 0; j < copies; ++j)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + ((i * threads + t) * copies + j) * 16), "r"(0u) : "memory");
+                    at += 2 * copies * threads * 16;
+                }
+            }
+        }
 #pragma unroll
         for (int i = 0; i < STAGES; ++i) copy(first + i * step, i);
     }
@@ -532,8 +544,8 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
             Pair* g = dy + 4 * i;
             Pair* hat = s + 4 * i;
             if constexpr (STAGES > 0) {
-                ring_half<DT>(at_dy, i, threads, t, h, g);
-                ring_half<ST>(at_s, i, threads, t, h, hat);
+                ring_half<DT>(at_dy, i, threads, t, g);
+                ring_half<ST>(at_s, i, threads, t, hat);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -555,9 +567,9 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
             Pair* hat = s + 4 * i;
             Pair d[4] = {0ull, 0ull, 0ull, 0ull};
             if constexpr (STAGES > 0) {
-                ring_half<DT>(at_dy, i, threads, t, h, g);
-                ring_half<ST>(at_s, i, threads, t, h, hat);
-                if (p.dsum != nullptr) ring_half<ST>(at_ds, i, threads, t, h, d);
+                ring_half<DT>(at_dy, i, threads, t, g);
+                ring_half<ST>(at_s, i, threads, t, hat);
+                if (p.dsum != nullptr) ring_half<ST>(at_ds, i, threads, t, d);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     hat[j] = mul2(hat[j], rstd2);
