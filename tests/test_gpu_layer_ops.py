@@ -4,7 +4,7 @@ import threading
 import pytest
 import torch
 
-from layer_cases import group64
+from layer_cases import group64, norm64, norm_grad_tol, norm_grads64, norm_tol, weight_grad_tol, within
 from umdk_original_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -162,6 +162,76 @@ def test_norm_past_32_bits():
     q, s, _, _ = ops.rms_norm_quant(x.detach(), w.detach(), 3)
     q2, s2, _, _ = ops.rms_norm_quant(part.detach(), w.detach(), 3)
     assert torch.equal(q[-300:].view(torch.int8), q2.view(torch.int8)) and torch.equal(s[-300:], s2)
+
+
+@pytest.mark.parametrize("dtype,residual,weight", [(BF, BF, BF), (torch.float16, torch.float32, torch.float16), (torch.float32, torch.float32, torch.float32),
+                                                   (BF, None, torch.float32)])
+@pytest.mark.parametrize("rows,h", [(40001, 72), (20003, 504), (11000, 520), (9999, 1000), (6007, 2056), (3001, 4096), (1301, 7168), (701, 8200), (700, 16384), (5003, 333)])
+def test_norm_gradients_of_many_rows(dtype, residual, weight, rows, h):
+    """More than two turns of all blocks: rows are loaded ahead (or, with an odd width, not), in both directions and with both gradients."""
+    g = torch.Generator(device=DEV).manual_seed(h)
+    r = lambda *s, d: torch.randn(*s, device=DEV, generator=g).to(d)  # noqa: E731
+    x, w, dy = r(rows, h, d=dtype), r(h, d=weight), r(rows, h, d=dtype)
+    res, ds = (None, None) if residual is None else (r(rows, h, d=residual), r(rows, h, d=residual))
+    leaves = [t.requires_grad_() for t in (x, res, w) if t is not None]
+    out = (ops.rms_norm(x, w),) if res is None else ops.add_rms_norm(x, res, w)
+    grads = torch.autograd.grad(out, leaves, [t for t in (dy, ds) if t is not None])
+    with torch.no_grad():
+        y64, total, _ = norm64(x, res, w, 1e-6)
+        within(out[0].detach(), y64, norm_tol(y64, dtype), "y")
+        del y64
+        assert res is None or torch.equal(out[1], total)
+        d, size, dw, dw_size = norm_grads64(dy, ds, total, w, 1e-6)
+        within(grads[0], d, norm_grad_tol(d, size, dtype), "dx")
+        if res is not None:
+            within(grads[1], d, norm_grad_tol(d, size, residual), "dresidual")
+        within(grads[-1], dw, weight_grad_tol(dw, dw_size, rows, weight), "dweight")
+        # a row's numbers do not depend on how many there are
+        few = ops.rms_norm_train(x[5:9].contiguous(), None if res is None else res[5:9].contiguous(), w)
+        if h % 8 == 0:
+            assert torch.equal(few[0], out[0][5:9])
+            back = ops.rms_norm_backward(dy[5:9].contiguous(), None if ds is None else ds[5:9].contiguous(), total[5:9].contiguous(), w, few[2])
+            assert torch.equal(back[0], grads[0][5:9])
+
+
+@pytest.mark.parametrize("mode", [2, 3, 4])
+def test_norm_quant_at_16_bytes(mode):
+    """Operands at 16 bytes that are not at 32: the same bits."""
+    def at_16(t):
+        buf = torch.zeros(t.numel() + 8, device=DEV, dtype=t.dtype)
+        return buf[8:].view(t.shape).copy_(t)
+    x, r, w = (torch.randn(*s, device=DEV).to(BF) for s in ((300, 1280), (300, 1280), (1280,)))
+    a, b = ops.rms_norm_quant(x, w, mode, r, 1e-6, True), ops.rms_norm_quant(at_16(x), at_16(w), mode, at_16(r), 1e-6, True)
+    assert all(torch.equal(u.view(torch.int8) if u.dtype == torch.float8_e4m3fn else u, v.view(torch.int8) if v.dtype == torch.float8_e4m3fn else v) for u, v in zip(a, b))
+
+
+@pytest.mark.parametrize("t,k,h,dtype", [(3000, 8, 2047, BF), (3000, 4, 1023, torch.float32), (2500, 2, 4095, torch.float16), (3000, 3, 8, BF), (1100, 32, 512, torch.float32)])
+def test_many_rows_there_and_back(t, k, h, dtype):
+    """Sizes at which every form of the kernels goes round: the identity of both directions, gradients against index arithmetic."""
+    g = torch.Generator(device=DEV).manual_seed(t + h)
+    idx = torch.rand(t, 40, device=DEV, generator=g).topk(k, -1).indices
+    idx = torch.where(torch.rand(t, k, device=DEV, generator=g) < 0.1, torch.full_like(idx, -1), idx)
+    x = torch.randn(t, h, device=DEV, generator=g).to(dtype).requires_grad_()
+    rows, _, off, slots = ops.moe_group_rows(x, idx, 40)
+    n, valid = int(off[-1]), slots >= 0
+    assert n == int(valid.sum()) and not rows[n:].any()
+    back = rows[slots.clamp(min=0).long()]
+    assert torch.equal(back[valid], x[:, None].expand(-1, k, -1)[valid])
+    results, w = torch.randn(t * k, h, device=DEV, generator=g).to(dtype).requires_grad_(), torch.rand(t, k, device=DEV, generator=g).requires_grad_()
+    out = ops.moe_ungroup_rows(results, slots, w)
+    dout, drows = torch.randn(t, h, device=DEV, generator=g).to(dtype), torch.randn(t * k, h, device=DEV, generator=g).to(dtype)
+    dx, dres, dw = torch.autograd.grad((rows, out), (x, results, w), (drows, dout))
+    half, tiny, u = {BF: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 0.0}[dtype], 2.0 ** -24, 2.0 ** -24
+    at = slots.clamp(min=0).long()
+    for got, terms in ((out, torch.where(valid[..., None], results.detach().double()[at] * w.detach().double()[..., None], 0.0)),
+                       (dx, torch.where(valid[..., None], drows.double()[at], 0.0))):
+        want = terms.sum(1)
+        within(got.detach(), want, want.abs() * half + terms.abs().sum(1) * (k + 3) * u + tiny)
+    want = torch.zeros(t * k, h, device=DEV, dtype=torch.float64)
+    want[slots[valid].long()] = (dout.double()[:, None] * w.detach().double()[..., None])[valid]
+    within(dres, want, want.abs() * (half + 2 * u) + tiny)
+    terms = torch.where(valid[..., None], results.detach().double()[at], 0.0) * dout.double()[:, None]
+    within(dw, terms.sum(-1), terms.abs().sum(-1) * (h / 16 + 64) * u + 2.0 ** -140)
 
 
 def test_rows_past_32_bits():

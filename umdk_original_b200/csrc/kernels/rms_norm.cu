@@ -731,8 +731,8 @@ template <int DT, int ST, int WT>
 int launch_backward_types(RmsNormBackwardParams p, cudaStream_t stream) {
     int access = access_of(p.h, p.dy, p.dsum, p.sum, p.weight, p.dx, p.dres, p.partial);
     // fp32 goes by 32 bytes
-    const bool all32 = aligned32(p.dy) && aligned32(p.dsum) && aligned32(p.sum) && aligned32(p.weight) && aligned32(p.dx) && aligned32(p.dres) && aligned32(p.partial);
-    if (!all32 && (DT == kDtFp32 || ST == kDtFp32 || WT == kDtFp32 || !aligned32(p.partial))) access = kByOne;
+    auto whole = [](int type, auto... ps) { return type != kDtFp32 || (aligned32(ps) && ...); };
+    if (!whole(DT, p.dy, p.dx) || !whole(ST, p.sum, p.dsum, p.dres) || !whole(WT, p.weight) || !whole(kDtFp32, p.partial)) access = kByOne;
     const Backward r = backward_of(p, DT, access != kByOne);
     const int64_t blocks = static_cast<int64_t>(r.blocks) * sm_count_of_current_device();
     p.parts = static_cast<int>(p.parts < blocks ? p.parts : blocks);
