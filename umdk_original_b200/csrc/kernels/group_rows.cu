@@ -362,13 +362,13 @@ struct Piece {
 
 // A piece of its token's rows per thread, weighted and summed in the order of the choices, U of them in flight
 template <int DT, int B, int U, class Index>
-__global__ void __launch_bounds__(256) ungroup_rows_kernel(const UngroupRowsParams p) {
+__global__ void __launch_bounds__(128) ungroup_rows_kernel(const UngroupRowsParams p) {
     using P = Piece<DT, B>;
     constexpr int N = P::N, H = N / 2;
     const Index pieces = static_cast<Index>(p.h / N);
     pdl_wait();
     pdl_release();
-    const Index i = static_cast<Index>(blockIdx.x) * 256 + threadIdx.x;
+    const Index i = static_cast<Index>(blockIdx.x) * 128 + threadIdx.x;
     if (i >= static_cast<Index>(p.tokens) * pieces) return;
     const Index token = i / pieces;
     const int64_t c = static_cast<int64_t>(i - token * pieces) * N, pair0 = static_cast<int64_t>(token) * p.k, to = static_cast<int64_t>(token) * p.h + c;
@@ -378,14 +378,19 @@ __global__ void __launch_bounds__(256) ungroup_rows_kernel(const UngroupRowsPara
     for (int j0 = 0; j0 < p.k; j0 += U) {
         P row[U];
         float w[U];
+        int slot[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int s = j0 + u < p.k ? __ldg(p.slots + pair0 + j0 + u) : -1;
-            const bool in = s >= 0 && s < p.num_rows;
-            w[u] = !in ? 0.f : p.weights != nullptr ? __ldg(p.weights + pair0 + j0 + u) : 1.f;
-            row[u].clear();
-            if (in) row[u].load(p.rows, static_cast<int64_t>(s) * p.h + c);
+            slot[u] = j0 + u < p.k ? __ldg(p.slots + pair0 + j0 + u) : -1;
+            if (slot[u] >= p.num_rows) slot[u] = -1;
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            row[u].clear();
+            if (slot[u] >= 0) row[u].load(p.rows, static_cast<int64_t>(slot[u]) * p.h + c);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = slot[u] < 0 ? 0.f : p.weights != nullptr ? __ldg(p.weights + pair0 + j0 + u) : 1.f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const Pair w2 = pair(w[u], w[u]);
@@ -651,10 +656,10 @@ int piece_of(const UngroupRowsParams& p, int bytes) {
 
 template <int DT, int B, int U>
 int launch_ungroup(const UngroupRowsParams& p, cudaStream_t stream) {
-    const int64_t n = p.tokens * (p.h / Piece<DT, B>::N), blocks = (n + 255) / 256;
+    const int64_t n = p.tokens * (p.h / Piece<DT, B>::N), blocks = (n + 127) / 128;
     if (blocks > 0x7FFFFFFF) return static_cast<int>(cudaErrorInvalidValue);
     const dim3 grid(static_cast<unsigned>(blocks));
-    return blocks * 256 < 0x7FFFFFFF ? launch_pdl(ungroup_rows_kernel<DT, B, U, uint32_t>, grid, 256, 0, stream, p) : launch_pdl(ungroup_rows_kernel<DT, B, U, uint64_t>, grid, 256, 0, stream, p);
+    return blocks * 128 < 0x7FFFFFFF ? launch_pdl(ungroup_rows_kernel<DT, B, U, uint32_t>, grid, 128, 0, stream, p) : launch_pdl(ungroup_rows_kernel<DT, B, U, uint64_t>, grid, 128, 0, stream, p);
 }
 
 template <int DT, int B>
