@@ -194,6 +194,23 @@ def test_norm_gradients_of_many_rows(dtype, residual, weight, rows, h):
             assert torch.equal(back[0], grads[0][5:9])
 
 
+@pytest.mark.parametrize("dtype,sums", [(BF, BF), (torch.float16, torch.float32), (torch.float32, torch.float32)])
+@pytest.mark.parametrize("rows,h,shift", [(9001, 255, 0), (9001, 257, 0), (1201, 4097, 0), (601, 8191, 0), (601, 8193, 0), (4001, 256, 1), (4001, 264, 1),
+                                          (601, 8192, 1), (601, 8200, 1)])
+def test_norm_gradients_value_by_value(dtype, sums, rows, h, shift):
+    """Odd widths, and rows that start off every boundary, where the threads' share of a row changes."""
+    g = torch.Generator(device=DEV).manual_seed(h)
+    r = lambda *s, d: torch.randn(*s, device=DEV, generator=g).to(d)  # noqa: E731
+    total, dy, ds = (r(rows * h + shift, d=d)[shift:].view(rows, h) for d in (sums, dtype, sums))
+    w = r(h, d=dtype)
+    rstd = (total.double().square().mean(1) + 1e-6).rsqrt().float()
+    dx, dres, dw = ops.rms_norm_backward(dy, ds, total, w, rstd, True, True, True)
+    d, size, want, dw_size = norm_grads64(dy, ds, total, w, 1e-6)
+    within(dx, d, norm_grad_tol(d, size, dtype), "dx")
+    within(dx if sums == dtype else dres, d, norm_grad_tol(d, size, sums), "dresidual")  # one tensor where they are of one type
+    within(dw, want, weight_grad_tol(want, dw_size, rows, dtype), "dweight")
+
+
 @pytest.mark.parametrize("mode", [2, 3, 4])
 def test_norm_quant_at_16_bytes(mode):
     """Operands at 16 bytes that are not at 32: the same bits."""

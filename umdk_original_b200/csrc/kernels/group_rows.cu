@@ -5,7 +5,7 @@
 // sort by one cluster: every warp counts a stretch of pairs (lanes with the same expert find each other with a ballot per bit of its
 // index), sums over warps, blocks and experts give every pair its row.  Everything else is bound by memory: a token is read once and written
 // to its k rows, or its k rows are read and summed, whole sectors per thread.  8192 tokens of 4096 bf16 to 8 of 128 experts, 604 MB each way:
-// sort and copy 106 us, back 101 us (0.91 of the copy rate), gradients of rows and weights 179 us (1.14 GB, 0.97 of it).
+// sort and copy 106 us, back 92 us (the copy rate), gradients of rows and weights 179 us (1.14 GB, 0.97 of it).
 #include <cooperative_groups.h>
 
 #include "launch.h"

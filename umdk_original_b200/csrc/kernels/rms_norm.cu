@@ -470,11 +470,12 @@ __device__ __forceinline__ void ring_half(uint32_t ring, int i, int threads, int
 }
 
 // Registers of a thread at most; the launcher counts with them
-template <int ST, int STAGES>
-constexpr int kBackwardRegisters = STAGES == 0 ? 128 : ST == kDtFp32 ? 96 : 64;
+template <int ST, int HALVES, int STAGES>
+constexpr int kBackwardRegisters = HALVES == 1 ? 64 : STAGES == 0 ? 128 : ST == kDtFp32 ? 96 : 64;
 
-template <int DT, int ST, int WT, int VEC, bool WARP, int THREADS, int STAGES>
-__global__ void __launch_bounds__(THREADS, THREADS > 512 ? 1 : 65536 / (THREADS * kBackwardRegisters<ST, STAGES>))
+// HALVES: eights of values per thread
+template <int DT, int ST, int WT, int VEC, int HALVES, bool WARP, int THREADS, int STAGES>
+__global__ void __launch_bounds__(THREADS, THREADS > 512 ? 1 : 65536 / (THREADS * kBackwardRegisters<ST, HALVES, STAGES>))
 rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
     extern __shared__ __align__(16) uint8_t dynamic[];  // WARP: per warp; the stages, and at the end the warps' sums
     __shared__ __align__(16) float red[128];
@@ -513,35 +514,35 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
     }
     Raw16<WT> w;  // as it lies in memory: sixteen values in two halves
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < HALVES; ++i) {
         Pair f[4];
         load_half<WT, VEC>(p.weight, Place{0, t, threads, h}, i, f);
 #pragma unroll
         for (int j = 0; j < 4; ++j) narrow2<WT>(w, 4 * i + j, f[j]);
     }
-    Pair acc[8];
+    Pair acc[4 * HALVES];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = 0ull;
+    for (int i = 0; i < 4 * HALVES; ++i) acc[i] = 0ull;
     int stage = 0, turn = 0;
     for (int64_t row = first; row < p.rows; row += step) {
         const Place at{row * h, t, threads, h};
         const float rstd = __ldg(p.rstd + row);
         const Pair rstd2 = pair(rstd, rstd);
         const uint32_t at_dy = slots + stage * stage_bytes, at_s = at_dy + 2 * kCopies<DT> * threads * 16, at_ds = at_s + 2 * kCopies<ST> * threads * 16;
-        Pair dy[8], s[8];
+        Pair dy[4 * HALVES], s[4 * HALVES];
         if constexpr (STAGES > 0) {
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES > 0 ? STAGES - 1 : 0) : "memory");
             if (DT == kDtFp32 || ST == kDtFp32) __syncwarp();
         } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < HALVES; ++i) {
                 load_half<DT, VEC>(p.dy, at, i, dy + 4 * i);
                 load_half<ST, VEC>(p.sum, at, i, s + 4 * i);
             }
         }
         Pair products = 0ull;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < HALVES; ++i) {
             Pair* g = dy + 4 * i;
             Pair* hat = s + 4 * i;
             if constexpr (STAGES > 0) {
@@ -563,7 +564,7 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
         const float share = -along / static_cast<float>(h);
         const Pair share2 = pair(share, share);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < HALVES; ++i) {
             Pair* g = dy + 4 * i;
             Pair* hat = s + 4 * i;
             Pair d[4] = {0ull, 0ull, 0ull, 0ull};
@@ -599,7 +600,7 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
         if (STAGES > 0) asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < 8 * HALVES; ++j) {
             const int c = half_column<VEC>(cols_at, j / 8, j % 8);
             const float2 f = split(acc[j / 2]);
             if (c < h) cols[warp * h + c] = j % 2 ? f.y : f.x;
@@ -612,8 +613,8 @@ rms_norm_backward_kernel(const RmsNormBackwardParams p, uint32_t stage_bytes) {
             mine[c] = a;
         }
     } else {
-        store_half<kDtFp32, VEC>(mine, cols_at, 0, acc);
-        store_half<kDtFp32, VEC>(mine, cols_at, 1, acc + 4);
+#pragma unroll
+        for (int i = 0; i < HALVES; ++i) store_half<kDtFp32, VEC>(mine, cols_at, i, acc + 4 * i);
     }
 }
 
@@ -692,12 +693,23 @@ struct Backward {
 
 int blocks_by_registers(const Shape& s, int registers) { return s.threads > 512 ? 1 : 65536 / (registers * s.threads); }
 
+// Eight values per thread
+Shape shape_by_eights(int h) {
+    const int pieces = (h + 7) / 8;
+    return pieces <= 32 ? Shape{true, kWarpRows * 32, 1} : Shape{false, (pieces + 31) / 32 * 32, 1};
+}
+
+// Values loaded one by one: eight per thread where a block has the threads for it.  8192 x 4095 bf16 107 us, with sixteen 197 us
+// (128 registers a thread leave half the loads in flight).
+int halves_of(int h, bool single) { return single && h <= 8192 ? 1 : 2; }
+
 Backward backward_of(const RmsNormBackwardParams& p, int dtype, bool ring) {
-    Backward r{shape_of(p.h, 1), 0, 0, 0, 0};
+    const int halves = halves_of(p.h, !ring);
+    Backward r{halves == 1 ? shape_by_eights(p.h) : shape_of(p.h, 1), 0, 0, 0, 0};
     const int group = r.shape.warp ? 32 : r.shape.threads, groups = r.shape.threads / group;
     const int size = dtype == kDtFp32 ? 4 : 2, sum = p.sum_type == kDtFp32 ? 4 : size, copies = size + sum + (p.dsum != nullptr ? sum : 0);
     const int sums = r.shape.warp ? kWarpRows * p.h * 4 : 0, room = 220 * 1024;
-    const Backward plain{r.shape, blocks_by_registers(r.shape, 128), 0, 0, sums};
+    const Backward plain{r.shape, blocks_by_registers(r.shape, halves == 1 ? 64 : 128), 0, 0, sums};
     r.blocks = blocks_by_registers(r.shape, sum == 2 ? 64 : 96);
     // below two turns of all blocks there is nothing to load ahead
     if (!ring || turns_of(r.shape, p.rows) <= 2 * static_cast<int64_t>(r.blocks) * sm_count_of_current_device()) return plain;
@@ -712,19 +724,19 @@ Backward backward_of(const RmsNormBackwardParams& p, int dtype, bool ring) {
     return r;
 }
 
-template <int DT, int ST, int WT, int VEC, bool WARP, int THREADS, int STAGES>
+template <int DT, int ST, int WT, int VEC, int HALVES, bool WARP, int THREADS, int STAGES>
 int launch_backward_kernel(const RmsNormBackwardParams& p, const Backward& r, cudaStream_t stream) {
     static SmemLimitCache limit;
-    auto kernel = rms_norm_backward_kernel<DT, ST, WT, VEC, WARP, THREADS, STAGES>;
+    auto kernel = rms_norm_backward_kernel<DT, ST, WT, VEC, HALVES, WARP, THREADS, STAGES>;
     const cudaError_t err = limit.ensure(kernel, r.smem);
     if (err != cudaSuccess) return static_cast<int>(err);
     return launch_pdl(kernel, dim3(static_cast<unsigned>(p.parts)), r.shape.threads, static_cast<size_t>(r.smem), stream, p, static_cast<uint32_t>(r.stage_bytes));
 }
 
-template <int DT, int ST, int WT, int VEC, int STAGES>
+template <int DT, int ST, int WT, int VEC, int HALVES, int STAGES>
 int launch_backward(const RmsNormBackwardParams& p, const Backward& r, cudaStream_t stream) {
-    if (r.shape.warp) return launch_backward_kernel<DT, ST, WT, VEC, true, 256, STAGES>(p, r, stream);
-    return r.shape.threads <= 512 ? launch_backward_kernel<DT, ST, WT, VEC, false, 512, STAGES>(p, r, stream) : launch_backward_kernel<DT, ST, WT, VEC, false, 1024, STAGES>(p, r, stream);
+    if (r.shape.warp) return launch_backward_kernel<DT, ST, WT, VEC, HALVES, true, 256, STAGES>(p, r, stream);
+    return r.shape.threads <= 512 ? launch_backward_kernel<DT, ST, WT, VEC, HALVES, false, 512, STAGES>(p, r, stream) : launch_backward_kernel<DT, ST, WT, VEC, HALVES, false, 1024, STAGES>(p, r, stream);
 }
 
 template <int DT, int ST, int WT>
@@ -736,10 +748,9 @@ int launch_backward_types(RmsNormBackwardParams p, cudaStream_t stream) {
     const Backward r = backward_of(p, DT, access != kByOne);
     const int64_t blocks = static_cast<int64_t>(r.blocks) * sm_count_of_current_device();
     p.parts = static_cast<int>(p.parts < blocks ? p.parts : blocks);
-    const int rc = access == kByOne  ? launch_backward<DT, ST, WT, kByOne, 0>(p, r, stream)
-                   : r.stages == 4   ? launch_backward<DT, ST, WT, kBy16, 4>(p, r, stream)
-                   : r.stages == 2   ? launch_backward<DT, ST, WT, kBy16, 2>(p, r, stream)
-                                     : launch_backward<DT, ST, WT, kBy16, 0>(p, r, stream);
+    int rc;
+    if (access == kByOne) rc = halves_of(p.h, true) == 1 ? launch_backward<DT, ST, WT, kByOne, 1, 0>(p, r, stream) : launch_backward<DT, ST, WT, kByOne, 2, 0>(p, r, stream);
+    else rc = r.stages == 4 ? launch_backward<DT, ST, WT, kBy16, 2, 4>(p, r, stream) : r.stages == 2 ? launch_backward<DT, ST, WT, kBy16, 2, 2>(p, r, stream) : launch_backward<DT, ST, WT, kBy16, 2, 0>(p, r, stream);
     if (rc != 0 || p.dweight == nullptr) return rc;
     return launch_pdl(add_parts_kernel<WT>, dim3(static_cast<unsigned>((p.h + 31) / 32)), 1024, 0, stream, static_cast<const float*>(p.partial), p.parts, p.h, p.dweight);
 }
@@ -764,7 +775,8 @@ extern "C" int cam_launch_rms_norm(const cam::RmsNormParams* p, int dtype, cudaS
 // Most blocks that a launch for these rows has
 extern "C" int cam_rms_norm_backward_blocks(int64_t rows, int h) {
     using namespace cam;
-    const Shape s = shape_of(h, 1);
+    // an upper bound: operands of a width in eights that are not aligned get by with what their aligned kin have
+    const Shape s = h % 8 != 0 && halves_of(h, true) == 1 ? shape_by_eights(h) : shape_of(h, 1);
     const int64_t turns = turns_of(s, rows), most = static_cast<int64_t>(sm_count_of_current_device()) * blocks_by_registers(s, 64);
     return static_cast<int>(turns < most ? turns : most);
 }
