@@ -194,6 +194,24 @@ def test_norm_gradients_of_many_rows(dtype, residual, weight, rows, h):
             assert torch.equal(back[0], grads[0][5:9])
 
 
+@pytest.mark.parametrize("dtype,residual", [(BF, BF), (torch.float16, torch.float32), (torch.float32, None)])
+@pytest.mark.parametrize("rows,h,shift", [(2003, 255, 0), (2003, 257, 0), (2001, 256, 1), (301, 4097, 0), (201, 8191, 0), (201, 8193, 0), (201, 8192, 1), (101, 12008, 3)])
+def test_norm_value_by_value(dtype, residual, rows, h, shift):
+    g = torch.Generator(device=DEV).manual_seed(h + shift)
+    r = lambda n, d: torch.randn(n + shift, device=DEV, generator=g).to(d)[shift:]  # noqa: E731
+    x, w = r(rows * h, dtype).view(rows, h), r(h, dtype)
+    res = None if residual is None else r(rows * h, residual).view(rows, h)
+    y64, total, _ = norm64(x, res, w, 1e-6)
+    y = ops.rms_norm(x, w) if res is None else ops.add_rms_norm(x, res, w)[0]
+    within(y, y64, norm_tol(y64, dtype), "rows")
+    q, s, kept, rows8 = ops.rms_norm_quant(x, w, 2, res, 1e-6, True)
+    assert torch.equal(rows8, y) and (res is None or torch.equal(kept, total))
+    rel = 40 * 2.0 ** -24  # of a value of y (32 u), a scale's division and product
+    top = y64.abs().amax(-1)
+    within(s, top / 127, top / 127 * rel, "scales")
+    within(q.double() * s.double()[:, None], y64, s.double()[:, None] * (0.5 + 127 * 3 * rel), "values")
+
+
 @pytest.mark.parametrize("dtype,sums", [(BF, BF), (torch.float16, torch.float32), (torch.float32, torch.float32)])
 @pytest.mark.parametrize("rows,h,shift", [(9001, 255, 0), (9001, 257, 0), (1201, 4097, 0), (601, 8191, 0), (601, 8193, 0), (4001, 256, 1), (4001, 264, 1),
                                           (601, 8192, 1), (601, 8200, 1)])

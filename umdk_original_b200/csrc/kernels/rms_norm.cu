@@ -82,10 +82,15 @@ struct Place {
     int t, threads, h;
 };
 
-// Column of the first of a thread's sixteen values (kByOne: of value j)
+// Pairs of a piece: sixteen values, but eight where they go one by one, so that twice the threads have loads in flight: 8192 x 4095 bf16
+// 88 us instead of 103, 20000 x 1023 fp16 50 instead of 63.
+template <int VEC>
+constexpr int kPairs = VEC == kByOne ? 4 : 8;
+
+// Column of the first value of a thread's piece (kByOne: of value j)
 template <int VEC>
 __device__ __forceinline__ int column(const Place& at, int v, int j) {
-    return VEC == kByOne ? (v * 16 + j) * at.threads + at.t : (v * at.threads + at.t) * 16 + j;
+    return VEC == kByOne ? (v * 8 + j) * at.threads + at.t : (v * at.threads + at.t) * 16 + j;
 }
 
 // Zeros past the row
@@ -96,7 +101,7 @@ __device__ __forceinline__ Raw16<DT> load16(const void* base, const Place& at, i
     const char* p = static_cast<const char*>(base) + (at.row0 + c) * kBytes<DT>;
     if constexpr (VEC == kByOne) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < 2 * kPairs<VEC>; ++j) {
             const int d = column<VEC>(at, v, j);
             if constexpr (DT == kDtFp32) r.w[j] = d < at.h ? __float_as_uint(load1<DT>(base, at.row0 + d)) : 0u;
             else {
@@ -130,7 +135,7 @@ __device__ __forceinline__ void store16(void* base, const Place& at, int v, cons
     char* p = static_cast<char*>(base) + (at.row0 + c) * kBytes<DT>;
     if constexpr (VEC == kByOne) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < 2 * kPairs<VEC>; ++j) {
             const int d = column<VEC>(at, v, j);
             if (d >= at.h) continue;
             if constexpr (DT == kDtFp32) static_cast<uint32_t*>(base)[at.row0 + d] = r.w[j];
@@ -170,7 +175,7 @@ __device__ __forceinline__ void load_weight_as(const void* w, const Place& at, i
         }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = widen2<DT>(r, i);
+    for (int i = 0; i < kPairs<VEC>; ++i) out[i] = widen2<DT>(r, i);
 }
 template <int DT, int VEC>
 __device__ __forceinline__ void load_weight(const void* w, bool fp32, const Place& at, int v, Pair* out) {
@@ -220,14 +225,14 @@ template <int VEC>
 __device__ __forceinline__ void store_int8(void* q, const Place& at, int v, const Pair* y, float inv) {
     uint32_t o[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 2 * kPairs<VEC>; ++j) {
         const float2 f = split(y[j / 2]);
         const int a = max(-127, min(127, __float2int_rn((j % 2 ? f.y : f.x) * inv)));  // NaN becomes 0; the row's scale is NaN then
         o[j / 4] |= (static_cast<uint32_t>(a) & 0xFFu) << (j % 4 * 8);
     }
     int8_t* row = static_cast<int8_t*>(q) + at.row0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kPairs<VEC> / 4; ++i) {
         const int c = column<VEC>(at, v, VEC == kByOne ? 0 : 8 * i);
         if constexpr (VEC != kByOne) {
             if (c < at.h) *reinterpret_cast<uint2*>(row + c) = make_uint2(o[2 * i], o[2 * i + 1]);
@@ -256,7 +261,7 @@ __device__ __forceinline__ void block_scale(float amax, bool power_of_two, float
 }
 
 template <int DT, int MODE, int NP, int VEC, bool WARP>
-__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : NP == 2 ? 512 : 1024)
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : NP == 2 && VEC != kByOne ? 512 : 1024, VEC == kByOne && !WARP && NP == 1 ? 2 : 1)  // int8 one by one in 50 registers: 127 us, in 32 92
 rms_norm_kernel(const RmsNormParams p) {
     __shared__ __align__(16) float red[64];
     clear_sums<WARP>(red);
@@ -266,7 +271,7 @@ rms_norm_kernel(const RmsNormParams p) {
     pdl_wait();
     pdl_release();
     if (WARP && row >= p.rows) return;
-    Pair s[NP][8];
+    Pair s[NP][kPairs<VEC>];
     {
         Raw16<DT> x[NP];
 #pragma unroll
@@ -275,7 +280,7 @@ rms_norm_kernel(const RmsNormParams p) {
 #pragma unroll
             for (int v = 0; v < NP; ++v) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) s[v][i] = widen2<DT>(x[v], i);
+                for (int i = 0; i < kPairs<VEC>; ++i) s[v][i] = widen2<DT>(x[v], i);
             }
         } else if (DT != kDtFp32 && p.res_type == kDtFp32) {
             Raw16<kDtFp32> r[NP];
@@ -284,7 +289,7 @@ rms_norm_kernel(const RmsNormParams p) {
 #pragma unroll
             for (int v = 0; v < NP; ++v) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < kPairs<VEC>; ++i) {
                     s[v][i] = add2(widen2<DT>(x[v], i), widen2<kDtFp32>(r[v], i));
                     narrow2<kDtFp32>(r[v], i, s[v][i]);
                 }
@@ -298,7 +303,7 @@ rms_norm_kernel(const RmsNormParams p) {
             for (int v = 0; v < NP; ++v) {
                 r[v] = add16<DT>(x[v], r[v]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) s[v][i] = widen2<DT>(r[v], i);
+                for (int i = 0; i < kPairs<VEC>; ++i) s[v][i] = widen2<DT>(r[v], i);
                 store16<DT, VEC>(p.sum, at, v, r[v]);
             }
         }
@@ -307,17 +312,17 @@ rms_norm_kernel(const RmsNormParams p) {
 #pragma unroll
     for (int v = 0; v < NP; ++v) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) squares = fma2(s[v][i], s[v][i], squares);
+        for (int i = 0; i < kPairs<VEC>; ++i) squares = fma2(s[v][i], s[v][i], squares);
     }
     const float2 halves = split(squares);
     float sum = halves.x + halves.y, top = 0.f;
     // times the weight already: int8 needs the largest product along with the sum
 #pragma unroll
     for (int v = 0; v < NP; ++v) {
-        Pair w[8];
+        Pair w[kPairs<VEC>];
         load_weight<DT, VEC>(p.weight, p.weight_type == kDtFp32, at, v, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kPairs<VEC>; ++i) {
             s[v][i] = mul2(s[v][i], w[i]);
             if (MODE == kInt8) {
                 const float2 f = split(s[v][i]);
@@ -334,11 +339,11 @@ rms_norm_kernel(const RmsNormParams p) {
 #pragma unroll
     for (int v = 0; v < NP; ++v) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[v][i] = mul2(s[v][i], rstd2);
+        for (int i = 0; i < kPairs<VEC>; ++i) s[v][i] = mul2(s[v][i], rstd2);
         if (MODE == kRowsOnly || p.y != nullptr) {
             Raw16<DT> y;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) narrow2<DT>(y, i, s[v][i]);
+            for (int i = 0; i < kPairs<VEC>; ++i) narrow2<DT>(y, i, s[v][i]);
             store16<DT, VEC>(p.y, at, v, y);
         }
         if constexpr (MODE == kInt8) store_int8<VEC>(p.q, at, v, s[v], inv8);
@@ -641,11 +646,11 @@ __global__ void __launch_bounds__(1024) add_parts_kernel(const float* __restrict
 // ------------------------------------------------------------------------------------------------
 // Launches
 // ------------------------------------------------------------------------------------------------
-// Threads that share a row and sixteens of values per thread.  They follow from the width alone: a row's sums are added in the same
+// Threads that share a row and sixteens of values per thread (pieces).  They follow from the width alone: a row's sums are added in the same
 // order however many rows there are.
 struct Shape {
     bool warp;
-    int threads, sixteens;
+    int threads, pieces;
 };
 
 Shape shape_of(int h, int most) {
@@ -653,17 +658,24 @@ Shape shape_of(int h, int most) {
     if (pieces <= 32 * most) return {true, kWarpRows * 32, pieces <= 32 ? 1 : 2};
     return {false, ((pieces + most - 1) / most + 31) / 32 * 32, most};
 }
+// The same for values that go one by one, by eights
+Shape shape_by_eights(int h) {
+    const int pieces = (h + 7) / 8;
+    if (pieces <= 32) return {true, kWarpRows * 32, 1};
+    return pieces <= 1024 ? Shape{false, (pieces + 31) / 32 * 32, 1} : Shape{false, ((pieces + 1) / 2 + 31) / 32 * 32, 2};
+}
 static_assert(kWarpRows * 32 == 256 && 512 * 2 * 16 >= kNormMaxHidden, "every row has its threads");
 
 int64_t turns_of(const Shape& s, int64_t rows) { return s.warp ? (rows + kWarpRows - 1) / kWarpRows : rows; }
 
 template <int DT, int MODE, int VEC>
 int launch_norm(const RmsNormParams& p, cudaStream_t stream) {
-    constexpr int most = VEC == kByOne ? 1 : 2;  // with two, single values leave too few threads: 8192 x 4095 bf16 178 us instead of 103
-    const Shape s = shape_of(p.h, most);
+    const Shape s = VEC == kByOne ? shape_by_eights(p.h) : shape_of(p.h, 2);
     const dim3 grid(static_cast<unsigned>(turns_of(s, p.rows)));
-    if (!s.warp) return launch_pdl(rms_norm_kernel<DT, MODE, most, VEC, false>, grid, s.threads, 0, stream, p);
-    return s.sixteens == 1 ? launch_pdl(rms_norm_kernel<DT, MODE, 1, VEC, true>, grid, s.threads, 0, stream, p) : launch_pdl(rms_norm_kernel<DT, MODE, most, VEC, true>, grid, s.threads, 0, stream, p);
+    // by eights a warp has one piece and a block one or two, by sixteens a warp has one or two and a block two
+    constexpr int most = VEC == kByOne ? 1 : 2;
+    if (s.warp) return s.pieces == 1 ? launch_pdl(rms_norm_kernel<DT, MODE, 1, VEC, true>, grid, s.threads, 0, stream, p) : launch_pdl(rms_norm_kernel<DT, MODE, most, VEC, true>, grid, s.threads, 0, stream, p);
+    return s.pieces == 1 ? launch_pdl(rms_norm_kernel<DT, MODE, most, VEC, false>, grid, s.threads, 0, stream, p) : launch_pdl(rms_norm_kernel<DT, MODE, 2, VEC, false>, grid, s.threads, 0, stream, p);
 }
 
 // How all operands of a launch can be read
@@ -692,12 +704,6 @@ struct Backward {
 };
 
 int blocks_by_registers(const Shape& s, int registers) { return s.threads > 512 ? 1 : 65536 / (registers * s.threads); }
-
-// Eight values per thread
-Shape shape_by_eights(int h) {
-    const int pieces = (h + 7) / 8;
-    return pieces <= 32 ? Shape{true, kWarpRows * 32, 1} : Shape{false, (pieces + 31) / 32 * 32, 1};
-}
 
 // Values loaded one by one: eight per thread where a block has the threads for it.  8192 x 4095 bf16 107 us, with sixteen 197 us
 // (128 registers a thread leave half the loads in flight).
