@@ -212,6 +212,26 @@ def test_norm_value_by_value(dtype, residual, rows, h, shift):
     within(q.double() * s.double()[:, None], y64, s.double()[:, None] * (0.5 + 127 * 3 * rel), "values")
 
 
+@pytest.mark.parametrize("h", [96, 203, 1024, 4096, 7168, 9001])
+def test_norm_int8_rows_that_are_not_finite(h):
+    """NaN, or an infinity before the norm: the scale is NaN; an infinity behind it: infinite.  The values are zero, other rows as without."""
+    g = torch.Generator(device=DEV).manual_seed(h)
+    x, w = torch.randn(9, h, device=DEV, generator=g), torch.rand(h, device=DEV, generator=g) + 0.5
+    want = ops.rms_norm_quant(x, w, 2)
+    bad = x.clone()
+    bad[1, h - 1], bad[3, 0], bad[6] = float("nan"), float("inf"), float("-inf")
+    q, s, _, _ = ops.rms_norm_quant(bad, w, 2)
+    assert s[[1, 3, 6]].isnan().all() and not q[[1, 3, 6]].any()
+    keep = [0, 2, 4, 5, 7, 8]
+    assert torch.equal(q[keep], want[0][keep]) and torch.equal(s[keep], want[1][keep])
+    for value in (float("nan"), float("inf")):
+        wrong = w.clone()
+        wrong[h // 2] = value
+        q, s, _, y = ops.rms_norm_quant(x, wrong, 2, None, 1e-6, True)
+        assert (s.isnan() if value != value else s.isinf()).all() and not q.any()
+        assert y.isfinite().sum() == 9 * (h - 1)
+
+
 @pytest.mark.parametrize("dtype,sums", [(BF, BF), (torch.float16, torch.float32), (torch.float32, torch.float32)])
 @pytest.mark.parametrize("rows,h,shift", [(9001, 255, 0), (9001, 257, 0), (1201, 4097, 0), (601, 8191, 0), (601, 8193, 0), (4001, 256, 1), (4001, 264, 1),
                                           (601, 8192, 1), (601, 8200, 1)])

@@ -4,8 +4,8 @@
 //   dx = dresidual = ds + r (w dy - s r mean(w dy s r)),   dw = sum over the rows of dy s r
 //
 // Bound by memory in both directions, with the issue slots close behind: arithmetic runs on pairs (16-bit sums in one instruction,
-// products and sums of two fp32 values in one).  16384 x 4096 with an fp32 residual 119 us, 32768 x 7168 to e4m3 240 us (1.03 of a plain
-// copy's rate both), backward 8192 x 7168 bf16 81 us (0.88).  A row stays in the registers of the threads that share it: read once, summed, scaled and
+// products and sums of two fp32 values in one).  16384 x 4096 with an fp32 residual 119 us, 32768 x 7168 to e4m3 or int8 240 us
+// (1.03 of a plain copy's rate all), backward 8192 x 7168 bf16 81 us (0.88).  A row stays in the registers of the threads that share it: read once, summed, scaled and
 // written.  A thread owns 16 consecutive values at a time, so blocks of 128 for e4m3 are eight lanes.  The norm is that of the
 // rounded sum, so a backward pass (or a later layer) that reads the stored sum sees the numbers that were normalised.
 #include "../common/quant.cuh"
@@ -200,10 +200,13 @@ __device__ __forceinline__ void clear_sums(float (&red)[N]) {
     if (!WARP && threadIdx.x < N && (threadIdx.x & 31) >= blockDim.x >> 5) red[threadIdx.x] = 0.f;
     if (!WARP && blockDim.x < N && threadIdx.x + blockDim.x < N && ((threadIdx.x + blockDim.x) & 31) >= blockDim.x >> 5) red[threadIdx.x + blockDim.x] = 0.f;
 }
+// Magnitudes compare as integers, and NaN is the largest.
+__device__ __forceinline__ float larger(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
+
 template <bool WARP, bool MAX>
 __device__ __forceinline__ void over_row(float& sum, float& top, float* red) {
     sum = warp_sum(sum);
-    if (MAX) top = warp_max(top);
+    if (MAX) top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top)));
     if constexpr (WARP) {
         __syncwarp();
     } else {
@@ -220,7 +223,7 @@ __device__ __forceinline__ void over_row(float& sum, float& top, float* red) {
             sum += v.x + v.y + (v.z + v.w);
             if (MAX) {
                 const float4 m = *reinterpret_cast<const float4*>(red + 32 + i);
-                top = fmaxf(fmaxf(top, fmaxf(m.x, m.y)), fmaxf(m.z, m.w));
+                top = larger(larger(top, larger(m.x, m.y)), larger(m.z, m.w));
             }
         }
     }
@@ -229,15 +232,20 @@ __device__ __forceinline__ void over_row(float& sum, float& top, float* red) {
 // ------------------------------------------------------------------------------------------------
 // Forward
 // ------------------------------------------------------------------------------------------------
-// Sixteen values of a row in 8 bits
+// Sixteen values of a row in 8 bits.  Adding 1.5 x 2^23 rounds to the nearest whole number and leaves it in the low byte; no value is above
+// 127 / inv.  A conversion and a clamp for each took 257 us for 32768 x 7168 bf16
+// instead of 235 (142 with the registers below).  inv is NaN for a row with NaN, or with an
+// infinity before the norm, and zero for one with an infinity behind it: its scale says so, its values are zero.
 template <int VEC>
 __device__ __forceinline__ void store_int8(void* q, const Place& at, int v, const Pair* y, float inv) {
+    const uint32_t keep = inv > 0.f ? 0xFFFFFFFFu : 0u;
+    const Pair inv2 = pair(inv, inv), whole = pair(12582912.f, 12582912.f);
     uint32_t o[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int j = 0; j < 2 * kPairs<VEC>; ++j) {
-        const float2 f = split(y[j / 2]);
-        const int a = max(-127, min(127, __float2int_rn((j % 2 ? f.y : f.x) * inv)));  // NaN becomes 0; the row's scale is NaN then
-        o[j / 4] |= (static_cast<uint32_t>(a) & 0xFFu) << (j % 4 * 8);
+    for (int j = 0; j < kPairs<VEC>; j += 2) {
+        const float2 a = split(add2(mul2(y[j], inv2), whole)), b = split(add2(mul2(y[j + 1], inv2), whole));
+        const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
+        o[j / 2] = __byte_perm(lo, hi, 0x5410) & keep;
     }
     int8_t* row = static_cast<int8_t*>(q) + at.row0;
 #pragma unroll
@@ -269,8 +277,14 @@ __device__ __forceinline__ void block_scale(float amax, bool power_of_two, float
     }
 }
 
+// Blocks of an SM, as a bound on registers.  Rows in 8 bits: 64 instead of 80 and 86, so that four blocks of 7168 columns have loads on their way
+// and not three: 32768 x 7168 bf16 to e4m3 174 -> 144 us, to int8 235 -> 142, with a residual 244 -> 239 and 294 -> 237; fp32 does not fit
+// (16384 x 4096 to int8 128 -> 137).  Values one by one: 32 registers, 8192 x 4095 bf16 to int8 92 us, with 50 127.
 template <int DT, int MODE, int NP, int VEC, bool WARP>
-__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : NP == 2 && VEC != kByOne ? 512 : 1024, VEC == kByOne && !WARP && NP == 1 ? 2 : 1)  // int8 one by one in 50 registers: 127 us, in 32 92
+constexpr int kNormBlocks = !WARP && (VEC == kByOne ? NP == 1 : NP == 2 && MODE != kRowsOnly && DT != kDtFp32) ? 2 : 1;
+
+template <int DT, int MODE, int NP, int VEC, bool WARP>
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : NP == 2 && VEC != kByOne ? 512 : 1024, kNormBlocks<DT, MODE, NP, VEC, WARP>)
 rms_norm_kernel(const RmsNormParams p) {
     __shared__ __align__(16) float red[64];
     clear_sums<WARP>(red);
@@ -335,7 +349,7 @@ rms_norm_kernel(const RmsNormParams p) {
             s[v][i] = mul2(s[v][i], w[i]);
             if (MODE == kInt8) {
                 const float2 f = split(s[v][i]);
-                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(f.x), "f"(f.y));
             }
         }
     }
