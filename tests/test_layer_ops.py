@@ -259,6 +259,21 @@ def test_route(device, dtype, with_bias, name):
     within(w, w64, route_weight_tol(w64) * 4, "weights")
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("score,group_top", [("sigmoid", 2), ("softmax", 1), ("softmax", 2)])
+@pytest.mark.parametrize("e,groups,open_groups,k", [(34, 2, 1, 5), (126, 2, 1, 9), (252, 4, 3, 8), (300, 4, 2, 7), (320, 4, 1, 3), (510, 5, 2, 6), (999, 3, 2, 12), (21, 7, 4, 2)])
+def test_route_groups_that_end_inside_a_lane(device, dtype, score, group_top, e, groups, open_groups, k):
+    g = gen(device, e + k)
+    x, bias = masked_logits(g, 13, e, dtype), 0.1 * randn(g, e)
+    kw = dict(k=k, score=score, num_groups=groups, topk_groups=open_groups, group_top=group_top)
+    for b in (None, bias):
+        idx, w = ops.moe_route(x, bias=b, **kw)
+        idx64, w64 = route64(x, bias=b, **kw)
+        assert torch.equal(idx, idx64)
+        within(w, w64, route_weight_tol(w64) * 4, "weights")
+
+
 @native
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -276,16 +276,26 @@ __device__ __forceinline__ uint32_t open_groups(const RouteParams& p, int64_t ro
             if (first + i < p.experts) all[first + i] = value[i];
         }
         __syncwarp();
-        if (sub < p.groups) {
-            int i = sub % size;  // lanes start at different banks
-            for (int n = 0; n < size; ++n) {
-                const float v = all[sub * size + i];
+        // as many lanes per group as there are, a power of two of them: 17885 x 300 in 4 groups 55 us, with one lane each 71
+        int share = 1;
+        while (2 * share * p.groups <= L) share *= 2;
+        const int group = sub / share;
+        if (group < p.groups) {
+            for (int i = sub % share; i < size; i += share) {
+                const float v = all[group * size + i];
                 two = fmaxf(two, fminf(one, v));
                 one = fmaxf(one, v);
-                i = i + 1 == size ? 0 : i + 1;
             }
         }
         __syncwarp();
+        for (int o = 1; o < share; o <<= 1) {
+            const float a = __shfl_xor_sync(0xFFFFFFFFu, one, o), b = __shfl_xor_sync(0xFFFFFFFFu, two, o);
+            two = fmaxf(fminf(one, a), fmaxf(two, b));
+            one = fmaxf(one, a);
+        }
+        const int from = min(L - 1, sub * share);
+        one = __shfl_sync(0xFFFFFFFFu, one, from, L);
+        two = __shfl_sync(0xFFFFFFFFu, two, from, L);
     }
     const float mine = p.group_top == 2 && two > -CUDART_INF_F ? one + two : one;
     const bool some = sub < p.groups && mine > -CUDART_INF_F;
@@ -407,9 +417,14 @@ __global__ void __launch_bounds__(128, VPL <= 16 ? 6 : 4) moe_route_kernel(const
         if (size % VPL == 0) {
             closed = first < p.experts && !(open >> (first / size) & 1u);
         } else {
+            int group = first / size, end = (group + 1) * size;  // past the row: groups there are none of
 #pragma unroll
             for (int i = 0; i < VPL; ++i) {
-                if (first + i < p.experts && !(open >> ((first + i) / size) & 1u)) value[i] = x[i] = -CUDART_INF_F;
+                if (first + i == end) {
+                    ++group;
+                    end += size;
+                }
+                if (first + i < p.experts && !(open >> group & 1u)) value[i] = x[i] = -CUDART_INF_F;
             }
             odd = true;
         }
