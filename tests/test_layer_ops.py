@@ -173,6 +173,35 @@ def test_norm_quant(device, dtype, residual, mode, h):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, FL])
+@pytest.mark.parametrize("mode", [3, 4])
+@pytest.mark.parametrize("h", [128, 1152, 7168])
+def test_norm_e4m3_rows_that_are_not_finite(device, dtype, mode, h):
+    """NaN behind the norm: its block has a NaN scale and NaN codes.  An infinity: an infinite scale, a NaN code, zeros beside it.  Other
+    blocks and rows are as without."""
+    g = gen(device, h)
+    x, w = randn(g, 5, h, dtype=dtype), torch.rand(h, generator=g, device=device) + 0.5
+    want_q, want_s = (t.float() for t in ops.rms_norm_quant(x, w, mode)[:2])
+    n, at = h // 128 - 1, torch.arange(h, device=device) == h - 3
+    for value in (float("nan"), float("inf"), -float("inf")):
+        wrong = w.clone()
+        wrong[h - 3] = value
+        q, s = (t.float() for t in ops.rms_norm_quant(x, wrong, mode)[:2])
+        assert torch.equal(q[:, : n * 128], want_q[:, : n * 128]) and torch.equal(s[:, :n], want_s[:, :n])
+        if value != value:
+            assert s[:, n].isnan().all() and q[:, n * 128:].isnan().all()
+        else:
+            assert (s[:, n] == float("inf")).all() and q[:, at].isnan().all() and not q[:, n * 128:][:, ~at[n * 128:]].any()
+    # before the norm: 1 / rms is NaN, or it is zero and an infinity times that is NaN
+    bad = x.clone()
+    bad[1, 5], bad[3, h - 1] = float("nan"), float("inf")
+    q, s = (t.float() for t in ops.rms_norm_quant(bad, w, mode)[:2])
+    assert s[1].isnan().all() and q[1].isnan().all() and s[3, n].isnan() and q[3, n * 128:].isnan().all()
+    assert s[3, :n].isfinite().all() and not q[3, : n * 128].any()
+    assert torch.equal(q[[0, 2, 4]], want_q[[0, 2, 4]]) and torch.equal(s[[0, 2, 4]], want_s[[0, 2, 4]])
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_norm_shapes(device):
     """Leading dimensions, no rows, rows that start anywhere in memory."""
     g = gen(device, 5)

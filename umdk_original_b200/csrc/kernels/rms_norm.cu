@@ -202,6 +202,10 @@ __device__ __forceinline__ void clear_sums(float (&red)[N]) {
 }
 // Magnitudes compare as integers, and NaN is the largest.
 __device__ __forceinline__ float larger(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
+__device__ __forceinline__ float widest(float top, float a, float b) {
+    asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(a), "f"(b));
+    return top;
+}
 
 template <bool WARP, bool MAX>
 __device__ __forceinline__ void over_row(float& sum, float& top, float* red) {
@@ -264,13 +268,15 @@ __device__ __forceinline__ void store_int8(void* q, const Place& at, int v, cons
 }
 
 // Power-of-two scale: the least 2^k >= max(amax, 1e-4) / 448.  448 = 1.75 x 2^8, so k is the exponent of amax less 8, one more where the
-// significand is above 1.75: exact, without a division.
+// significand is above 1.75: exact, without a division.  A block with NaN has a NaN scale and NaN codes; one with an infinity has an
+// infinite scale, NaN in the infinity's place and zeros in the others, so no product of it is finite.
 __device__ __forceinline__ void block_scale(float amax, bool power_of_two, float& scale, float& inv) {
-    const float a = fmaxf(amax, 1e-4f);
+    const float a = larger(amax, 1e-4f);
     if (power_of_two) {
         const uint32_t b = __float_as_uint(a), e = (b >> 23) - 8u + ((b & 0x7FFFFFu) > 0x600000u ? 1u : 0u);
-        scale = __uint_as_float(e << 23);
-        inv = __uint_as_float((254u - e) << 23);
+        const bool finite = b < 0x7F800000u;
+        scale = finite ? __uint_as_float(e << 23) : a;
+        inv = finite ? __uint_as_float((254u - e) << 23) : b == 0x7F800000u ? 0.f : a;
     } else {
         scale = a * (1.f / 448.f);
         inv = __fdividef(448.f, a);
@@ -349,7 +355,7 @@ rms_norm_kernel(const RmsNormParams p) {
             s[v][i] = mul2(s[v][i], w[i]);
             if (MODE == kInt8) {
                 const float2 f = split(s[v][i]);
-                asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(f.x), "f"(f.y));
+                top = widest(top, f.x, f.y);
             }
         }
     }
@@ -376,10 +382,10 @@ rms_norm_kernel(const RmsNormParams p) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float2 f = split(s[v][i]);
-                amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                amax = widest(amax, f.x, f.y);
             }
 #pragma unroll
-            for (int o = 4; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+            for (int o = 4; o >= 1; o >>= 1) amax = larger(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
             float scale, inv;
             block_scale(amax, p.quant_mode == 4, scale, inv);
             const Pair inv2 = pair(inv, inv);

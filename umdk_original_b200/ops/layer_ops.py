@@ -124,6 +124,7 @@ def rms_norm_quant_cpu(x, weight, quant_mode, residual=None, eps=1e-6, with_rows
         s = s.view(x.shape[:-1])
     else:
         q, s = ref.quant_fp8_1x128(flat, quant_mode == 4)
+        s = torch.where(flat.view(-1, h // 128, 128).isnan().any(-1), torch.full_like(s, float("nan")), s)  # rounding up to a power of two loses it
         s = s.view(*x.shape[:-1], h // 128)
     return q.view(x.shape), s, x.new_empty(0) if residual is None else total, y.to(x.dtype) if with_rows else x.new_empty(0)
 
