@@ -5,7 +5,7 @@ import torch
 from layer_cases import (U, group64, half_step, norm64, norm_grad_tol, norm_grads64, norm_tol, route64, route_grad64, route_weight_tol, weight_grad_tol,
                          within)
 from umdk_original_b200 import ops
-from umdk_original_b200.ops import cam_ops
+from umdk_original_b200.ops import cam_ops, reference as ref
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -170,6 +170,20 @@ def test_norm_quant(device, dtype, residual, mode, h):
     v = y64 / s.double().repeat_interleave(128, -1)
     step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)  # 2^-9 at the least
     within(q, v.clamp(-448, 448), step / 2 + v.abs() * 3 * rel, "codes")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("mode", [2, 3, 4])
+@pytest.mark.parametrize("h", [128, 1024, 7168])
+def test_norm_quant_is_that_of_the_dispatch(device, mode, h):
+    """fp32 rows come out as they were quantised: codes and scales are the bits that the dispatch's formula has for them, up to 3e38."""
+    g = gen(device, h)
+    x, w = randn(g, 64, h), randn(g, h)
+    w[1] = 5e37
+    for weight in (w[2:3].expand(h).contiguous(), w):
+        q, s, _, y = (t.cpu() for t in ops.rms_norm_quant(x, weight, mode, None, 1e-6, True))
+        q2, s2 = ref.quant_int8_token(y) if mode == 2 else ref.quant_fp8_1x128(y, mode == 4)
+        assert y.isfinite().all() and torch.equal(s.view(s2.shape), s2) and torch.equal(q.float(), q2.float())
 
 
 @pytest.mark.parametrize("device", DEVICES)

@@ -278,8 +278,8 @@ __device__ __forceinline__ void block_scale(float amax, bool power_of_two, float
         scale = finite ? __uint_as_float(e << 23) : a;
         inv = finite ? __uint_as_float((254u - e) << 23) : b == 0x7F800000u ? 0.f : a;
     } else {
-        scale = a * (1.f / 448.f);
-        inv = __fdividef(448.f, a);
+        scale = a / 448.f;  // both divided as the dispatch does: the same bits from the same rows
+        inv = 448.f / a;
     }
 }
 
