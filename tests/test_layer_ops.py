@@ -391,6 +391,30 @@ def test_route_special_rows(device):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("group_top", [1, 2])
+@pytest.mark.parametrize("e", [16, 60])
+def test_route_groups_of_rows_that_are_not_finite(device, dtype, score, with_bias, group_top, e):
+    """A softmax of NaN or infinity has no value: where groups or experts are ranked by it nothing is chosen; elsewhere logits rank as they
+    are and NaN is left out."""
+    g = gen(device, 13)
+    x, bias = randn(g, 7, e, dtype=dtype), 0.1 * randn(g, e) if with_bias else None
+    x[0, 3], x[1, 4], x[2] = float("nan"), float("inf"), float("nan")
+    x[3, 1] = x[3, e - 2] = float("inf")
+    x[4, : e // 4] = -float("inf")
+    kw = dict(bias=bias, score=score, num_groups=4, topk_groups=2, group_top=group_top)
+    idx, w = ops.moe_route(x, 3, **kw)
+    want, w64 = route64(x, 3, **kw)
+    if score == "softmax" and (with_bias or group_top == 2):
+        want[:4] = -1
+    assert torch.equal(idx, want)
+    assert w[[0, 1, 2, 3] if score == "softmax" else [0, 2]].isnan().all()
+    within(w[4:], w64[4:], route_weight_tol(w64[4:]), "weights")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_route_close_scores(device, dtype):
     """Many rows with sigmoid and bias: neighbours closer than fp32 can tell are ranked in 64 bits."""
     g = gen(device, 8)

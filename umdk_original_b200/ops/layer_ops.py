@@ -170,7 +170,7 @@ def moe_route_cpu(logits, k, bias=None, score="softmax", num_groups=1, topk_grou
         best = value.view(t, num_groups, -1).sort(-1, descending=True).values[..., :group_top]
         best = torch.where(best[..., :1] > float("-inf"), best.masked_fill(best == float("-inf"), 0.0).sum(-1, keepdim=True), best[..., :1]).squeeze(-1)
         top = best.sort(dim=-1, descending=True, stable=True).indices[:, :topk_groups]
-        open_ = torch.zeros(t, num_groups, dtype=torch.bool).scatter_(1, top, True)
+        open_ = torch.zeros(t, num_groups, dtype=torch.bool).scatter_(1, top, True) & (best > float("-inf"))
         rank = torch.where(open_.repeat_interleave(e // num_groups, 1), rank, low)
     value, idx = rank.sort(dim=-1, descending=True, stable=True)
     empty = value[:, :k] == float("-inf")
