@@ -260,6 +260,22 @@ def test_norm_quant_at_16_bytes(mode):
     assert all(torch.equal(u.view(torch.int8) if u.dtype == torch.float8_e4m3fn else u, v.view(torch.int8) if v.dtype == torch.float8_e4m3fn else v) for u, v in zip(a, b))
 
 
+def test_softmax_weights_and_their_gradient_are_of_one_softmax():
+    """Two experts, weights as they are: the gradient of the first weight by the second logit is minus the product of both weights, to the
+    bit, and the weights are an fp32 softmax."""
+    d = torch.linspace(0.0, 12.0, 1 << 14, device=DEV)
+    x = torch.stack([torch.zeros_like(d), -d], 1).contiguous().requires_grad_()
+    idx, w = ops.moe_route(x, 2, None, "softmax", renormalize=False)
+    assert torch.equal(idx, torch.tensor([0, 1], device=DEV).expand_as(idx))
+    (dx,) = torch.autograd.grad(w, x, torch.tensor([1.0, 0.0], device=DEV).expand_as(w).contiguous())
+    w = w.detach()
+    assert torch.equal(dx[:, 1], -(w[:, 0] * w[:, 1]))
+    # u = 2^-24: expf 2 u, of which the first weight takes the second's share, a sum, a reciprocal, and one product for the second
+    want = torch.softmax(x.detach().double(), -1)
+    share, u = want[:, 1:], 2.0 ** -24
+    within(w, want, want * (torch.cat([2 + 2 * share, 5 + 2 * share], 1) * u))
+
+
 @pytest.mark.parametrize("t,k,h,dtype", [(3000, 8, 2047, BF), (3000, 4, 1023, torch.float32), (2500, 2, 4095, torch.float16), (3000, 3, 8, BF), (1100, 32, 512, torch.float32)])
 def test_many_rows_there_and_back(t, k, h, dtype):
     """Sizes at which every form of the kernels goes round: the identity of both directions, gradients against index arithmetic."""

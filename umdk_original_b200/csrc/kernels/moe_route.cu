@@ -371,8 +371,13 @@ __global__ void __launch_bounds__(128, VPL <= 16 ? 6 : 4) moe_route_kernel(const
         top = seg_max<L>(top);
         nan = nan || top == CUDART_INF_F;  // a softmax of infinity has no value
         float sum = 0.f;
+        if (p.renormalize) {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) sum += quick_exp(x[i] - top);
+            for (int i = 0; i < VPL; ++i) sum += quick_exp(x[i] - top);
+        } else {  // the weights are divided by it: the terms that the backward pass adds
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) sum += expf(x[i] - top);
+        }
         inv_sum = 1.f / seg_sum<L>(sum);
     }
     // what a group's score is made of, and, with a bias, what experts are ranked by; -inf: cannot be chosen
