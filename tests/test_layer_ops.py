@@ -519,6 +519,21 @@ def test_ungroup_rows_and_gradients(device, dtype, t, k, h, weighted, with_resid
         assert torch.equal(grads[-1], dout)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h", [7, 8, 264, 2048, 2050])
+def test_ungroup_weight_gradients_of_places_without_a_row(device, dtype, h):
+    """They are zero whatever the token's gradient holds."""
+    g = gen(device, h)
+    rows, w = randn(g, 6, h, dtype=dtype), torch.rand(2, 3, generator=g, device=device)
+    slots = torch.tensor([[0, -1, 9], [-1, -1, 3]], device=device, dtype=torch.int32)
+    dout = torch.ones(2, h, device=device, dtype=dtype)
+    dout[0, h // 2], dout[1, h - 1] = float("inf"), float("nan")
+    _, dw = ops.moe_ungroup_rows_backward(dout, rows, slots, w)
+    none = (slots < 0) | (slots >= 6)
+    assert not dw[none].any() and not dw[~none].isfinite().any()
+
+
 @native
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(256) ungroup_rows_backward_kernel(const Ungrou
 #pragma unroll
                     for (int v = 0; v < H; ++v) sum = fma2(d.get(v), row[u].get(v), sum);
                     const float2 f = split(sum);
-                    dot[u] += f.x + f.y;
+                    dot[u] += slot[u] >= 0 ? f.x + f.y : 0.f;  // an infinity times the zeros of no row is not one
                 }
             }
         }

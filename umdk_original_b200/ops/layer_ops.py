@@ -296,7 +296,7 @@ def moe_ungroup_rows_backward_cpu(dout, rows, slots, topk_weights=None, need_dro
         drows[slots[valid].long()] = (d[:, None] * w[..., None])[valid]
         drows = drows.to(rows.dtype)
     if need_dweights:
-        dw = (picked * d[:, None]).sum(-1)
+        dw = torch.where(valid, (picked * d[:, None]).sum(-1), torch.zeros(()))
     return drows, dw
 
 
