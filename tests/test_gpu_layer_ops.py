@@ -305,6 +305,77 @@ def test_many_rows_there_and_back(t, k, h, dtype):
     within(dw, terms.sum(-1), terms.abs().sum(-1) * (h / 16 + 64) * u + 2.0 ** -140)
 
 
+def many_slots(t, k, m, g, drop=0.1):
+    """Slots of t tokens among m rows, some of none; in every 512 rows some that nobody names, and the last ones."""
+    free = torch.arange(m, device=DEV)
+    free = free[(free % 512 > 2) & (free < m - 40)]
+    slots = free[torch.randperm(free.numel(), device=DEV, generator=g)[: t * k]].to(torch.int32).view(t, k)
+    return torch.where(torch.rand(t, k, device=DEV, generator=g) < drop, torch.full_like(slots, -1), slots)
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("t,k,h", [(40000, 8, 16), (131072, 8, 8), (70000, 2, 21), (20000, 8, 1032), (16400, 8, 40)])
+def test_gradients_of_many_rows_of_which_some_have_no_token(dtype, t, k, h):
+    """More rows and slots than the blocks that write zeros look at in one go; rows of no slot lie everywhere.  Any alignment of the slots."""
+    g = torch.Generator(device=DEV).manual_seed(h)
+    m = t * k + t * k // 64 + 77
+    slots = many_slots(t, k, m, g)
+    w, dout, rows = torch.rand(t, k, device=DEV, generator=g), torch.randn(t, h, device=DEV, generator=g).to(dtype), torch.randn(m, h, device=DEV, generator=g).to(dtype)
+    drows, dw = ops.moe_ungroup_rows_backward(dout, rows, slots, w)
+    valid = slots >= 0
+    unused = torch.ones(m, dtype=torch.bool, device=DEV)
+    unused[slots[valid].long()] = False
+    assert unused[-40:].all() and unused.view(-1)[: m // 512 * 512].view(-1, 512).any(1).all() and not drows[unused].any()
+    half, tiny = (2.0 ** -8 if dtype == BF else 0.0), 2.0 ** -130
+    want = dout.double()[:, None] * w.double()[..., None]
+    at = slots.clamp(min=0).long()
+    within(torch.where(valid[..., None], drows[at], 0.0), torch.where(valid[..., None], want, 0.0), want.abs() * (half + 2.0 ** -23) + tiny)
+    terms = torch.where(valid[..., None], rows[at], 0.0).double() * dout.double()[:, None]
+    within(dw, terms.sum(-1), terms.abs().sum(-1) * (h / 16 + 64) * 2.0 ** -24 + 2.0 ** -140)
+    odd = torch.empty(t * k + 1, dtype=torch.int32, device=DEV)[1:].view(t, k).copy_(slots)
+    assert same(ops.moe_ungroup_rows_backward(dout, rows, odd, w), (drows, dw))
+    assert torch.equal(ops.moe_ungroup_rows_backward(dout, rows, slots, w, True, False)[0], drows)
+
+
+def test_gradients_of_many_rows_in_two_graphs():
+    """The map of used rows belongs to a call: graphs that are replayed in turn, with other slots each time."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    t, k, h = 20000, 8, 24
+    m = t * k + 5000
+    inputs = [[torch.randn(t, h, device=DEV, generator=g).to(BF), torch.randn(m, h, device=DEV, generator=g).to(BF), many_slots(t, k, m, g), torch.rand(t, k, device=DEV, generator=g)]
+              for _ in range(2)]
+    ops.moe_ungroup_rows_backward(*inputs[0])
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph, args in zip(graphs, inputs):
+        with torch.cuda.graph(graph):
+            outs.append(ops.moe_ungroup_rows_backward(*args))
+    for i in range(3):
+        for args in inputs:
+            args[2].copy_(many_slots(t, k, m, g, 0.3 * i))
+        for j in ((0, 1), (1, 0), (0, 1))[i]:
+            graphs[j].replay()
+        for args, out in zip(inputs, outs):
+            assert same(ops.moe_ungroup_rows_backward(*args), out)
+
+
+def test_gradients_of_many_rows_take_time_like_their_number():
+    """Eight times the rows take at most 24 times the time, whatever part of the small case is launches."""
+    def milliseconds(t, k, h):
+        g = torch.Generator(device=DEV).manual_seed(7)
+        m = t * k * 65 // 64 + 100
+        args = torch.randn(t, h, device=DEV, generator=g).to(BF), torch.randn(m, h, device=DEV, generator=g).to(BF), many_slots(t, k, m, g), torch.rand(t, k, device=DEV, generator=g)
+        times = []
+        for _ in range(6):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            ops.moe_ungroup_rows_backward(*args)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+    assert milliseconds(131072, 8, 16) <= 24 * milliseconds(16384, 8, 16)
+
+
 def test_rows_past_32_bits():
     t, k, h, e = 40000, 8, 8192, 16
     g = torch.Generator(device=DEV).manual_seed(1)

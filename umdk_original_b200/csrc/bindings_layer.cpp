@@ -275,9 +275,11 @@ Two moe_ungroup_rows_backward_cuda(const at::Tensor& dout, const at::Tensor& row
     c10::cuda::CUDAGuard guard(rows.device());
     at::Tensor drows = need_drows ? cuda_like(rows) : cuda_none(rows);
     at::Tensor dw = need_dweights ? cuda_empty({p.tokens, p.k}, at::kFloat, rows) : cuda_empty({0}, at::kFloat, rows);
+    const int64_t words = need_drows ? cam_moe_ungroup_rows_backward_words(p.dtype, p.num_rows, p.h, p.tokens, p.k) : 0;
+    at::Tensor used = words > 0 ? cuda_empty({words}, at::kInt, rows) : at::Tensor();
     CAM_RT(cam_moe_ungroup_rows_backward(data_or_null(dout), data_or_null(rows), p.dtype, p.num_rows, p.h, static_cast<const int*>(data_or_null(slots)),
                                          p.tokens, p.k, given(weights) ? floats_or_null(*weights) : nullptr, data_or_null(drows), floats_or_null(dw),
-                                         stream_now()));
+                                         static_cast<uint32_t*>(data_or_null(used)), stream_now()));
     return {drows, dw};
 }
 

@@ -490,9 +490,32 @@ __device__ __forceinline__ float warp_sums8(const float (&v)[8]) {
 }
 
 constexpr int kZeroRange = 4096;  // rows that a block looks after at a time: a bit each
+// Slots that such a block reads in all its rounds at most; beyond, they are marked in a map first, which is two launches more.  Looking / map,
+// bf16: 98304 rows of 256 29 / 30 us, of 2048 182 / 184; 131072 of 256 (two rounds) 74 / 37; 262144 of 256 297 / 70; 1048576 of 16 16000 / 203.
+constexpr int64_t kMostLooks = 1 << 17;
+
+// Which rows a slot names, a bit each, for the blocks that write zeros to the others: one look at the slots by all SMs.
+__global__ void __launch_bounds__(256) clear_used_kernel(uint32_t* used, int64_t words) {
+    pdl_wait();
+    pdl_release();
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i < words) used[i] = 0u;
+}
+__global__ void __launch_bounds__(256) mark_used_kernel(const int* slots, int64_t pairs, int64_t num_rows, uint32_t* used) {
+    pdl_wait();
+    pdl_release();
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x;
+    int s[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s[u] = first + u * 256 < pairs ? __ldg(slots + first + u * 256) : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        if (s[u] >= 0 && s[u] < num_rows) atomicOr(used + s[u] / 32, 1u << (s[u] % 32));
+    }
+}
 
 // Gradients of rows (weight x gradient of the token) and of weights (row . gradient of the token), a token per warp or block.  The first
-// `zero_blocks` write zeros to rows that no token uses: each marks its share of the rows by looking at all slots.
+// `zero_blocks` write zeros to rows that no token uses: they read p.used, or each marks its share of the rows by looking at all slots.
 constexpr int kOddRows = 0;  // B: rows that start anywhere, in pieces of sixteen bytes of each row
 
 template <int DT, int B, int U, bool WARP>
@@ -512,19 +535,23 @@ __global__ void __launch_bounds__(256) ungroup_rows_backward_kernel(const Ungrou
         const int64_t pairs = p.tokens * p.k;
         for (int64_t from = static_cast<int64_t>(blockIdx.x) * range; from < p.num_rows; from += static_cast<int64_t>(zero_blocks) * range) {
             const int n = static_cast<int>(p.num_rows - from < range ? p.num_rows - from : range);
-            for (int i = threadIdx.x; i * 32 < n; i += blockDim.x) used[i] = 0u;
-            __syncthreads();
-            auto mark = [&](int slot) {
-                const int64_t s = slot - from;
-                if (s >= 0 && s < n) atomicOr(used + s / 32, 1u << (s % 32));
-            };
-            const int64_t fours = aligned16(p.slots) ? pairs / 4 : 0;
+            if (p.used != nullptr) {
+                for (int i = threadIdx.x; i * 32 < n; i += blockDim.x) used[i] = __ldg(p.used + from / 32 + i);
+            } else {
+                for (int i = threadIdx.x; i * 32 < n; i += blockDim.x) used[i] = 0u;
+                __syncthreads();
+                auto mark = [&](int slot) {
+                    const int64_t s = slot - from;
+                    if (s >= 0 && s < n) atomicOr(used + s / 32, 1u << (s % 32));
+                };
+                const int64_t fours = aligned16(p.slots) ? pairs / 4 : 0;
 #pragma unroll 4
-            for (int64_t i = threadIdx.x; i < fours; i += blockDim.x) {
-                const int4 s = __ldg(reinterpret_cast<const int4*>(p.slots) + i);
-                mark(s.x), mark(s.y), mark(s.z), mark(s.w);
+                for (int64_t i = threadIdx.x; i < fours; i += blockDim.x) {
+                    const int4 s = __ldg(reinterpret_cast<const int4*>(p.slots) + i);
+                    mark(s.x), mark(s.y), mark(s.z), mark(s.w);
+                }
+                for (int64_t i = 4 * fours + threadIdx.x; i < pairs; i += blockDim.x) mark(__ldg(p.slots + i));
             }
-            for (int64_t i = 4 * fours + threadIdx.x; i < pairs; i += blockDim.x) mark(__ldg(p.slots + i));
             __syncthreads();
             for (int i = warp; i * 32 < n; i += warps) {
                 uint32_t left = ~used[i] & (n - i * 32 < 32 ? (1u << (n - i * 32)) - 1u : 0xFFFFFFFFu);
@@ -682,26 +709,48 @@ int launch_ungroup_type(const UngroupRowsParams& p, cudaStream_t stream) {
     return piece == 32 ? launch_ungroup_piece<DT, 32>(p, stream) : piece == 16 ? launch_ungroup_piece<DT, 16>(p, stream) : launch_ungroup_odd<DT>(p, stream);
 }
 
+// Who writes zeros to the rows without a token
+struct ZeroPlan {
+    int64_t blocks, range, words;  // rows per block and round; words of the map (0: the blocks look at the slots themselves)
+};
+
+ZeroPlan zero_plan(int64_t num_rows, int64_t row_bytes, int64_t pairs) {
+    if (num_rows == 0) return {0, 32, 0};
+    const int64_t sms = sm_count_of_current_device();
+    auto plan = [&](int64_t most) {
+        // 64 rows a block at least
+        int64_t blocks = (num_rows + 63) / 64;
+        blocks = blocks < most ? blocks : most < 1 ? 1 : most;
+        const int64_t range = ((num_rows + blocks - 1) / blocks + 31) / 32 * 32;
+        return ZeroPlan{blocks, range < kZeroRange ? range : kZeroRange, 0};
+    };
+    // Blocks that look for themselves each read all slots in every round: all together a 64th of what the rows move, or 16 MB, a round.  One
+    // block for 1554 rows of 1000: 13 us instead of 4; 148 for 65536 of 4096: 185 instead of 176.
+    const int64_t share = row_bytes / 128, few = (1 << 22) / (pairs + 1), by_bytes = share > few ? share : few;
+    ZeroPlan p = plan(sms < by_bytes ? sms : by_bytes);
+    const int64_t rounds = (num_rows + p.blocks * p.range - 1) / (p.blocks * p.range);
+    if (rounds * pairs <= kMostLooks) return p;
+    p = plan(sms);
+    p.words = (num_rows + 31) / 32;
+    return p;
+}
+
 template <int DT, int B, int U>
-int launch_ungroup_backward(const UngroupRowsParams& p, cudaStream_t stream) {
+int launch_ungroup_backward(UngroupRowsParams p, cudaStream_t stream) {
     const bool warp = p.h <= 1024;
-    const int64_t tokens = warp ? (p.tokens + 7) / 8 : p.tokens;
-    int64_t zero = 0, range = 32;
-    if (p.drows != nullptr && p.num_rows > 0) {
-        // Blocks that look for rows without a token, each of which reads all slots: 64 rows each at least, and all together a 64th of what the
-        // rows move, or 16 MB.  One block for 1554 rows of 1000: 13 us instead of 4; 148 for 65536 of 4096: 185 instead of 176.
-        const int64_t by_rows = (p.num_rows + 63) / 64, share = static_cast<int64_t>(p.h) * kBytes<DT> / 128;
-        const int64_t few = (1 << 22) / (p.tokens * p.k + 1), by_bytes = share > few ? share : few;
-        zero = sm_count_of_current_device();
-        zero = zero < by_rows ? zero : by_rows;
-        zero = zero < by_bytes ? zero : by_bytes < 1 ? 1 : by_bytes;
-        range = ((p.num_rows + zero - 1) / zero + 31) / 32 * 32;
-        range = range < kZeroRange ? range : kZeroRange;
+    const int64_t tokens = warp ? (p.tokens + 7) / 8 : p.tokens, pairs = p.tokens * p.k;
+    const ZeroPlan zero = p.drows != nullptr ? zero_plan(p.num_rows, static_cast<int64_t>(p.h) * kBytes<DT>, pairs) : ZeroPlan{0, 32, 0};
+    if (tokens + zero.blocks > 0x7FFFFFFF) return static_cast<int>(cudaErrorInvalidValue);
+    if (tokens + zero.blocks == 0) return 0;
+    if (zero.words == 0) {
+        p.used = nullptr;
+    } else {
+        int rc = launch_pdl(clear_used_kernel, dim3(static_cast<unsigned>((zero.words + 255) / 256)), 256, 0, stream, p.used, zero.words);
+        if (rc == 0) rc = launch_pdl(mark_used_kernel, dim3(static_cast<unsigned>((pairs + 1023) / 1024)), 256, 0, stream, p.slots, pairs, p.num_rows, p.used);
+        if (rc != 0) return rc;
     }
-    if (tokens + zero > 0x7FFFFFFF) return static_cast<int>(cudaErrorInvalidValue);
-    if (tokens + zero == 0) return 0;
-    const dim3 grid(static_cast<unsigned>(tokens + zero));
-    return warp ? launch_pdl(ungroup_rows_backward_kernel<DT, B, U, true>, grid, 256, 0, stream, p, static_cast<unsigned>(zero), static_cast<int>(range)) : launch_pdl(ungroup_rows_backward_kernel<DT, B, U, false>, grid, 256, 0, stream, p, static_cast<unsigned>(zero), static_cast<int>(range));
+    const dim3 grid(static_cast<unsigned>(tokens + zero.blocks));
+    return launch_pdl(warp ? ungroup_rows_backward_kernel<DT, B, U, true> : ungroup_rows_backward_kernel<DT, B, U, false>, grid, 256, 0, stream, p, static_cast<unsigned>(zero.blocks), static_cast<int>(zero.range));
 }
 
 template <int DT, int B>
@@ -741,6 +790,12 @@ extern "C" int cam_launch_ungroup_rows(const cam::UngroupRowsParams* p, int dtyp
     return dtype == kDtBf16 ? launch_ungroup_type<kDtBf16>(*p, stream) : dtype == kDtFp16 ? launch_ungroup_type<kDtFp16>(*p, stream) : launch_ungroup_type<kDtFp32>(*p, stream);
 }
 
+extern "C" int64_t cam_ungroup_rows_backward_map_words(int64_t num_rows, int h, int dtype, int64_t pairs) {
+    using namespace cam;
+    return zero_plan(num_rows, static_cast<int64_t>(h) * (dtype == kDtFp32 ? 4 : 2), pairs).words;
+}
+
+// `used` (the words above, where there are any) with `drows`
 extern "C" int cam_launch_ungroup_rows_backward(const cam::UngroupRowsParams* p, int dtype, cudaStream_t stream) {
     using namespace cam;
     return dtype == kDtBf16 ? launch_ungroup_backward_type<kDtBf16>(*p, stream) : dtype == kDtFp16 ? launch_ungroup_backward_type<kDtFp16>(*p, stream) : launch_ungroup_backward_type<kDtFp32>(*p, stream);

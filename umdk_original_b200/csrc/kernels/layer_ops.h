@@ -84,6 +84,7 @@ struct UngroupRowsParams {
     const void* dout;       // backward
     void* drows;            // [num_rows, h] or null
     float* dweights;        // [tokens, k] or null
+    uint32_t* used;         // a bit per row, or null: workspace of gradients of many rows
 };
 
 }  // namespace cam
@@ -95,5 +96,6 @@ int cam_launch_rms_norm_backward(const cam::RmsNormBackwardParams* p, int dtype,
 int cam_launch_moe_route(const cam::RouteParams* p, int dtype, cudaStream_t stream);
 int cam_launch_group_rows(const cam::GroupRowsParams* p, cudaStream_t stream);
 int cam_launch_ungroup_rows(const cam::UngroupRowsParams* p, int dtype, cudaStream_t stream);
+int64_t cam_ungroup_rows_backward_map_words(int64_t num_rows, int h, int dtype, int64_t pairs);
 int cam_launch_ungroup_rows_backward(const cam::UngroupRowsParams* p, int dtype, cudaStream_t stream);
 }

@@ -217,13 +217,18 @@ extern "C" int cam_moe_ungroup_rows(const void* rows, int dtype, int64_t num_row
     return launched(cam_launch_ungroup_rows(&p, dtype, stream), "moe_ungroup_rows");
 }
 
+extern "C" int64_t cam_moe_ungroup_rows_backward_words(int dtype, int64_t num_rows, int h, int64_t tokens, int k) {
+    return cam_ungroup_rows_backward_map_words(num_rows, h, dtype, tokens * k);
+}
+
 extern "C" int cam_moe_ungroup_rows_backward(const void* dout, const void* rows, int dtype, int64_t num_rows, int h, const int* slots,
                                              int64_t tokens, int k, const float* weights, void* drows, float* dweights,
-                                             cudaStream_t stream) {
+                                             uint32_t* used, cudaStream_t stream) {
     if (check_ungroup("moe_ungroup_rows_backward", dtype, num_rows, h, tokens, k) != 0) return -1;
     LAYER_CHECK(tokens == 0 || (dout && slots), "moe_ungroup_rows_backward: null operand");
     LAYER_CHECK(dweights == nullptr || rows != nullptr || num_rows == 0, "moe_ungroup_rows_backward: null rows");
     if (drows == nullptr && dweights == nullptr) return 0;
+    LAYER_CHECK(drows == nullptr || used != nullptr || cam_moe_ungroup_rows_backward_words(dtype, num_rows, h, tokens, k) == 0, "moe_ungroup_rows_backward: no workspace");
     cam::UngroupRowsParams p{};
     p.rows = rows;
     p.num_rows = num_rows;
@@ -235,5 +240,6 @@ extern "C" int cam_moe_ungroup_rows_backward(const void* dout, const void* rows,
     p.dout = dout;
     p.drows = drows;
     p.dweights = dweights;
+    p.used = used;
     return launched(cam_launch_ungroup_rows_backward(&p, dtype, stream), "moe_ungroup_rows_backward");
 }

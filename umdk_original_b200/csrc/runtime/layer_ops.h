@@ -33,9 +33,11 @@ int cam_moe_group_rows(const void* x, int64_t row_bytes, int elem_bytes, const f
 // out[t] = residual[t] + sum_j weights[t, j] rows[slots[t, j]]; slots outside [0, num_rows) add nothing
 int cam_moe_ungroup_rows(const void* rows, int dtype, int64_t num_rows, int h, const int* slots, int64_t tokens, int k, const float* weights,
                          const void* residual, void* out, cudaStream_t stream);
+// 32-bit words of the workspace `used` that gradients of rows need; 0: none
+int64_t cam_moe_ungroup_rows_backward_words(int dtype, int64_t num_rows, int h, int64_t tokens, int k);
 // A row belongs to one slot at most; rows of no slot get zeros.
 int cam_moe_ungroup_rows_backward(const void* dout, const void* rows, int dtype, int64_t num_rows, int h, const int* slots, int64_t tokens,
-                                  int k, const float* weights, void* drows, float* dweights, cudaStream_t stream);
+                                  int k, const float* weights, void* drows, float* dweights, uint32_t* used, cudaStream_t stream);
 
 #ifdef __cplusplus
 }
