@@ -1,4 +1,7 @@
 """Norm, routing and rows grouped by expert against their definitions in 64 bits: the CPU implementations here, the kernels on a B200."""
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -517,6 +520,39 @@ def test_ungroup_rows_and_gradients(device, dtype, t, k, h, weighted, with_resid
         assert torch.equal(torch.autograd.grad(ops.moe_ungroup_rows(rows, slots, only, res), only, dout)[0], grads[1])
     if with_residual:
         assert torch.equal(grads[-1], dout)
+
+
+@native
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h", [7, 40, 1032])
+@pytest.mark.parametrize("weighted", [False, True])
+def test_rows_that_no_gradient_reads_are_not_kept(device, dtype, h, weighted):
+    """Weights without a gradient, or none: the rows may change and their memory may go before the backward pass."""
+    g = gen(device, h)
+    z = randn(g, 6, h, dtype=dtype).requires_grad_()
+    slots = torch.tensor([[0, 4], [-1, 2], [5, 1]], device=device, dtype=torch.int32)
+    w = torch.rand(3, 2, generator=g, device=device) if weighted else None
+    dout = randn(g, 3, h, dtype=dtype)
+    rows = z * 1
+    held = weakref.ref(rows.untyped_storage())
+    out = ops.moe_ungroup_rows(rows, slots, w)
+    with torch.no_grad():
+        rows.add_(1)
+    del rows
+    gc.collect()
+    assert held() is None
+    (got,) = torch.autograd.grad(out, z, dout)
+    weights = torch.ones(3, 2, device=device) if w is None else w
+    want, _ = ops.moe_ungroup_rows_backward(dout, z.detach(), slots, weights)
+    assert torch.equal(got, want)
+    # the operator itself: rows [M, 0] stand for their number, but not where they are read
+    none = z.detach()[:, :0].contiguous()
+    assert torch.equal(ops.moe_ungroup_rows_backward(dout, none, slots, weights, True, False)[0], want)
+    with pytest.raises(RuntimeError, match="rows must be"):
+        ops.moe_ungroup_rows_backward(dout, none, slots, weights)
+    with pytest.raises(RuntimeError, match="rows must be"):
+        ops.moe_ungroup_rows_backward(dout[:, :0].contiguous(), none, slots, weights, True, False)
 
 
 @pytest.mark.parametrize("device", DEVICES)

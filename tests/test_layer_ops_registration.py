@@ -62,6 +62,16 @@ def test_all_cases_are_checked():
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_opcheck_of_rows_that_are_only_numbered(device):
+    gen = torch.Generator().manual_seed(2)
+    dout, wt = torch.randn(3, 64, generator=gen).to(device), torch.rand(3, 2, generator=gen).to(device)
+    slots = torch.tensor([[0, 4], [-1, 2], [5, 1]], dtype=torch.int32, device=device)
+    lib = torch.ops.umdk_cam_op_lib
+    opcheck(lib.moe_ungroup_rows_backward.default, (dout, dout.new_empty(6, 0), slots, wt, True, False), test_utils=ALL)
+    opcheck(lib.moe_ungroup_rows.default, (torch.randn(6, 64, generator=gen).to(device).requires_grad_(), slots, wt), test_utils=ALL)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_compiled_program(device):
     """A traced program of all of them, with its backward pass, gives the bits of the eager one."""
     gen = torch.Generator().manual_seed(1)

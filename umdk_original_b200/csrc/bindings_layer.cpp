@@ -231,12 +231,14 @@ struct UngroupProblem {
     int h, k, dtype;
 };
 
-UngroupProblem check_ungroup(const char* op, const at::Tensor& rows, const at::Tensor& slots, const OptTensor& weights) {
+// `h` 0: the width is that of the rows
+UngroupProblem check_ungroup(const char* op, const at::Tensor& rows, const at::Tensor& slots, const OptTensor& weights, int64_t h = 0) {
     check_operand(rows, rows, "rows");
     check_operand(slots, rows, "slots");
     UngroupProblem p{};
     p.dtype = dtype_of(rows.scalar_type(), "rows");
-    CAM_ASSERT(rows.dim() == 2 && rows.size(1) >= 1 && rows.size(1) < (1 << 26) && rows.size(0) < (1ll << 31) - 512, op, ": rows must be [M, h]");
+    if (h == 0 && rows.dim() == 2) h = rows.size(1);
+    CAM_ASSERT(rows.dim() == 2 && h >= 1 && h < (1 << 26) && rows.size(0) < (1ll << 31) - 512, op, ": rows must be [M, h]");
     CAM_ASSERT(slots.dim() == 2 && slots.scalar_type() == at::kInt && slots.size(1) >= 1 && slots.size(1) <= 32, op, ": slots must be int32 [T, k] with k of 1 to 32");
     CAM_ASSERT(slots.numel() < (1ll << 31) - 512, op, ": ", num(slots.numel()), " slots");
     if (given(weights)) {
@@ -244,7 +246,7 @@ UngroupProblem check_ungroup(const char* op, const at::Tensor& rows, const at::T
         CAM_ASSERT(weights->scalar_type() == at::kFloat && weights->sizes() == slots.sizes(), op, ": topk_weights must be float32 ", shape(slots.sizes()));
     }
     p.num_rows = rows.size(0);
-    p.h = static_cast<int>(rows.size(1));
+    p.h = static_cast<int>(h);
     p.tokens = slots.size(0);
     p.k = static_cast<int>(slots.size(1));
     return p;
@@ -268,12 +270,14 @@ at::Tensor moe_ungroup_rows_cuda(const at::Tensor& rows, const at::Tensor& slots
 
 Two moe_ungroup_rows_backward_cuda(const at::Tensor& dout, const at::Tensor& rows, const at::Tensor& slots, const OptTensor& weights,
                                    bool need_drows, bool need_dweights) {
-    const UngroupProblem p = check_ungroup("moe_ungroup_rows_backward", rows, slots, weights);
+    // gradients of rows alone need their number: rows [M, 0] will do
+    const bool numbered = !need_dweights && rows.dim() == 2 && rows.size(1) == 0 && dout.dim() == 2;
+    const UngroupProblem p = check_ungroup("moe_ungroup_rows_backward", rows, slots, weights, numbered ? dout.size(1) : 0);
     check_operand(dout, rows, "dout");
     CAM_ASSERT(dout.scalar_type() == rows.scalar_type() && dout.dim() == 2 && dout.size(0) == p.tokens && dout.size(1) == p.h,
                "moe_ungroup_rows_backward: dout must be [T, h] of the rows' type");
     c10::cuda::CUDAGuard guard(rows.device());
-    at::Tensor drows = need_drows ? cuda_like(rows) : cuda_none(rows);
+    at::Tensor drows = need_drows ? cuda_empty({p.num_rows, p.h}, rows.scalar_type(), rows) : cuda_none(rows);
     at::Tensor dw = need_dweights ? cuda_empty({p.tokens, p.k}, at::kFloat, rows) : cuda_empty({0}, at::kFloat, rows);
     const int64_t words = need_drows ? cam_moe_ungroup_rows_backward_words(p.dtype, p.num_rows, p.h, p.tokens, p.k) : 0;
     at::Tensor used = words > 0 ? cuda_empty({words}, at::kInt, rows) : at::Tensor();
@@ -324,9 +328,9 @@ Four moe_group_rows_meta(const at::Tensor& x, const at::Tensor& topk_idx, int64_
 at::Tensor moe_ungroup_rows_meta(const at::Tensor& rows, const at::Tensor& slots, const OptTensor&, const OptTensor&) {
     return at::empty_symint({slots.sym_size(0), rows.sym_size(1)}, rows.options());
 }
-Two moe_ungroup_rows_backward_meta(const at::Tensor&, const at::Tensor& rows, const at::Tensor& slots, const OptTensor&, bool need_drows, bool need_dweights) {
+Two moe_ungroup_rows_backward_meta(const at::Tensor& dout, const at::Tensor& rows, const at::Tensor& slots, const OptTensor&, bool need_drows, bool need_dweights) {
     const auto floats = rows.options().dtype(at::kFloat);
-    return {need_drows ? at::empty_like(rows) : none_of(rows), need_dweights ? at::empty_symint(slots.sym_sizes(), floats) : at::empty({0}, floats)};
+    return {need_drows ? at::empty_symint({rows.sym_size(0), dout.sym_size(1)}, rows.options()) : none_of(rows), need_dweights ? at::empty_symint(slots.sym_sizes(), floats) : at::empty({0}, floats)};
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -474,9 +478,10 @@ struct UngroupRowsFunction : public torch::autograd::Function<UngroupRowsFunctio
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows, const at::Tensor& slots, const OptTensor& weights, const OptTensor& residual) {
         at::AutoDispatchBelowADInplaceOrView guard;
         at::Tensor out = call_ungroup(rows, slots, weights, residual);
-        // the rows themselves enter the gradient of the weights only
+        // the rows themselves enter the gradient of the weights only; without it their number does, and they are free to change or go
         const bool rows_read = given(weights) && weights->requires_grad();
-        variable_list kept = {rows_read ? kept_for_backward(rows) : rows, kept_for_backward(slots), given(weights) ? kept_for_backward(*weights) : at::Tensor()};
+        variable_list kept = {rows_read ? kept_for_backward(rows) : at::empty_symint({rows.sym_size(0), 0}, rows.options()), kept_for_backward(slots),
+                              given(weights) ? kept_for_backward(*weights) : at::Tensor()};
         if (given(residual)) kept.emplace_back();  // its place says that there was one
         ctx->save_for_backward(kept);
         return out;

@@ -254,10 +254,10 @@ def moe_group_rows_cpu(x, topk_idx, num_experts, scales=None):
     return rows, row_scales, offsets.to(torch.int32), slots.view(t, k)
 
 
-def _check_ungroup(op: str, rows, slots, weights) -> None:
+def _check_ungroup(op: str, rows, slots, weights, numbered: bool = False) -> None:
     _contiguous((rows, "rows"), (slots, "slots"), (weights, "topk_weights"))
     _check_float(rows, "rows")
-    _check(rows.dim() == 2 and rows.shape[1] >= 1, f"{op}: rows must be [M, h]")
+    _check(rows.dim() == 2 and (rows.shape[1] >= 1 or numbered), f"{op}: rows must be [M, h]")
     _check(slots.dim() == 2 and slots.dtype == torch.int32 and 1 <= slots.shape[1] <= MAX_TOPK, f"{op}: slots must be int32 [T, k] with k of 1 to {MAX_TOPK}")
     _check(weights is None or (weights.dtype == torch.float32 and weights.shape == slots.shape), f"{op}: topk_weights must be float32 {list(slots.shape)}")
 
@@ -283,16 +283,19 @@ def moe_ungroup_rows_cpu(rows, slots, topk_weights=None, residual=None):
 
 def moe_ungroup_rows_backward_cpu(dout, rows, slots, topk_weights=None, need_drows=True, need_dweights=True):
     op = "moe_ungroup_rows_backward"
-    _check_ungroup(op, rows, slots, topk_weights)
+    # gradients of rows alone need their number: rows [M, 0] will do
+    numbered = not need_dweights and rows.dim() == 2 and rows.shape[1] == 0 and dout.dim() == 2 and dout.shape[1] >= 1
+    _check_ungroup(op, rows, slots, topk_weights, numbered)
     _contiguous((dout, "dout"))
-    _check(dout.dtype == rows.dtype and tuple(dout.shape) == (slots.shape[0], rows.shape[1]), f"{op}: dout must be [T, h] of the rows' type")
+    h = dout.shape[1] if numbered else rows.shape[1]
+    _check(dout.dtype == rows.dtype and tuple(dout.shape) == (slots.shape[0], h), f"{op}: dout must be [T, h] of the rows' type")
     valid, picked, w = _picked(rows, slots, topk_weights)
     d = dout.float()
     drows, dw = rows.new_empty(0), torch.empty(0)
     if need_drows:
         named = slots[valid]
         _check(named.unique().numel() == named.numel(), f"{op}: a row belongs to one slot at most")
-        drows = torch.zeros(rows.shape, dtype=torch.float32)
+        drows = torch.zeros(rows.shape[0], h, dtype=torch.float32)
         drows[slots[valid].long()] = (d[:, None] * w[..., None])[valid]
         drows = drows.to(rows.dtype)
     if need_dweights:
