@@ -102,3 +102,16 @@ def test_block_without_tokens(device):
         out, s = block(x[:0], res[:0])
     assert out.shape == s.shape == (0, TINY.hidden)
     assert dataclasses.replace(block.routing, topk=1).topk == 1
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_the_8_bit_block_is_a_snapshot(device, score):
+    """What is trained after it was taken does not reach it: not the norm and the router either."""
+    block, x, res, _, _ = make(GROUPED, device, score)
+    fp8 = block.quantized()
+    with torch.no_grad():
+        want = [t.clone() for t in fp8(x, res)]
+        for t in (*block.parameters(), *block.buffers()):
+            t.add_(0.5)
+        assert all(torch.equal(a, b) for a, b in zip(fp8(x, res), want))

@@ -65,8 +65,10 @@ class MoEBlock(torch.nn.Module):
         return ops.moe_ungroup_rows(self.experts(rows, offsets), slots, weights), total
 
     def quantized(self) -> "Fp8MoEBlock":
+        """The block as it is now: training it further leaves the copy alone."""
         w = ExpertWeights(*quantize_fp8_block(self.experts.w1.detach()), *quantize_fp8_block(self.experts.w2.detach()))
-        return Fp8MoEBlock(self.routing, self.norm_weight.detach(), self.gate_weight.detach(), self.route_bias, w, self.eps)
+        bias = None if self.route_bias is None else self.route_bias.clone()
+        return Fp8MoEBlock(self.routing, self.norm_weight.detach().clone(), self.gate_weight.detach().clone(), bias, w, self.eps)
 
 
 @dataclass
