@@ -115,3 +115,19 @@ def test_the_8_bit_block_is_a_snapshot(device, score):
         for t in (*block.parameters(), *block.buffers()):
             t.add_(0.5)
         assert all(torch.equal(a, b) for a, b in zip(fp8(x, res), want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_block_of_another_type(device, score):
+    """A block that was made in one 16-bit type runs in the other; the selection bias stays as it is, in fp32, wherever the block goes."""
+    block, x, res, _, _ = make(GROUPED, device, score, torch.float16)
+    bias = None if block.route_bias is None else block.route_bias.clone()
+    block = block.to(torch.bfloat16)
+    with torch.no_grad():
+        out, s = block(x.bfloat16(), res.bfloat16())
+        assert out.dtype == s.dtype == torch.bfloat16 and block.quantized()(x.bfloat16(), res.bfloat16())[0].shape == out.shape
+    assert bias is None if score == "softmax" else block.route_bias.dtype == torch.float32 and torch.equal(block.route_bias, bias)
+    back = block.half().cpu()
+    assert all(p.dtype == torch.float16 and p.device.type == "cpu" for p in back.parameters())
+    assert bias is None or torch.equal(back.state_dict()["route_bias"], bias.cpu())

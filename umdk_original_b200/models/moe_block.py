@@ -53,6 +53,14 @@ class MoEBlock(torch.nn.Module):
         self.register_buffer("route_bias", torch.zeros(cfg.num_experts, device=device) if score == "sigmoid" else None)
         self.experts = ExpertMLP(cfg.num_experts, cfg.hidden, cfg.intermediate, dtype, device, seed)
 
+    def _apply(self, fn, recurse=True):
+        # a change of the block's type leaves the bias in fp32: the router takes no other, and its small steps would be lost in 16 bits
+        bias = self.route_bias
+        super()._apply(fn, recurse)
+        if bias is not None and self.route_bias.dtype != bias.dtype:
+            self.route_bias = bias.to(self.route_bias.device)
+        return self
+
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """x [T, h], residual [T, h] (or None) -> (what the experts add [T, h], the residual stream after ``x`` [T, h]).  The next block
         takes both as they are."""
