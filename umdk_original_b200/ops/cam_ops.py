@@ -12,6 +12,7 @@ pybind/pybind.cpp:23-42.  This module
 """
 from __future__ import annotations
 
+import sys
 from typing import List, Optional
 
 import torch
@@ -58,7 +59,8 @@ SCHEMAS = [
 ]
 
 if _C is None:
-    if torch.cuda.is_available():
+    # `python -m umdk_original_b200._build` imports the package before it can build the extension
+    if torch.cuda.is_available() and "umdk_original_b200._build" not in sys.orig_argv:
         raise ImportError(
             "umdk_original_b200: the native extension is not built but a GPU is present; run "
             "`python -m umdk_original_b200._build` (refusing to fall back to the CPU path)") from _IMPORT_ERROR
