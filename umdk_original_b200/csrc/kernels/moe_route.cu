@@ -12,9 +12,11 @@
 // only find candidates: k + 1 of them, whose own ranks are then taken exactly (in 64 bits where scores are ranked) and put in order;
 // where the next key is so close that it might belong to them, the row is ranked again by the whole warp.
 //
-// Bound by instructions: 620 for four tokens of 128 bf16 logits and k = 8 (32768 tokens 9.2 us, 11.5 MB), 1450 for two tokens of 256 fp32
-// logits with sigmoid, bias and 4 of 8 groups (16384 tokens 18 us).  A whole warp per token took three times as many.  Rows of
-// nothing but equal logits cost four times as much (16384 x 256: 12 and 38 us; with bias and groups 18 and 108).
+// 620 instructions for four tokens of 128 bf16 logits and k = 8 (32768 tokens 9.2 us, 11.5 MB), 1460 for two tokens of 256 fp32 logits with
+// sigmoid, bias and 4 of 8 groups (16384 tokens 18 us); a whole warp per token took three times as many.  Bound by latency rather
+// than by their issue (1.9 and 2.1 a cycle of 4, five warps a scheduler): of the 10.8 and 9.3 cycles from one to the next a warp waits 3.0 and 1.7
+// for logits, 2.0 and 1.7 for shuffles and shared memory, whose rounds depend on one another, and 1.6 and 2.1 for results of arithmetic.  Rows
+// of nothing but equal logits cost four times as much (16384 x 256: 12 and 38 us; with bias and groups 18 and 108).
 #include <math_constants.h>
 
 #include "layer_ops.h"

@@ -286,7 +286,8 @@ __device__ __forceinline__ void block_scale(float amax, bool power_of_two, float
 }
 
 // Blocks of an SM, as a bound on registers.  Rows in 8 bits: 64 instead of 80 and 86, so that four blocks of 7168 columns have loads on their way
-// and not three: 32768 x 7168 bf16 to e4m3 174 -> 144 us, to int8 235 -> 142, with a residual 244 -> 239 and 294 -> 237; fp32 does not fit
+// and not three: 32768 x 7168 bf16 to e4m3 174 -> 144 us (150 to 158 with what marks blocks that are not finite), to int8 235 -> 142, with a residual
+// 244 -> 239 and 294 -> 237; fp32 does not fit
 // (16384 x 4096 with a residual to int8 128 -> 137).  Values one by one: 32 registers, 8192 x 4095 bf16 to int8 92 us, with 50 127.
 template <int DT, int MODE, int NP, int VEC, bool WARP>
 constexpr int kNormBlocks = !WARP && (VEC == kByOne ? NP == 1 : NP == 2 && MODE != kRowsOnly && DT != kDtFp32) ? 2 : 1;

@@ -68,6 +68,7 @@ class MoEBlock(torch.nn.Module):
             y, total = ops.rms_norm(x, self.norm_weight, self.eps), x
         else:
             y, total = ops.add_rms_norm(x, residual, self.norm_weight, self.eps)
+        # logits of y's type: the product's fp32 sums rounded once, so that the gate reads the rows as they are; equal ones go to the lowest expert
         idx, weights = self.routing(y @ self.gate_weight.t(), self.route_bias)
         rows, _, offsets, slots = ops.moe_group_rows(y, idx, self.gate_weight.shape[0])
         return ops.moe_ungroup_rows(self.experts(rows, offsets), slots, weights), total
